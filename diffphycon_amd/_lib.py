@@ -59,6 +59,29 @@ class SmokeOut(C.Structure):
                 ("frame_stride", C.c_int32), ("space_stride", C.c_int32)]
 
 
+class SeqTensor(C.Structure):
+    """dpc_seq_tensor (include/dpc.h)."""
+    _fields_ = [("p", C.c_void_p), ("stride_b", C.c_int64), ("stride_t", C.c_int64), ("stride_h", C.c_int64)]
+
+
+class SeqRotary(C.Structure):
+    """dpc_seq_rotary (include/dpc.h)."""
+    _fields_ = [("xq", SeqTensor), ("xk", SeqTensor), ("yq", SeqTensor), ("yk", SeqTensor), ("table", C.c_void_p), ("positions", C.c_void_p),
+                ("pos_stride_b", C.c_int64), ("start", C.c_int64), ("max_positions", C.c_int64), ("type", C.c_int32), ("batch", C.c_int32),
+                ("tokens", C.c_int32), ("heads", C.c_int32), ("kv_heads", C.c_int32), ("head_dim", C.c_int32), ("rotary_dim", C.c_int32),
+                ("interleaved", C.c_int32), ("transpose", C.c_int32)]
+
+
+class SeqAttn(C.Structure):
+    """dpc_seq_attn (include/dpc.h)."""
+    _fields_ = [("q", SeqTensor), ("k", SeqTensor), ("v", SeqTensor), ("out", SeqTensor), ("lse", C.c_void_p), ("lse_stride_b", C.c_int64),
+                ("lse_stride_h", C.c_int64), ("dout", SeqTensor), ("dq", SeqTensor), ("dk", SeqTensor), ("dv", SeqTensor),
+                ("key_mask", C.c_void_p), ("mask_stride_b", C.c_int64), ("seqs", C.c_void_p), ("q_tiles", C.c_void_p), ("k_tiles", C.c_void_p),
+                ("n_q_tiles", C.c_int32), ("n_k_tiles", C.c_int32), ("type", C.c_int32), ("batch", C.c_int32), ("heads", C.c_int32),
+                ("kv_heads", C.c_int32), ("head_dim", C.c_int32), ("q_len", C.c_int32), ("k_len", C.c_int32), ("causal", C.c_int32),
+                ("lse_rows", C.c_int64), ("scale", C.c_float)]
+
+
 class ProfileRow(C.Structure):
     """dpc_profile_row (include/dpc.h)."""
     _fields_ = [("name", C.c_char_p), ("launches", C.c_int64), ("total_ms", C.c_double), ("flops", C.c_double),
@@ -173,6 +196,13 @@ _SIGNATURES = {
     "dpc_l2_norm": (C.c_int, [_P, _L, C.c_float, _P, _P, _Z, _P]),
     "dpc_adam_ema_step": (C.c_int, [_P, _P, _P, _P, _P, _L, _P, C.c_float, C.c_float, _D, _D, _D, _D, _I, _I,
                                     C.c_float, _P]),
+    "dpc_seq_norm_fwd": (C.c_int, [_P] * 5 + [_L, _I, _L, C.c_float, _I, _I, _P]),
+    "dpc_seq_norm_bwd_workspace_bytes": (_Z, [_L, _I]),
+    "dpc_seq_norm_bwd": (C.c_int, [_P] * 7 + [_L, _I, _L, _L, _I, _I, _P, _Z, _P]),
+    "dpc_seq_rotary_run": (C.c_int, [C.POINTER(SeqRotary), _P]),
+    "dpc_seq_attn_workspace_bytes": (_Z, [C.POINTER(SeqAttn), _I]),
+    "dpc_seq_attn_fwd": (C.c_int, [C.POINTER(SeqAttn), _P, _Z, _P]),
+    "dpc_seq_attn_bwd": (C.c_int, [C.POINTER(SeqAttn), _P, _Z, _P]),
     "dpc_burgers_fd": (C.c_int, [_P, _P, _P, _I, _I, _I, _D, _D, _D, _P]),
     "dpc_unet2d_create": (C.c_int, [C.POINTER(Unet2DCfg), C.POINTER(_P)]),
     "dpc_unet2d_destroy": (None, [_P]),

@@ -412,6 +412,69 @@ int dpc_adam_ema_step(float* w, const float* g, float* m, float* v, float* ema, 
                       float grad_inv_scale, double lr, double beta1, double beta2, double eps, int step, int ema_mode, float ema_weight,
                       dpc_stream_t stream);
 
+/* ------------------------------------------------------------------ operators on token sequences
+ * Layer norm, rotary positions and attention, forward and backward, for the element types below; they stand beside the fp32
+ * operators above (dpc_ln_*, the rotary inside dpc_attention_core, dpc_attention_core / dpc_attention_bwd), which are bound to
+ * the U-Nets' packed fp32 layout.  Python surface: diffphycon_amd/sequence.py.  Sums, softmax statistics and norms are fp32
+ * whatever the element type; nothing is accumulated with atomics, so results repeat bit for bit. */
+enum dpc_seq_type { DPC_SEQ_F32 = 0, DPC_SEQ_F16 = 1, DPC_SEQ_BF16 = 2 };
+
+/* y = (x - mean) * rstd * weight + bias over the last axis of x [rows][C] (x rows x_stride elements apart, y contiguous);
+ * weight / bias [C] of type wtype (fp32 or type) or NULL; stats [rows][2] = (mean, rstd), rstd = (variance + eps)^-1/2. */
+int dpc_seq_norm_fwd(const void* x, const void* weight, const void* bias, void* y, float* stats, int64_t rows, int C,
+                     int64_t x_stride, float eps, int type, int wtype, dpc_stream_t stream);
+/* dx [rows][C] contiguous; dweight / dbias [C] of type wtype, each NULL: skipped.  ws: partial sums of the two [C] rows. */
+size_t dpc_seq_norm_bwd_workspace_bytes(int64_t rows, int C);
+int dpc_seq_norm_bwd(const void* dy, const void* x, const float* stats, const void* weight, void* dx, void* dweight, void* dbias,
+                     int64_t rows, int C, int64_t dy_stride, int64_t x_stride, int type, int wtype, void* ws, size_t ws_bytes,
+                     dpc_stream_t stream);
+
+/* A [batch][token][head][head_dim] tensor: strides in elements, head_dim contiguous.  Packed sequences: one batch. */
+typedef struct dpc_seq_tensor {
+    void* p;
+    int64_t stride_b, stride_t, stride_h;
+} dpc_seq_tensor;
+
+/* Rotary positions: pair i < rotary_dim / 2 of every head, (2i, 2i + 1) when interleaved != 0, else (i, i + rotary_dim / 2), is
+ * turned by the angle in table [max_positions][rotary_dim / 2][2] = (cos, sin) at the token's position (transpose != 0: by minus
+ * that angle, the gradient); the rest of the head is copied.  xk.p / yk.p NULL: one tensor.  y may be x (in place: the pass-through
+ * part is then not touched).  positions: int64 [batch][tokens] with pos_stride_b elements between batches (0: shared), or NULL:
+ * start + token.  A position outside [0, max_positions) gives NaN in its pairs. */
+typedef struct dpc_seq_rotary {
+    dpc_seq_tensor xq, xk, yq, yk;
+    const float* table;
+    const int64_t* positions;
+    int64_t pos_stride_b, start, max_positions;
+    int32_t type, batch, tokens, heads, kv_heads, head_dim, rotary_dim, interleaved, transpose;
+} dpc_seq_rotary;
+int dpc_seq_rotary_run(const dpc_seq_rotary* a, dpc_stream_t stream);
+
+/* Attention: S_ij = scale q_i k_j over the keys j that query i sees, P = softmax_j(S), out = P v; query head h reads key / value
+ * head h / (heads / kv_heads).  Visible: key_mask[j] != 0 (uint8, NULL: all) and, with causal, j <= i + k_len - q_len of the
+ * sequence.  A query that sees nothing gives out = 0, lse = -inf and no gradient.  Keys that the mask takes out are never read into a product:
+ * they may hold anything.  lse [batch][heads][tokens] = log sum exp S (natural), contiguous in tokens.
+ * Dense: every sequence has q_len / k_len tokens, seqs == NULL.  Otherwise seqs [batch][4] = (first query row, queries, first key row,
+ * keys), rows counted from the batch's own base (stride_b = 0: packed), q_len / k_len the longest; q_tiles / k_tiles [n][2] =
+ * (sequence, block of 128 rows) list every block once, in launch order; rows that no sequence covers are not written.
+ * head_dim: a multiple of 8, at most 128.  Tensor bases and strides: multiples of 16 bytes. */
+typedef struct dpc_seq_attn {
+    dpc_seq_tensor q, k, v, out;             /* forward: out is written; backward: read */
+    float* lse;
+    int64_t lse_stride_b, lse_stride_h;
+    dpc_seq_tensor dout, dq, dk, dv;         /* backward only */
+    const uint8_t* key_mask;
+    int64_t mask_stride_b;
+    const int32_t *seqs, *q_tiles, *k_tiles;
+    int32_t n_q_tiles, n_k_tiles;
+    int32_t type, batch, heads, kv_heads, head_dim, q_len, k_len, causal;
+    int64_t lse_rows;                        /* batch * heads * tokens of lse */
+    float scale;                             /* > 0 */
+} dpc_seq_attn;
+size_t dpc_seq_attn_workspace_bytes(const dpc_seq_attn* a, int backward);
+int dpc_seq_attn_fwd(const dpc_seq_attn* a, void* ws, size_t ws_bytes, dpc_stream_t stream);
+/* dq, dk, dv from dout and the forward's out and lse: the probabilities are computed again from q, k and lse. */
+int dpc_seq_attn_bwd(const dpc_seq_attn* a, void* ws, size_t ws_bytes, dpc_stream_t stream);
+
 /* ------------------------------------------------------------------ Burgers finite-difference solver
  * Replaces dataset/apps/generate_burgers.py:207-299 burgers_numeric_solve_free (fp32, explicit Euler).
  * u0 [N,nx], f [N,num_t,nx] -> traj [N,num_t+1,nx]. */
