@@ -34,15 +34,14 @@ typedef float f32x8 __attribute__((ext_vector_type(8)));
 typedef short s16x4 __attribute__((__vector_size__(8)));
 typedef __attribute__((address_space(3))) s16x4* lds_s16x4;
 
-// LDS image of a tile: rows of DP elements in 16-byte chunks.
-//  16 bits: pitch DP * 2, chunk c of row r stored at c ^ swz(r): the row read (8 lanes = 8 rows, one chunk) and the transpose read (4
-//  rows x 64 bytes) both spread over all banks.  fp32: pitch + 16 bytes does the same for the row read; column reads are contiguous.
+// LDS image of a tile: rows of DP elements in 16-byte chunks, filled 16 bytes a lane straight from global memory (Stage), so the image
+// has no padding; chunk c of row r is stored at c ^ swz(r), which spreads both kinds of read over the banks.  16 bits: the row read (8
+// lanes = 8 rows, one chunk) and the transpose read (4 rows x 64 bytes); fp32: the row read (column reads are whole 128-byte lines).
 template <class T, int DP>
 struct Image {
-    static constexpr int CH = DP * (int)sizeof(T) / 16;
-    static constexpr int PITCH = sizeof(T) == 2 ? DP * 2 : DP * 4 + 16;
+    static constexpr int CH = DP * (int)sizeof(T) / 16, PITCH = CH * 16;
     __device__ static __forceinline__ int swz(int r) {
-        if (sizeof(T) == 4) return 0;
+        if (sizeof(T) == 4) return r & 7;
         return (DP / 32) % 2 ? (r >> 1) & 3 : ((r & 1) << 2) | ((r >> 1) & 3);
     }
     __device__ static __forceinline__ int off(int r, int c) { return r * PITCH + ((c ^ swz(r)) << 4); }
@@ -95,7 +94,8 @@ template <> struct Mma<float> {
         const int h = lane >> 5;
         Frag f;
 #pragma unroll
-        for (int e = 0; e < 4; ++e) f[e] = *reinterpret_cast<const float*>(img + (r0 + 8 * s + 4 * h + e) * Image<float, DP>::PITCH + (32 * dt + (lane & 31)) * 4);
+        for (int e = 0; e < 4; ++e)
+            f[e] = *reinterpret_cast<const float*>(img + Image<float, DP>::off(r0 + 8 * s + 4 * h + e, 8 * dt + ((lane & 31) >> 2)) + (lane & 3) * 4);
         return f;
     }
     __device__ static __forceinline__ Frag from_acc(const f32x16& v, int s) { return Frag{v[4 * s], v[4 * s + 1], v[4 * s + 2], v[4 * s + 3]}; }
@@ -106,13 +106,15 @@ struct Ten { char* p; long long b, t, h; };        // strides in bytes
 struct Params {
     Ten q, k, v, out, dout, dq, dk, dv;
     float* lse;
-    long long lse_b, lse_h;
+    long long lse_b, lse_h, krow_b, krow_h;        // row numbers of q (as in lse) and of k
     const unsigned char* key_mask;
     long long mask_b;
     const int* seqs;
-    const int* tiles;                              // [grid / heads][2] or null (dense)
-    float *lse2, *delta;                           // backward: lse in powers of two (+inf: a row that sees nothing) and D; lse's addressing
-    int heads, kv_heads, group, D, q_len, k_len, causal, tiles_per_seq;
+    const int* tiles;                              // [..][2] = (sequence, block) or null (dense)
+    float *lse2, *ndelta;                          // backward: lse in powers of two (+inf: a row that sees nothing) and -D, numbered like lse
+    float *part, *part_ml;                         // splits: partial sums [split][row][D] and per-row scalars (layout at each kernel)
+    long long part_rows;
+    int heads, kv_heads, group, D, q_len, k_len, causal, n_tiles, tiles_per_seq, subs, splits;
     float scale;
 };
 
@@ -125,28 +127,67 @@ __device__ __forceinline__ Seq sequence(const Params& p, int b) {
     return s;
 }
 
-// ROWS x DP tile, global -> registers -> LDS by 256 threads; rows that `ok` refuses and columns >= D become zero.
-template <class T, int DP, int ROWS>
-struct Stage {
-    static constexpr int CH = Image<T, DP>::CH, N = (ROWS * CH + 255) / 256;
-    static_assert(ROWS * CH % 256 == 0, "whole rounds");
-    uint4 r[N];
-    template <class F> __device__ __forceinline__ void issue(const char* base, long long st, int D, F ok) {
-#pragma unroll
-        for (int i = 0; i < N; ++i) {
-            const int e = threadIdx.x + 256 * i, row = e / CH, c = e % CH;
-            r[i] = uint4{0, 0, 0, 0};
-            if (c * 16 < D * (int)sizeof(T) && ok(row)) r[i] = *reinterpret_cast<const uint4*>(base + row * st + c * 16);
-        }
+// Which block of which (sequence, key head) a workgroup has.  Workgroups go round the 8 XCDs, each with its own L2: the blocks of one
+// (sequence, key head), which read the same keys and values, stay on one XCD where the pairs divide evenly; the blocks with most work
+// (the last ones under a causal mask) come first.  A query block is `subs` sub-blocks of QB rows (rows = tokens x heads of the group).
+struct Where { int b, tile, kvh, sub, split; };
+__device__ __forceinline__ Where where(const Params& p, bool last_first) {
+    Where w;
+    int id = blockIdx.x;
+    if (p.tiles) {
+        w.split = id % p.splits; id /= p.splits;
+        w.sub = id % p.subs; id /= p.subs;
+        w.kvh = id % p.kv_heads;
+        id /= p.kv_heads;
+        w.b = p.tiles[2 * id];
+        w.tile = p.tiles[2 * id + 1];
+        return w;
     }
-    __device__ __forceinline__ void store(char* img) {
+    const int per = p.tiles_per_seq * p.subs * p.splits, pairs = p.n_tiles / p.tiles_per_seq * p.kv_heads;
+    int pair, i;
+    if (pairs % 8 == 0) { const int x = id & 7, j = id >> 3; pair = x * (pairs / 8) + j / per; i = j % per; }
+    else { pair = id % pairs; i = id / pairs; }
+    w.split = i % p.splits; i /= p.splits;
+    w.sub = i % p.subs; i /= p.subs;
+    w.tile = last_first ? p.tiles_per_seq - 1 - i : i;
+    w.b = pair / p.kv_heads;
+    w.kvh = pair % p.kv_heads;
+    return w;
+}
+
+// Sources of 16 (4) bytes for rows and columns that are not there: zeros, and +inf for their lse
+__device__ __attribute__((aligned(16))) const float FILL[8] = {0.f, 0.f, 0.f, 0.f, INFINITY, 0.f, 0.f, 0.f};
+
+// Copies 16 (4) bytes a lane from global memory to LDS at `lds` + 16 (4) * lane, past the registers.  Written out, because the compiler would wait for
+// every such copy in flight before any LDS read; copies_done() is the wait, followed by a barrier.  (A write to m0 needs one wait state before its use.)
+__device__ __forceinline__ void copy16(const char* src, unsigned lds) {
+    asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, off" :: "v"(src), "s"(lds) : "memory", "m0");
+}
+__device__ __forceinline__ void copy4(const char* src, unsigned lds) {
+    asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dword %0, off" :: "v"(src), "s"(lds) : "memory", "m0");
+}
+__device__ __forceinline__ void copies_done() { asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); }
+__device__ __forceinline__ unsigned lds_offset(const void* p) {
+    return __builtin_amdgcn_readfirstlane((unsigned)(size_t)(__attribute__((address_space(3))) const char*)p);
+}
+
+// KB x DP tile, global -> LDS by 256 threads; rows whose bit is 0 and columns >= D become zero.
+template <class T, int DP>
+struct Stage {
+    static constexpr int CH = Image<T, DP>::CH, N = KB * CH / 256;
+    static_assert(KB * CH % 256 == 0, "whole rounds");
+    __device__ static __forceinline__ void issue(char* img, const char* base, long long st, int D, unsigned long long bits) {
+        const unsigned at = lds_offset(img) + (threadIdx.x >> 6) * 1024;
 #pragma unroll
         for (int i = 0; i < N; ++i) {
-            const int e = threadIdx.x + 256 * i, row = e / CH, c = e % CH;
-            *reinterpret_cast<uint4*>(img + Image<T, DP>::off(row, c)) = r[i];
+            const int e = threadIdx.x + 256 * i, row = e / CH, c = (e % CH) ^ Image<T, DP>::swz(row);
+            const char* src = base + row * st + c * 16;
+            if (!((bits >> row) & 1) || c * 16 >= D * (int)sizeof(T)) src = reinterpret_cast<const char*>(FILL);
+            copy16(src, __builtin_amdgcn_readfirstlane(at + i * 4096));
         }
     }
 };
+__device__ __forceinline__ unsigned long long first_bits(int n) { return n >= 64 ? ~0ull : n <= 0 ? 0ull : (1ull << n) - 1; }
 
 // operand fragments of one row (this lane's column of the product), zero where !ok
 template <class T, int DP>
@@ -161,7 +202,7 @@ __device__ __forceinline__ void load_row(typename Mma<T>::Frag (&f)[DP / Mma<T>:
 }
 
 // acc[dt] (rows = columns 32 dt .. of the tensor, column = this lane's row) * mul -> row
-template <class T, int DP>
+template <class T, int DP, class Q = typename Mma<T>::Quad>
 __device__ __forceinline__ void store_row(const f32x16 (&acc)[DP / 32], char* row, int h, int D, float mul) {
 #pragma unroll
     for (int dt = 0; dt < DP / 32; ++dt)
@@ -170,7 +211,7 @@ __device__ __forceinline__ void store_row(const f32x16 (&acc)[DP / 32], char* ro
             const int d = 32 * dt + 8 * g + 4 * h;
             if (d < D) {
                 const f32x4 v = {acc[dt][4 * g] * mul, acc[dt][4 * g + 1] * mul, acc[dt][4 * g + 2] * mul, acc[dt][4 * g + 3] * mul};
-                *reinterpret_cast<typename Mma<T>::Quad*>(row + d * (int)sizeof(T)) = __builtin_convertvector(v, typename Mma<T>::Quad);
+                *reinterpret_cast<Q*>(row + d * (int)(sizeof(Q) / 4)) = __builtin_convertvector(v, Q);
             }
         }
 }
@@ -187,13 +228,17 @@ template <int N> __device__ __forceinline__ void times(f32x16 (&a)[N], float m) 
 #pragma unroll
         for (int r = 0; r < 16; ++r) a[i][r] *= m;
 }
+__device__ __forceinline__ float other_half(float v) {               // the value of lane l ^ 32
+    const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    return __uint_as_float(threadIdx.x & 32 ? r[0] : r[1]);
+}
 
 // fp16 only: keep |t| * sc inside fp16 by a power of two per column; when it has to shrink, the column's sum follows.
 template <int N> __device__ __forceinline__ void scale_col(f32x16& t, float& sc, f32x16 (&acc)[N]) {
     float m = 0.f;
 #pragma unroll
     for (int r = 0; r < 16; ++r) m = fmaxf(m, fabsf(t[r]));
-    m = fmaxf(m, __shfl_xor(m, 32, 64));
+    m = fmaxf(m, other_half(m));
     if (__any(m * sc > 32768.f)) {
         float ns = sc;
         if (m * sc > 32768.f) ns = ldexpf(1.f, 14 - min(ilogbf(m), 127));
@@ -205,353 +250,503 @@ template <int N> __device__ __forceinline__ void scale_col(f32x16& t, float& sc,
 }
 
 template <class T> __device__ __forceinline__ constexpr bool is_f16() { return __is_same(T, _Float16); }
+template <class T, int DP> constexpr int WAVES = sizeof(T) == 2 || DP <= 64 ? 2 : 1;       // workgroups of a CU that the registers have to allow
 
-// Which keys of the staged tile take part: bit j.  Without a key mask only the sequence's end matters.
-__device__ __forceinline__ unsigned long long key_bits(const unsigned char* mask, int kt, int kl, int lane) {
-    const int j = kt + lane;
-    return __ballot(j < kl && (!mask || mask[j]));
-}
+// The keys of a tile that take part, one tile ahead: without a key mask by the sequence's end, with one by a byte a lane
+struct KeyBits {
+    const unsigned char* mask;
+    int kl, lane;
+    unsigned char next;
+    __device__ __forceinline__ void fetch(int kt) { if (mask) next = kt + lane < kl ? mask[kt + lane] : 0; }
+    __device__ __forceinline__ unsigned long long bits(int kt) const { return mask ? __ballot(next != 0) : first_bits(kl - kt); }
+};
 
+// Rows of a query block: row r = token r / group, head kvh * group + r % group, so that heads which share keys share the tile's loads.
 template <class T, int DP>
-__global__ __launch_bounds__(256) void fwd_kernel(const Params p) {
+__global__ __launch_bounds__(256, (WAVES<T, DP>)) void fwd_kernel(const Params p) {
     typedef Mma<T> M;
-    constexpr int NF = DP / M::KS, NP = 32 / M::KS, ND = DP / 32;
-    extern __shared__ __attribute__((aligned(16))) char smem[];
-    char* const img_k = smem;
-    char* const img_v = smem + KB * Image<T, DP>::PITCH;
+    constexpr int NF = DP / M::KS, NP = 32 / M::KS, ND = DP / 32, IMG = KB * Image<T, DP>::PITCH;
+    extern __shared__ __attribute__((aligned(16))) char smem[];       // [2][K, V]
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, l31 = lane & 31, h = lane >> 5;
-    const int head = blockIdx.x % p.heads, ti = blockIdx.x / p.heads;
-    const int b = p.tiles ? p.tiles[2 * ti] : ti / p.tiles_per_seq, tile = p.tiles ? p.tiles[2 * ti + 1] : ti % p.tiles_per_seq;
-    const Seq s = sequence(p, b);
-    if (tile * QB >= s.ql) return;
-    const int kvh = head / p.group, off = s.kl - s.ql;
-    const int qw = tile * QB + wave * 32, qi = qw + l31;            // this wave's first query, this lane's
-    const bool qok = qi < s.ql;
-    const int kend = p.causal ? min(s.kl, min(tile * QB + QB, s.ql) + off) : s.kl;
-    const char* const kbase = p.k.p + b * p.k.b + s.k0 * p.k.t + kvh * p.k.h;
-    const char* const vbase = p.v.p + b * p.v.b + s.k0 * p.v.t + kvh * p.v.h;
-    const unsigned char* const mask = p.key_mask ? p.key_mask + b * p.mask_b + s.k0 : nullptr;
+    const Where w = where(p, true);
+    const Seq s = sequence(p, w.b);
+    const int rows = s.ql * p.group, r0 = w.tile * QB * p.group + w.sub * QB;       // (tokens < 2^31 / 128 a sequence is far beyond memory x heads)
+    if (r0 >= min(rows, (w.tile + 1) * QB * p.group)) return;
+    const int off = s.kl - s.ql, rw = r0 + wave * 32, r = rw + l31;   // this wave's first row, this lane's
+    const bool rok = r < rows;
+    const int token = (rok ? r : r0) / p.group, head = w.kvh * p.group + (rok ? r : r0) % p.group;
+    const int t_first = rw / p.group, t_last = (rw + 31) / p.group;   // this wave's tokens
+    int kend = p.causal ? min(s.kl, min((r0 + QB - 1) / p.group, s.ql - 1) + 1 + off) : s.kl, kbegin = 0;
+    if (p.splits > 1) {                                              // whole tiles, at least four
+        const int per = max(4, (max(kend, 0) + KB * p.splits - 1) / (KB * p.splits)) * KB;
+        kbegin = w.split * per;
+        kend = min(kend, kbegin + per);
+    }
+    const char* const kbase = p.k.p + w.b * p.k.b + s.k0 * p.k.t + w.kvh * p.k.h;
+    const char* const vbase = p.v.p + w.b * p.v.b + s.k0 * p.v.t + w.kvh * p.v.h;
+    KeyBits kb{p.key_mask ? p.key_mask + w.b * p.mask_b + s.k0 : nullptr, s.kl, lane, 0};
     typename M::Frag qf[NF];
-    load_row<T, DP>(qf, p.q.p + b * p.q.b + (s.q0 + (qok ? qi : 0)) * p.q.t + head * p.q.h, h, p.D, qok);
+    load_row<T, DP>(qf, p.q.p + w.b * p.q.b + (s.q0 + token) * p.q.t + head * p.q.h, h, p.D, rok);
     f32x16 o[ND];
     clear(o);
-    // exponents in powers of two; fp16 carries 2^15 P so that small probabilities keep their bits
-    const float c = p.scale * LOG2E, lift = is_f16<T>() ? 15.f : 0.f;
-    float m = -INFINITY, l = 0.f;                                    // running maximum (scaled), this lane's part of the sum
-    Stage<T, DP, KB> sk, sv;
-    auto issue = [&](int kt) {
-        auto ok = [&](int r) { return kt + r < s.kl && (!mask || mask[kt + r]); };
-        sk.issue(kbase + kt * p.k.t, p.k.t, p.D, ok);
-        sv.issue(vbase + kt * p.v.t, p.v.t, p.D, ok);
+    // Exponents in powers of two.  The running maximum m is only raised when a score exceeds it by 2^8, so the sums are rarely rescaled;
+    // probabilities are then at most 2^8, and fp16 carries 2^7 P on top of that so that small ones keep their bits.
+    const float c = p.scale * LOG2E, lift = is_f16<T>() ? 7.f : 0.f;
+    float m = -INFINITY, l = 0.f;                                    // maximum (scaled), this lane's part of the sum
+    unsigned long long cur = 0;
+    auto issue = [&](int kt, int buf) {
+        cur = kb.bits(kt);
+        Stage<T, DP>::issue(smem + buf * 2 * IMG, kbase + kt * p.k.t, p.k.t, p.D, cur);
+        Stage<T, DP>::issue(smem + buf * 2 * IMG + IMG, vbase + kt * p.v.t, p.v.t, p.D, cur);
+        kb.fetch(kt + KB);
     };
-    if (kend > 0) issue(0);
-    for (int kt = 0; kt < kend; kt += KB) {
-        sk.store(img_k);
-        sv.store(img_v);
-        __syncthreads();
-        if (kt + KB < kend) issue(kt + KB);
-        if (!p.causal || kt <= qw + 31 + off) {
-            f32x16 st[2];
-            clear(st);
+    if (kbegin < kend) { kb.fetch(kbegin); issue(kbegin, 0); }
+    int buf = 0;
+    for (int kt = kbegin; kt < kend; kt += KB, buf ^= 1) {
+        const unsigned long long bits = cur;
+        copies_done();
+        __syncthreads();                                             // this tile is there, and everyone is done with the other buffer
+        if (kt + KB < kend) issue(kt + KB, buf ^ 1);
+        if (rw >= rows || (p.causal && kt > t_last + off)) continue;
+        const char* const img_k = smem + buf * 2 * IMG;
+        const char* const img_v = img_k + IMG;
+        f32x16 st[2];
+        clear(st);
+#pragma unroll
+        for (int f = 0; f < NF; ++f)
+#pragma unroll
+            for (int sub = 0; sub < 2; ++sub) st[sub] = M::mma(M::template row<DP>(img_k, sub * 32 + l31, f, h), qf[f], st[sub]);
+        if (bits != ~0ull || (p.causal && kt + KB - 1 > t_first + off)) {
+            const int last = p.causal ? token + off - kt : KB;       // last visible key of the tile
 #pragma unroll
             for (int sub = 0; sub < 2; ++sub)
 #pragma unroll
-                for (int f = 0; f < NF; ++f) st[sub] = M::mma(M::template row<DP>(img_k, sub * 32 + l31, f, h), qf[f], st[sub]);
-            if (mask || kt + KB > s.kl || (p.causal && kt + KB - 1 > qw + off)) {
-                const unsigned long long bits = key_bits(mask, kt, s.kl, lane);
-                const int last = p.causal ? qi + off - kt : KB;      // last visible key of the tile
+                for (int x = 0; x < 16; ++x) {
+                    const int j = sub * 32 + rowmap(x, h);
+                    if (!((bits >> j) & 1) || j > last) st[sub][x] = -INFINITY;
+                }
+        }
+        float tm = fmaxf(st[0][0], st[1][0]);
 #pragma unroll
-                for (int sub = 0; sub < 2; ++sub)
-#pragma unroll
-                    for (int r = 0; r < 16; ++r) {
-                        const int j = sub * 32 + rowmap(r, h);
-                        if (!((bits >> j) & 1) || j > last) st[sub][r] = -INFINITY;
-                    }
-            }
-            float tm = fmaxf(st[0][0], st[1][0]);
-#pragma unroll
-            for (int r = 1; r < 16; ++r) tm = fmaxf(tm, fmaxf(st[0][r], st[1][r]));
-            tm = fmaxf(tm, __shfl_xor(tm, 32, 64));
-            const float mn = fmaxf(m, tm * c);
-            const float sub0 = (mn == -INFINITY ? 0.f : mn) - lift;
-            const float alpha = exp2f(m - (mn == -INFINITY ? 0.f : mn));
+        for (int x = 1; x < 16; ++x) tm = fmaxf(fmaxf(tm, st[0][x]), st[1][x]);
+        tm = fmaxf(tm, other_half(tm)) * c;
+        if (__any(tm > m + 8.f)) {
+            const float mn = fmaxf(m, tm), alpha = mn == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m - mn);
             m = mn;
-            float sum = 0.f;
-#pragma unroll
-            for (int sub = 0; sub < 2; ++sub)
-#pragma unroll
-                for (int r = 0; r < 16; ++r) {
-                    st[sub][r] = __builtin_amdgcn_exp2f(__builtin_fmaf(st[sub][r], c, -sub0));
-                    sum += st[sub][r];
-                }
-            l = l * alpha + sum;
+            l *= alpha;
             times(o, alpha);
-#pragma unroll
-            for (int sub = 0; sub < 2; ++sub)
-#pragma unroll
-                for (int f = 0; f < NP; ++f) {
-                    const typename M::Frag pf = M::from_acc(st[sub], f);
-#pragma unroll
-                    for (int dt = 0; dt < ND; ++dt) o[dt] = M::mma(M::template col<DP>(img_v, sub * 32, f, dt, lane), pf, o[dt]);
-                }
         }
-        __syncthreads();
+        const float sub0 = (m == -INFINITY ? 0.f : m) - lift;
+        float sum[2] = {0.f, 0.f};
+#pragma unroll
+        for (int sub = 0; sub < 2; ++sub)
+#pragma unroll
+            for (int x = 0; x < 16; ++x) {
+                st[sub][x] = __builtin_amdgcn_exp2f(__builtin_fmaf(st[sub][x], c, -sub0));
+                sum[sub] += st[sub][x];
+            }
+        l += sum[0] + sum[1];
+#pragma unroll
+        for (int sub = 0; sub < 2; ++sub)
+#pragma unroll
+            for (int f = 0; f < NP; ++f) {
+                const typename M::Frag pf = M::from_acc(st[sub], f);
+#pragma unroll
+                for (int dt = 0; dt < ND; ++dt) o[dt] = M::mma(M::template col<DP>(img_v, sub * 32, f, dt, lane), pf, o[dt]);
+            }
     }
-    l += __shfl_xor(l, 32, 64);
-    if (!qok) return;
-    store_row<T, DP>(o, p.out.p + b * p.out.b + (s.q0 + qi) * p.out.t + head * p.out.h, h, p.D, l == 0.f ? 0.f : 1.f / l);
-    if (h == 0) p.lse[b * p.lse_b + head * p.lse_h + s.q0 + qi] = l == 0.f ? -INFINITY : (m - lift + log2f(l)) * LN2;
+    l += other_half(l);
+    if (!rok) return;
+    const long long at = w.b * p.lse_b + head * p.lse_h + s.q0 + token;
+    if (p.splits > 1) {                                              // part: sums, part_ml [split][row][2]: maximum and sum
+        store_row<T, DP, f32x4>(o, reinterpret_cast<char*>(p.part + (w.split * p.part_rows + at) * p.D), h, p.D, 1.f);
+        if (h == 0) {
+            float* ml = p.part_ml + 2 * (w.split * p.part_rows + at);
+            ml[0] = m - lift;
+            ml[1] = l;
+        }
+        return;
+    }
+    store_row<T, DP>(o, p.out.p + w.b * p.out.b + (s.q0 + token) * p.out.t + head * p.out.h, h, p.D, l == 0.f ? 0.f : 1.f / l);
+    if (h == 0) p.lse[at] = l == 0.f ? -INFINITY : (m - lift + __builtin_amdgcn_logf(l)) * LN2;
 }
 
-// lse2 = lse in powers of two (+inf where the row saw nothing: e^(S - inf) = 0), delta = sum_d dO O; 16 lanes a row
+// The blocks of 16 rows that join the splits: 16 lanes a row, 8 elements a lane.
+template <class F> __device__ __forceinline__ void join_rows(const Params& p, F f) {
+    Params one = p;
+    one.splits = QB / 16;                                            // (the same block numbering, 16 rows each)
+    const Where w = where(one, true);
+    const Seq s = sequence(p, w.b);
+    const int rows = s.ql * p.group, r = w.tile * QB * p.group + w.sub * QB + w.split * 16 + (threadIdx.x >> 4);
+    if (r >= min(rows, (w.tile + 1) * QB * p.group)) return;
+    const int token = r / p.group, head = w.kvh * p.group + r % p.group;
+    f(w, s, token, head, w.b * p.lse_b + head * p.lse_h + s.q0 + token, (int)(threadIdx.x & 15) * 8);
+}
+
+template <class T> __device__ __forceinline__ void store8(char* row, int d, const float (&v)[8]) {
+#pragma unroll
+    for (int e = 0; e < 8; e += 4)
+        *reinterpret_cast<typename Mma<T>::Quad*>(row + (d + e) * (int)sizeof(T)) = __builtin_convertvector((f32x4{v[e], v[e + 1], v[e + 2], v[e + 3]}), typename Mma<T>::Quad);
+}
+
 template <class T>
-__global__ __launch_bounds__(256) void delta_kernel(const Params p) {
-    const int head = blockIdx.x % p.heads, ti = blockIdx.x / p.heads;
-    const int b = p.tiles ? p.tiles[2 * ti] : ti / p.tiles_per_seq, tile = p.tiles ? p.tiles[2 * ti + 1] : ti % p.tiles_per_seq;
-    const Seq s = sequence(p, b);
-    constexpr int E = 16 / (int)sizeof(T);
-    typedef T V __attribute__((ext_vector_type(E)));
-    const int part = threadIdx.x & 15;
-    for (int r = threadIdx.x >> 4; r < QB; r += 16) {
-        const int i = tile * QB + r;
-        if (i >= s.ql) break;
-        const char* o = p.out.p + b * p.out.b + (s.q0 + i) * p.out.t + head * p.out.h;
-        const char* g = p.dout.p + b * p.dout.b + (s.q0 + i) * p.dout.t + head * p.dout.h;
-        float acc = 0.f;
-        for (int c = part; c * E < p.D; c += 16) {
-            const V a = *reinterpret_cast<const V*>(o + c * 16), e = *reinterpret_cast<const V*>(g + c * 16);
-#pragma unroll
-            for (int k = 0; k < E; ++k) acc = __builtin_fmaf((float)a[k], (float)e[k], acc);
+__global__ __launch_bounds__(256) void fwd_join_kernel(const Params p) {
+    join_rows(p, [&](const Where& w, const Seq& s, int token, int head, long long at, int d) {
+        float m = -INFINITY;
+        for (int i = 0; i < p.splits; ++i) {
+            const float* ml = p.part_ml + 2 * (i * p.part_rows + at);
+            if (ml[1] != 0.f) m = fmaxf(m, ml[0]);                   // (NaN sums count: they have to come out)
         }
+        float l = 0.f, v[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+        for (int i = 0; i < p.splits; ++i) {
+            const float* ml = p.part_ml + 2 * (i * p.part_rows + at);
+            if (ml[1] == 0.f) continue;
+            const float a = __builtin_amdgcn_exp2f(ml[0] - m);
+            l += ml[1] * a;
+            if (d < p.D) {
+                const f32x4* x = reinterpret_cast<const f32x4*>(p.part + (i * p.part_rows + at) * p.D + d);
 #pragma unroll
-        for (int x = 8; x; x >>= 1) acc += __shfl_xor(acc, x, 64);
-        if (part == 0) {
-            const long long at = b * p.lse_b + head * p.lse_h + s.q0 + i;
-            const float v = p.lse[at];
-            p.lse2[at] = v == -INFINITY ? INFINITY : v * LOG2E;
-            p.delta[at] = v == -INFINITY ? 0.f : acc;
+                for (int e = 0; e < 8; ++e) v[e] += x[e / 4][e % 4] * a;
+            }
         }
-    }
+        const float inv = l == 0.f ? 0.f : 1.f / l;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) v[e] *= inv;
+        if (d < p.D) store8<T>(p.out.p + w.b * p.out.b + (s.q0 + token) * p.out.t + head * p.out.h, d, v);
+        if (d == 0) p.lse[at] = l == 0.f ? -INFINITY : (m + __builtin_amdgcn_logf(l)) * LN2;
+    });
 }
 
+// dQ, and for the dK/dV kernel lse2 and -D.  D = sum_d dO O with the 16-bit O misses what O's rounding lost; since the probabilities of a
+// row add up to 1, sum_j P (dP - D) is exactly that error, so the sweep adds it up and hands the corrected D on.  Rows that see at most
+// 256 keys -- where dP and D are of one size -- are swept once for D alone before they are swept for dQ.
 template <class T, int DP>
-__global__ __launch_bounds__(256) void dq_kernel(const Params p) {
+__global__ __launch_bounds__(256, (WAVES<T, DP>)) void dq_kernel(const Params p) {
     typedef Mma<T> M;
-    constexpr int NF = DP / M::KS, NP = 32 / M::KS, ND = DP / 32;
-    extern __shared__ __attribute__((aligned(16))) char smem[];
-    char* const img_k = smem;
-    char* const img_v = smem + KB * Image<T, DP>::PITCH;
+    constexpr int NF = DP / M::KS, NP = 32 / M::KS, ND = DP / 32, IMG = KB * Image<T, DP>::PITCH;
+    constexpr bool FIX = sizeof(T) == 2;
+    extern __shared__ __attribute__((aligned(16))) char smem[];       // [2][K, V]
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, l31 = lane & 31, h = lane >> 5;
-    const int head = blockIdx.x % p.heads, ti = blockIdx.x / p.heads;
-    const int b = p.tiles ? p.tiles[2 * ti] : ti / p.tiles_per_seq, tile = p.tiles ? p.tiles[2 * ti + 1] : ti % p.tiles_per_seq;
-    const Seq s = sequence(p, b);
-    if (tile * QB >= s.ql) return;
-    const int kvh = head / p.group, off = s.kl - s.ql;
-    const int qw = tile * QB + wave * 32, qi = qw + l31;
-    const bool in = qi < s.ql;
-    const int kend = p.causal ? min(s.kl, min(tile * QB + QB, s.ql) + off) : s.kl;
-    const char* const kbase = p.k.p + b * p.k.b + s.k0 * p.k.t + kvh * p.k.h;
-    const char* const vbase = p.v.p + b * p.v.b + s.k0 * p.v.t + kvh * p.v.h;
-    const unsigned char* const mask = p.key_mask ? p.key_mask + b * p.mask_b + s.k0 : nullptr;
-    const long long at = b * p.lse_b + head * p.lse_h + s.q0 + (in ? qi : 0);
-    const float lse2 = in ? p.lse2[at] : INFINITY, delta = in ? p.delta[at] : 0.f;
-    const bool sees = lse2 != INFINITY;                              // (a row that sees nothing takes no part, whatever it holds)
+    const Where w = where(p, true);
+    const Seq s = sequence(p, w.b);
+    const int rows = s.ql * p.group, r0 = w.tile * QB * p.group + w.sub * QB;
+    if (r0 >= min(rows, (w.tile + 1) * QB * p.group)) return;
+    const int off = s.kl - s.ql, rw = r0 + wave * 32, r = rw + l31;
+    const bool rok = r < rows;
+    const int token = (rok ? r : r0) / p.group, head = w.kvh * p.group + (rok ? r : r0) % p.group;
+    const int t_first = rw / p.group, t_last = (rw + 31) / p.group;
+    int kend = p.causal ? min(s.kl, min((r0 + QB - 1) / p.group, s.ql - 1) + 1 + off) : s.kl, kbegin = 0;
+    if (p.splits > 1) {
+        const int per = max(4, (max(kend, 0) + KB * p.splits - 1) / (KB * p.splits)) * KB;
+        kbegin = w.split * per;
+        kend = min(kend, kbegin + per);
+    }
+    const char* const kbase = p.k.p + w.b * p.k.b + s.k0 * p.k.t + w.kvh * p.k.h;
+    const char* const vbase = p.v.p + w.b * p.v.b + s.k0 * p.v.t + w.kvh * p.v.h;
+    KeyBits kb{p.key_mask ? p.key_mask + w.b * p.mask_b + s.k0 : nullptr, s.kl, lane, 0};
+    const long long at = w.b * p.lse_b + head * p.lse_h + s.q0 + token;
+    const float lse = rok ? p.lse[at] : -INFINITY;
+    const bool sees = lse != -INFINITY;                              // (a row that sees nothing takes no part, whatever it holds)
+    const float lse2 = sees ? lse * LOG2E : INFINITY;
     typename M::Frag qf[NF], gf[NF];
-    const long long row = s.q0 + (in ? qi : 0);
-    load_row<T, DP>(qf, p.q.p + b * p.q.b + row * p.q.t + head * p.q.h, h, p.D, sees);
-    load_row<T, DP>(gf, p.dout.p + b * p.dout.b + row * p.dout.t + head * p.dout.h, h, p.D, sees);
+    load_row<T, DP>(qf, p.q.p + w.b * p.q.b + (s.q0 + token) * p.q.t + head * p.q.h, h, p.D, sees);
+    load_row<T, DP>(gf, p.dout.p + w.b * p.dout.b + (s.q0 + token) * p.dout.t + head * p.dout.h, h, p.D, sees);
+    float nd = 0.f, rho = 0.f;                                       // -D, what D still misses
+    {
+        typename M::Frag of[NF];
+        load_row<T, DP>(of, p.out.p + w.b * p.out.b + (s.q0 + token) * p.out.t + head * p.out.h, h, p.D, sees);
+#pragma unroll
+        for (int f = 0; f < NF; ++f)
+#pragma unroll
+            for (int e = 0; e < M::KS / 2; ++e) nd = __builtin_fmaf(-(float)of[f][e], (float)gf[f][e], nd);
+        nd += other_half(nd);
+    }
     f32x16 acc[ND];
     clear(acc);
     const float c = p.scale * LOG2E;
     float sc = is_f16<T>() ? 0x1p100f : 1.f;
-    Stage<T, DP, KB> sk, sv;
-    auto issue = [&](int kt) {
-        auto ok = [&](int r) { return kt + r < s.kl && (!mask || mask[kt + r]); };
-        sk.issue(kbase + kt * p.k.t, p.k.t, p.D, ok);
-        sv.issue(vbase + kt * p.v.t, p.v.t, p.D, ok);
+    unsigned long long cur = 0;
+    auto issue = [&](int kt, int buf) {
+        cur = kb.bits(kt);
+        Stage<T, DP>::issue(smem + buf * 2 * IMG, kbase + kt * p.k.t, p.k.t, p.D, cur);
+        Stage<T, DP>::issue(smem + buf * 2 * IMG + IMG, vbase + kt * p.v.t, p.v.t, p.D, cur);
     };
-    if (kend > 0) issue(0);
-    for (int kt = 0; kt < kend; kt += KB) {
-        sk.store(img_k);
-        sv.store(img_v);
+    const int tiles = kend > kbegin ? (kend - kbegin + KB - 1) / KB : 0;
+    const int first = FIX && p.splits == 1 && tiles <= 4 ? tiles : 0;             // tiles of the sweep for D alone
+    auto key = [&](int i) { return kbegin + (i < first ? i : i - first) * KB; };
+    if (tiles) { kb.fetch(key(0)); issue(key(0), 0); if (first + tiles > 1) kb.fetch(key(1)); }
+    for (int i = 0; i < first + tiles; ++i) {
+        const unsigned long long bits = cur;
+        const int kt = key(i), buf = i & 1;
+        copies_done();
         __syncthreads();
-        if (kt + KB < kend) issue(kt + KB);
-        if (!p.causal || kt <= qw + 31 + off) {
-            const bool partial = mask || kt + KB > s.kl || (p.causal && kt + KB - 1 > qw + off);
-            const unsigned long long bits = partial ? key_bits(mask, kt, s.kl, lane) : ~0ull;
-            const int last = p.causal ? qi + off - kt : KB;
+        if (i + 1 < first + tiles) {
+            issue(key(i + 1), buf ^ 1);
+            if (i + 2 < first + tiles) kb.fetch(key(i + 2));
+        }
+        if (FIX && i == first && first) { nd -= rho + other_half(rho); rho = 0.f; }
+        if (rw >= rows || (p.causal && kt > t_last + off)) continue;
+        const char* const img_k = smem + buf * 2 * IMG;
+        const char* const img_v = img_k + IMG;
+        const bool partial = bits != ~0ull || (p.causal && kt + KB - 1 > t_first + off);
+        const int last = p.causal ? token + off - kt : KB;
 #pragma unroll
-            for (int sub = 0; sub < 2; ++sub) {
-                f32x16 st[1], dp[1];
-                clear(st);
-                clear(dp);
+        for (int sub = 0; sub < 2; ++sub) {
+            f32x16 st, dp;
 #pragma unroll
-                for (int f = 0; f < NF; ++f) st[0] = M::mma(M::template row<DP>(img_k, sub * 32 + l31, f, h), qf[f], st[0]);
+            for (int x = 0; x < 16; ++x) { st[x] = 0.f; dp[x] = nd; }
 #pragma unroll
-                for (int f = 0; f < NF; ++f) dp[0] = M::mma(M::template row<DP>(img_v, sub * 32 + l31, f, h), gf[f], dp[0]);
+            for (int f = 0; f < NF; ++f) {
+                st = M::mma(M::template row<DP>(img_k, sub * 32 + l31, f, h), qf[f], st);
+                dp = M::mma(M::template row<DP>(img_v, sub * 32 + l31, f, h), gf[f], dp);
+            }
 #pragma unroll
-                for (int r = 0; r < 16; ++r) st[0][r] = __builtin_amdgcn_exp2f(__builtin_fmaf(st[0][r], c, -lse2)) * (dp[0][r] - delta);
-                if (partial) {
+            for (int x = 0; x < 16; ++x) st[x] = __builtin_amdgcn_exp2f(__builtin_fmaf(st[x], c, -lse2)) * dp[x];
+            if (partial) {
 #pragma unroll
-                    for (int r = 0; r < 16; ++r) {
-                        const int j = sub * 32 + rowmap(r, h);
-                        if (!((bits >> j) & 1) || j > last) st[0][r] = 0.f;
-                    }
-                }
-                if (is_f16<T>()) scale_col(st[0], sc, acc);
-#pragma unroll
-                for (int f = 0; f < NP; ++f) {
-                    const typename M::Frag df = M::from_acc(st[0], f);
-#pragma unroll
-                    for (int dt = 0; dt < ND; ++dt) acc[dt] = M::mma(M::template col<DP>(img_k, sub * 32, f, dt, lane), df, acc[dt]);
+                for (int x = 0; x < 16; ++x) {
+                    const int j = sub * 32 + rowmap(x, h);
+                    if (!((bits >> j) & 1) || j > last) st[x] = 0.f;
                 }
             }
+            if (FIX) {
+                float a = 0.f;
+#pragma unroll
+                for (int x = 0; x < 16; ++x) a += st[x];
+                rho += a;
+                if (i < first) continue;
+            }
+            if (is_f16<T>()) scale_col(st, sc, acc);
+#pragma unroll
+            for (int f = 0; f < NP; ++f) {
+                const typename M::Frag df = M::from_acc(st, f);
+#pragma unroll
+                for (int dt = 0; dt < ND; ++dt) acc[dt] = M::mma(M::template col<DP>(img_k, sub * 32, f, dt, lane), df, acc[dt]);
+            }
         }
-        __syncthreads();
     }
-    if (in) store_row<T, DP>(acc, p.dq.p + b * p.dq.b + row * p.dq.t + head * p.dq.h, h, p.D, p.scale / sc);
+    rho += other_half(rho);
+    if (!rok) return;
+    const float un = p.scale / sc;
+    if (p.splits > 1) {                                              // part: sums, part_ml [split][row]: rho
+        store_row<T, DP, f32x4>(acc, reinterpret_cast<char*>(p.part + (w.split * p.part_rows + at) * p.D), h, p.D, un);
+        if (h == 0) p.part_ml[w.split * p.part_rows + at] = rho;
+        if (h == 0 && w.split == 0) { p.lse2[at] = lse2; p.ndelta[at] = nd; }
+        return;
+    }
+    store_row<T, DP>(acc, p.dq.p + w.b * p.dq.b + (s.q0 + token) * p.dq.t + head * p.dq.h, h, p.D, un);
+    if (h == 0) { p.lse2[at] = lse2; p.ndelta[at] = nd - rho; }
+}
+
+template <class T>
+__global__ __launch_bounds__(256) void dq_join_kernel(const Params p) {
+    join_rows(p, [&](const Where& w, const Seq& s, int token, int head, long long at, int d) {
+        float v[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f}, rho = 0.f;
+        for (int i = 0; i < p.splits; ++i) {
+            rho += p.part_ml[i * p.part_rows + at];
+            if (d < p.D) {
+                const f32x4* x = reinterpret_cast<const f32x4*>(p.part + (i * p.part_rows + at) * p.D + d);
+#pragma unroll
+                for (int e = 0; e < 8; ++e) v[e] += x[e / 4][e % 4];
+            }
+        }
+        if (d < p.D) store8<T>(p.dq.p + w.b * p.dq.b + (s.q0 + token) * p.dq.t + head * p.dq.h, d, v);
+        if (d == 0) p.ndelta[at] -= rho;
+    });
 }
 
 template <class T, int DP>
-__global__ __launch_bounds__(256) void dkv_kernel(const Params p) {
+__global__ __launch_bounds__(256, (WAVES<T, DP>)) void dkv_kernel(const Params p) {
     typedef Mma<T> M;
-    constexpr int NF = DP / M::KS, NP = 32 / M::KS, ND = DP / 32;
-    extern __shared__ __attribute__((aligned(16))) char smem[];
-    char* const img_q = smem;
-    char* const img_g = smem + KB * Image<T, DP>::PITCH;
-    float* const s_lse = reinterpret_cast<float*>(smem + 2 * KB * Image<T, DP>::PITCH);     // [64] lse2, [64] delta
+    constexpr int NF = DP / M::KS, NP = 32 / M::KS, ND = DP / 32, IMG = KB * Image<T, DP>::PITCH;
+    extern __shared__ __attribute__((aligned(16))) char smem[];       // [2][Q, dO], then [2][lse2, -D][64]
+    float* const s_row = reinterpret_cast<float*>(smem + 4 * IMG);
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, l31 = lane & 31, h = lane >> 5;
-    const int kvh = blockIdx.x % p.kv_heads, ti = blockIdx.x / p.kv_heads;
-    const int b = p.tiles ? p.tiles[2 * ti] : ti / p.tiles_per_seq, tile = p.tiles ? p.tiles[2 * ti + 1] : ti % p.tiles_per_seq;
-    const Seq s = sequence(p, b);
-    if (tile * QB >= s.kl) return;
+    const Where w = where(p, false);
+    const Seq s = sequence(p, w.b);
+    if (w.tile * QB >= s.kl) return;
     const int off = s.kl - s.ql;
-    const int kw = tile * QB + wave * 32, kj = kw + l31;             // this wave's first key, this lane's
+    const int kw = w.tile * QB + wave * 32, kj = kw + l31;           // this wave's first key, this lane's
     const bool in = kj < s.kl;
     const long long row = s.k0 + (in ? kj : 0);
-    const bool live = in && (!p.key_mask || p.key_mask[b * p.mask_b + row]);
+    const bool live = in && (!p.key_mask || p.key_mask[w.b * p.mask_b + row]);
     typename M::Frag kf[NF], vf[NF];
-    load_row<T, DP>(kf, p.k.p + b * p.k.b + row * p.k.t + kvh * p.k.h, h, p.D, live);
-    load_row<T, DP>(vf, p.v.p + b * p.v.b + row * p.v.t + kvh * p.v.h, h, p.D, live);
+    load_row<T, DP>(kf, p.k.p + w.b * p.k.b + row * p.k.t + w.kvh * p.k.h, h, p.D, live);
+    load_row<T, DP>(vf, p.v.p + w.b * p.v.b + row * p.v.t + w.kvh * p.v.h, h, p.D, live);
     f32x16 dk[ND], dv[ND];
     clear(dk);
     clear(dv);
     const float c = p.scale * LOG2E, lift = is_f16<T>() ? 15.f : 0.f;
     float sc = is_f16<T>() ? 0x1p100f : 1.f;
-    const int qbegin = p.causal ? max(0, tile * QB - off) / KB * KB : 0;        // first tile with a query that sees the first key
-    const int per_head = qbegin < s.ql ? (s.ql - qbegin + KB - 1) / KB : 0, steps = per_head * p.group;
-    Stage<T, DP, KB> sq, sg;
-    float r_lse = INFINITY, r_delta = 0.f;
-    auto issue = [&](int step) {
-        const int head = kvh * p.group + step / per_head, qt = qbegin + step % per_head * KB;
-        const long long first = s.q0 + qt, at = b * p.lse_b + head * p.lse_h + first;
-        const float* const lse2 = p.lse2 + at;
-        auto ok = [&](int r) { return qt + r < s.ql && lse2[r] != INFINITY; };
-        sq.issue(p.q.p + b * p.q.b + first * p.q.t + head * p.q.h, p.q.t, p.D, ok);
-        sg.issue(p.dout.p + b * p.dout.b + first * p.dout.t + head * p.dout.h, p.dout.t, p.D, ok);
-        if (tid < KB) {
-            r_lse = qt + tid < s.ql ? lse2[tid] : INFINITY;
-            r_delta = qt + tid < s.ql ? p.delta[at + tid] : 0.f;
-        }
+    const int qbegin = p.causal ? max(0, w.tile * QB - off) : 0;                 // first query that sees the first key
+    const int per_head = qbegin < s.ql ? (s.ql - qbegin + KB - 1) / KB : 0;
+    int step = 0, steps = per_head * p.group;
+    if (p.splits > 1) {
+        const int per = (steps + p.splits - 1) / p.splits;
+        step = min(steps, w.split * per);
+        steps = min(steps, step + per);
+    }
+    // Rows that see nothing are not read (their lse2 is +inf).  Under a causal mask alone they lie before qbegin; a key mask can leave any
+    // row empty, so its lse2 is looked at first, a tile ahead.
+    float ahead = 0.f;
+    auto fetch = [&](int i) {
+        const int qt = qbegin + i % per_head * KB + lane;
+        if (p.key_mask) ahead = qt < s.ql ? p.lse2[w.b * p.lse_b + (w.kvh * p.group + i / per_head) * p.lse_h + s.q0 + qt] : INFINITY;
     };
-    if (steps > 0) issue(0);
-    for (int step = 0; step < steps; ++step) {
-        const int qt = qbegin + step % per_head * KB;
-        sq.store(img_q);
-        sg.store(img_g);
-        if (tid < KB) { s_lse[tid] = r_lse - lift; s_lse[KB + tid] = r_delta; }
+    auto issue = [&](int i, int buf) {
+        const int head = w.kvh * p.group + i / per_head, qt = qbegin + i % per_head * KB;
+        const long long first = s.q0 + qt, at = w.b * p.lse_b + head * p.lse_h + first;
+        const unsigned long long bits = p.key_mask ? __ballot(ahead != INFINITY) : first_bits(s.ql - qt);
+        Stage<T, DP>::issue(smem + buf * 2 * IMG, p.q.p + w.b * p.q.b + first * p.q.t + head * p.q.h, p.q.t, p.D, bits);
+        Stage<T, DP>::issue(smem + buf * 2 * IMG + IMG, p.dout.p + w.b * p.dout.b + first * p.dout.t + head * p.dout.h, p.dout.t, p.D, bits);
+        const bool there = (bits >> lane) & 1;
+        if (wave == 0) copy4(reinterpret_cast<const char*>(there ? p.lse2 + at + lane : FILL + 4), lds_offset(s_row + buf * 128));
+        if (wave == 1) copy4(reinterpret_cast<const char*>(there ? p.ndelta + at + lane : FILL), lds_offset(s_row + buf * 128 + 64));
+    };
+    if (step < steps) { fetch(step); issue(step, step & 1); if (step + 1 < steps) fetch(step + 1); }
+    for (; step < steps; ++step) {
+        const int qt = qbegin + step % per_head * KB, buf = step & 1;
+        copies_done();
         __syncthreads();
-        if (step + 1 < steps) issue(step + 1);
-        if (!p.causal || qt + KB - 1 >= kw - off) {
-            const bool partial = p.causal && kw + 31 - off > qt;
+        if (step + 1 < steps) {
+            issue(step + 1, buf ^ 1);
+            if (step + 2 < steps) fetch(step + 2);
+        }
+        if (kw >= s.kl || (p.causal && qt + KB - 1 < kw - off)) continue;
+        const char* const img_q = smem + buf * 2 * IMG;
+        const char* const img_g = img_q + IMG;
+        const bool partial = p.causal && kw + 31 - off > qt;
 #pragma unroll
-            for (int sub = 0; sub < 2; ++sub) {
-                f32x16 st[1], dp[1];
-                clear(st);
-                clear(dp);
+        for (int sub = 0; sub < 2; ++sub) {
+            const float* const sl = s_row + buf * 128 + sub * 32 + 4 * h;
+            f32x16 st, dp;
 #pragma unroll
-                for (int f = 0; f < NF; ++f) st[0] = M::mma(M::template row<DP>(img_q, sub * 32 + l31, f, h), kf[f], st[0]);
+            for (int g = 0; g < 4; ++g) {
+                const f32x4 de = *reinterpret_cast<const f32x4*>(sl + 64 + 8 * g);
 #pragma unroll
-                for (int f = 0; f < NF; ++f) dp[0] = M::mma(M::template row<DP>(img_g, sub * 32 + l31, f, h), vf[f], dp[0]);
-                const float* const sl = s_lse + sub * 32 + 4 * h;
+                for (int e = 0; e < 4; ++e) { st[4 * g + e] = 0.f; dp[4 * g + e] = de[e]; }
+            }
 #pragma unroll
-                for (int g = 0; g < 4; ++g) {
-                    const f32x4 le = *reinterpret_cast<const f32x4*>(sl + 8 * g), de = *reinterpret_cast<const f32x4*>(sl + KB + 8 * g);
+            for (int f = 0; f < NF; ++f) {
+                st = M::mma(M::template row<DP>(img_q, sub * 32 + l31, f, h), kf[f], st);
+                dp = M::mma(M::template row<DP>(img_g, sub * 32 + l31, f, h), vf[f], dp);
+            }
 #pragma unroll
-                    for (int e = 0; e < 4; ++e) {
-                        const int r = 4 * g + e;
-                        float pr = __builtin_amdgcn_exp2f(__builtin_fmaf(st[0][r], c, -le[e]));
-                        if (partial && kj - off > qt + sub * 32 + rowmap(r, h)) pr = 0.f;
-                        st[0][r] = pr;
-                        dp[0][r] = pr * (dp[0][r] - de[e]);
-                    }
+            for (int g = 0; g < 4; ++g) {
+                const f32x4 le = *reinterpret_cast<const f32x4*>(sl + 8 * g);
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    const int x = 4 * g + e;
+                    float pr = __builtin_amdgcn_exp2f(__builtin_fmaf(st[x], c, lift - le[e]));
+                    if (partial && kj - off > qt + sub * 32 + rowmap(x, h)) pr = 0.f;
+                    st[x] = pr;
+                    dp[x] *= pr;
                 }
-                if (is_f16<T>()) scale_col(dp[0], sc, dk);
+            }
+            if (is_f16<T>()) scale_col(dp, sc, dk);
 #pragma unroll
-                for (int f = 0; f < NP; ++f) {
-                    const typename M::Frag pf = M::from_acc(st[0], f), df = M::from_acc(dp[0], f);
+            for (int f = 0; f < NP; ++f) {
+                const typename M::Frag pf = M::from_acc(st, f), df = M::from_acc(dp, f);
 #pragma unroll
-                    for (int dt = 0; dt < ND; ++dt) dv[dt] = M::mma(M::template col<DP>(img_g, sub * 32, f, dt, lane), pf, dv[dt]);
-#pragma unroll
-                    for (int dt = 0; dt < ND; ++dt) dk[dt] = M::mma(M::template col<DP>(img_q, sub * 32, f, dt, lane), df, dk[dt]);
+                for (int dt = 0; dt < ND; ++dt) {
+                    dv[dt] = M::mma(M::template col<DP>(img_g, sub * 32, f, dt, lane), pf, dv[dt]);
+                    dk[dt] = M::mma(M::template col<DP>(img_q, sub * 32, f, dt, lane), df, dk[dt]);
                 }
             }
         }
-        __syncthreads();
     }
     if (!in) return;
     if (!live) { clear(dk); clear(dv); }
     const float un = is_f16<T>() ? 0x1p-15f : 1.f;                   // (P and with it dS carry 2^15)
-    store_row<T, DP>(dk, p.dk.p + b * p.dk.b + row * p.dk.t + kvh * p.dk.h, h, p.D, p.scale * un / sc);
-    store_row<T, DP>(dv, p.dv.p + b * p.dv.b + row * p.dv.t + kvh * p.dv.h, h, p.D, un);
+    if (p.splits > 1) {                                              // part: [split][dK, dV][row][D]
+        const long long at = w.b * p.krow_b + w.kvh * p.krow_h + row;
+        store_row<T, DP, f32x4>(dk, reinterpret_cast<char*>(p.part + ((2 * w.split) * p.part_rows + at) * p.D), h, p.D, p.scale * un / sc);
+        store_row<T, DP, f32x4>(dv, reinterpret_cast<char*>(p.part + ((2 * w.split + 1) * p.part_rows + at) * p.D), h, p.D, un);
+        return;
+    }
+    store_row<T, DP>(dk, p.dk.p + w.b * p.dk.b + row * p.dk.t + w.kvh * p.dk.h, h, p.D, p.scale * un / sc);
+    store_row<T, DP>(dv, p.dv.p + w.b * p.dv.b + row * p.dv.t + w.kvh * p.dv.h, h, p.D, un);
 }
 
+template <class T>
+__global__ __launch_bounds__(256) void dkv_join_kernel(const Params p) {
+    Params one = p;
+    one.splits = QB / 16;
+    const Where w = where(one, false);
+    const Seq s = sequence(p, w.b);
+    const int j = w.tile * QB + w.split * 16 + (threadIdx.x >> 4), d = (threadIdx.x & 15) * 8;
+    if (j >= s.kl || d >= p.D) return;
+    const long long row = s.k0 + j, at = w.b * p.krow_b + w.kvh * p.krow_h + row;
+#pragma unroll
+    for (int which = 0; which < 2; ++which) {
+        float v[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+        for (int i = 0; i < p.splits; ++i) {
+            const f32x4* x = reinterpret_cast<const f32x4*>(p.part + ((2 * i + which) * p.part_rows + at) * p.D + d);
+#pragma unroll
+            for (int e = 0; e < 8; ++e) v[e] += x[e / 4][e % 4];
+        }
+        const Ten& t = which ? p.dv : p.dk;
+        store8<T>(t.p + w.b * t.b + row * t.t + w.kvh * t.h, d, v);
+    }
+}
+
+inline int grid_of(const Params& p, int splits) { return p.n_tiles * p.kv_heads * p.subs * splits; }
+
 template <class T, int DP>
-int run_fwd(const Params& p, int grid, hipStream_t s) {
-    constexpr int lds = 2 * KB * Image<T, DP>::PITCH;
+int run_fwd(const Params& p, hipStream_t s) {
+    constexpr int lds = 4 * KB * Image<T, DP>::PITCH;
     static DeviceOnce once;
     if (!once) { DPC_HIP(hipFuncSetAttribute((const void*)fwd_kernel<T, DP>, hipFuncAttributeMaxDynamicSharedMemorySize, lds)); once = true; }
-    hipLaunchKernelGGL((fwd_kernel<T, DP>), dim3(grid), dim3(256), lds, s, p);
+    hipLaunchKernelGGL((fwd_kernel<T, DP>), dim3(grid_of(p, p.splits)), dim3(256), lds, s, p);
     DPC_LAUNCH_CHECK();
+    if (p.splits > 1) {
+        hipLaunchKernelGGL((fwd_join_kernel<T>), dim3(grid_of(p, QB / 16)), dim3(256), 0, s, p);
+        DPC_LAUNCH_CHECK();
+    }
     return DPC_OK;
 }
 
 template <class T, int DP>
-int run_bwd(const Params& pq, int grid_q, const Params& pk, int grid_k, hipStream_t s) {
-    constexpr int lds = 2 * KB * Image<T, DP>::PITCH, lds_k = lds + 2 * KB * 4;
+int run_bwd(const Params& pq, const Params& pk, hipStream_t s) {
+    constexpr int lds = 4 * KB * Image<T, DP>::PITCH, lds_k = lds + 4 * KB * 4;
     static DeviceOnce once;
     if (!once) {
         DPC_HIP(hipFuncSetAttribute((const void*)dq_kernel<T, DP>, hipFuncAttributeMaxDynamicSharedMemorySize, lds));
         DPC_HIP(hipFuncSetAttribute((const void*)dkv_kernel<T, DP>, hipFuncAttributeMaxDynamicSharedMemorySize, lds_k));
         once = true;
     }
-    if (grid_q) {
-        hipLaunchKernelGGL((delta_kernel<T>), dim3(grid_q), dim3(256), 0, s, pq);
+    if (pq.n_tiles) {
+        hipLaunchKernelGGL((dq_kernel<T, DP>), dim3(grid_of(pq, pq.splits)), dim3(256), lds, s, pq);
         DPC_LAUNCH_CHECK();
-        hipLaunchKernelGGL((dq_kernel<T, DP>), dim3(grid_q), dim3(256), lds, s, pq);
-        DPC_LAUNCH_CHECK();
+        if (pq.splits > 1) {
+            hipLaunchKernelGGL((dq_join_kernel<T>), dim3(grid_of(pq, QB / 16)), dim3(256), 0, s, pq);
+            DPC_LAUNCH_CHECK();
+        }
     }
-    if (grid_k) {
-        hipLaunchKernelGGL((dkv_kernel<T, DP>), dim3(grid_k), dim3(256), lds_k, s, pk);
+    if (pk.n_tiles) {
+        hipLaunchKernelGGL((dkv_kernel<T, DP>), dim3(grid_of(pk, pk.splits)), dim3(256), lds_k, s, pk);
         DPC_LAUNCH_CHECK();
+        if (pk.splits > 1) {
+            hipLaunchKernelGGL((dkv_join_kernel<T>), dim3(grid_of(pk, QB / 16)), dim3(256), 0, s, pk);
+            DPC_LAUNCH_CHECK();
+        }
     }
     return DPC_OK;
 }
 
 // one element type's kernels live in one translation unit (seq_attn_{f32,f16,bf16}.hip)
-template <class T> int fwd(const Params& p, int grid, hipStream_t s) {
-    return p.D <= 32 ? run_fwd<T, 32>(p, grid, s) : p.D <= 64 ? run_fwd<T, 64>(p, grid, s) : p.D <= 96 ? run_fwd<T, 96>(p, grid, s) : run_fwd<T, 128>(p, grid, s);
+template <class T> int fwd(const Params& p, hipStream_t s) {
+    return p.D <= 32 ? run_fwd<T, 32>(p, s) : p.D <= 64 ? run_fwd<T, 64>(p, s) : p.D <= 96 ? run_fwd<T, 96>(p, s) : run_fwd<T, 128>(p, s);
 }
-template <class T> int bwd(const Params& pq, int gq, const Params& pk, int gk, hipStream_t s) {
-    return pq.D <= 32 ? run_bwd<T, 32>(pq, gq, pk, gk, s) : pq.D <= 64 ? run_bwd<T, 64>(pq, gq, pk, gk, s)
-         : pq.D <= 96 ? run_bwd<T, 96>(pq, gq, pk, gk, s) : run_bwd<T, 128>(pq, gq, pk, gk, s);
+template <class T> int bwd(const Params& pq, const Params& pk, hipStream_t s) {
+    return pq.D <= 32 ? run_bwd<T, 32>(pq, pk, s) : pq.D <= 64 ? run_bwd<T, 64>(pq, pk, s) : pq.D <= 96 ? run_bwd<T, 96>(pq, pk, s) : run_bwd<T, 128>(pq, pk, s);
 }
-int fwd_f32(const Params&, int, hipStream_t);
-int fwd_f16(const Params&, int, hipStream_t);
-int fwd_bf16(const Params&, int, hipStream_t);
-int bwd_f32(const Params&, int, const Params&, int, hipStream_t);
-int bwd_f16(const Params&, int, const Params&, int, hipStream_t);
-int bwd_bf16(const Params&, int, const Params&, int, hipStream_t);
+int fwd_f32(const Params&, hipStream_t);
+int fwd_f16(const Params&, hipStream_t);
+int fwd_bf16(const Params&, hipStream_t);
+int bwd_f32(const Params&, const Params&, hipStream_t);
+int bwd_f16(const Params&, const Params&, hipStream_t);
+int bwd_bf16(const Params&, const Params&, hipStream_t);
 
 }  // namespace seqattn
 }  // namespace dpc

@@ -1,4 +1,5 @@
 // Entry points of the attention on token sequences (include/dpc.h: dpc_seq_attn); the kernels are in seq_attn.h.
+#include <algorithm>
 #include <cmath>
 
 #include "seq_attn.h"
@@ -16,6 +17,7 @@ static int check(const dpc_seq_attn* a, bool backward) {
     DPC_REQUIRE(a->batch >= 0 && a->q_len >= 0 && a->k_len >= 0, "seq_attn: negative size");
     DPC_REQUIRE(a->heads >= 1 && a->kv_heads >= 1 && a->heads % a->kv_heads == 0, "seq_attn: heads must be a multiple of kv_heads");
     DPC_REQUIRE(a->head_dim >= 8 && a->head_dim <= 128 && a->head_dim % 8 == 0, "seq_attn: head_dim must be a multiple of 8 up to 128");
+    DPC_REQUIRE((a->q_len + 2ll * QB) * (a->heads / a->kv_heads) < (1ll << 31) && a->k_len < (1ll << 31) - 2 * QB, "seq_attn: sequence too long");
     DPC_REQUIRE(a->scale > 0.f && std::isfinite(a->scale), "seq_attn: scale must be positive and finite");
     DPC_REQUIRE(!a->seqs || ((a->q_tiles || !a->n_q_tiles) && (a->k_tiles || !a->n_k_tiles) && a->n_q_tiles >= 0 && a->n_k_tiles >= 0),
                 "seq_attn: sequences need their block lists");
@@ -39,19 +41,49 @@ static Params params(const dpc_seq_attn* a) {
     p.q = ten(a->q); p.k = ten(a->k); p.v = ten(a->v); p.out = ten(a->out);
     p.dout = ten(a->dout); p.dq = ten(a->dq); p.dk = ten(a->dk); p.dv = ten(a->dv);
     p.lse = a->lse; p.lse_b = a->lse_stride_b; p.lse_h = a->lse_stride_h;
+    p.krow_b = a->k_row_stride_b; p.krow_h = a->k_row_stride_h;
     p.key_mask = a->key_mask; p.mask_b = a->mask_stride_b;
     p.seqs = a->seqs;
     p.heads = a->heads; p.kv_heads = a->kv_heads; p.group = a->heads / a->kv_heads; p.D = a->head_dim;
-    p.q_len = a->q_len; p.k_len = a->k_len; p.causal = a->causal; p.scale = a->scale;
+    p.q_len = a->q_len; p.k_len = a->k_len; p.causal = a->causal != 0; p.scale = a->scale;
     return p;
 }
 
-// workgroups of a kernel that walks over blocks of QB rows; < 0: too many
-static int blocks(Params& p, const dpc_seq_attn* a, bool keys) {
+// Blocks and splits.  A CU holds two workgroups, the card 512.  Where the blocks alone do not fill 3/4 of them, the axis that a block walks
+// along (keys; for dK/dV the query rows of the group) is split over as many workgroups as fit, each with at least four tiles to walk;
+// the partial sums are joined in order by a second launch.  Returns false when the grid would pass 2^31.
+constexpr int SLOTS = 512;
+static bool plan_grid(Params& p, const dpc_seq_attn* a, bool keys) {
     p.tiles = a->seqs ? (keys ? a->k_tiles : a->q_tiles) : nullptr;
     p.tiles_per_seq = cdiv(keys ? a->k_len : a->q_len, QB);
-    const long long n = (a->seqs ? (keys ? a->n_k_tiles : a->n_q_tiles) : (long long)a->batch * p.tiles_per_seq) * (keys ? a->kv_heads : a->heads);
-    return n < (1ll << 31) ? (int)n : -1;
+    const long long n = a->seqs ? (keys ? a->n_k_tiles : a->n_q_tiles) : (long long)a->batch * p.tiles_per_seq;
+    p.subs = keys ? 1 : cdiv((long long)std::min(a->q_len, QB) * p.group, QB);
+    const long long blocks = n * p.kv_heads * p.subs;
+    const long long walk = keys ? (long long)p.group * cdiv(a->q_len, KB) : cdiv(a->k_len, KB);
+    p.splits = blocks == 0 || blocks >= SLOTS * 3 / 4 ? 1 : (int)std::max<long long>(1, std::min<long long>(SLOTS / blocks, walk / 4));
+    p.n_tiles = (int)n;
+    p.part_rows = keys ? a->k_rows : a->lse_rows;
+    return n < (1ll << 31) && blocks * std::max(p.splits, QB / 16) < (1ll << 31);
+}
+
+static size_t part_bytes(const Params& p, int per_row) {
+    return p.splits > 1 ? align_up((size_t)p.splits * p.part_rows * per_row * sizeof(float), 256) : 0;
+}
+
+struct Plan { Params q, k; size_t rows, bytes; bool ok; };
+static Plan plan_of(const dpc_seq_attn* a, bool backward) {
+    Plan w{};
+    w.q = params(a);
+    w.k = w.q;
+    w.ok = plan_grid(w.q, a, false) && (!backward || plan_grid(w.k, a, true));
+    if (backward) {
+        w.rows = align_up((size_t)a->lse_rows * sizeof(float), 256);
+        w.bytes = 2 * w.rows + std::max(part_bytes(w.q, a->head_dim + 1), part_bytes(w.k, 2 * a->head_dim));
+    } else {
+        w.bytes = part_bytes(w.q, a->head_dim + 2);
+    }
+    if (w.bytes) w.bytes += 256;
+    return w;
 }
 
 }  // namespace seqattn
@@ -63,37 +95,42 @@ using namespace dpc::seqattn;
 extern "C" {
 
 size_t dpc_seq_attn_workspace_bytes(const dpc_seq_attn* a, int backward) {
-    if (!a || !backward || a->lse_rows <= 0) return 256;
-    return 2 * align_up((size_t)a->lse_rows * sizeof(float), 256) + 256;
+    if (check(a, backward != 0) != DPC_OK || a->batch == 0) return 0;
+    return plan_of(a, backward != 0).bytes;
 }
 
 int dpc_seq_attn_fwd(const dpc_seq_attn* a, void* ws, size_t ws_bytes, dpc_stream_t stream) {
     const int rc = check(a, false);
     if (rc != DPC_OK) return rc;
-    (void)ws; (void)ws_bytes;
-    Params p = params(a);
-    const int grid = blocks(p, a, false);
-    DPC_REQUIRE(grid >= 0, "seq_attn: grid too large");
-    if (grid == 0) return DPC_OK;
+    if (a->batch == 0) return DPC_OK;
+    Plan w = plan_of(a, false);
+    DPC_REQUIRE(w.ok, "seq_attn: grid too large");
+    DPC_REQUIRE(w.bytes == 0 || (ws && ws_bytes >= w.bytes), "seq_attn: workspace too small");
+    if (w.q.n_tiles == 0) return DPC_OK;
+    w.q.part = reinterpret_cast<float*>(align_up((size_t)ws, 256));
+    w.q.part_ml = w.q.part + (size_t)w.q.splits * a->lse_rows * a->head_dim;
     hipStream_t s = (hipStream_t)stream;
     ProfScope prof(PROF_ATTN, 4.0 * a->batch * a->heads * (double)a->q_len * a->k_len * a->head_dim, 0, s);
-    return a->type == DPC_SEQ_F32 ? fwd_f32(p, grid, s) : a->type == DPC_SEQ_F16 ? fwd_f16(p, grid, s) : fwd_bf16(p, grid, s);
+    return a->type == DPC_SEQ_F32 ? fwd_f32(w.q, s) : a->type == DPC_SEQ_F16 ? fwd_f16(w.q, s) : fwd_bf16(w.q, s);
 }
 
 int dpc_seq_attn_bwd(const dpc_seq_attn* a, void* ws, size_t ws_bytes, dpc_stream_t stream) {
     const int rc = check(a, true);
     if (rc != DPC_OK) return rc;
     if (a->batch == 0) return DPC_OK;
-    DPC_REQUIRE(a->q_len == 0 || (ws && ws_bytes >= dpc_seq_attn_workspace_bytes(a, 1)), "seq_attn_bwd: workspace too small");
-    Params p = params(a);
-    p.lse2 = reinterpret_cast<float*>(align_up((size_t)ws, 256));
-    p.delta = reinterpret_cast<float*>(align_up((size_t)ws, 256) + align_up((size_t)a->lse_rows * sizeof(float), 256));
-    Params pk = p;
-    const int gq = blocks(p, a, false), gk = blocks(pk, a, true);
-    DPC_REQUIRE(gq >= 0 && gk >= 0, "seq_attn_bwd: grid too large");
+    Plan w = plan_of(a, true);
+    DPC_REQUIRE(w.ok, "seq_attn_bwd: grid too large");
+    DPC_REQUIRE(w.bytes == 0 || (ws && ws_bytes >= w.bytes), "seq_attn_bwd: workspace too small");
+    const size_t base = align_up((size_t)ws, 256);
+    for (Params* p : {&w.q, &w.k}) {
+        p->lse2 = reinterpret_cast<float*>(base);
+        p->ndelta = reinterpret_cast<float*>(base + w.rows);
+        p->part = reinterpret_cast<float*>(base + 2 * w.rows);
+        p->part_ml = p->part + (size_t)p->splits * p->part_rows * a->head_dim;
+    }
     hipStream_t s = (hipStream_t)stream;
     ProfScope prof(PROF_ATTN_BWD, 10.0 * a->batch * a->heads * (double)a->q_len * a->k_len * a->head_dim, 0, s);
-    return a->type == DPC_SEQ_F32 ? bwd_f32(p, gq, pk, gk, s) : a->type == DPC_SEQ_F16 ? bwd_f16(p, gq, pk, gk, s) : bwd_bf16(p, gq, pk, gk, s);
+    return a->type == DPC_SEQ_F32 ? bwd_f32(w.q, w.k, s) : a->type == DPC_SEQ_F16 ? bwd_f16(w.q, w.k, s) : bwd_bf16(w.q, w.k, s);
 }
 
 }  // extern "C"

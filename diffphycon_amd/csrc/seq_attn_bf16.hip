@@ -3,7 +3,7 @@
 
 namespace dpc {
 namespace seqattn {
-int fwd_bf16(const Params& p, int grid, hipStream_t s) { return fwd<__bf16>(p, grid, s); }
-int bwd_bf16(const Params& pq, int gq, const Params& pk, int gk, hipStream_t s) { return bwd<__bf16>(pq, gq, pk, gk, s); }
+int fwd_bf16(const Params& p, hipStream_t s) { return fwd<__bf16>(p, s); }
+int bwd_bf16(const Params& pq, const Params& pk, hipStream_t s) { return bwd<__bf16>(pq, pk, s); }
 }  // namespace seqattn
 }  // namespace dpc

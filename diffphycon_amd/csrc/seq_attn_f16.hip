@@ -3,7 +3,7 @@
 
 namespace dpc {
 namespace seqattn {
-int fwd_f16(const Params& p, int grid, hipStream_t s) { return fwd<_Float16>(p, grid, s); }
-int bwd_f16(const Params& pq, int gq, const Params& pk, int gk, hipStream_t s) { return bwd<_Float16>(pq, gq, pk, gk, s); }
+int fwd_f16(const Params& p, hipStream_t s) { return fwd<_Float16>(p, s); }
+int bwd_f16(const Params& pq, const Params& pk, hipStream_t s) { return bwd<_Float16>(pq, pk, s); }
 }  // namespace seqattn
 }  // namespace dpc

@@ -3,7 +3,7 @@
 
 namespace dpc {
 namespace seqattn {
-int fwd_f32(const Params& p, int grid, hipStream_t s) { return fwd<float>(p, grid, s); }
-int bwd_f32(const Params& pq, int gq, const Params& pk, int gk, hipStream_t s) { return bwd<float>(pq, gq, pk, gk, s); }
+int fwd_f32(const Params& p, hipStream_t s) { return fwd<float>(p, s); }
+int bwd_f32(const Params& pq, const Params& pk, hipStream_t s) { return bwd<float>(pq, pk, s); }
 }  // namespace seqattn
 }  // namespace dpc

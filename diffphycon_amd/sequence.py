@@ -426,7 +426,8 @@ def _attention_args(q, k, v, causal, scale, key_mask, plan):
     lse_shape = (H, q.shape[0]) if packed else (q.shape[0], H, q.shape[1])
     a = _lib.SeqAttn(key_mask=key_mask.data_ptr() if key_mask is not None else None, mask_stride_b=0 if packed else k.shape[1], type=_TYPE[t], batch=B, heads=H,
                      kv_heads=Hk, head_dim=D, q_len=q_len, k_len=k_len, causal=1 if causal else 0, lse_rows=math.prod(lse_shape), scale=scale,
-                     lse_stride_b=0 if packed else H * q.shape[1], lse_stride_h=lse_shape[-1])
+                     lse_stride_b=0 if packed else H * q.shape[1], lse_stride_h=lse_shape[-1], k_rows=k.numel() // D,
+                     k_row_stride_b=0 if packed else Hk * k.shape[1], k_row_stride_h=k.shape[-3])
     if plan is not None:
         a.seqs, a.q_tiles, a.k_tiles = (plan._pointer(i) for i in range(3))
         a.n_q_tiles, a.n_k_tiles = plan.counts
@@ -459,8 +460,9 @@ def attention_forward(q, k, v, *, causal=False, scale=None, key_mask=None, plan=
             return out, lse
         a.out, a.lse = _seq_tensor(out), lse.data_ptr()
         L = _lib.lib()
-        ws = _lib.workspace(L.dpc_seq_attn_workspace_bytes(C.byref(a), 0), dev)
-        _lib.check(L.dpc_seq_attn_fwd(C.byref(a), _p(ws), ws.numel(), _stream(dev)))
+        nbytes = L.dpc_seq_attn_workspace_bytes(C.byref(a), 0)
+        ws = _lib.workspace(nbytes, dev) if nbytes else None
+        _lib.check(L.dpc_seq_attn_fwd(C.byref(a), _p(ws), nbytes, _stream(dev)))
     return out, lse
 
 
@@ -493,6 +495,7 @@ def attention_backward(dout, q, k, v, out, lse, *, causal=False, scale=None, key
         a.dout, a.out, a.dq, a.dk, a.dv = (_seq_tensor(x) for x in (dout, out, dq, dk, dv))
         a.lse = lse.data_ptr()
         L = _lib.lib()
-        ws = _lib.workspace(L.dpc_seq_attn_workspace_bytes(C.byref(a), 1), dev)
-        _lib.check(L.dpc_seq_attn_bwd(C.byref(a), _p(ws), ws.numel(), _stream(dev)))
+        nbytes = L.dpc_seq_attn_workspace_bytes(C.byref(a), 1)
+        ws = _lib.workspace(nbytes, dev) if nbytes else None
+        _lib.check(L.dpc_seq_attn_bwd(C.byref(a), _p(ws), nbytes, _stream(dev)))
     return dq, dk, dv
