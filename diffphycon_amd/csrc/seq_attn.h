@@ -129,7 +129,7 @@ __device__ __forceinline__ Seq sequence(const Params& p, int b) {
 
 // Which block of which (sequence, key head) a workgroup has.  Workgroups go round the 8 XCDs, each with its own L2: the blocks of one
 // (sequence, key head), which read the same keys and values, stay on one XCD where the pairs divide evenly; the blocks with most work
-// (the last ones under a causal mask) come first.  A query block is `subs` sub-blocks of QB rows (rows = tokens x heads of the group).
+// (under a causal mask the last queries', the first keys') come first.  A query block is `subs` sub-blocks of QB rows (rows = tokens x heads of the group).
 struct Where { int b, tile, kvh, sub, split; };
 __device__ __forceinline__ Where where(const Params& p, bool last_first) {
     Where w;
@@ -163,6 +163,9 @@ __device__ __attribute__((aligned(16))) const float FILL[8] = {0.f, 0.f, 0.f, 0.
 __device__ __forceinline__ void copy16(const char* src, unsigned lds) {
     asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, off" :: "v"(src), "s"(lds) : "memory", "m0");
 }
+__device__ __forceinline__ void copy16(const char* base, unsigned off, unsigned lds) {          // one base for the wave
+    asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, %1" :: "v"(off), "s"(base), "s"(lds) : "memory", "m0");
+}
 __device__ __forceinline__ void copy4(const char* src, unsigned lds) {
     asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dword %0, off" :: "v"(src), "s"(lds) : "memory", "m0");
 }
@@ -171,22 +174,43 @@ __device__ __forceinline__ unsigned lds_offset(const void* p) {
     return __builtin_amdgcn_readfirstlane((unsigned)(size_t)(__attribute__((address_space(3))) const char*)p);
 }
 
-// KB x DP tile, global -> LDS by 256 threads; rows whose bit is 0 and columns >= D become zero.
-template <class T, int DP>
+// ROWS x DP tiles of one tensor, global -> LDS by 256 threads.  The tile's base is the wave's, a lane adds one 32-bit offset (64 rows
+// stay within 2^31 bytes: checked at the entry), so a whole tile costs no address arithmetic.  Rows whose bit is 0 become zero; columns >= D
+// are never written: zero_images() clears them once.
+template <class T, int DP, int ROWS = KB>
 struct Stage {
-    static constexpr int CH = Image<T, DP>::CH, N = KB * CH / 256;
-    static_assert(KB * CH % 256 == 0, "whole rounds");
-    __device__ static __forceinline__ void issue(char* img, const char* base, long long st, int D, unsigned long long bits) {
-        const unsigned at = lds_offset(img) + (threadIdx.x >> 6) * 1024;
+    static constexpr int CH = Image<T, DP>::CH, N = ROWS * CH / 256, STEP = 256 / CH;
+    static constexpr bool EVEN = 256 % CH == 0;                       // round i is round 0, STEP rows further (a multiple of 8: same swizzle)
+    static_assert(ROWS * CH % 256 == 0 && (!EVEN || STEP % 8 == 0), "whole rounds");
+    unsigned off[EVEN ? 1 : N];
+    long long st;
+    int width;                                                       // bytes of a row
+    __device__ static __forceinline__ int row(int i) { return (threadIdx.x + 256 * i) / CH; }
+    __device__ static __forceinline__ int col(int i) { return (((threadIdx.x + 256 * i) % CH) ^ Image<T, DP>::swz(row(i))) * 16; }
+    __device__ __forceinline__ Stage(long long stride, int D) : st(stride), width(D * (int)sizeof(T)) {
+#pragma unroll
+        for (int i = 0; i < (EVEN ? 1 : N); ++i) off[i] = (unsigned)(row(i) * st + col(i));
+    }
+    __device__ __forceinline__ void issue(char* img, const char* base, unsigned long long bits) const {
+        const unsigned at = lds_offset(img) + __builtin_amdgcn_readfirstlane((threadIdx.x >> 6) * 1024);
+        const bool all = ROWS == 64 ? bits == ~0ull : (unsigned)bits == ~0u;
+        if (all && width == DP * (int)sizeof(T)) {
+#pragma unroll
+            for (int i = 0; i < N; ++i) copy16(EVEN ? base + i * STEP * st : base, off[EVEN ? 0 : i], at + i * 4096);
+            return;
+        }
 #pragma unroll
         for (int i = 0; i < N; ++i) {
-            const int e = threadIdx.x + 256 * i, row = e / CH, c = (e % CH) ^ Image<T, DP>::swz(row);
-            const char* src = base + row * st + c * 16;
-            if (!((bits >> row) & 1) || c * 16 >= D * (int)sizeof(T)) src = reinterpret_cast<const char*>(FILL);
-            copy16(src, __builtin_amdgcn_readfirstlane(at + i * 4096));
+            const char* src = base + (EVEN ? i * STEP * st : 0) + off[EVEN ? 0 : i];
+            if (!((bits >> row(i)) & 1)) src = reinterpret_cast<const char*>(FILL);
+            if (col(i) < width) copy16(src, at + i * 4096);
         }
     }
 };
+__device__ __forceinline__ void zero_images(char* smem, int bytes) {  // (followed by the barrier before the first read)
+    for (int i = threadIdx.x * 16; i < bytes; i += 256 * 16) *reinterpret_cast<uint4*>(smem + i) = uint4{0, 0, 0, 0};
+    __syncthreads();
+}
 __device__ __forceinline__ unsigned long long first_bits(int n) { return n >= 64 ? ~0ull : n <= 0 ? 0ull : (1ull << n) - 1; }
 
 // operand fragments of one row (this lane's column of the product), zero where !ok
@@ -251,6 +275,16 @@ template <int N> __device__ __forceinline__ void scale_col(f32x16& t, float& sc,
 
 template <class T> __device__ __forceinline__ constexpr bool is_f16() { return __is_same(T, _Float16); }
 template <class T, int DP> constexpr int WAVES = sizeof(T) == 2 || DP <= 64 ? 2 : 1;       // workgroups of a CU that the registers have to allow
+#ifndef DKVW
+#define DKVW 2
+#endif
+#ifndef LV
+#define LV 1
+#endif
+// dK/dV at head size 128: the two sums alone take 128 registers; the values' fragments wait in LDS (V_LDS) and the staged tile has 32 rows
+template <class T, int DP> constexpr bool V_LDS = LV && DP == 128;
+template <class T, int DP> constexpr int RB = V_LDS<T, DP> ? 32 : 64;
+template <class T, int DP> constexpr int DKV_WAVES = DP == 128 && sizeof(T) == 2 ? DKVW : WAVES<T, DP>;
 
 // The keys of a tile that take part, one tile ahead: without a key mask by the sequence's end, with one by a byte a lane
 struct KeyBits {
@@ -294,10 +328,12 @@ __global__ __launch_bounds__(256, (WAVES<T, DP>)) void fwd_kernel(const Params p
     const float c = p.scale * LOG2E, lift = is_f16<T>() ? 7.f : 0.f;
     float m = -INFINITY, l = 0.f;                                    // maximum (scaled), this lane's part of the sum
     unsigned long long cur = 0;
+    const Stage<T, DP> sk(p.k.t, p.D), sv(p.v.t, p.D);
+    if (p.D < DP) zero_images(smem, 4 * IMG);
     auto issue = [&](int kt, int buf) {
         cur = kb.bits(kt);
-        Stage<T, DP>::issue(smem + buf * 2 * IMG, kbase + kt * p.k.t, p.k.t, p.D, cur);
-        Stage<T, DP>::issue(smem + buf * 2 * IMG + IMG, vbase + kt * p.v.t, p.v.t, p.D, cur);
+        sk.issue(smem + buf * 2 * IMG, kbase + kt * p.k.t, cur);
+        sv.issue(smem + buf * 2 * IMG + IMG, vbase + kt * p.v.t, cur);
         kb.fetch(kt + KB);
     };
     if (kbegin < kend) { kb.fetch(kbegin); issue(kbegin, 0); }
@@ -466,10 +502,12 @@ __global__ __launch_bounds__(256, (WAVES<T, DP>)) void dq_kernel(const Params p)
     const float c = p.scale * LOG2E;
     float sc = is_f16<T>() ? 0x1p100f : 1.f;
     unsigned long long cur = 0;
+    const Stage<T, DP> sk(p.k.t, p.D), sv(p.v.t, p.D);
+    if (p.D < DP) zero_images(smem, 4 * IMG);
     auto issue = [&](int kt, int buf) {
         cur = kb.bits(kt);
-        Stage<T, DP>::issue(smem + buf * 2 * IMG, kbase + kt * p.k.t, p.k.t, p.D, cur);
-        Stage<T, DP>::issue(smem + buf * 2 * IMG + IMG, vbase + kt * p.v.t, p.v.t, p.D, cur);
+        sk.issue(smem + buf * 2 * IMG, kbase + kt * p.k.t, cur);
+        sv.issue(smem + buf * 2 * IMG + IMG, vbase + kt * p.v.t, cur);
     };
     const int tiles = kend > kbegin ? (kend - kbegin + KB - 1) / KB : 0;
     const int first = FIX && p.splits == 1 && tiles <= 4 ? tiles : 0;             // tiles of the sweep for D alone
@@ -556,10 +594,11 @@ __global__ __launch_bounds__(256) void dq_join_kernel(const Params p) {
 }
 
 template <class T, int DP>
-__global__ __launch_bounds__(256, (WAVES<T, DP>)) void dkv_kernel(const Params p) {
+__global__ __launch_bounds__(256, (DKV_WAVES<T, DP>)) void dkv_kernel(const Params p) {
     typedef Mma<T> M;
-    constexpr int NF = DP / M::KS, NP = 32 / M::KS, ND = DP / 32, IMG = KB * Image<T, DP>::PITCH;
-    extern __shared__ __attribute__((aligned(16))) char smem[];       // [2][Q, dO], then [2][lse2, -D][64]
+    constexpr int NF = DP / M::KS, NP = 32 / M::KS, ND = DP / 32, R = RB<T, DP>, IMG = R * Image<T, DP>::PITCH;
+    constexpr bool VL = V_LDS<T, DP>;
+    extern __shared__ __attribute__((aligned(16))) char smem[];       // [2][Q, dO], [2][lse2, -D][64], then the waves' V fragments
     float* const s_row = reinterpret_cast<float*>(smem + 4 * IMG);
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, l31 = lane & 31, h = lane >> 5;
     const Where w = where(p, false);
@@ -573,51 +612,71 @@ __global__ __launch_bounds__(256, (WAVES<T, DP>)) void dkv_kernel(const Params p
     typename M::Frag kf[NF], vf[NF];
     load_row<T, DP>(kf, p.k.p + w.b * p.k.b + row * p.k.t + w.kvh * p.k.h, h, p.D, live);
     load_row<T, DP>(vf, p.v.p + w.b * p.v.b + row * p.v.t + w.kvh * p.v.h, h, p.D, live);
+    typename M::Frag* const s_v = reinterpret_cast<typename M::Frag*>(smem + 4 * IMG + 1024) + wave * NF * 64 + lane;     // (each lane its own)
+    if (VL) {
+#pragma unroll
+        for (int f = 0; f < NF; ++f) s_v[f * 64] = vf[f];
+    }
     f32x16 dk[ND], dv[ND];
     clear(dk);
     clear(dv);
     const float c = p.scale * LOG2E, lift = is_f16<T>() ? 15.f : 0.f;
     float sc = is_f16<T>() ? 0x1p100f : 1.f;
     const int qbegin = p.causal ? max(0, w.tile * QB - off) : 0;                 // first query that sees the first key
-    const int per_head = qbegin < s.ql ? (s.ql - qbegin + KB - 1) / KB : 0;
+    const int per_head = qbegin < s.ql ? (s.ql - qbegin + R - 1) / R : 0;
     int step = 0, steps = per_head * p.group;
     if (p.splits > 1) {
         const int per = (steps + p.splits - 1) / p.splits;
         step = min(steps, w.split * per);
         steps = min(steps, step + per);
     }
+    // The walk: tiles of R queries, head after head.
+    struct At { int head, qt; } next{w.kvh * p.group, qbegin};
+    if (step < steps) { next.head += step / per_head; next.qt += step % per_head * R; }
+    auto advance = [&](At a) { return a.qt + R < s.ql ? At{a.head, a.qt + R} : At{a.head + 1, qbegin}; };
+    const Stage<T, DP, R> sq(p.q.t, p.D), sg(p.dout.t, p.D);
+    const char* const qbase = p.q.p + w.b * p.q.b + s.q0 * p.q.t;
+    const char* const gbase = p.dout.p + w.b * p.dout.b + s.q0 * p.dout.t;
+    const long long first_row = w.b * p.lse_b + s.q0;
+    if (p.D < DP) zero_images(smem, 4 * IMG);
     // Rows that see nothing are not read (their lse2 is +inf).  Under a causal mask alone they lie before qbegin; a key mask can leave any
     // row empty, so its lse2 is looked at first, a tile ahead.
     float ahead = 0.f;
-    auto fetch = [&](int i) {
-        const int qt = qbegin + i % per_head * KB + lane;
-        if (p.key_mask) ahead = qt < s.ql ? p.lse2[w.b * p.lse_b + (w.kvh * p.group + i / per_head) * p.lse_h + s.q0 + qt] : INFINITY;
+    auto fetch = [&](At a) {
+        if (p.key_mask) ahead = a.qt + lane < s.ql ? p.lse2[first_row + a.head * p.lse_h + a.qt + lane] : INFINITY;
     };
-    auto issue = [&](int i, int buf) {
-        const int head = w.kvh * p.group + i / per_head, qt = qbegin + i % per_head * KB;
-        const long long first = s.q0 + qt, at = w.b * p.lse_b + head * p.lse_h + first;
-        const unsigned long long bits = p.key_mask ? __ballot(ahead != INFINITY) : first_bits(s.ql - qt);
-        Stage<T, DP>::issue(smem + buf * 2 * IMG, p.q.p + w.b * p.q.b + first * p.q.t + head * p.q.h, p.q.t, p.D, bits);
-        Stage<T, DP>::issue(smem + buf * 2 * IMG + IMG, p.dout.p + w.b * p.dout.b + first * p.dout.t + head * p.dout.h, p.dout.t, p.D, bits);
-        const bool there = (bits >> lane) & 1;
-        if (wave == 0) copy4(reinterpret_cast<const char*>(there ? p.lse2 + at + lane : FILL + 4), lds_offset(s_row + buf * 128));
-        if (wave == 1) copy4(reinterpret_cast<const char*>(there ? p.ndelta + at + lane : FILL), lds_offset(s_row + buf * 128 + 64));
+    auto issue = [&](At a, int buf) {
+        const long long at = first_row + a.head * p.lse_h + a.qt + lane;
+        const unsigned long long bits = p.key_mask ? __ballot(ahead != INFINITY) : first_bits(s.ql - a.qt);
+        sq.issue(smem + buf * 2 * IMG, qbase + a.qt * p.q.t + a.head * p.q.h, bits);
+        sg.issue(smem + buf * 2 * IMG + IMG, gbase + a.qt * p.dout.t + a.head * p.dout.h, bits);
+        const bool there = (bits >> lane) & 1;                       // (R = 32: the upper half is never read)
+        if (wave == 0) copy4(reinterpret_cast<const char*>(there ? p.lse2 + at : FILL + 4), lds_offset(s_row + buf * 128));
+        if (wave == 1) copy4(reinterpret_cast<const char*>(there ? p.ndelta + at : FILL), lds_offset(s_row + buf * 128 + 64));
     };
-    if (step < steps) { fetch(step); issue(step, step & 1); if (step + 1 < steps) fetch(step + 1); }
-    for (; step < steps; ++step) {
-        const int qt = qbegin + step % per_head * KB, buf = step & 1;
+    At now = next;
+    if (step < steps) {
+        fetch(now);
+        issue(now, 0);
+        next = advance(now);
+        if (step + 1 < steps) fetch(next);
+    }
+    for (int buf = 0; step < steps; ++step, buf ^= 1) {
+        const int qt = now.qt;
         copies_done();
         __syncthreads();
         if (step + 1 < steps) {
-            issue(step + 1, buf ^ 1);
-            if (step + 2 < steps) fetch(step + 2);
+            issue(next, buf ^ 1);
+            now = next;
+            next = advance(next);
+            if (step + 2 < steps) fetch(next);
         }
-        if (kw >= s.kl || (p.causal && qt + KB - 1 < kw - off)) continue;
+        if (kw >= s.kl || (p.causal && qt + R - 1 < kw - off)) continue;
         const char* const img_q = smem + buf * 2 * IMG;
         const char* const img_g = img_q + IMG;
         const bool partial = p.causal && kw + 31 - off > qt;
 #pragma unroll
-        for (int sub = 0; sub < 2; ++sub) {
+        for (int sub = 0; sub < R / 32; ++sub) {
             const float* const sl = s_row + buf * 128 + sub * 32 + 4 * h;
             f32x16 st, dp;
 #pragma unroll
@@ -629,7 +688,7 @@ __global__ __launch_bounds__(256, (WAVES<T, DP>)) void dkv_kernel(const Params p
 #pragma unroll
             for (int f = 0; f < NF; ++f) {
                 st = M::mma(M::template row<DP>(img_q, sub * 32 + l31, f, h), kf[f], st);
-                dp = M::mma(M::template row<DP>(img_g, sub * 32 + l31, f, h), vf[f], dp);
+                dp = M::mma(M::template row<DP>(img_g, sub * 32 + l31, f, h), VL ? s_v[f * 64] : vf[f], dp);
             }
 #pragma unroll
             for (int g = 0; g < 4; ++g) {
@@ -708,7 +767,7 @@ int run_fwd(const Params& p, hipStream_t s) {
 
 template <class T, int DP>
 int run_bwd(const Params& pq, const Params& pk, hipStream_t s) {
-    constexpr int lds = 4 * KB * Image<T, DP>::PITCH, lds_k = lds + 4 * KB * 4;
+    constexpr int lds = 4 * KB * Image<T, DP>::PITCH, lds_k = 4 * RB<T, DP> * Image<T, DP>::PITCH + 1024 + (V_LDS<T, DP> ? QB * Image<T, DP>::PITCH : 0);
     static DeviceOnce once;
     if (!once) {
         DPC_HIP(hipFuncSetAttribute((const void*)dq_kernel<T, DP>, hipFuncAttributeMaxDynamicSharedMemorySize, lds));

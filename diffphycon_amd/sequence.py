@@ -61,12 +61,13 @@ def _p(t):
 
 
 def _rows16(x):
-    """x with a contiguous last axis and every other stride and the base on 16 bytes: itself or a contiguous copy."""
+    """x with a contiguous last axis, every other stride and the base on 16 bytes and tokens less than 2^25 bytes apart: itself or a contiguous copy."""
     es = x.element_size()
     if x.numel() == 0:
         return x
     if x.stride(-1) == 1 and x.data_ptr() % 16 == 0 and all(s * es % 16 == 0 for s, n in zip(x.stride()[:-1], x.shape[:-1]) if n > 1):
-        return x
+        if x.shape[-3] == 1 or x.stride(-3) * es < 1 << 25:
+            return x
     return x.clone(memory_format=torch.contiguous_format)
 
 

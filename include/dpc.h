@@ -456,7 +456,8 @@ int dpc_seq_rotary_run(const dpc_seq_rotary* a, dpc_stream_t stream);
  * Dense: every sequence has q_len / k_len tokens, seqs == NULL.  Otherwise seqs [batch][4] = (first query row, queries, first key row,
  * keys), rows counted from the batch's own base (stride_b = 0: packed), q_len / k_len the longest; q_tiles / k_tiles [n][2] =
  * (sequence, block of 128 rows) list every block once, in launch order; rows that no sequence covers are not written.
- * head_dim: a multiple of 8, at most 128.  Tensor bases and strides: multiples of 16 bytes. */
+ * head_dim: a multiple of 8, at most 128.  Tensor bases and strides: multiples of 16 bytes; token
+ * strides below 2^25 bytes. */
 typedef struct dpc_seq_attn {
     dpc_seq_tensor q, k, v, out;             /* forward: out is written; backward: read */
     float* lse;
