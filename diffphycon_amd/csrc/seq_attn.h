@@ -35,14 +35,14 @@ typedef short s16x4 __attribute__((__vector_size__(8)));
 typedef __attribute__((address_space(3))) s16x4* lds_s16x4;
 
 // LDS image of a tile: rows of DP elements in 16-byte chunks, filled 16 bytes a lane straight from global memory (Stage), so the image
-// has no padding; chunk c of row r is stored at c ^ swz(r), which spreads both kinds of read over the banks.  16 bits: the row read (8
-// lanes = 8 rows, one chunk) and the transpose read (4 rows x 64 bytes); fp32: the row read (column reads are whole 128-byte lines).
+// has no padding; chunk c of row r is stored at c ^ swz(r).  LDS serves a 16-byte read 16 lanes at a time over 64 banks (256 bytes): the row read
+// (lane = row, one chunk) wants 16 rows in 16 different 16-byte slots, the transpose read (4 rows x 64 bytes) 4 rows in 4 different
+// 64-byte ones.  With rows of 256 bytes all of that has to come from swz, with shorter ones a part comes from where the row starts.
 template <class T, int DP>
 struct Image {
     static constexpr int CH = DP * (int)sizeof(T) / 16, PITCH = CH * 16;
     __device__ static __forceinline__ int swz(int r) {
-        if (sizeof(T) == 4) return r & 7;
-        return (DP / 32) % 2 ? (r >> 1) & 3 : ((r & 1) << 2) | ((r >> 1) & 3);
+        return CH % 16 == 0 ? ((r & 3) << 2) | ((r >> 2) & 3) : CH % 8 == 0 ? ((r & 2) << 1) | ((r >> 2) & 3) : (r >> 2) & 3;
     }
     __device__ static __forceinline__ int off(int r, int c) { return r * PITCH + ((c ^ swz(r)) << 4); }
 };
@@ -58,9 +58,9 @@ template <class T, class F> struct Mma16 {   // the two 16-bit types
     template <int DP> __device__ static __forceinline__ Frag col(const char* img, int r0, int s, int dt, int lane) {
         const int i = lane & 15, g = (lane >> 4) & 1, h = lane >> 5;
         const int r = 4 * h + (i >> 2);
-        const int o = (r0 + 16 * s) * Image<T, DP>::PITCH + Image<T, DP>::off(r, 4 * dt + 2 * g + ((i & 3) >> 1)) + (i & 1) * 8;
-        const s16x4 a = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4)(img + o));
-        const s16x4 b = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4)(img + o + 8 * Image<T, DP>::PITCH));
+        const int c = 4 * dt + 2 * g + ((i & 3) >> 1), o = (r0 + 16 * s) * Image<T, DP>::PITCH + (i & 1) * 8;       // (swz repeats every 16 rows)
+        const s16x4 a = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4)(img + o + Image<T, DP>::off(r, c)));
+        const s16x4 b = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4)(img + o + Image<T, DP>::off(r + 8, c)));
         return __builtin_bit_cast(Frag, __builtin_shufflevector(a, b, 0, 1, 2, 3, 4, 5, 6, 7));
     }
     __device__ static __forceinline__ Frag from_acc(const f32x16& v, int s) {
@@ -180,8 +180,8 @@ __device__ __forceinline__ unsigned lds_offset(const void* p) {
 template <class T, int DP, int ROWS = KB>
 struct Stage {
     static constexpr int CH = Image<T, DP>::CH, N = ROWS * CH / 256, STEP = 256 / CH;
-    static constexpr bool EVEN = 256 % CH == 0;                       // round i is round 0, STEP rows further (a multiple of 8: same swizzle)
-    static_assert(ROWS * CH % 256 == 0 && (!EVEN || STEP % 8 == 0), "whole rounds");
+    static constexpr bool EVEN = 256 % CH == 0 && STEP % 16 == 0;     // round i is round 0, STEP rows further, with the same swizzle
+    static_assert(ROWS * CH % 256 == 0, "whole rounds");
     unsigned off[EVEN ? 1 : N];
     long long st;
     int width;                                                       // bytes of a row
