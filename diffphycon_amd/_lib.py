@@ -2,6 +2,7 @@
 to load, importing any compute entry raises — the product path never silently runs on something else."""
 import ctypes as C
 import os
+import struct
 
 import torch
 
@@ -80,6 +81,12 @@ class SeqAttn(C.Structure):
                 ("n_q_tiles", C.c_int32), ("n_k_tiles", C.c_int32), ("type", C.c_int32), ("batch", C.c_int32), ("heads", C.c_int32),
                 ("kv_heads", C.c_int32), ("head_dim", C.c_int32), ("q_len", C.c_int32), ("k_len", C.c_int32), ("causal", C.c_int32),
                 ("lse_rows", C.c_int64), ("k_rows", C.c_int64), ("k_row_stride_b", C.c_int64), ("k_row_stride_h", C.c_int64), ("scale", C.c_float)]
+
+
+# The two structures above as one struct.pack each: a call per microsecond matters for single tokens, and ctypes takes one per field.
+SEQ_ROTARY_BYTES = struct.Struct("<21q9i4x")
+SEQ_ATTN_BYTES = struct.Struct("<40q10i4qf4x")
+assert SEQ_ROTARY_BYTES.size == C.sizeof(SeqRotary) and SEQ_ATTN_BYTES.size == C.sizeof(SeqAttn)
 
 
 class ProfileRow(C.Structure):
@@ -199,10 +206,10 @@ _SIGNATURES = {
     "dpc_seq_norm_fwd": (C.c_int, [_P] * 5 + [_L, _I, _L, C.c_float, _I, _I, _P]),
     "dpc_seq_norm_bwd_workspace_bytes": (_Z, [_L, _I]),
     "dpc_seq_norm_bwd": (C.c_int, [_P] * 7 + [_L, _I, _L, _L, _I, _I, _P, _Z, _P]),
-    "dpc_seq_rotary_run": (C.c_int, [C.POINTER(SeqRotary), _P]),
-    "dpc_seq_attn_workspace_bytes": (_Z, [C.POINTER(SeqAttn), _I]),
-    "dpc_seq_attn_fwd": (C.c_int, [C.POINTER(SeqAttn), _P, _Z, _P]),
-    "dpc_seq_attn_bwd": (C.c_int, [C.POINTER(SeqAttn), _P, _Z, _P]),
+    "dpc_seq_rotary_run": (C.c_int, [_P, _P]),                        # (SeqRotary / SeqAttn by reference, or their bytes)
+    "dpc_seq_attn_workspace_bytes": (_Z, [_P, _I]),
+    "dpc_seq_attn_fwd": (C.c_int, [_P, _P, _Z, _P]),
+    "dpc_seq_attn_bwd": (C.c_int, [_P, _P, _Z, _P]),
     "dpc_burgers_fd": (C.c_int, [_P, _P, _P, _I, _I, _I, _D, _D, _D, _P]),
     "dpc_unet2d_create": (C.c_int, [C.POINTER(Unet2DCfg), C.POINTER(_P)]),
     "dpc_unet2d_destroy": (None, [_P]),

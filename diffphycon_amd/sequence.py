@@ -14,7 +14,6 @@ Element types: float32, float16, bfloat16 (one type per call); sums, statistics 
 current stream of the tensors' device and never synchronise; outputs and scratch come from torch's allocator on that stream, so calls may be
 captured into graphs.  Nothing is accumulated with atomics: results repeat bit for bit.  Arguments are checked on the host (ValueError /
 TypeError / RuntimeError); tensors must live on the GPU (no CPU path)."""
-import ctypes as C
 import math
 
 import torch
@@ -22,53 +21,72 @@ import torch
 from . import _lib
 
 _TYPE = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}
+_BYTES = {torch.float32: 4, torch.float16: 2, torch.bfloat16: 2}
 
 
 # ------------------------------------------------------------------------------------------------------------------ checks
-def _type(*tensors):
-    t = tensors[0].dtype
+def _type(x, *more):
+    t = x.dtype
     if t not in _TYPE:
         raise TypeError(f"element type {t}: float32, float16 and bfloat16 are supported")
-    for x in tensors[1:]:
-        if x.dtype != t:
-            raise TypeError(f"one element type per call, got {t} and {x.dtype}")
+    for y in more:
+        if y.dtype != t:
+            raise TypeError(f"one element type per call, got {t} and {y.dtype}")
     return t
 
 
-def _device(*tensors):
-    d = tensors[0].device
-    for x in tensors:
-        if not x.is_cuda:
-            raise RuntimeError("libdpc needs device tensors (there is no CPU implementation)")
-        if x.device != d:
-            raise RuntimeError(f"tensors on {d} and {x.device}")
+def _device(x, *more):
+    """The index of the device that all tensors (None: absent) are on."""
+    d = x.get_device()
+    if d < 0:
+        raise RuntimeError("libdpc needs device tensors (there is no CPU implementation)")
+    for y in more:
+        if y is not None and y.get_device() != d:
+            raise RuntimeError(f"tensors on {x.device} and {y.device}")
     return d
 
 
-def _stream(device):
-    return C.c_void_p(torch.cuda.current_stream(device).cuda_stream)
+def _elsewhere(x):
+    """Whether x is on a GPU that is not the current one: the public functions then call themselves there."""
+    d = x.get_device()
+    return d >= 0 and d != torch.cuda.current_device()
 
 
-def _in_use(owner):
+def _stream(d):
+    return torch._C._cuda_getCurrentRawStream(d)
+
+
+def _in_use(owner, d):
     """The owner's table is read on the current stream: its memory is not handed on before that stream is done with it."""
-    current = torch.cuda.current_stream(owner.table.device)
-    if current != owner.stream:
-        owner.table.record_stream(current)
+    if _stream(d) != owner.stream:
+        owner.table.record_stream(torch.cuda.current_stream(d))
 
 
-def _p(t):
-    return C.c_void_p(t.data_ptr()) if t is not None else None
+def _ok16(x, es):
+    """Whether a kernel can read x as it lies: last axis contiguous, base and strides on 16 bytes, tokens less than 2^25 bytes apart."""
+    s = [n if m > 1 else 0 for n, m in zip(x.stride()[:-1], x.shape[:-1])]
+    return x.stride(-1) == 1 and not any(n * es & 15 for n in s) and x.data_ptr() & 15 == 0 and s[-2] * es < 1 << 25
 
 
-def _rows16(x):
-    """x with a contiguous last axis, every other stride and the base on 16 bytes and tokens less than 2^25 bytes apart: itself or a contiguous copy."""
-    es = x.element_size()
-    if x.numel() == 0:
-        return x
-    if x.stride(-1) == 1 and x.data_ptr() % 16 == 0 and all(s * es % 16 == 0 for s, n in zip(x.stride()[:-1], x.shape[:-1]) if n > 1):
-        if x.shape[-3] == 1 or x.stride(-3) * es < 1 << 25:
-            return x
-    return x.clone(memory_format=torch.contiguous_format)
+def _lay(x, es):
+    """(x or a contiguous copy that a kernel can read; its address, strides of batch, token, head) for [B, T, H, D] or packed [T, H, D]."""
+    if x.dim() == 4:
+        b, t, h, d = x.stride()
+    else:
+        b = 0
+        t, h, d = x.stride()
+    p = x.data_ptr()
+    if d == 1 and not (p | b * es | t * es | h * es) & 15 and t * es < 1 << 25:
+        return x, p, b, t, h
+    if x.numel() and not _ok16(x, es):
+        x = x.clone(memory_format=torch.contiguous_format)
+    return x, x.data_ptr(), *_strides(x)
+
+
+def _strides(x):
+    """Strides of batch, token, head; 0 for an axis of one element, whose stride means nothing."""
+    s = [n if m > 1 else 0 for n, m in zip(x.stride()[:-1], x.shape[:-1])]
+    return s if len(s) == 3 else [0] + s
 
 
 def _shares(a, b):
@@ -99,7 +117,7 @@ def _written(x, like, name, inputs):
         if s <= reach:
             raise ValueError(f"{name}: elements of the buffer overlap")
         reach += s * (n - 1)
-    if x.numel() and _rows16(x) is not x:
+    if x.numel() and not _ok16(x, x.element_size()):
         raise ValueError(f"{name}: the last axis must be contiguous, base and strides multiples of 16 bytes")
     if any(_overlap(x, i) for i in inputs):
         raise ValueError(f"{name}: the buffer overlaps an input")
@@ -107,28 +125,29 @@ def _written(x, like, name, inputs):
 
 # ------------------------------------------------------------------------------------------------------------------ layer norm
 def _norm_params(x, weight, bias):
-    for name, p in (("weight", weight), ("bias", bias)):
+    """The type of weight and bias."""
+    t = None
+    for p in (weight, bias):
         if p is None:
             continue
         if p.shape != x.shape[-1:]:
-            raise ValueError(f"{name}: expected shape {tuple(x.shape[-1:])}, got {tuple(p.shape)}")
-        if p.dtype not in (torch.float32, x.dtype):
-            raise TypeError(f"{name}: float32 or {x.dtype}, got {p.dtype}")
-    if weight is not None and bias is not None and weight.dtype != bias.dtype:
-        raise TypeError("weight and bias must have one type")
-    p = weight if weight is not None else bias
-    return _TYPE[torch.float32] if p is None else _TYPE[p.dtype]
+            raise ValueError(f"weight, bias: expected shape {tuple(x.shape[-1:])}, got {tuple(p.shape)}")
+        if p.dtype not in (torch.float32, x.dtype) or t not in (None, p.dtype):
+            raise TypeError(f"weight, bias: both float32 or both {x.dtype}, got {p.dtype}")
+        t = p.dtype
+    return 0 if t is None else _TYPE[t]
 
 
-def _matrix(x):
-    """x as [rows, C] with one row stride (a view where the layout allows it, else a copy); broadcast rows are copied."""
-    n = x.shape[-1]
-    if x.dim() == 2 and x.stride(1) == 1 and (x.shape[0] == 1 or x.stride(0) >= n):
-        return x
+def _matrix(x, n):
+    """(x as [rows, n] with one row stride: a view where the layout allows it, else a copy; its row stride).  Broadcast rows are copied."""
+    if x.dim() == 2:
+        r, c = x.stride()
+        if (c == 1 or n == 1) and (r >= n or x.shape[0] == 1):
+            return x, max(r, n)
     y = x.reshape(-1, n)
-    if y.stride(1) != 1 or (y.shape[0] > 1 and y.stride(0) < n):
+    if (y.stride(1) != 1 and n > 1) or (y.shape[0] > 1 and y.stride(0) < n):
         y = y.clone(memory_format=torch.contiguous_format)
-    return y
+    return y, max(y.stride(0), n)
 
 
 def layer_norm_forward(x, weight=None, bias=None, eps=1e-5):
@@ -136,36 +155,42 @@ def layer_norm_forward(x, weight=None, bias=None, eps=1e-5):
 
     x: any shape [..., C], C >= 1, any strides; weight, bias: [C] of float32 or of x's type, or None.  stats [rows, 2] float32 = (mean,
     1 / sqrt(variance + eps)) is what `layer_norm_backward` needs."""
+    if _elsewhere(x):
+        with torch.cuda.device(x.device):
+            return layer_norm_forward(x, weight, bias, eps)
     if x.dim() < 1 or x.shape[-1] < 1:
         raise ValueError("x: at least one axis of at least one element")
-    eps = float(eps)
-    if not (eps > 0 and math.isfinite(eps)):
+    if not 0 < eps < math.inf:
         raise ValueError("eps must be positive and finite")
     t = _TYPE[_type(x)]
     wt = _norm_params(x, weight, bias)
-    dev = _device(*[v for v in (x, weight, bias) if v is not None])
-    y = torch.empty(x.shape, dtype=x.dtype, device=dev)
-    rows = x.numel() // x.shape[-1]
-    stats = torch.empty(rows, 2, dtype=torch.float32, device=dev)
+    d = _device(x, weight, bias)
+    n = x.shape[-1]
+    rows = x.numel() // n
+    y = x.new_empty(x.shape)
+    stats = x.new_empty((rows, 2), dtype=torch.float32)
     if rows == 0:
         return y, stats
-    with torch.cuda.device(dev):
-        m = _matrix(x)
-        w, b = (v.contiguous() if v is not None else None for v in (weight, bias))
-        _lib.check(_lib.lib().dpc_seq_norm_fwd(_p(m), _p(w), _p(b), _p(y), _p(stats), rows, x.shape[-1], m.stride(0) if rows > 1 else x.shape[-1],
-                                               eps, t, wt, _stream(dev)))
+    m, stride = _matrix(x, n)
+    w = None if weight is None else weight.contiguous()
+    b = None if bias is None else bias.contiguous()
+    _lib.check(_lib.lib().dpc_seq_norm_fwd(m.data_ptr(), None if w is None else w.data_ptr(), None if b is None else b.data_ptr(), y.data_ptr(),
+                                           stats.data_ptr(), rows, n, stride, eps, t, wt, _stream(d)))
     return y, stats
 
 
 def layer_norm_backward(dy, x, stats, weight=None, param_grads=True, param_dtype=None):
     """Gradients of `layer_norm_forward` -> (dx, dweight, dbias): dx in x's shape, dweight and dbias [C] in weight's type (without a weight:
     `param_dtype`, float32 by default).  param_grads=False skips the two sums (None, None)."""
+    if _elsewhere(x):
+        with torch.cuda.device(x.device):
+            return layer_norm_backward(dy, x, stats, weight, param_grads, param_dtype)
     if dy.shape != x.shape:
         raise ValueError(f"dy {tuple(dy.shape)} must have x's shape {tuple(x.shape)}")
     if x.dim() < 1 or x.shape[-1] < 1:
         raise ValueError("x: at least one axis of at least one element")
     t = _TYPE[_type(x, dy)]
-    wt = _norm_params(x, weight, None)
+    _norm_params(x, weight, None)
     n = x.shape[-1]
     rows = x.numel() // n
     if stats.shape != (rows, 2) or stats.dtype != torch.float32 or not stats.is_contiguous():
@@ -173,20 +198,19 @@ def layer_norm_backward(dy, x, stats, weight=None, param_grads=True, param_dtype
     pt = weight.dtype if weight is not None else param_dtype or torch.float32
     if pt not in (torch.float32, x.dtype) or (weight is not None and param_dtype not in (None, pt)):
         raise TypeError(f"param_dtype: float32 or {x.dtype}; with a weight, the weight's type")
-    if weight is None:
-        wt = _TYPE[pt]
-    dev = _device(*[v for v in (x, dy, stats, weight) if v is not None])
-    dx = torch.empty(x.shape, dtype=x.dtype, device=dev)
-    dw, db = (torch.empty(n, dtype=pt, device=dev) for _ in range(2)) if param_grads else (None, None)
+    d = _device(x, dy, stats, weight)
+    dx = x.new_empty(x.shape)
+    dw, db = (x.new_empty(n, dtype=pt), x.new_empty(n, dtype=pt)) if param_grads else (None, None)
     if rows == 0:
         return dx, dw.zero_() if dw is not None else None, db.zero_() if db is not None else None
     L = _lib.lib()
-    with torch.cuda.device(dev):
-        mx, mdy = _matrix(x), _matrix(dy)
-        w = weight.contiguous() if weight is not None else None
-        ws = _lib.workspace(L.dpc_seq_norm_bwd_workspace_bytes(rows, n), dev) if param_grads else None
-        _lib.check(L.dpc_seq_norm_bwd(_p(mdy), _p(mx), _p(stats), _p(w), _p(dx), _p(dw), _p(db), rows, n, mdy.stride(0) if rows > 1 else n,
-                                      mx.stride(0) if rows > 1 else n, t, wt, _p(ws), ws.numel() if ws is not None else 0, _stream(dev)))
+    (mx, sx), (mdy, sdy) = _matrix(x, n), _matrix(dy, n)
+    w = None if weight is None else weight.contiguous()
+    nbytes = L.dpc_seq_norm_bwd_workspace_bytes(rows, n) if param_grads else 0
+    ws = x.new_empty(nbytes, dtype=torch.uint8) if nbytes else None
+    _lib.check(L.dpc_seq_norm_bwd(mdy.data_ptr(), mx.data_ptr(), stats.data_ptr(), None if w is None else w.data_ptr(), dx.data_ptr(),
+                                  dw.data_ptr() if param_grads else None, db.data_ptr() if param_grads else None, rows, n, sdy, sx, t, _TYPE[pt],
+                                  ws.data_ptr() if nbytes else None, nbytes, _stream(d)))
     return dx, dw, db
 
 
@@ -238,82 +262,78 @@ class RotaryTable:
         angle = torch.arange(max_positions, dtype=torch.float64, device=device)[:, None] * f.to(device)
         z = torch.polar(torch.full((), self.attention_factor, dtype=torch.float64, device=device), angle)
         self.table = torch.view_as_real(z).float().contiguous()                        # [max_positions, rotary_dim / 2, 2]
-        self.stream = torch.cuda.current_stream(self.table.device)
-        self.stream.synchronize()                                                      # whole for whatever stream uses it
-
-
-def _as_btd(x):
-    """(strides of batch, token, head; batch, tokens) of [B, T, H, D] or packed [T, H, D]."""
-    if x.dim() == 4:
-        return x.stride()[:3], x.shape[0], x.shape[1]
-    return (0,) + x.stride()[:2], 1, x.shape[0]
-
-
-def _seq_tensor(x):
-    if x is None:
-        return _lib.SeqTensor(None, 0, 0, 0)
-    (b, t, h), _, _ = _as_btd(x)
-    n = x.shape if x.dim() == 4 else (1,) + tuple(x.shape)
-    return _lib.SeqTensor(x.data_ptr(), *(s if m > 1 else 0 for s, m in zip((b, t, h), n)))
+        torch.cuda.current_stream(self.table.device).synchronize()                     # whole for whatever stream uses it
+        self.stream = _stream(self.table.get_device())
 
 
 def _rotary(q, k, table, positions, start, out, transpose):
-    both = [q] if k is None else [q, k]
-    for x in both:
-        if x.dim() not in (3, 4):
-            raise ValueError("expected [batch, tokens, heads, head_dim] or packed [tokens, heads, head_dim]")
-    if k is not None and (k.dim() != q.dim() or k.shape[:-2] != q.shape[:-2] or k.shape[-1] != q.shape[-1]):
-        raise ValueError(f"q {tuple(q.shape)} and k {tuple(k.shape)} must agree but for the heads")
-    t = _TYPE[_type(*both)]
-    D = q.shape[-1]
+    if _elsewhere(q):
+        with torch.cuda.device(q.device):
+            return _rotary(q, k, table, positions, start, out, transpose)
+    packed, start = q.dim() == 3, int(start)
+    if not packed and q.dim() != 4:
+        raise ValueError("expected [batch, tokens, heads, head_dim] or packed [tokens, heads, head_dim]")
+    t = _TYPE[_type(q) if k is None else _type(q, k)]
+    shape = q.shape
+    B, T, H, D = (1, *shape) if packed else shape
+    Hk = 0
+    if k is not None:
+        if k.shape[:-2] != shape[:-2] or k.shape[-1] != D:
+            raise ValueError(f"q {tuple(shape)} and k {tuple(k.shape)} must agree but for the heads")
+        Hk = k.shape[-2]
     if table.rotary_dim > D:
         raise ValueError(f"the table's rotary_dim {table.rotary_dim} exceeds the head's {D}")
-    _, B, T = _as_btd(q)
-    start = int(start)
     pos_b = 0
     if positions is not None:
         if start != 0:
             raise ValueError("give positions or start, not both")
         if positions.dtype not in (torch.int64, torch.int32):
             raise TypeError("positions: int64 or int32")
-        if tuple(positions.shape) not in ((T,), (B, T) if q.dim() == 4 else (T,)):
-            raise ValueError(f"positions: shape ({T},)" + (f" or ({B}, {T})" if q.dim() == 4 else "") + f", got {tuple(positions.shape)}")
-        if positions.dim() == 2:
+        if positions.shape == (B, T) and not packed:
             pos_b = T
+        elif positions.shape != (T,):
+            raise ValueError(f"positions: shape ({T},)" + ("" if packed else f" or ({B}, {T})") + f", got {tuple(positions.shape)}")
     elif start < 0 or start + T > table.max_positions:
         raise ValueError(f"positions {start} .. {start + T - 1} leave the table's 0 .. {table.max_positions - 1}")
-    dev = _device(table.table, *both, *([positions] if positions is not None else []))
-    _in_use(table)
-    with torch.cuda.device(dev):
-        if out is None:
-            ys = [torch.empty(x.shape, dtype=x.dtype, device=dev) for x in both]
-        else:
-            ys = [out] if k is None and torch.is_tensor(out) else list(out)
-            ys = ys[:1] if k is None else ys
-            if len(ys) != len(both):
-                raise ValueError("out: one buffer per tensor")
-            for y, x in zip(ys, both):
-                if y.shape != x.shape or y.dtype != x.dtype or y.device != x.device:
-                    raise ValueError("out: shape, type and device of the input")
-                if y.numel() and y.stride(-1) != 1 or any(s == 0 and n > 1 for s, n in zip(y.stride(), y.shape)):
-                    raise ValueError("out: the last axis must be contiguous and elements distinct")
-                for z in both:
-                    itself = z is x and y.data_ptr() == z.data_ptr() and y.stride() == z.stride()
-                    if _shares(y, z) and not itself and _overlap(y, z):
-                        raise ValueError("out: a buffer that overlaps an input must be that input")
-            if k is not None and _overlap(*ys):
-                raise ValueError("out: the two buffers overlap")
-        if q.numel() == 0 and (k is None or k.numel() == 0):
-            return (ys[0], ys[1] if k is not None else None)
-        xs = [x if x.stride(-1) == 1 else x.contiguous() for x in both]
-        pos = None if positions is None else positions.to(torch.int64).contiguous()
-        a = _lib.SeqRotary(xq=_seq_tensor(xs[0]), yq=_seq_tensor(ys[0]), xk=_seq_tensor(xs[1] if k is not None else None),
-                           yk=_seq_tensor(ys[1] if k is not None else None), table=table.table.data_ptr(),
-                           positions=pos.data_ptr() if pos is not None else None, pos_stride_b=pos_b, start=start,
-                           max_positions=table.max_positions, type=t, batch=B, tokens=T, heads=q.shape[-2], kv_heads=k.shape[-2] if k is not None else 0,
-                           head_dim=D, rotary_dim=table.rotary_dim, interleaved=1 if table.layout == "interleaved" else 0, transpose=1 if transpose else 0)
-        _lib.check(_lib.lib().dpc_seq_rotary_run(C.byref(a), _stream(dev)))
-    return (ys[0], ys[1] if k is not None else None)
+    d = _device(q, k, positions, table.table)
+    _in_use(table, d)
+    if out is None:
+        yq, yk = q.new_empty(shape), None if k is None else k.new_empty(k.shape)
+    else:
+        yq, yk = _rotary_out(q, k, out)
+    if B * T * H * D == 0 and (k is None or k.numel() == 0):
+        return yq, yk
+    q = q if q.stride(-1) == 1 else q.contiguous()
+    k = k if k is None or k.stride(-1) == 1 else k.contiguous()
+    if positions is not None and not (positions.dtype == torch.int64 and positions.is_contiguous()):
+        positions = positions.to(torch.int64).contiguous()
+    none = (0, 0, 0, 0)
+    a = _lib.SEQ_ROTARY_BYTES.pack(q.data_ptr(), *_strides(q), *(none if k is None else (k.data_ptr(), *_strides(k))),
+                                   yq.data_ptr(), *_strides(yq), *(none if k is None else (yk.data_ptr(), *_strides(yk))), table.table.data_ptr(),
+                                   0 if positions is None else positions.data_ptr(), pos_b, start, table.max_positions, t, B, T, H, Hk, D,
+                                   table.rotary_dim, table.layout == "interleaved", transpose)
+    _lib.check(_lib.lib().dpc_seq_rotary_run(a, _stream(d)))
+    return yq, yk
+
+
+def _rotary_out(q, k, out):
+    """Checks the caller's buffers: an input itself, or something that shares no element with any input or the other buffer."""
+    ys = [out] if k is None and torch.is_tensor(out) else list(out)[:1 if k is None else None]
+    xs = [q] if k is None else [q, k]
+    if len(ys) != len(xs):
+        raise ValueError("out: one buffer per tensor")
+    for y, x in zip(ys, xs):
+        if y.shape != x.shape or y.dtype != x.dtype or y.device != x.device:
+            raise ValueError("out: shape, type and device of the input")
+        if y.numel() and y.stride(-1) != 1 or any(s == 0 and n > 1 for s, n in zip(y.stride(), y.shape)):
+            raise ValueError("out: the last axis must be contiguous and elements distinct")
+        for z in xs:
+            itself = z is x and y.data_ptr() == z.data_ptr() and y.stride() == z.stride()
+            if not itself and _overlap(y, z):
+                raise ValueError("out: a buffer that overlaps an input must be that input")
+    if k is not None and _overlap(*ys):
+        raise ValueError("out: the two buffers overlap")
+    return ys[0], None if k is None else ys[1]
 
 
 def rotary_forward(q, k, table, positions=None, start=0, out=None):
@@ -368,9 +388,11 @@ class SequencePlan:
         tiles = [self._tiles(ql, kl), self._tiles(kl, ql)]
         flat = torch.tensor([v for r in rows for v in r] + [v for t in tiles for e in t for v in e], dtype=torch.int32)
         self.table = flat.to(device)                                    # (a blocking copy: whole for whatever stream uses it)
-        self.stream = torch.cuda.current_stream(self.table.device)
+        self.stream = _stream(self.table.get_device())
         self.counts = tuple(len(t) for t in tiles)
-        self._offsets = (0, 4 * len(rows), 4 * len(rows) + 2 * len(tiles[0]))
+        at = self.table.data_ptr()
+        self.pointers = (at, at + 16 * len(rows), at + 16 * len(rows) + 8 * len(tiles[0]))
+        self.q_longest, self.k_longest, self.q_total, self.k_total = max(ql), max(kl), sum(ql), sum(kl)
 
     @staticmethod
     def _tiles(lengths, other):
@@ -386,55 +408,48 @@ class SequencePlan:
     def padded(cls, q_lengths, q_max, k_lengths=None, k_max=None, device="cuda"):
         return cls(q_lengths, k_lengths, q_max, k_max, device)
 
-    def _pointer(self, i):
-        return self.table.data_ptr() + 4 * self._offsets[i]
-
 
 def _attention_args(q, k, v, causal, scale, key_mask, plan):
-    """Checks the inputs -> (16-byte-row forms of q, k, v; filled dpc_seq_attn; the shape of lse; device)."""
+    """Checks the inputs -> (device; q, k, v in layouts a kernel can read, each with address and strides; the lse's shape; the rest of dpc_seq_attn)."""
     t = _type(q, k, v)
     packed = plan is not None and plan.packed_layout
-    want = 3 if packed else 4
-    if q.dim() != want or k.dim() != want or v.dim() != want:
+    if q.dim() != (3 if packed else 4) or k.dim() != q.dim():
         raise ValueError("expected " + ("packed [tokens, heads, head_dim]" if packed else "[batch, tokens, heads, head_dim]") + " tensors")
     if k.shape != v.shape:
         raise ValueError(f"k {tuple(k.shape)} and v {tuple(v.shape)} must have one shape")
-    H, Hk, D = q.shape[-2], k.shape[-2], q.shape[-1]
-    if k.shape[-1] != D or Hk < 1 or H < 1 or H % Hk:
+    B, Tq, H, D = (1, *q.shape) if packed else q.shape
+    Bk, Tk, Hk, Dk = (1, *k.shape) if packed else k.shape
+    if Dk != D or Hk < 1 or H < 1 or H % Hk:
         raise ValueError(f"q {tuple(q.shape)} and k {tuple(k.shape)}: one head size, query heads a multiple of the key heads")
-    if D % 8 or not 8 <= D <= 128:
+    if D & 7 or not 8 <= D <= 128:
         raise ValueError(f"head size {D}: multiples of 8 up to 128 are supported")
-    if not packed and q.shape[0] != k.shape[0]:
+    if B != Bk:
         raise ValueError("q and k must have one batch size")
     scale = D ** -0.5 if scale is None else float(scale)
-    if not (scale > 0 and math.isfinite(scale)):
+    if not 0 < scale < math.inf:
         raise ValueError("scale must be positive and finite")
-    if key_mask is not None:
-        if key_mask.dtype != torch.bool or key_mask.shape != k.shape[:-2]:
-            raise ValueError(f"key_mask: bool of shape {tuple(k.shape[:-2])}")
+    if key_mask is not None and (key_mask.dtype != torch.bool or key_mask.shape != k.shape[:-2]):
+        raise ValueError(f"key_mask: bool of shape {tuple(k.shape[:-2])}")
+    d = _device(q, k, v, key_mask, plan and plan.table)
     if plan is None:
-        B, q_len, k_len = q.shape[0], q.shape[1], k.shape[1]
+        seqs, sizes, n_seq, q_len, k_len = (0, 0, 0), (0, 0), B, Tq, Tk
     else:
-        B, q_len, k_len = len(plan.q_lengths), max(plan.q_lengths), max(plan.k_lengths)
-        shape = ((sum(plan.q_lengths),), (sum(plan.k_lengths),)) if packed else ((B, plan.q_max), (B, plan.k_max))
-        if (tuple(q.shape[:-2]), tuple(k.shape[:-2])) != shape:
-            raise ValueError(f"the plan is for q {shape[0]} and k {shape[1]} tokens, got {tuple(q.shape[:-2])} and {tuple(k.shape[:-2])}")
-    dev = _device(q, k, v, *([key_mask] if key_mask is not None else []), *([plan.table] if plan is not None else []))
-    if plan is not None:
-        _in_use(plan)
+        n_seq, q_len, k_len = len(plan.q_lengths), plan.q_longest, plan.k_longest
+        want = ((1, plan.q_total), (1, plan.k_total)) if packed else ((n_seq, plan.q_max), (n_seq, plan.k_max))
+        if ((B, Tq), (Bk, Tk)) != want:
+            raise ValueError(f"the plan is for q {want[0]} and k {want[1]} (batch, tokens), got {(B, Tq)} and {(Bk, Tk)}")
+        _in_use(plan, d)
+        seqs, sizes = plan.pointers, plan.counts
     if key_mask is not None:
         key_mask = key_mask.contiguous()
-    lse_shape = (H, q.shape[0]) if packed else (q.shape[0], H, q.shape[1])
-    a = _lib.SeqAttn(key_mask=key_mask.data_ptr() if key_mask is not None else None, mask_stride_b=0 if packed else k.shape[1], type=_TYPE[t], batch=B, heads=H,
-                     kv_heads=Hk, head_dim=D, q_len=q_len, k_len=k_len, causal=1 if causal else 0, lse_rows=math.prod(lse_shape), scale=scale,
-                     lse_stride_b=0 if packed else H * q.shape[1], lse_stride_h=lse_shape[-1], k_rows=k.numel() // D,
-                     k_row_stride_b=0 if packed else Hk * k.shape[1], k_row_stride_h=k.shape[-3])
-    if plan is not None:
-        a.seqs, a.q_tiles, a.k_tiles = (plan._pointer(i) for i in range(3))
-        a.n_q_tiles, a.n_k_tiles = plan.counts
-    q, k, v = _rows16(q), _rows16(k), _rows16(v)
-    a.q, a.k, a.v = _seq_tensor(q), _seq_tensor(k), _seq_tensor(v)
-    return (q, k, v, key_mask), a, lse_shape, dev
+    es = _BYTES[t]
+    lse_b, mask_b, krow_b = (0, 0, 0) if packed else (H * Tq, Tk, Hk * Tk)
+    tail = (0 if key_mask is None else key_mask.data_ptr(), mask_b, *seqs, *sizes, _TYPE[t], n_seq, H, Hk, D, q_len, k_len, 1 if causal else 0,
+            B * H * Tq, B * Hk * Tk, krow_b, Tk, scale)
+    return d, _lay(q, es), _lay(k, es), _lay(v, es), ((H, Tq) if packed else (B, H, Tq)), (lse_b, Tq), tail, key_mask
+
+
+_ABSENT = (0,) * 16
 
 
 def attention_forward(q, k, v, *, causal=False, scale=None, key_mask=None, plan=None, out=None):
@@ -442,28 +457,32 @@ def attention_forward(q, k, v, *, causal=False, scale=None, key_mask=None, plan=
 
     q [B, Lq, H, D], k and v [B, Lk, Hk, D] (or packed, see `SequencePlan`), H a multiple of Hk: query head h reads key / value head
     h // (H / Hk); D a multiple of 8 up to 128; scale defaults to D^-0.5.  causal: query i sees keys j <= i + Lk - Lq of its sequence.
-    key_mask: bool [B, Lk] (packed: [tokens]), True = takes part; what masked keys and values hold never matters.  A query that sees
-    nothing gives zeros and lse -inf.  lse [B, H, Lq] (packed: [H, tokens]) float32 is the log of the softmax's denominator, which
-    `attention_backward` needs.  Any strides; layouts whose head rows do not start on 16 bytes are copied first.  Rows of a padded plan
-    that belong to no sequence are zero (lse -inf), or left as they were in a given `out` buffer."""
-    (q, k, v, key_mask), a, lse_shape, dev = _attention_args(q, k, v, causal, scale, key_mask, plan)
+    key_mask: bool [B, Lk] (packed: [tokens]), True = takes part; what masked keys and values hold never matters.  (A NaN or infinity in a
+    key or value that some query of the call sees may reach queries that the causal mask keeps from it, as 0 * NaN does in the formula.)  A
+    query that sees nothing gives zeros and lse -inf.  lse [B, H, Lq] (packed: [H, tokens]) float32 is the log of the softmax's
+    denominator, which `attention_backward` needs.  Any strides; layouts whose head rows do not start on 16 bytes are copied first.  Rows of a padded
+    plan that belong to no sequence are zero (lse -inf), or left as they were in a given `out` buffer."""
+    if _elsewhere(q):
+        with torch.cuda.device(q.device):
+            return attention_forward(q, k, v, causal=causal, scale=scale, key_mask=key_mask, plan=plan, out=out)
+    d, lq, lk, lv, lse_shape, lse_strides, tail, key_mask = _attention_args(q, k, v, causal, scale, key_mask, plan)
     whole = plan is None or plan.q_whole
-    with torch.cuda.device(dev):
-        if out is None:
-            out = (torch.empty if whole else torch.zeros)(q.shape, dtype=q.dtype, device=dev)
-        else:
-            _device(q, out)
-            _written(out, q, "out", (q, k, v))
-        lse = torch.empty(lse_shape, dtype=torch.float32, device=dev)
-        if not whole:
-            lse.fill_(-math.inf)
-        if q.numel() == 0:
-            return out, lse
-        a.out, a.lse = _seq_tensor(out), lse.data_ptr()
-        L = _lib.lib()
-        nbytes = L.dpc_seq_attn_workspace_bytes(C.byref(a), 0)
-        ws = _lib.workspace(nbytes, dev) if nbytes else None
-        _lib.check(L.dpc_seq_attn_fwd(C.byref(a), _p(ws), nbytes, _stream(dev)))
+    if out is None:
+        out = (q.new_empty if whole else q.new_zeros)(q.shape)
+    else:
+        _device(q, out)
+        _written(out, q, "out", (q, k, v))
+    lse = q.new_empty(lse_shape, dtype=torch.float32)
+    if not whole:
+        lse.fill_(-math.inf)
+    if lse.numel() == 0:
+        return out, lse
+    es = _BYTES[q.dtype]
+    a = _lib.SEQ_ATTN_BYTES.pack(*lq[1:], *lk[1:], *lv[1:], *_lay(out, es)[1:], lse.data_ptr(), *lse_strides, *_ABSENT, *tail)
+    L = _lib.lib()
+    nbytes = L.dpc_seq_attn_workspace_bytes(a, 0)
+    ws = q.new_empty(nbytes, dtype=torch.uint8) if nbytes else None
+    _lib.check(L.dpc_seq_attn_fwd(a, ws.data_ptr() if nbytes else None, nbytes, _stream(d)))
     return out, lse
 
 
@@ -472,31 +491,35 @@ def attention_backward(dout, q, k, v, out, lse, *, causal=False, scale=None, key
 
     The probabilities are computed again from q, k and lse.  Gradients of a key / value head are summed over the query heads that read it.  Masked
     keys get zero gradients.  grads: buffers for (dq, dk, dv), e.g. views of one packed projection gradient; they must not overlap."""
-    _type(q, dout, out)
+    if _elsewhere(q):
+        with torch.cuda.device(q.device):
+            return attention_backward(dout, q, k, v, out, lse, causal=causal, scale=scale, key_mask=key_mask, plan=plan, grads=grads)
+    t = _type(q, dout, out)
     if dout.shape != q.shape or out.shape != q.shape:
         raise ValueError(f"dout {tuple(dout.shape)} and out {tuple(out.shape)} must have q's shape {tuple(q.shape)}")
-    (q, k, v, key_mask), a, lse_shape, dev = _attention_args(q, k, v, causal, scale, key_mask, plan)
+    d, lq, lk, lv, lse_shape, lse_strides, tail, key_mask = _attention_args(q, k, v, causal, scale, key_mask, plan)
     _device(q, dout, out, lse)
-    if tuple(lse.shape) != tuple(lse_shape) or lse.dtype != torch.float32 or not lse.is_contiguous():
-        raise ValueError(f"lse: the contiguous float32 {tuple(lse_shape)} of attention_forward")
-    with torch.cuda.device(dev):
-        dout, out = _rows16(dout), _rows16(out)
-        if grads is None:
-            dq = (torch.empty if plan is None or plan.q_whole else torch.zeros)(q.shape, dtype=q.dtype, device=dev)
-            dk, dv = ((torch.empty if plan is None or plan.k_whole else torch.zeros)(k.shape, dtype=k.dtype, device=dev) for _ in range(2))
-        else:
-            dq, dk, dv = grads
-            _device(q, dq, dk, dv)
-            for name, g, like in (("dq", dq, q), ("dk", dk, k), ("dv", dv, v)):
-                _written(g, like, name, (q, k, v, dout, out))
-            if _overlap(dq, dk) or _overlap(dq, dv) or _overlap(dk, dv):
-                raise ValueError("grads: the buffers overlap")
-        if q.numel() == 0 and k.numel() == 0:
-            return dq, dk, dv
-        a.dout, a.out, a.dq, a.dk, a.dv = (_seq_tensor(x) for x in (dout, out, dq, dk, dv))
-        a.lse = lse.data_ptr()
-        L = _lib.lib()
-        nbytes = L.dpc_seq_attn_workspace_bytes(C.byref(a), 1)
-        ws = _lib.workspace(nbytes, dev) if nbytes else None
-        _lib.check(L.dpc_seq_attn_bwd(C.byref(a), _p(ws), nbytes, _stream(dev)))
+    if lse.shape != lse_shape or lse.dtype != torch.float32 or not lse.is_contiguous():
+        raise ValueError(f"lse: the contiguous float32 {lse_shape} of attention_forward")
+    if grads is None:
+        dq = (q.new_empty if plan is None or plan.q_whole else q.new_zeros)(q.shape)
+        new = k.new_empty if plan is None or plan.k_whole else k.new_zeros
+        dk, dv = new(k.shape), new(k.shape)
+    else:
+        dq, dk, dv = grads
+        _device(q, dq, dk, dv)
+        for name, g, like in (("dq", dq, q), ("dk", dk, k), ("dv", dv, v)):
+            _written(g, like, name, (q, k, v, dout, out))
+        if _overlap(dq, dk) or _overlap(dq, dv) or _overlap(dk, dv):
+            raise ValueError("grads: the buffers overlap")
+    if lse.numel() == 0 and k.numel() == 0:
+        return dq, dk, dv
+    es = _BYTES[t]
+    lout, ldout = _lay(out, es), _lay(dout, es)
+    a = _lib.SEQ_ATTN_BYTES.pack(*lq[1:], *lk[1:], *lv[1:], *lout[1:], lse.data_ptr(), *lse_strides, *ldout[1:], *_lay(dq, es)[1:], *_lay(dk, es)[1:],
+                                 *_lay(dv, es)[1:], *tail)
+    L = _lib.lib()
+    nbytes = L.dpc_seq_attn_workspace_bytes(a, 1)
+    ws = q.new_empty(nbytes, dtype=torch.uint8) if nbytes else None
+    _lib.check(L.dpc_seq_attn_bwd(a, ws.data_ptr() if nbytes else None, nbytes, _stream(d)))
     return dq, dk, dv
