@@ -204,7 +204,7 @@ _SIGNATURES = {
     "dpc_adam_ema_step": (C.c_int, [_P, _P, _P, _P, _P, _L, _P, C.c_float, C.c_float, _D, _D, _D, _D, _I, _I,
                                     C.c_float, _P]),
     "dpc_seq_norm_fwd": (C.c_int, [_P] * 5 + [_L, _I, _L, C.c_float, _I, _I, _P]),
-    "dpc_seq_norm_bwd_workspace_bytes": (_Z, [_L, _I]),
+    "dpc_seq_norm_bwd_workspace_bytes": (_Z, [_L, _I, _I]),
     "dpc_seq_norm_bwd": (C.c_int, [_P] * 7 + [_L, _I, _L, _L, _I, _I, _P, _Z, _P]),
     "dpc_seq_rotary_run": (C.c_int, [_P, _P]),                        # (SeqRotary / SeqAttn by reference, or their bytes)
     "dpc_seq_attn_workspace_bytes": (_Z, [_P, _I]),

@@ -2,11 +2,14 @@
 //   mu = sum x / C, var = sum (x - mu)^2 / C, s = (var + eps)^-1/2, xh = (x - mu) s, y = xh w + b
 //   g = dy w, dx = s (g - mean(g) - xh mean(g xh)), dw = sum_rows dy xh, db = sum_rows dy
 // Bound by bytes: the forward reads x and writes y, the backward reads x and dy and writes dx, each once.  A row lives in the registers
-// of G lanes (4, 16, 64 or a whole workgroup of 256; N accesses of 16 bytes a lane), so that the centred second sum of the variance -- no
+// of G lanes (4, 16, 64 or a whole workgroup; N accesses of 16 bytes a lane), so that the centred second sum of the variance -- no
 // E[x^2] - mu^2 cancellation -- costs no second read.  Rows too wide for that (over 2048 accesses) are read again from L2.
 // The backward pass keeps dw and db in registers over all rows of a group, adds the groups of a workgroup in LDS and writes one row of
 // partial sums per workgroup; a second kernel adds those in fixed order.
 #include <algorithm>
+#include <initializer_list>
+#include <type_traits>
+#include <utility>
 
 #include "common.h"
 
@@ -14,38 +17,44 @@ namespace dpc {
 namespace seqnorm {
 
 template <class T> constexpr int VEC = 16 / (int)sizeof(T);
+template <class T, int E> struct Pack { typedef T type __attribute__((ext_vector_type(E))); };
 
-// Element e of access n of a lane.  Rows that start on 16 bytes and hold whole accesses: 16 consecutive bytes; other rows: one element at a
-// time, consecutive lanes on consecutive elements.
-template <class T, int G> struct Map {
-    int lane; bool vec;
-    __device__ __forceinline__ int at(int n, int e) const { return vec ? (n * G + lane) * VEC<T> + e : n * G * VEC<T> + e * G + lane; }
-};
-
-template <class T, int G>
-__device__ __forceinline__ void load(const T* __restrict__ row, const Map<T, G>& m, int n, int C, float (&v)[VEC<T>]) {
-    typedef T Q __attribute__((ext_vector_type(VEC<T>)));
-    if (m.vec) {
-        const int c = m.at(n, 0);
-        if (c < C) {
-            const Q q = *reinterpret_cast<const Q*>(row + c);
-#pragma unroll
-            for (int e = 0; e < VEC<T>; ++e) v[e] = (float)q[e];
-            return;
-        }
-#pragma unroll
-        for (int e = 0; e < VEC<T>; ++e) v[e] = 0.f;
-    } else {
-#pragma unroll
-        for (int e = 0; e < VEC<T>; ++e) { const int c = m.at(n, e); v[e] = c < C ? (float)row[c] : 0.f; }
-    }
+// Element e of access n of a lane.  VECT: rows start on 16 bytes and hold whole accesses; a lane has 16 consecutive bytes.  Otherwise: one
+// element at a time, consecutive lanes on consecutive elements.
+template <class T, int G, bool VECT> __device__ __forceinline__ int at(int lane, int n, int e) {
+    return VECT ? (n * G + lane) * VEC<T> + e : n * G * VEC<T> + e * G + lane;
 }
 
-template <class T, int G>
-__device__ __forceinline__ void store(T* __restrict__ row, const Map<T, G>& m, int n, int C, const float (&v)[VEC<T>]) {
-    typedef T Q __attribute__((ext_vector_type(VEC<T>)));
-    if (m.vec) {
-        const int c = m.at(n, 0);
+// The elements of P (T, or fp32 parameters) that a lane holds, as they lie in memory; `none` past the row's end
+template <class T, class P, int G, int N, bool VECT> struct Held {
+    typedef typename Pack<P, VEC<T>>::type Q;
+    Q v[N];
+    __device__ __forceinline__ void load(const P* __restrict__ row, int lane, int C, float none) {
+#pragma unroll
+        for (int n = 0; n < N; ++n) {
+            if (VECT) {
+                const int c = at<T, G, VECT>(lane, n, 0);
+                if (c < C) { v[n] = *reinterpret_cast<const Q*>(row + c); continue; }
+            }
+#pragma unroll
+            for (int e = 0; e < VEC<T>; ++e) {
+                const int c = at<T, G, VECT>(lane, n, e);
+                v[n][e] = !VECT && c < C ? row[c] : (P)none;
+            }
+        }
+    }
+    __device__ __forceinline__ void fill(float x) {
+#pragma unroll
+        for (int n = 0; n < N; ++n)
+#pragma unroll
+            for (int e = 0; e < VEC<T>; ++e) v[n][e] = (P)x;
+    }
+};
+
+template <class T, int G, bool VECT> __device__ __forceinline__ void store(T* __restrict__ row, int lane, int n, int C, const float (&v)[VEC<T>]) {
+    typedef typename Pack<T, VEC<T>>::type Q;
+    if (VECT) {
+        const int c = at<T, G, VECT>(lane, n, 0);
         if (c < C) {
             Q q;
 #pragma unroll
@@ -54,25 +63,23 @@ __device__ __forceinline__ void store(T* __restrict__ row, const Map<T, G>& m, i
         }
     } else {
 #pragma unroll
-        for (int e = 0; e < VEC<T>; ++e) { const int c = m.at(n, e); if (c < C) row[c] = (T)v[e]; }
+        for (int e = 0; e < VEC<T>; ++e) { const int c = at<T, G, VECT>(lane, n, e); if (c < C) row[c] = (T)v[e]; }
     }
 }
 
-// weight / bias element, fp32 or T (null: the identity's value)
-template <class T> __device__ __forceinline__ float param(const void* w, int w32, int c, float none) {
-    return !w ? none : w32 ? reinterpret_cast<const float*>(w)[c] : (float)reinterpret_cast<const T*>(w)[c];
-}
-
-template <int G> __device__ __forceinline__ float group_sum(float v, float* s_red) {
+// Sums of a and b over the G lanes of a group.  A group that is a whole workgroup (256, 1024) meets in LDS; `turn` alternates between two slots, so one
+// barrier a call is enough.  (Every thread of the workgroup makes every call.)
+template <int G> __device__ __forceinline__ void group_sum(float& a, float& b, float2 (*s_red)[16], int& turn) {
 #pragma unroll
-    for (int x = (G < 64 ? G : 64) / 2; x; x >>= 1) v += __shfl_xor(v, x, 64);
-    if (G == 256) {
+    for (int x = (G < 64 ? G : 64) / 2; x; x >>= 1) { a += __shfl_xor(a, x, 64); b += __shfl_xor(b, x, 64); }
+    if (G > 64) {
+        if ((threadIdx.x & 63) == 0) s_red[turn][threadIdx.x >> 6] = float2{a, b};
         __syncthreads();
-        if ((threadIdx.x & 63) == 0) s_red[threadIdx.x >> 6] = v;
-        __syncthreads();
-        v = (s_red[0] + s_red[1]) + (s_red[2] + s_red[3]);
+        a = b = 0.f;
+#pragma unroll
+        for (int w = 0; w < G / 64; ++w) { a += s_red[turn][w].x; b += s_red[turn][w].y; }
+        turn ^= 1;
     }
-    return v;
 }
 
 struct FwdParams {
@@ -84,227 +91,257 @@ struct FwdParams {
     float eps;
 };
 
-template <class T, int G, int N>
-__global__ __launch_bounds__(256) void fwd_kernel(const FwdParams p) {
-    __shared__ float s_red[4];
-    constexpr int V = VEC<T>, R = 256 / G;
-    const Map<T, G> m{(int)(threadIdx.x & (G - 1)), p.vec != 0};
+template <class T, class P, int G, int N, bool VECT, int THREADS>
+__global__ __launch_bounds__(THREADS) void fwd_kernel(const FwdParams p) {
+    __shared__ float2 s_red[2][16];
+    constexpr int V = VEC<T>, R = THREADS / G;
+    const int lane = threadIdx.x & (G - 1);
+    int turn = 0;
     const float inv_c = 1.f / (float)p.C;
-    for (long long r0 = (long long)blockIdx.x * R; r0 < p.rows; r0 += (long long)gridDim.x * R) {      // (uniform over the workgroup)
-        const long long r = r0 + threadIdx.x / G;
-        const bool ok = r < p.rows;
-        const T* x = reinterpret_cast<const T*>(p.x) + (ok ? r : 0) * p.xs;
-        float v[N][V], sum = 0.f;
+    Held<T, P, G, N, VECT> w, b;
+    if (p.w) w.load(reinterpret_cast<const P*>(p.w), lane, p.C, 0.f); else w.fill(1.f);
+    if (p.b) b.load(reinterpret_cast<const P*>(p.b), lane, p.C, 0.f); else b.fill(0.f);
+    const long long step = (long long)gridDim.x * R;
+    long long r = (long long)blockIdx.x * R + threadIdx.x / G;
+    const T* x = reinterpret_cast<const T*>(p.x);
+    Held<T, T, G, N, VECT> next;
+    next.load(x + min(r, p.rows - 1) * p.xs, lane, p.C, 0.f);
+    for (long long r0 = (long long)blockIdx.x * R; r0 < p.rows; r0 += step, r += step) {      // (uniform over the workgroup)
+        Held<T, T, G, N, VECT> cur = next;
+        if (r0 + step < p.rows) next.load(x + min(r + step, p.rows - 1) * p.xs, lane, p.C, 0.f);
+        float v[N][V], sum = 0.f, none = 0.f;
 #pragma unroll
-        for (int n = 0; n < N; ++n) {
-            load<T, G>(x, m, n, p.C, v[n]);
+        for (int n = 0; n < N; ++n)
 #pragma unroll
-            for (int e = 0; e < V; ++e) sum += v[n][e];
-        }
-        const float mu = group_sum<G>(sum, s_red) * inv_c;
+            for (int e = 0; e < V; ++e) { v[n][e] = (float)cur.v[n][e]; sum += v[n][e]; }
+        group_sum<G>(sum, none, s_red, turn);
+        const float mu = sum * inv_c;
         sum = 0.f;
 #pragma unroll
         for (int n = 0; n < N; ++n)
 #pragma unroll
             for (int e = 0; e < V; ++e) {
                 v[n][e] -= mu;
-                if (m.at(n, e) < p.C) sum += v[n][e] * v[n][e];
+                if (at<T, G, VECT>(lane, n, e) < p.C) sum = __builtin_fmaf(v[n][e], v[n][e], sum);
             }
-        const float rstd = 1.f / sqrtf(group_sum<G>(sum, s_red) * inv_c + p.eps);
-        if (ok) {
+        group_sum<G>(sum, none, s_red, turn);
+        const float rstd = 1.f / sqrtf(sum * inv_c + p.eps);
+        if (r < p.rows) {
             T* y = reinterpret_cast<T*>(p.y) + r * (long long)p.C;
 #pragma unroll
             for (int n = 0; n < N; ++n) {
 #pragma unroll
-                for (int e = 0; e < V; ++e) {
-                    const int c = min(m.at(n, e), p.C - 1);
-                    v[n][e] = v[n][e] * rstd * param<T>(p.w, p.w32, c, 1.f) + param<T>(p.b, p.w32, c, 0.f);
-                }
-                store<T, G>(y, m, n, p.C, v[n]);
+                for (int e = 0; e < V; ++e) v[n][e] = __builtin_fmaf(v[n][e] * rstd, (float)w.v[n][e], (float)b.v[n][e]);
+                store<T, G, VECT>(y, lane, n, p.C, v[n]);
             }
-            if (m.lane == 0) { p.stats[2 * r] = mu; p.stats[2 * r + 1] = rstd; }
+            if (lane == 0) *reinterpret_cast<float2*>(p.stats + 2 * r) = float2{mu, rstd};
         }
     }
 }
 
 // rows wider than 2048 accesses: one workgroup a row, three reads of x (the later two from L2)
-template <class T>
+template <class T, class P, bool VECT>
 __global__ __launch_bounds__(256) void fwd_wide_kernel(const FwdParams p) {
-    __shared__ float s_red[4];
-    constexpr int V = VEC<T>;
-    const Map<T, 256> m{(int)threadIdx.x, p.vec != 0};
+    __shared__ float2 s_red[2][16];
+    constexpr int V = VEC<T>, S = 256 * V;
+    const int lane = threadIdx.x;
+    int turn = 0;
     const float inv_c = 1.f / (float)p.C;
-    const int N = (p.C + 256 * V - 1) / (256 * V);
     for (long long r = blockIdx.x; r < p.rows; r += gridDim.x) {
         const T* x = reinterpret_cast<const T*>(p.x) + r * p.xs;
-        float v[V], sum = 0.f;
-        for (int n = 0; n < N; ++n) {
-            load<T, 256>(x, m, n, p.C, v);
+        Held<T, T, 256, 1, VECT> h;
+        float sum = 0.f, none = 0.f;
+        for (int c0 = 0; c0 < p.C; c0 += S) {
+            h.load(x + c0, lane, p.C - c0, 0.f);
 #pragma unroll
-            for (int e = 0; e < V; ++e) sum += v[e];
+            for (int e = 0; e < V; ++e) sum += (float)h.v[0][e];
         }
-        const float mu = group_sum<256>(sum, s_red) * inv_c;
+        group_sum<256>(sum, none, s_red, turn);
+        const float mu = sum * inv_c;
         sum = 0.f;
-        for (int n = 0; n < N; ++n) {
-            load<T, 256>(x, m, n, p.C, v);
-#pragma unroll
-            for (int e = 0; e < V; ++e) if (m.at(n, e) < p.C) sum += (v[e] - mu) * (v[e] - mu);
-        }
-        const float rstd = 1.f / sqrtf(group_sum<256>(sum, s_red) * inv_c + p.eps);
-        T* y = reinterpret_cast<T*>(p.y) + r * (long long)p.C;
-        for (int n = 0; n < N; ++n) {
-            load<T, 256>(x, m, n, p.C, v);
+        for (int c0 = 0; c0 < p.C; c0 += S) {
+            h.load(x + c0, lane, p.C - c0, 0.f);
 #pragma unroll
             for (int e = 0; e < V; ++e) {
-                const int c = min(m.at(n, e), p.C - 1);
-                v[e] = (v[e] - mu) * rstd * param<T>(p.w, p.w32, c, 1.f) + param<T>(p.b, p.w32, c, 0.f);
+                const float d = (float)h.v[0][e] - mu;
+                if (c0 + at<T, 256, VECT>(lane, 0, e) < p.C) sum = __builtin_fmaf(d, d, sum);
             }
-            store<T, 256>(y, m, n, p.C, v);
         }
-        if (threadIdx.x == 0) { p.stats[2 * r] = mu; p.stats[2 * r + 1] = rstd; }
+        group_sum<256>(sum, none, s_red, turn);
+        const float rstd = 1.f / sqrtf(sum * inv_c + p.eps);
+        T* y = reinterpret_cast<T*>(p.y) + r * (long long)p.C;
+        for (int c0 = 0; c0 < p.C; c0 += S) {
+            Held<T, P, 256, 1, VECT> w, b;
+            h.load(x + c0, lane, p.C - c0, 0.f);
+            if (p.w) w.load(reinterpret_cast<const P*>(p.w) + c0, lane, p.C - c0, 0.f); else w.fill(1.f);
+            if (p.b) b.load(reinterpret_cast<const P*>(p.b) + c0, lane, p.C - c0, 0.f); else b.fill(0.f);
+            float v[V];
+#pragma unroll
+            for (int e = 0; e < V; ++e) v[e] = __builtin_fmaf(((float)h.v[0][e] - mu) * rstd, (float)w.v[0][e], (float)b.v[0][e]);
+            store<T, 256, VECT>(y + c0, lane, 0, p.C - c0, v);
+        }
+        if (lane == 0) *reinterpret_cast<float2*>(p.stats + 2 * r) = float2{mu, rstd};
     }
 }
 
 struct BwdParams {
     const void *dy, *x, *w;
     const float* stats;
-    void* dx;
-    float* part;               // [gridDim.x][2][C] sums of dy xh and dy, or null
+    void *dx, *dw, *db;        // dw, db: written by the kernel itself when it is one workgroup (part null)
+    float* part;               // [gridDim.x][2][C] sums of dy xh and dy
     long long rows, dys, xs;
-    int C, w32, vec;
+    int C, w32, vec, sums;
 };
 
-template <class T, int G, int N>
-__global__ __launch_bounds__(256) void bwd_kernel(const BwdParams p) {
-    constexpr int V = VEC<T>, R = 256 / G;
-    __shared__ float s_red[4];
-    __shared__ float s_sum[G < 256 ? 2 * 256 * N * V : 1];
-    const Map<T, G> m{(int)(threadIdx.x & (G - 1)), p.vec != 0};
+template <class P> __device__ __forceinline__ void put_param(void* dst, int c, float v) { if (dst) reinterpret_cast<P*>(dst)[c] = (P)v; }
+
+template <class T, class P, int G, int N, bool VECT, int THREADS>
+__global__ __launch_bounds__(THREADS) void bwd_kernel(const BwdParams p) {
+    constexpr int V = VEC<T>, R = THREADS / G;
+    __shared__ float2 s_red[2][16];
+    __shared__ float s_sum[R > 1 ? THREADS * N * V : 1];
+    const int lane = threadIdx.x & (G - 1), grp = threadIdx.x / G;
+    int turn = 0;
     const float inv_c = 1.f / (float)p.C;
     float dw[N][V], db[N][V];
 #pragma unroll
     for (int n = 0; n < N; ++n)
 #pragma unroll
         for (int e = 0; e < V; ++e) dw[n][e] = db[n][e] = 0.f;
-    for (long long r0 = (long long)blockIdx.x * R; r0 < p.rows; r0 += (long long)gridDim.x * R) {
-        const long long r = r0 + threadIdx.x / G;
-        const bool ok = r < p.rows;
-        const long long at = ok ? r : 0;
-        const T* x = reinterpret_cast<const T*>(p.x) + at * p.xs;
-        const T* dy = reinterpret_cast<const T*>(p.dy) + at * p.dys;
-        const float mu = p.stats[2 * at], rstd = p.stats[2 * at + 1];
+    Held<T, P, G, N, VECT> w;
+    if (p.w) w.load(reinterpret_cast<const P*>(p.w), lane, p.C, 0.f); else w.fill(1.f);
+    const T* x = reinterpret_cast<const T*>(p.x);
+    const T* dy = reinterpret_cast<const T*>(p.dy);
+    const long long step = (long long)gridDim.x * R;
+    long long r = (long long)blockIdx.x * R + grp;
+    Held<T, T, G, N, VECT> nx, ny;
+    float2 ns;
+    auto fetch = [&](long long row) {
+        row = min(row, p.rows - 1);
+        nx.load(x + row * p.xs, lane, p.C, 0.f);
+        ny.load(dy + row * p.dys, lane, p.C, 0.f);
+        ns = *reinterpret_cast<const float2*>(p.stats + 2 * row);
+    };
+    fetch(r);
+    for (long long r0 = (long long)blockIdx.x * R; r0 < p.rows; r0 += step, r += step) {
+        const Held<T, T, G, N, VECT> hx = nx, hy = ny;
+        const float mu = ns.x, rstd = ns.y;
+        if (r0 + step < p.rows) fetch(r + step);
         float xh[N][V], g[N][V], a = 0.f, b = 0.f;
-#pragma unroll
-        for (int n = 0; n < N; ++n) {
-            load<T, G>(x, m, n, p.C, xh[n]);
-            load<T, G>(dy, m, n, p.C, g[n]);
-#pragma unroll
-            for (int e = 0; e < V; ++e) {
-                const int c = m.at(n, e);
-                xh[n][e] = (xh[n][e] - mu) * rstd;
-                if (c >= p.C) xh[n][e] = 0.f;
-                if (ok) { dw[n][e] += g[n][e] * xh[n][e]; db[n][e] += g[n][e]; }
-                g[n][e] *= param<T>(p.w, p.w32, min(c, p.C - 1), 1.f);
-                a += g[n][e];
-                b += g[n][e] * xh[n][e];
-            }
-        }
-        a = group_sum<G>(a, s_red) * inv_c;
-        b = group_sum<G>(b, s_red) * inv_c;
-        if (ok) {
-            T* dx = reinterpret_cast<T*>(p.dx) + r * (long long)p.C;
-#pragma unroll
-            for (int n = 0; n < N; ++n) {
-#pragma unroll
-                for (int e = 0; e < V; ++e) xh[n][e] = rstd * (g[n][e] - a - xh[n][e] * b);
-                store<T, G>(dx, m, n, p.C, xh[n]);
-            }
-        }
-    }
-    if (!p.part) return;
-    float* part = p.part + (long long)blockIdx.x * 2 * p.C;
-    if (G == 256) {
 #pragma unroll
         for (int n = 0; n < N; ++n)
 #pragma unroll
             for (int e = 0; e < V; ++e) {
-                const int c = m.at(n, e);
-                if (c < p.C) { part[c] = dw[n][e]; part[p.C + c] = db[n][e]; }
+                xh[n][e] = ((float)hx.v[n][e] - mu) * rstd;
+                g[n][e] = (float)hy.v[n][e];                          // (0 past the row's end)
+                if (r >= p.rows) g[n][e] = 0.f;                      // (a group without a row reads the last one again)
+                dw[n][e] = __builtin_fmaf(g[n][e], xh[n][e], dw[n][e]);
+                db[n][e] += g[n][e];
+                g[n][e] *= (float)w.v[n][e];
+                a += g[n][e];
+                b = __builtin_fmaf(g[n][e], xh[n][e], b);
             }
-        return;
-    }
-    constexpr int W = G * N * V;                                     // columns a group holds
-    const int grp = threadIdx.x / G;
+        group_sum<G>(a, b, s_red, turn);
+        a *= inv_c;
+        b *= inv_c;
+        if (r < p.rows) {
+            T* dx = reinterpret_cast<T*>(p.dx) + r * (long long)p.C;
 #pragma unroll
-    for (int n = 0; n < N; ++n)
+            for (int n = 0; n < N; ++n) {
 #pragma unroll
-        for (int e = 0; e < V; ++e) {
-            s_sum[(grp * N * V + n * V + e) * G + m.lane] = dw[n][e];
-            s_sum[((R + grp) * N * V + n * V + e) * G + m.lane] = db[n][e];
+                for (int e = 0; e < V; ++e) xh[n][e] = rstd * (g[n][e] - __builtin_fmaf(xh[n][e], b, a));
+                store<T, G, VECT>(dx, lane, n, p.C, xh[n]);
+            }
         }
-    __syncthreads();
-    for (int i = threadIdx.x; i < 2 * W; i += 256) {
-        const int half = i / W, k = i % W;                           // k = (n * V + e) * G + lane
-        float sum = 0.f;
+    }
+    if (!p.sums) return;
+    // the groups of the workgroup are added in order, first dw, then db
+    float* part = p.part ? p.part + (long long)blockIdx.x * 2 * p.C : nullptr;
 #pragma unroll
-        for (int q = 0; q < R; ++q) sum += s_sum[(half * R + q) * W + k];
-        const Map<T, G> mm{k % G, p.vec != 0};
-        const int c = mm.at(k / G / V, k / G % V);
-        if (c < p.C) part[half * p.C + c] = sum;
+    for (int half = 0; half < 2; ++half) {
+        if (R > 1) {
+            __syncthreads();
+#pragma unroll
+            for (int n = 0; n < N; ++n)
+#pragma unroll
+                for (int e = 0; e < V; ++e) s_sum[(grp * N * V + n * V + e) * G + lane] = half ? db[n][e] : dw[n][e];
+            __syncthreads();
+        }
+        constexpr int W = G * N * V;                                 // columns a group holds: index (n V + e) G + lane
+        for (int i = threadIdx.x; i < W; i += THREADS) {
+            float sum = 0.f;
+            if (R > 1) {
+#pragma unroll 8
+                for (int q = 0; q < R; ++q) sum += s_sum[q * W + i];
+            }
+            const int c = at<T, G, VECT>(i % G, i / G / V, i / G % V);
+            if (R == 1) {                                            // (i = (n V + e) 256 + thread: this thread's own)
+#pragma unroll
+                for (int n = 0; n < N; ++n)
+#pragma unroll
+                    for (int e = 0; e < V; ++e) if (n * V + e == i / G) sum = half ? db[n][e] : dw[n][e];
+            }
+            if (c >= p.C) continue;
+            if (part) part[half * p.C + c] = sum;
+            else put_param<P>(half ? p.db : p.dw, c, sum);
+        }
     }
 }
 
-template <class T>
+template <class T, class P, bool VECT>
 __global__ __launch_bounds__(256) void bwd_wide_kernel(const BwdParams p) {
-    __shared__ float s_red[4];
-    constexpr int V = VEC<T>;
-    const Map<T, 256> m{(int)threadIdx.x, p.vec != 0};
+    __shared__ float2 s_red[2][16];
+    constexpr int V = VEC<T>, S = 256 * V;
+    const int lane = threadIdx.x;
+    int turn = 0;
     const float inv_c = 1.f / (float)p.C;
-    const int N = (p.C + 256 * V - 1) / (256 * V);
-    float* part = p.part ? p.part + (long long)blockIdx.x * 2 * p.C : nullptr;
+    float* part = p.sums ? p.part + (long long)blockIdx.x * 2 * p.C : nullptr;
     bool first = true;
     for (long long r = blockIdx.x; r < p.rows; r += gridDim.x) {
         const T* x = reinterpret_cast<const T*>(p.x) + r * p.xs;
         const T* dy = reinterpret_cast<const T*>(p.dy) + r * p.dys;
         const float mu = p.stats[2 * r], rstd = p.stats[2 * r + 1];
-        float xh[V], g[V], a = 0.f, b = 0.f;
-        for (int n = 0; n < N; ++n) {
-            load<T, 256>(x, m, n, p.C, xh);
-            load<T, 256>(dy, m, n, p.C, g);
+        Held<T, T, 256, 1, VECT> hx, hy;
+        Held<T, P, 256, 1, VECT> w;
+        w.fill(1.f);
+        float a = 0.f, b = 0.f;
+        for (int c0 = 0; c0 < p.C; c0 += S) {
+            hx.load(x + c0, lane, p.C - c0, 0.f);
+            hy.load(dy + c0, lane, p.C - c0, 0.f);
+            if (p.w) w.load(reinterpret_cast<const P*>(p.w) + c0, lane, p.C - c0, 0.f);
 #pragma unroll
             for (int e = 0; e < V; ++e) {
-                const int c = m.at(n, e);
+                const int c = c0 + at<T, 256, VECT>(lane, 0, e);
                 if (c >= p.C) continue;
-                xh[e] = (xh[e] - mu) * rstd;
+                const float xh = ((float)hx.v[0][e] - mu) * rstd, g = (float)hy.v[0][e];
                 if (part) {                                          // (this thread's own columns: no other touches them)
-                    part[c] = (first ? 0.f : part[c]) + g[e] * xh[e];
-                    part[p.C + c] = (first ? 0.f : part[p.C + c]) + g[e];
+                    part[c] = (first ? 0.f : part[c]) + g * xh;
+                    part[p.C + c] = (first ? 0.f : part[p.C + c]) + g;
                 }
-                g[e] *= param<T>(p.w, p.w32, c, 1.f);
-                a += g[e];
-                b += g[e] * xh[e];
+                a += g * (float)w.v[0][e];
+                b = __builtin_fmaf(g * (float)w.v[0][e], xh, b);
             }
         }
         first = false;
-        a = group_sum<256>(a, s_red) * inv_c;
-        b = group_sum<256>(b, s_red) * inv_c;
+        group_sum<256>(a, b, s_red, turn);
+        a *= inv_c;
+        b *= inv_c;
         T* dx = reinterpret_cast<T*>(p.dx) + r * (long long)p.C;
-        for (int n = 0; n < N; ++n) {
-            load<T, 256>(x, m, n, p.C, xh);
-            load<T, 256>(dy, m, n, p.C, g);
+        for (int c0 = 0; c0 < p.C; c0 += S) {
+            hx.load(x + c0, lane, p.C - c0, 0.f);
+            hy.load(dy + c0, lane, p.C - c0, 0.f);
+            if (p.w) w.load(reinterpret_cast<const P*>(p.w) + c0, lane, p.C - c0, 0.f);
+            float v[V];
 #pragma unroll
-            for (int e = 0; e < V; ++e) {
-                const int c = min(m.at(n, e), p.C - 1);
-                xh[e] = rstd * (g[e] * param<T>(p.w, p.w32, c, 1.f) - a - (xh[e] - mu) * rstd * b);
-            }
-            store<T, 256>(dx, m, n, p.C, xh);
+            for (int e = 0; e < V; ++e) v[e] = rstd * ((float)hy.v[0][e] * (float)w.v[0][e] - __builtin_fmaf(((float)hx.v[0][e] - mu) * rstd, b, a));
+            store<T, 256, VECT>(dx + c0, lane, 0, p.C - c0, v);
         }
     }
 }
 
 // dweight / dbias: 32 columns x 32 slices of the partial rows a workgroup; slices are joined in order
-template <class T>
-__global__ __launch_bounds__(1024) void param_kernel(const float* __restrict__ part, void* dw, void* db, int nblk, int C, int w32) {
+template <class P>
+__global__ __launch_bounds__(1024) void param_kernel(const float* __restrict__ part, void* dw, void* db, int nblk, int C) {
     __shared__ float s[32][33];
     const int half = blockIdx.y, col = threadIdx.x & 31, slice = threadIdx.x >> 5, c = blockIdx.x * 32 + col;
     void* out = half ? db : dw;
@@ -319,55 +356,82 @@ __global__ __launch_bounds__(1024) void param_kernel(const float* __restrict__ p
     if (slice == 0 && c < C) {
         double t = 0.0;
         for (int k = 0; k < 32; ++k) t += (double)s[k][col];
-        if (w32) reinterpret_cast<float*>(out)[c] = (float)t;
-        else reinterpret_cast<T*>(out)[c] = (T)(float)t;
+        put_param<P>(out, c, (float)t);
     }
 }
 
-// lanes a row and accesses a lane: the fewest lanes that hold the row in at most four accesses up to a wave, else a workgroup
-template <class F> int by_width(int acc, F f) {       // acc: 16-byte accesses of a row
-    if (acc <= 4) return f(std::integral_constant<int, 4>{}, std::integral_constant<int, 1>{});
-    if (acc <= 16) return f(std::integral_constant<int, 16>{}, std::integral_constant<int, 1>{});
-    if (acc <= 64) return f(std::integral_constant<int, 64>{}, std::integral_constant<int, 1>{});
-    if (acc <= 128) return f(std::integral_constant<int, 64>{}, std::integral_constant<int, 2>{});
-    if (acc <= 256) return f(std::integral_constant<int, 64>{}, std::integral_constant<int, 4>{});
-    if (acc <= 512) return f(std::integral_constant<int, 256>{}, std::integral_constant<int, 2>{});
-    if (acc <= 1024) return f(std::integral_constant<int, 256>{}, std::integral_constant<int, 4>{});
-    if (acc <= 2048) return f(std::integral_constant<int, 256>{}, std::integral_constant<int, 8>{});
-    return f(std::integral_constant<int, 256>{}, std::integral_constant<int, 0>{});
+// Lanes a row (G) and accesses a lane (N) by the row's 16-byte accesses: the fewest lanes that hold it in at most four accesses up to a wave
+// -- no barrier -- else a workgroup.  More accesses a lane cost registers, that is waves, that is loads in flight: bf16 rows of 4096 forward in
+// one wave of 8 accesses 41 us for 8191 rows, in four waves of 2 accesses 23 us (5.7 TB/s).
+template <int A, int B> using Shape = std::pair<std::integral_constant<int, A>, std::integral_constant<int, B>>;
+template <class F> int by_width(int acc, F f) {
+    if (acc <= 4) return f(Shape<4, 1>{});
+    if (acc <= 16) return f(Shape<16, 1>{});
+    if (acc <= 64) return f(Shape<64, 1>{});
+    if (acc <= 128) return f(Shape<64, 2>{});
+    if (acc <= 256) return f(Shape<64, 4>{});
+    if (acc <= 512) return f(Shape<256, 2>{});
+    if (acc <= 1024) return f(Shape<256, 4>{});
+    if (acc <= 2048) return f(Shape<1024, 2>{});
+    return f(Shape<256, 0>{});
 }
-static inline int rows_per_group(int acc) { return acc <= 4 ? 64 : acc <= 16 ? 16 : acc <= 256 ? 4 : 1; }
 
-constexpr int FWD_BLOCKS = 2048, BWD_BLOCKS = 512;
-template <class T> int fwd(const FwdParams& p, hipStream_t s) {
+constexpr int FWD_BLOCKS = 2048;
+// Workgroups of the backward pass: each writes one row of partial sums (8 C bytes, read once more), which may cost some 10 % of the rows' own traffic,
+// but two workgroups a CU are there in any case.
+static int bwd_blocks(long long rows, int es) { return (int)std::min(rows, std::min(2048ll, std::max(512ll, rows * es / 64))); }
+constexpr long long ONE_BLOCK = 32768;       // elements that one workgroup of 1024 threads takes alone: the sums then need no second launch
+
+static bool one_block(long long rows, int C, int es) { return rows * C <= ONE_BLOCK && (C * es + 15) / 16 <= 64; }
+
+template <class T, class P, bool VECT> int fwd(const FwdParams& p, hipStream_t s) {
     const int acc = (p.C + VEC<T> - 1) / VEC<T>;
-    const int grid = (int)std::min<long long>(FWD_BLOCKS, (p.rows + rows_per_group(acc) - 1) / rows_per_group(acc));
-    return by_width(acc, [&](auto g, auto n) {
-        if constexpr (n() == 0) hipLaunchKernelGGL((fwd_wide_kernel<T>), dim3(grid), dim3(256), 0, s, p);
-        else hipLaunchKernelGGL((fwd_kernel<T, g(), n()>), dim3(grid), dim3(256), 0, s, p);
+    return by_width(acc, [&](auto shape) {
+        constexpr int G = decltype(shape.first)::value, N = decltype(shape.second)::value;
+        constexpr int THREADS = G > 256 ? G : 256, R = THREADS / G;
+        const int grid = (int)std::min<long long>(FWD_BLOCKS, (p.rows + R - 1) / R);
+        if constexpr (N == 0) hipLaunchKernelGGL((fwd_wide_kernel<T, P, VECT>), dim3(grid), dim3(256), 0, s, p);
+        else hipLaunchKernelGGL((fwd_kernel<T, P, G, N, VECT, THREADS>), dim3(grid), dim3(THREADS), 0, s, p);
         DPC_LAUNCH_CHECK();
         return (int)DPC_OK;
     });
 }
 
-template <class T> int bwd(const BwdParams& p, void* dw, void* db, hipStream_t s) {
+template <class T, class P, bool VECT> int bwd(const BwdParams& p, hipStream_t s) {
     const int acc = (p.C + VEC<T> - 1) / VEC<T>;
-    const int grid = (int)std::min<long long>(BWD_BLOCKS, (p.rows + rows_per_group(acc) - 1) / rows_per_group(acc));
-    const int rc = by_width(acc, [&](auto g, auto n) {
-        if constexpr (n() == 0) hipLaunchKernelGGL((bwd_wide_kernel<T>), dim3(grid), dim3(256), 0, s, p);
-        else hipLaunchKernelGGL((bwd_kernel<T, g(), n()>), dim3(grid), dim3(256), 0, s, p);
+    return by_width(acc, [&](auto shape) {
+        constexpr int G = decltype(shape.first)::value, N = decltype(shape.second)::value;
+        if constexpr (G <= 64 && N == 1) {
+            if (p.sums && !p.part) {
+                hipLaunchKernelGGL((bwd_kernel<T, P, G, N, VECT, 1024>), dim3(1), dim3(1024), 0, s, p);
+                DPC_LAUNCH_CHECK();
+                return (int)DPC_OK;
+            }
+        }
+        constexpr int THREADS = G > 256 ? G : 256, R = THREADS / G;
+        const int grid = (int)std::min<long long>(bwd_blocks(p.rows, sizeof(T)), (p.rows + R - 1) / R);
+        if constexpr (N == 0) hipLaunchKernelGGL((bwd_wide_kernel<T, P, VECT>), dim3(grid), dim3(256), 0, s, p);
+        else hipLaunchKernelGGL((bwd_kernel<T, P, G, N, VECT, THREADS>), dim3(grid), dim3(THREADS), 0, s, p);
+        DPC_LAUNCH_CHECK();
+        if (!p.sums) return (int)DPC_OK;
+        hipLaunchKernelGGL((param_kernel<P>), dim3((p.C + 31) / 32, 2), dim3(1024), 0, s, p.part, p.dw, p.db, grid, p.C);
         DPC_LAUNCH_CHECK();
         return (int)DPC_OK;
     });
-    if (rc != DPC_OK || !p.part) return rc;
-    hipLaunchKernelGGL((param_kernel<T>), dim3((p.C + 31) / 32, 2), dim3(1024), 0, s, p.part, dw, db, grid, p.C, p.w32);
-    DPC_LAUNCH_CHECK();
-    return DPC_OK;
 }
 
-static int vector_rows(const void* a, const void* b, const void* c, long long sa, long long sb, int C, int es) {
-    const size_t bits = (size_t)a | (size_t)b | (size_t)c | (size_t)(sa * es) | (size_t)(sb * es) | (size_t)((long long)C * es);
-    return bits % 16 == 0;
+template <class Prm, class F> int by_type(const Prm& p, int type, int wtype, F f) {
+    auto v = [&](auto t, auto w) { return p.vec ? f(t, w, std::true_type{}) : f(t, w, std::false_type{}); };
+    if (type == DPC_SEQ_F32) return v(float{}, float{});
+    if (type == DPC_SEQ_F16) return wtype == DPC_SEQ_F32 ? v(_Float16{}, float{}) : v(_Float16{}, _Float16{});
+    return wtype == DPC_SEQ_F32 ? v(__bf16{}, float{}) : v(__bf16{}, __bf16{});
+}
+
+// (parameters of fp32 beside a 16-bit x are read 32 bytes at a time)
+static int vector_rows(std::initializer_list<const void*> ptrs, long long sa, long long sb, int C, int es, const void* w, const void* b, int wes) {
+    size_t bits = (size_t)(sa * es) | (size_t)(sb * es) | (size_t)((long long)C * es);
+    for (const void* q : ptrs) bits |= (size_t)q;
+    return bits % 16 == 0 && ((size_t)w | (size_t)b) % (16 / es * wes) == 0;
 }
 
 }  // namespace seqnorm
@@ -387,14 +451,14 @@ int dpc_seq_norm_fwd(const void* x, const void* weight, const void* bias, void* 
     DPC_REQUIRE(x && y && stats && (rows == 1 || x_stride >= C), "seq_norm: null argument or overlapping rows");
     hipStream_t s = (hipStream_t)stream;
     const int es = type == DPC_SEQ_F32 ? 4 : 2;
-    const FwdParams p{x, weight, bias, y, stats, rows, x_stride, C, wtype == DPC_SEQ_F32, vector_rows(x, y, nullptr, x_stride, 0, C, es), eps};
+    const FwdParams p{x, weight, bias, y, stats, rows, x_stride, C, wtype == DPC_SEQ_F32, vector_rows({x, y}, x_stride, 0, C, es, weight, bias, wtype == DPC_SEQ_F32 ? 4 : 2), eps};
     ProfScope prof(PROF_LN, 0, 2.0 * (double)rows * C * es, s);
-    return type == DPC_SEQ_F32 ? fwd<float>(p, s) : type == DPC_SEQ_F16 ? fwd<_Float16>(p, s) : fwd<__bf16>(p, s);
+    return by_type(p, type, wtype, [&](auto t, auto w, auto v) { return fwd<decltype(t), decltype(w), decltype(v)::value>(p, s); });
 }
 
-size_t dpc_seq_norm_bwd_workspace_bytes(int64_t rows, int C) {
-    if (rows < 1 || C < 1) return 0;
-    return (size_t)std::min<long long>(BWD_BLOCKS, rows) * 2 * (size_t)C * sizeof(float) + 256;
+size_t dpc_seq_norm_bwd_workspace_bytes(int64_t rows, int C, int type) {
+    if (rows < 1 || C < 1 || one_block(rows, C, type == DPC_SEQ_F32 ? 4 : 2)) return 0;
+    return (size_t)bwd_blocks(rows, type == DPC_SEQ_F32 ? 4 : 2) * 2 * (size_t)C * sizeof(float) + 256;
 }
 
 int dpc_seq_norm_bwd(const void* dy, const void* x, const float* stats, const void* weight, void* dx, void* dweight, void* dbias,
@@ -404,14 +468,14 @@ int dpc_seq_norm_bwd(const void* dy, const void* x, const float* stats, const vo
     DPC_REQUIRE(wtype == DPC_SEQ_F32 || wtype == type, "seq_norm_bwd: weight and bias are fp32 or of the element type");
     DPC_REQUIRE(rows >= 1 && C >= 1, "seq_norm_bwd: rows >= 1, C >= 1");
     DPC_REQUIRE(dy && x && stats && dx && (rows == 1 || (x_stride >= C && (dy_stride >= C || dy_stride == 0))), "seq_norm_bwd: null argument or overlapping rows");
-    const bool sums = dweight || dbias;
-    DPC_REQUIRE(!sums || (ws && ws_bytes >= dpc_seq_norm_bwd_workspace_bytes(rows, C)), "seq_norm_bwd: workspace too small");
+    const int sums = dweight || dbias, es = type == DPC_SEQ_F32 ? 4 : 2;
+    const size_t need = sums ? dpc_seq_norm_bwd_workspace_bytes(rows, C, type) : 0;
+    DPC_REQUIRE(need == 0 || (ws && ws_bytes >= need), "seq_norm_bwd: workspace too small");
     hipStream_t s = (hipStream_t)stream;
-    const int es = type == DPC_SEQ_F32 ? 4 : 2;
-    const BwdParams p{dy, x, weight, stats, dx, sums ? reinterpret_cast<float*>(align_up((size_t)ws, 256)) : nullptr, rows, dy_stride, x_stride, C,
-                      wtype == DPC_SEQ_F32, vector_rows(dy, x, dx, dy_stride, x_stride, C, es)};
+    const BwdParams p{dy, x, weight, stats, dx, dweight, dbias, need ? reinterpret_cast<float*>(align_up((size_t)ws, 256)) : nullptr, rows, dy_stride, x_stride, C,
+                      wtype == DPC_SEQ_F32, vector_rows({dy, x, dx}, dy_stride, x_stride, C, es, weight, nullptr, wtype == DPC_SEQ_F32 ? 4 : 2), sums};
     ProfScope prof(PROF_LN, 0, 3.0 * (double)rows * C * es, s);
-    return type == DPC_SEQ_F32 ? bwd<float>(p, dweight, dbias, s) : type == DPC_SEQ_F16 ? bwd<_Float16>(p, dweight, dbias, s) : bwd<__bf16>(p, dweight, dbias, s);
+    return by_type(p, type, wtype, [&](auto t, auto w, auto v) { return bwd<decltype(t), decltype(w), decltype(v)::value>(p, s); });
 }
 
 }  // extern "C"

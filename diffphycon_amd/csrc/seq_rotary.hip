@@ -11,82 +11,95 @@ namespace dpc {
 namespace seqrot {
 
 struct Ten { char* p; long long b, t, h; };      // strides in elements
+
+// n / d for 0 <= n < 2^31 by a multiplication: with s = ceil(log2 d) and m = floor(2^32 (2^s - d) / d) + 1, n / d = (mulhi(n, m) + n) >> s
+struct Div {
+    unsigned d, m, s;
+    Div() : Div(1) {}
+    explicit Div(unsigned x) : d(x), m(0), s(0) {
+        while ((1ull << s) < d) ++s;
+        m = (unsigned)(((1ull << 32) * ((1ull << s) - d)) / d + 1);
+    }
+    __device__ __forceinline__ unsigned operator()(unsigned n) const { return (__umulhi(n, m) + n) >> s; }
+};
+
 struct Params {
     Ten xq, xk, yq, yk;
     const float* table;
     const long long* positions;
     long long pos_b, start, max_pos;
-    int tokens, total, heads, kv_heads, D, R, interleaved, items, rot_items, hgroups, per_wg;
+    int total, heads, all, D, R, interleaved, rot_items, per_wg, work;
+    Div tokens, items, per_token, groups;
     float sign;
 };
 
-template <class T, int V>        // V: elements of an access (16 bytes, or 1)
+// HEADS heads of one token and chunk: their loads are all in flight before the first is used
+template <class T, int V, int HEADS>
 __global__ __launch_bounds__(256) void rotary_kernel(const Params p) {
     typedef T Q __attribute__((ext_vector_type(V)));
-    constexpr int P = V > 1 ? V : 2;                                 // elements a chunk may hold per side
-    const int per_token = p.hgroups * p.items;
-    for (int w = threadIdx.x; w < p.per_wg * per_token; w += 256) {
-        const int lt = w / per_token, in = w % per_token, hg = in / p.items, it = in % p.items;
-        const long long n = (long long)blockIdx.x * p.per_wg + lt;
-        if (n >= p.total) return;
-        const int b = (int)n / p.tokens, t = (int)n % p.tokens;
-        const bool turn = it < p.rot_items;
-        // first element of the chunk, distance to the pair's other side (half layout), pairs in it
-        int c0, other = 0, i0 = 0;
-        if (!turn) c0 = p.R + (it - p.rot_items) * V;
-        else if (p.interleaved) { c0 = it * P; i0 = it * (P / 2); }
-        else { c0 = it * V; other = p.R / 2; i0 = it * V; }
-        constexpr int NP = V > 1 ? V : 1;                            // pairs held at most (half layout: V, interleaved: V / 2)
-        float cs[NP], sn[NP];
-        if (turn) {
-            const long long pos = p.positions ? p.positions[b * p.pos_b + t] : p.start + t;
-            const bool ok = pos >= 0 && pos < p.max_pos;
-            const float2* tab = reinterpret_cast<const float2*>(p.table) + (ok ? pos : 0) * (p.R / 2) + i0;
-            const int np = p.interleaved ? P / 2 : NP;
+    constexpr int NP = V > 1 ? V : 1, PAIR = V > 1 ? V : 2;          // pairs of a chunk at most; elements of an interleaved chunk
+    const unsigned w = threadIdx.x + blockIdx.y * 256;
+    if (w >= (unsigned)p.work) return;
+    const unsigned lt = p.per_token(w), in = w - lt * p.per_token.d, hg = p.items(in), it = in - hg * p.items.d;
+    const unsigned n = blockIdx.x * p.per_wg + lt;
+    if (n >= (unsigned)p.total) return;
+    const unsigned b = p.tokens(n), t = n - b * p.tokens.d;
+    const bool turn = (int)it < p.rot_items;
+    const int c0 = !turn ? p.R + ((int)it - p.rot_items) * V : p.interleaved ? it * PAIR : it * V;
+    const int other = p.interleaved || !turn ? (V > 1 ? 0 : turn) : p.R / 2;          // distance to the pair's second half (V = 1, interleaved: the next element)
+    float cs[NP], sn[NP];
 #pragma unroll
-            for (int k = 0; k < NP; ++k)
-                if (k < np) {
-                    const float2 z = tab[k];
-                    cs[k] = ok ? z.x : __builtin_nanf("");
-                    sn[k] = ok ? z.y * p.sign : __builtin_nanf("");
-                }
-        }
-        for (int hd = hg; hd < p.heads + p.kv_heads; hd += p.hgroups) {
-            const bool isq = hd < p.heads;
-            const Ten& X = isq ? p.xq : p.xk;
-            const Ten& Y = isq ? p.yq : p.yk;
-            const int h = isq ? hd : hd - p.heads;
-            const T* x = reinterpret_cast<const T*>(X.p) + b * X.b + t * X.t + h * X.h + c0;
-            T* y = reinterpret_cast<T*>(Y.p) + b * Y.b + t * Y.t + h * Y.h + c0;
-            if (!turn) {
-                *reinterpret_cast<Q*>(y) = *reinterpret_cast<const Q*>(x);
-            } else if (p.interleaved) {
-                if constexpr (V > 1) {
-                    Q q = *reinterpret_cast<const Q*>(x);
+    for (int k = 0; k < NP; ++k) { cs[k] = 1.f; sn[k] = 0.f; }
+    if (turn) {
+        const long long pos = p.positions ? p.positions[b * p.pos_b + t] : p.start + t;
+        const bool ok = pos >= 0 && pos < p.max_pos;
+        const int i0 = p.interleaved ? it * (PAIR / 2) : it * V;
+        const float2* tab = reinterpret_cast<const float2*>(p.table) + (ok ? pos : 0) * (p.R / 2) + i0;
 #pragma unroll
-                    for (int k = 0; k < V / 2; ++k) {
-                        const float a = (float)q[2 * k], c = (float)q[2 * k + 1];
-                        q[2 * k] = (T)(a * cs[k] - c * sn[k]);
-                        q[2 * k + 1] = (T)(a * sn[k] + c * cs[k]);
-                    }
-                    *reinterpret_cast<Q*>(y) = q;
-                } else {
-                    const float a = (float)x[0], c = (float)x[1];
-                    y[0] = (T)(a * cs[0] - c * sn[0]);
-                    y[1] = (T)(a * sn[0] + c * cs[0]);
-                }
-            } else {
-                Q q = *reinterpret_cast<const Q*>(x), u = *reinterpret_cast<const Q*>(x + other);
+        for (int k = 0; k < NP; ++k)
+            if (!p.interleaved || k < PAIR / 2) {
+                const float2 z = tab[k];
+                cs[k] = ok ? z.x : __builtin_nanf("");
+                sn[k] = ok ? z.y * p.sign : __builtin_nanf("");
+            }
+    }
+    Q q[HEADS], u[HEADS];
+    T* dst[HEADS];
 #pragma unroll
-                for (int k = 0; k < V; ++k) {
-                    const float a = (float)q[k], c = (float)u[k];
-                    q[k] = (T)(a * cs[k] - c * sn[k]);
-                    u[k] = (T)(a * sn[k] + c * cs[k]);
-                }
-                *reinterpret_cast<Q*>(y) = q;
-                *reinterpret_cast<Q*>(y + other) = u;
+    for (int i = 0; i < HEADS; ++i) {
+        const int hd = hg + i * p.groups.d;
+        dst[i] = nullptr;
+        if (hd >= p.all) continue;
+        const bool isq = hd < p.heads;
+        const Ten& X = isq ? p.xq : p.xk;
+        const Ten& Y = isq ? p.yq : p.yk;
+        const int h = isq ? hd : hd - p.heads;
+        const T* x = reinterpret_cast<const T*>(X.p) + b * X.b + t * X.t + h * X.h + c0;
+        dst[i] = reinterpret_cast<T*>(Y.p) + b * Y.b + t * Y.t + h * Y.h + c0;
+        q[i] = *reinterpret_cast<const Q*>(x);
+        u[i] = q[i];
+        if (other) u[i] = *reinterpret_cast<const Q*>(x + other);
+    }
+#pragma unroll
+    for (int i = 0; i < HEADS; ++i) {
+        if (!dst[i]) continue;
+        if (turn && p.interleaved && V > 1) {
+#pragma unroll
+            for (int k = 0; k < V / 2; ++k) {
+                const float x = (float)q[i][2 * k], y = (float)q[i][(2 * k + 1) % V];
+                q[i][2 * k] = (T)(x * cs[k] - y * sn[k]);
+                q[i][(2 * k + 1) % V] = (T)(x * sn[k] + y * cs[k]);
+            }
+        } else if (turn) {
+#pragma unroll
+            for (int k = 0; k < V; ++k) {
+                const float x = (float)q[i][k], y = (float)u[i][k];
+                q[i][k] = (T)(x * cs[k] - y * sn[k]);
+                u[i][k] = (T)(x * sn[k] + y * cs[k]);
             }
         }
+        *reinterpret_cast<Q*>(dst[i]) = q[i];
+        if (other) *reinterpret_cast<Q*>(dst[i] + other) = u[i];
     }
 }
 
@@ -108,18 +121,25 @@ template <class T> int run(const dpc_seq_rotary* a, hipStream_t s) {
     p.xq = ten(a->xq); p.xk = ten(a->xk); p.yq = ten(a->yq); p.yk = ten(a->yk);
     p.table = a->table; p.positions = reinterpret_cast<const long long*>(a->positions);
     p.pos_b = a->pos_stride_b; p.start = a->start; p.max_pos = a->max_positions;
-    p.tokens = a->tokens; p.total = a->batch * a->tokens; p.heads = a->heads; p.kv_heads = a->xk.p ? a->kv_heads : 0;
+    p.total = a->batch * a->tokens; p.heads = a->heads; p.all = a->heads + (a->xk.p ? a->kv_heads : 0);
     p.D = a->head_dim; p.R = a->rotary_dim; p.interleaved = a->interleaved != 0;
     const int w = vec ? V : 1;
     p.rot_items = p.interleaved ? p.R / (vec ? V : 2) : p.R / 2 / w;
-    p.items = p.rot_items + (inplace ? 0 : (p.D - p.R) / w);
-    const int all = p.heads + p.kv_heads;
-    p.hgroups = all;
-    p.per_wg = std::max(1, 256 / (p.hgroups * p.items));
+    const int items = p.rot_items + (inplace ? 0 : (p.D - p.R) / w);
+    // Four heads a thread once the card is full without that (2^20 threads): the angles, the index arithmetic and the position are then shared.
+    // Few tokens keep one head a thread, for latency.
+    const bool four = (long long)p.total * p.all * items >= (1ll << 20);
+    const int groups = four ? (p.all + 3) / 4 : p.all, per_token = groups * items;
+    p.tokens = Div(a->tokens); p.items = Div(items); p.per_token = Div(per_token); p.groups = Div(groups);
+    p.per_wg = std::max(1, 256 / per_token);
+    p.work = p.per_wg * per_token;
     p.sign = a->transpose ? -1.f : 1.f;
-    const int grid = (p.total + p.per_wg - 1) / p.per_wg;
-    if (vec) hipLaunchKernelGGL((rotary_kernel<T, 16 / (int)sizeof(T)>), dim3(grid), dim3(256), 0, s, p);
-    else hipLaunchKernelGGL((rotary_kernel<T, 1>), dim3(grid), dim3(256), 0, s, p);
+    const dim3 grid((p.total + p.per_wg - 1) / p.per_wg, (p.work + 255) / 256);
+    constexpr int VV = 16 / (int)sizeof(T);
+    if (vec && four) hipLaunchKernelGGL((rotary_kernel<T, VV, 4>), grid, dim3(256), 0, s, p);
+    else if (vec) hipLaunchKernelGGL((rotary_kernel<T, VV, 1>), grid, dim3(256), 0, s, p);
+    else if (four) hipLaunchKernelGGL((rotary_kernel<T, 1, 4>), grid, dim3(256), 0, s, p);
+    else hipLaunchKernelGGL((rotary_kernel<T, 1, 1>), grid, dim3(256), 0, s, p);
     DPC_LAUNCH_CHECK();
     return DPC_OK;
 }
@@ -138,7 +158,7 @@ extern "C" int dpc_seq_rotary_run(const dpc_seq_rotary* a, dpc_stream_t stream) 
     if ((int64_t)a->batch * a->tokens == 0) return DPC_OK;
     DPC_REQUIRE(a->xq.p && a->yq.p && a->table && a->max_positions >= 1, "seq_rotary: null argument");
     DPC_REQUIRE(!a->xk.p == !a->yk.p && (!a->xk.p || a->kv_heads >= 1), "seq_rotary: the second tensor needs input, output and heads");
-    DPC_REQUIRE((int64_t)(a->heads + a->kv_heads) * a->head_dim < (1 << 24), "seq_rotary: heads x head_dim");
+    DPC_REQUIRE((int64_t)(a->heads + a->kv_heads) * a->head_dim < (1 << 23), "seq_rotary: heads x head_dim");
     hipStream_t s = (hipStream_t)stream;
     const int es = a->type == DPC_SEQ_F32 ? 4 : 2;
     ProfScope prof(PROF_SMALL, 0, 2.0 * a->batch * a->tokens * (a->heads + (a->xk.p ? a->kv_heads : 0)) * (double)a->head_dim * es, s);

@@ -206,7 +206,7 @@ def layer_norm_backward(dy, x, stats, weight=None, param_grads=True, param_dtype
     L = _lib.lib()
     (mx, sx), (mdy, sdy) = _matrix(x, n), _matrix(dy, n)
     w = None if weight is None else weight.contiguous()
-    nbytes = L.dpc_seq_norm_bwd_workspace_bytes(rows, n) if param_grads else 0
+    nbytes = L.dpc_seq_norm_bwd_workspace_bytes(rows, n, t) if param_grads else 0
     ws = x.new_empty(nbytes, dtype=torch.uint8) if nbytes else None
     _lib.check(L.dpc_seq_norm_bwd(mdy.data_ptr(), mx.data_ptr(), stats.data_ptr(), None if w is None else w.data_ptr(), dx.data_ptr(),
                                   dw.data_ptr() if param_grads else None, db.data_ptr() if param_grads else None, rows, n, sdy, sx, t, _TYPE[pt],

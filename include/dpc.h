@@ -424,7 +424,7 @@ enum dpc_seq_type { DPC_SEQ_F32 = 0, DPC_SEQ_F16 = 1, DPC_SEQ_BF16 = 2 };
 int dpc_seq_norm_fwd(const void* x, const void* weight, const void* bias, void* y, float* stats, int64_t rows, int C,
                      int64_t x_stride, float eps, int type, int wtype, dpc_stream_t stream);
 /* dx [rows][C] contiguous; dweight / dbias [C] of type wtype, each NULL: skipped.  ws: partial sums of the two [C] rows. */
-size_t dpc_seq_norm_bwd_workspace_bytes(int64_t rows, int C);
+size_t dpc_seq_norm_bwd_workspace_bytes(int64_t rows, int C, int type);
 int dpc_seq_norm_bwd(const void* dy, const void* x, const float* stats, const void* weight, void* dx, void* dweight, void* dbias,
                      int64_t rows, int C, int64_t dy_stride, int64_t x_stride, int type, int wtype, void* ws, size_t ws_bytes,
                      dpc_stream_t stream);

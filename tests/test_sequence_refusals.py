@@ -167,6 +167,7 @@ def test_rotary_and_norm_entries_refuse():
     for args in [(None, None, None, p, p, 4, 8, 8, 1e-5, 0, 0), (p, None, None, p, p, 4, 0, 8, 1e-5, 0, 0), (p, None, None, p, p, 4, 8, 7, 1e-5, 0, 0),
                  (p, None, None, p, p, 4, 8, 8, 0.0, 0, 0), (p, None, None, p, p, 4, 8, 8, 1e-5, 3, 0), (p, None, None, p, p, 4, 8, 8, 1e-5, 1, 2)]:
         assert L.dpc_seq_norm_fwd(*args, None) < 0
-    need = L.dpc_seq_norm_bwd_workspace_bytes(4, 8)
-    assert L.dpc_seq_norm_bwd(p, p, p, None, p, p, p, 4, 8, 8, 8, 0, 0, p, need - 1, None) < 0
-    assert L.dpc_seq_norm_bwd(p, p, p, None, p, p, p, 0, 8, 8, 8, 0, 0, p, need, None) < 0
+    need = L.dpc_seq_norm_bwd_workspace_bytes(400, 800, 0)
+    assert need >= 2 * 800 * 4
+    assert L.dpc_seq_norm_bwd(p, p, p, None, p, p, p, 400, 800, 800, 800, 0, 0, p, need - 1, None) < 0
+    assert L.dpc_seq_norm_bwd(p, p, p, None, p, p, p, 0, 800, 800, 800, 0, 0, p, need, None) < 0
