@@ -77,7 +77,7 @@ class SeqAttn(C.Structure):
     """dpc_seq_attn (include/dpc.h)."""
     _fields_ = [("q", SeqTensor), ("k", SeqTensor), ("v", SeqTensor), ("out", SeqTensor), ("lse", C.c_void_p), ("lse_stride_b", C.c_int64),
                 ("lse_stride_h", C.c_int64), ("dout", SeqTensor), ("dq", SeqTensor), ("dk", SeqTensor), ("dv", SeqTensor),
-                ("key_mask", C.c_void_p), ("mask_stride_b", C.c_int64), ("seqs", C.c_void_p), ("q_tiles", C.c_void_p), ("k_tiles", C.c_void_p),
+                ("key_mask", C.c_void_p), ("mask_stride_b", C.c_int64), ("q_tiles", C.c_void_p), ("k_tiles", C.c_void_p),
                 ("n_q_tiles", C.c_int32), ("n_k_tiles", C.c_int32), ("type", C.c_int32), ("batch", C.c_int32), ("heads", C.c_int32),
                 ("kv_heads", C.c_int32), ("head_dim", C.c_int32), ("q_len", C.c_int32), ("k_len", C.c_int32), ("causal", C.c_int32),
                 ("lse_rows", C.c_int64), ("k_rows", C.c_int64), ("k_row_stride_b", C.c_int64), ("k_row_stride_h", C.c_int64), ("scale", C.c_float)]
@@ -85,7 +85,7 @@ class SeqAttn(C.Structure):
 
 # The two structures above as one struct.pack each: a call per microsecond matters for single tokens, and ctypes takes one per field.
 SEQ_ROTARY_BYTES = struct.Struct("<21q9i4x")
-SEQ_ATTN_BYTES = struct.Struct("<40q10i4qf4x")
+SEQ_ATTN_BYTES = struct.Struct("<39q10i4qf4x")
 assert SEQ_ROTARY_BYTES.size == C.sizeof(SeqRotary) and SEQ_ATTN_BYTES.size == C.sizeof(SeqAttn)
 
 

@@ -13,7 +13,7 @@
 // One source for the three element types: Mma<T> hides the instruction (32x32x16 for 16 bits; for fp32 four 32x32x2, which multiply
 // exact fp32) and the operand layouts.  P and dS are rounded to the element type for the second product, as any 16-bit matrix operand
 // is; sums and statistics stay fp32.  fp16 has only 2^-14 as its smallest full-precision number: P is carried as 2^15 P and dS under a running power of
-// two per column (scale_col), both undone in fp32 at the end.
+// two per column (shrink_col), both undone in fp32 at the end.
 #pragma once
 #include "common.h"
 
@@ -109,8 +109,7 @@ struct Params {
     long long lse_b, lse_h, krow_b, krow_h;        // row numbers of q (as in lse) and of k
     const unsigned char* key_mask;
     long long mask_b;
-    const int* seqs;
-    const int* tiles;                              // [..][2] = (sequence, block) or null (dense)
+    const int* tiles;                              // [..][8] = (sequence, block, first query, queries, first key, keys, ..) or null (dense)
     float *lse2, *ndelta;                          // backward: lse in powers of two (+inf: a row that sees nothing) and -D, numbered like lse
     float *part, *part_ml;                         // splits: partial sums [split][row][D] and per-row scalars (layout at each kernel)
     long long part_rows;
@@ -118,29 +117,21 @@ struct Params {
     float scale;
 };
 
-struct Seq { long long q0, k0; int ql, kl; };
-
-__device__ __forceinline__ Seq sequence(const Params& p, int b) {
-    Seq s;
-    if (p.seqs) { s.q0 = p.seqs[4 * b]; s.ql = p.seqs[4 * b + 1]; s.k0 = p.seqs[4 * b + 2]; s.kl = p.seqs[4 * b + 3]; }
-    else { s.q0 = 0; s.ql = p.q_len; s.k0 = 0; s.kl = p.k_len; }
-    return s;
-}
-
 // Which block of which (sequence, key head) a workgroup has.  Workgroups go round the 8 XCDs, each with its own L2: the blocks of one
 // (sequence, key head), which read the same keys and values, stay on one XCD where the pairs divide evenly; the blocks with most work
 // (under a causal mask the last queries', the first keys') come first.  A query block is `subs` sub-blocks of QB rows (rows = tokens x heads of the group).
-struct Where { int b, tile, kvh, sub, split; };
+struct Where { int b, tile, kvh, sub, split, ql, kl; long long q0, k0; };
 __device__ __forceinline__ Where where(const Params& p, bool last_first) {
     Where w;
     int id = blockIdx.x;
+    w.ql = p.q_len; w.kl = p.k_len; w.q0 = w.k0 = 0;
     if (p.tiles) {
         w.split = id % p.splits; id /= p.splits;
         w.sub = id % p.subs; id /= p.subs;
         w.kvh = id % p.kv_heads;
         id /= p.kv_heads;
-        w.b = p.tiles[2 * id];
-        w.tile = p.tiles[2 * id + 1];
+        const int* e = p.tiles + 8 * id;
+        w.b = e[0]; w.tile = e[1]; w.q0 = e[2]; w.ql = e[3]; w.k0 = e[4]; w.kl = e[5];
         return w;
     }
     const int per = p.tiles_per_seq * p.subs * p.splits, pairs = p.n_tiles / p.tiles_per_seq * p.kv_heads;
@@ -257,34 +248,28 @@ __device__ __forceinline__ float other_half(float v) {               // the valu
     return __uint_as_float(threadIdx.x & 32 ? r[0] : r[1]);
 }
 
-// fp16 only: keep |t| * sc inside fp16 by a power of two per column; when it has to shrink, the column's sum follows.
-template <int N> __device__ __forceinline__ void scale_col(f32x16& t, float& sc, f32x16 (&acc)[N]) {
+// fp16 only: t carries a power of two per column; where it outgrows fp16 (2^15), t and the column's sum shrink by the power of two returned.
+template <int N> __device__ __forceinline__ float shrink_col(f32x16& t, f32x16 (&acc)[N]) {
     float m = 0.f;
 #pragma unroll
     for (int r = 0; r < 16; ++r) m = fmaxf(m, fabsf(t[r]));
     m = fmaxf(m, other_half(m));
-    if (__any(m * sc > 32768.f)) {
-        float ns = sc;
-        if (m * sc > 32768.f) ns = ldexpf(1.f, 14 - min(ilogbf(m), 127));
-        times(acc, ns / sc);
-        sc = ns;
-    }
+    if (!__any(m > 32768.f)) return 1.f;
+    const float by = m > 32768.f ? ldexpf(1.f, 14 - min(ilogbf(m), 127)) : 1.f;
+    times(acc, by);
 #pragma unroll
-    for (int r = 0; r < 16; ++r) t[r] *= sc;
+    for (int r = 0; r < 16; ++r) t[r] *= by;
+    return by;
 }
 
 template <class T> __device__ __forceinline__ constexpr bool is_f16() { return __is_same(T, _Float16); }
-template <class T, int DP> constexpr int WAVES = sizeof(T) == 2 || DP <= 64 ? 2 : 1;       // workgroups of a CU that the registers have to allow
-#ifndef DKVW
-#define DKVW 2
-#endif
-#ifndef LV
-#define LV 1
-#endif
+// Workgroups of a CU that the registers have to allow.  Rows of at most 128 bytes: three (packed fp16, D 64: forward 119 -> 99 us, dQ 181 -> 157
+// against two; four spill), but for dK/dV, whose two sums would spill (211 us at two, 222 at three).
+template <class T, int DP> constexpr int WAVES = DP * sizeof(T) <= 128 ? 3 : sizeof(T) == 2 || DP <= 64 ? 2 : 1;
+template <class T, int DP> constexpr int DKV_WAVES = WAVES<T, DP> < 2 ? 1 : 2;
 // dK/dV at head size 128: the two sums alone take 128 registers; the values' fragments wait in LDS (V_LDS) and the staged tile has 32 rows
-template <class T, int DP> constexpr bool V_LDS = LV && DP == 128;
+template <class T, int DP> constexpr bool V_LDS = DP == 128;
 template <class T, int DP> constexpr int RB = V_LDS<T, DP> ? 32 : 64;
-template <class T, int DP> constexpr int DKV_WAVES = DP == 128 && sizeof(T) == 2 ? DKVW : WAVES<T, DP>;
 
 // The keys of a tile that take part, one tile ahead: without a key mask by the sequence's end, with one by a byte a lane
 struct KeyBits {
@@ -303,24 +288,23 @@ __global__ __launch_bounds__(256, (WAVES<T, DP>)) void fwd_kernel(const Params p
     extern __shared__ __attribute__((aligned(16))) char smem[];       // [2][K, V]
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, l31 = lane & 31, h = lane >> 5;
     const Where w = where(p, true);
-    const Seq s = sequence(p, w.b);
-    const int rows = s.ql * p.group, r0 = w.tile * QB * p.group + w.sub * QB;       // (tokens < 2^31 / 128 a sequence is far beyond memory x heads)
+    const int rows = w.ql * p.group, r0 = w.tile * QB * p.group + w.sub * QB;       // (tokens < 2^31 / 128 a sequence is far beyond memory x heads)
     if (r0 >= min(rows, (w.tile + 1) * QB * p.group)) return;
-    const int off = s.kl - s.ql, rw = r0 + wave * 32, r = rw + l31;   // this wave's first row, this lane's
+    const int off = w.kl - w.ql, rw = r0 + wave * 32, r = rw + l31;   // this wave's first row, this lane's
     const bool rok = r < rows;
     const int token = (rok ? r : r0) / p.group, head = w.kvh * p.group + (rok ? r : r0) % p.group;
     const int t_first = rw / p.group, t_last = (rw + 31) / p.group;   // this wave's tokens
-    int kend = p.causal ? min(s.kl, min((r0 + QB - 1) / p.group, s.ql - 1) + 1 + off) : s.kl, kbegin = 0;
+    int kend = p.causal ? min(w.kl, min((r0 + QB - 1) / p.group, w.ql - 1) + 1 + off) : w.kl, kbegin = 0;
     if (p.splits > 1) {                                              // whole tiles, at least four
         const int per = max(4, (max(kend, 0) + KB * p.splits - 1) / (KB * p.splits)) * KB;
         kbegin = w.split * per;
         kend = min(kend, kbegin + per);
     }
-    const char* const kbase = p.k.p + w.b * p.k.b + s.k0 * p.k.t + w.kvh * p.k.h;
-    const char* const vbase = p.v.p + w.b * p.v.b + s.k0 * p.v.t + w.kvh * p.v.h;
-    KeyBits kb{p.key_mask ? p.key_mask + w.b * p.mask_b + s.k0 : nullptr, s.kl, lane, 0};
+    const char* const kbase = p.k.p + w.b * p.k.b + w.k0 * p.k.t + w.kvh * p.k.h;
+    const char* const vbase = p.v.p + w.b * p.v.b + w.k0 * p.v.t + w.kvh * p.v.h;
+    KeyBits kb{p.key_mask ? p.key_mask + w.b * p.mask_b + w.k0 : nullptr, w.kl, lane, 0};
     typename M::Frag qf[NF];
-    load_row<T, DP>(qf, p.q.p + w.b * p.q.b + (s.q0 + token) * p.q.t + head * p.q.h, h, p.D, rok);
+    load_row<T, DP>(qf, p.q.p + w.b * p.q.b + (w.q0 + token) * p.q.t + head * p.q.h, h, p.D, rok);
     f32x16 o[ND];
     clear(o);
     // Exponents in powers of two.  The running maximum m is only raised when a score exceeds it by 2^8, so the sums are rarely rescaled;
@@ -343,7 +327,7 @@ __global__ __launch_bounds__(256, (WAVES<T, DP>)) void fwd_kernel(const Params p
         copies_done();
         __syncthreads();                                             // this tile is there, and everyone is done with the other buffer
         if (kt + KB < kend) issue(kt + KB, buf ^ 1);
-        if (rw >= rows || (p.causal && kt > t_last + off)) continue;
+        if (rw >= rows || bits == 0 || (p.causal && kt > t_last + off)) continue;
         const char* const img_k = smem + buf * 2 * IMG;
         const char* const img_v = img_k + IMG;
         f32x16 st[2];
@@ -393,7 +377,7 @@ __global__ __launch_bounds__(256, (WAVES<T, DP>)) void fwd_kernel(const Params p
     }
     l += other_half(l);
     if (!rok) return;
-    const long long at = w.b * p.lse_b + head * p.lse_h + s.q0 + token;
+    const long long at = w.b * p.lse_b + head * p.lse_h + w.q0 + token;
     if (p.splits > 1) {                                              // part: sums, part_ml [split][row][2]: maximum and sum
         store_row<T, DP, f32x4>(o, reinterpret_cast<char*>(p.part + (w.split * p.part_rows + at) * p.D), h, p.D, 1.f);
         if (h == 0) {
@@ -403,53 +387,84 @@ __global__ __launch_bounds__(256, (WAVES<T, DP>)) void fwd_kernel(const Params p
         }
         return;
     }
-    store_row<T, DP>(o, p.out.p + w.b * p.out.b + (s.q0 + token) * p.out.t + head * p.out.h, h, p.D, l == 0.f ? 0.f : 1.f / l);
+    store_row<T, DP>(o, p.out.p + w.b * p.out.b + (w.q0 + token) * p.out.t + head * p.out.h, h, p.D, l == 0.f ? 0.f : 1.f / l);
     if (h == 0) p.lse[at] = l == 0.f ? -INFINITY : (m - lift + __builtin_amdgcn_logf(l)) * LN2;
 }
 
-// The blocks of 16 rows that join the splits: 16 lanes a row, 8 elements a lane.
+// Joining the splits: a workgroup has 4 rows, a wave one: lane = 16 slices of 8 columns x 4 slices of the splits, whose loads are in flight together.
+constexpr int JOIN = 4;
 template <class F> __device__ __forceinline__ void join_rows(const Params& p, F f) {
     Params one = p;
-    one.splits = QB / 16;                                            // (the same block numbering, 16 rows each)
+    one.splits = QB / JOIN;                                          // (the same block numbering, JOIN rows each)
     const Where w = where(one, true);
-    const Seq s = sequence(p, w.b);
-    const int rows = s.ql * p.group, r = w.tile * QB * p.group + w.sub * QB + w.split * 16 + (threadIdx.x >> 4);
+    const int rows = w.ql * p.group, r = w.tile * QB * p.group + w.sub * QB + w.split * JOIN + (threadIdx.x >> 6);
     if (r >= min(rows, (w.tile + 1) * QB * p.group)) return;
     const int token = r / p.group, head = w.kvh * p.group + r % p.group;
-    f(w, s, token, head, w.b * p.lse_b + head * p.lse_h + s.q0 + token, (int)(threadIdx.x & 15) * 8);
+    f(w, token, head, w.b * p.lse_b + head * p.lse_h + w.q0 + token);
 }
-
+__device__ __forceinline__ void load8(const float* row, int d, int D, float (&v)[8]) {
+#pragma unroll
+    for (int e = 0; e < 8; e += 4) {
+        const f32x4 x = d < D ? *reinterpret_cast<const f32x4*>(row + d + e) : f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int i = 0; i < 4; ++i) v[e + i] = x[i];
+    }
+}
 template <class T> __device__ __forceinline__ void store8(char* row, int d, const float (&v)[8]) {
 #pragma unroll
     for (int e = 0; e < 8; e += 4)
         *reinterpret_cast<typename Mma<T>::Quad*>(row + (d + e) * (int)sizeof(T)) = __builtin_convertvector((f32x4{v[e], v[e + 1], v[e + 2], v[e + 3]}), typename Mma<T>::Quad);
 }
+// Sum over i of row i of part (rows `stride` apart), in a fixed order: v in the first 16 lanes
+__device__ __forceinline__ void sum_splits(const float* part, long long stride, int n, int D, float (&v)[8]) {
+    const int lane = threadIdx.x & 63, d = (lane & 15) * 8;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) v[e] = 0.f;
+#pragma unroll 4
+    for (int i = lane >> 4; i < n; i += 4) {
+        float x[8];
+        load8(part + i * stride, d, D, x);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) v[e] += x[e];
+    }
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+        v[e] += __shfl_xor(v[e], 16, 64);
+        v[e] += __shfl_xor(v[e], 32, 64);
+    }
+}
 
 template <class T>
 __global__ __launch_bounds__(256) void fwd_join_kernel(const Params p) {
-    join_rows(p, [&](const Where& w, const Seq& s, int token, int head, long long at, int d) {
+    join_rows(p, [&](const Where& w, int token, int head, long long at) {
+        const int lane = threadIdx.x & 63, d = (lane & 15) * 8;
+        // the largest maximum (splits that saw nothing have -inf and sum 0; a NaN sum counts whatever its maximum: it has to come out)
         float m = -INFINITY;
-        for (int i = 0; i < p.splits; ++i) {
-            const float* ml = p.part_ml + 2 * (i * p.part_rows + at);
-            if (ml[1] != 0.f) m = fmaxf(m, ml[0]);                   // (NaN sums count: they have to come out)
-        }
-        float l = 0.f, v[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
-        for (int i = 0; i < p.splits; ++i) {
-            const float* ml = p.part_ml + 2 * (i * p.part_rows + at);
-            if (ml[1] == 0.f) continue;
-            const float a = __builtin_amdgcn_exp2f(ml[0] - m);
-            l += ml[1] * a;
-            if (d < p.D) {
-                const f32x4* x = reinterpret_cast<const f32x4*>(p.part + (i * p.part_rows + at) * p.D + d);
+        for (int i = lane; i < p.splits; i += 64) m = fmaxf(m, p.part_ml[2 * (i * p.part_rows + at)]);
 #pragma unroll
-                for (int e = 0; e < 8; ++e) v[e] += x[e / 4][e % 4] * a;
-            }
+        for (int x = 32; x; x >>= 1) m = fmaxf(m, __shfl_xor(m, x, 64));
+        float l = 0.f, v[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+#pragma unroll 4
+        for (int i = lane >> 4; i < p.splits; i += 4) {
+            const float2 ml = *reinterpret_cast<const float2*>(p.part_ml + 2 * (i * p.part_rows + at));
+            float x[8];
+            load8(p.part + (i * p.part_rows + at) * p.D, d, p.D, x);
+            const float a = ml.y == 0.f ? 0.f : ml.x == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(ml.x - m);
+            l = __builtin_fmaf(ml.y, a, l);
+#pragma unroll
+            for (int e = 0; e < 8; ++e) v[e] = __builtin_fmaf(x[e], a, v[e]);
+        }
+#pragma unroll
+        for (int x = 16; x <= 32; x += 16) {
+            l += __shfl_xor(l, x, 64);
+#pragma unroll
+            for (int e = 0; e < 8; ++e) v[e] += __shfl_xor(v[e], x, 64);
         }
         const float inv = l == 0.f ? 0.f : 1.f / l;
 #pragma unroll
         for (int e = 0; e < 8; ++e) v[e] *= inv;
-        if (d < p.D) store8<T>(p.out.p + w.b * p.out.b + (s.q0 + token) * p.out.t + head * p.out.h, d, v);
-        if (d == 0) p.lse[at] = l == 0.f ? -INFINITY : (m + __builtin_amdgcn_logf(l)) * LN2;
+        if (lane < 16 && d < p.D) store8<T>(p.out.p + w.b * p.out.b + (w.q0 + token) * p.out.t + head * p.out.h, d, v);
+        if (lane == 0) p.lse[at] = l == 0.f ? -INFINITY : (m + __builtin_amdgcn_logf(l)) * LN2;
     });
 }
 
@@ -464,33 +479,36 @@ __global__ __launch_bounds__(256, (WAVES<T, DP>)) void dq_kernel(const Params p)
     extern __shared__ __attribute__((aligned(16))) char smem[];       // [2][K, V]
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, l31 = lane & 31, h = lane >> 5;
     const Where w = where(p, true);
-    const Seq s = sequence(p, w.b);
-    const int rows = s.ql * p.group, r0 = w.tile * QB * p.group + w.sub * QB;
+    const int rows = w.ql * p.group, r0 = w.tile * QB * p.group + w.sub * QB;
     if (r0 >= min(rows, (w.tile + 1) * QB * p.group)) return;
-    const int off = s.kl - s.ql, rw = r0 + wave * 32, r = rw + l31;
+    const int off = w.kl - w.ql, rw = r0 + wave * 32, r = rw + l31;
     const bool rok = r < rows;
     const int token = (rok ? r : r0) / p.group, head = w.kvh * p.group + (rok ? r : r0) % p.group;
     const int t_first = rw / p.group, t_last = (rw + 31) / p.group;
-    int kend = p.causal ? min(s.kl, min((r0 + QB - 1) / p.group, s.ql - 1) + 1 + off) : s.kl, kbegin = 0;
+    int kend = p.causal ? min(w.kl, min((r0 + QB - 1) / p.group, w.ql - 1) + 1 + off) : w.kl, kbegin = 0;
     if (p.splits > 1) {
         const int per = max(4, (max(kend, 0) + KB * p.splits - 1) / (KB * p.splits)) * KB;
         kbegin = w.split * per;
         kend = min(kend, kbegin + per);
     }
-    const char* const kbase = p.k.p + w.b * p.k.b + s.k0 * p.k.t + w.kvh * p.k.h;
-    const char* const vbase = p.v.p + w.b * p.v.b + s.k0 * p.v.t + w.kvh * p.v.h;
-    KeyBits kb{p.key_mask ? p.key_mask + w.b * p.mask_b + s.k0 : nullptr, s.kl, lane, 0};
-    const long long at = w.b * p.lse_b + head * p.lse_h + s.q0 + token;
+    const char* const kbase = p.k.p + w.b * p.k.b + w.k0 * p.k.t + w.kvh * p.k.h;
+    const char* const vbase = p.v.p + w.b * p.v.b + w.k0 * p.v.t + w.kvh * p.v.h;
+    KeyBits kb{p.key_mask ? p.key_mask + w.b * p.mask_b + w.k0 : nullptr, w.kl, lane, 0};
+    const long long at = w.b * p.lse_b + head * p.lse_h + w.q0 + token;
     const float lse = rok ? p.lse[at] : -INFINITY;
     const bool sees = lse != -INFINITY;                              // (a row that sees nothing takes no part, whatever it holds)
     const float lse2 = sees ? lse * LOG2E : INFINITY;
     typename M::Frag qf[NF], gf[NF];
-    load_row<T, DP>(qf, p.q.p + w.b * p.q.b + (s.q0 + token) * p.q.t + head * p.q.h, h, p.D, sees);
-    load_row<T, DP>(gf, p.dout.p + w.b * p.dout.b + (s.q0 + token) * p.dout.t + head * p.dout.h, h, p.D, sees);
-    float nd = 0.f, rho = 0.f;                                       // -D, what D still misses
+    load_row<T, DP>(qf, p.q.p + w.b * p.q.b + (w.q0 + token) * p.q.t + head * p.q.h, h, p.D, rok);
+    load_row<T, DP>(gf, p.dout.p + w.b * p.dout.b + (w.q0 + token) * p.dout.t + head * p.dout.h, h, p.D, rok);
+    float nd = 0.f, rho = 0.f;                                       // -D, what D still misses (times sc)
     {
         typename M::Frag of[NF];
-        load_row<T, DP>(of, p.out.p + w.b * p.out.b + (s.q0 + token) * p.out.t + head * p.out.h, h, p.D, sees);
+        load_row<T, DP>(of, p.out.p + w.b * p.out.b + (w.q0 + token) * p.out.t + head * p.out.h, h, p.D, rok);
+        if (!sees) {
+#pragma unroll
+            for (int f = 0; f < NF; ++f) qf[f] = gf[f] = of[f] = typename M::Frag{};
+        }
 #pragma unroll
         for (int f = 0; f < NF; ++f)
 #pragma unroll
@@ -500,7 +518,7 @@ __global__ __launch_bounds__(256, (WAVES<T, DP>)) void dq_kernel(const Params p)
     f32x16 acc[ND];
     clear(acc);
     const float c = p.scale * LOG2E;
-    float sc = is_f16<T>() ? 0x1p100f : 1.f;
+    float sc = is_f16<T>() ? 0x1p60f : 1.f, shift = lse2 - (is_f16<T>() ? 60.f : 0.f);      // (fp16: the exponent brings the column's power of two along)
     unsigned long long cur = 0;
     const Stage<T, DP> sk(p.k.t, p.D), sv(p.v.t, p.D);
     if (p.D < DP) zero_images(smem, 4 * IMG);
@@ -522,13 +540,13 @@ __global__ __launch_bounds__(256, (WAVES<T, DP>)) void dq_kernel(const Params p)
             issue(key(i + 1), buf ^ 1);
             if (i + 2 < first + tiles) kb.fetch(key(i + 2));
         }
-        if (FIX && i == first && first) { nd -= rho + other_half(rho); rho = 0.f; }
-        if (rw >= rows || (p.causal && kt > t_last + off)) continue;
+        if (FIX && i == first && first) { nd -= (rho + other_half(rho)) / sc; rho = 0.f; }
+        if (rw >= rows || bits == 0 || (p.causal && kt > t_last + off)) continue;
         const char* const img_k = smem + buf * 2 * IMG;
         const char* const img_v = img_k + IMG;
         const bool partial = bits != ~0ull || (p.causal && kt + KB - 1 > t_first + off);
         const int last = p.causal ? token + off - kt : KB;
-#pragma unroll
+#pragma unroll 1
         for (int sub = 0; sub < 2; ++sub) {
             f32x16 st, dp;
 #pragma unroll
@@ -539,7 +557,7 @@ __global__ __launch_bounds__(256, (WAVES<T, DP>)) void dq_kernel(const Params p)
                 dp = M::mma(M::template row<DP>(img_v, sub * 32 + l31, f, h), gf[f], dp);
             }
 #pragma unroll
-            for (int x = 0; x < 16; ++x) st[x] = __builtin_amdgcn_exp2f(__builtin_fmaf(st[x], c, -lse2)) * dp[x];
+            for (int x = 0; x < 16; ++x) st[x] = __builtin_amdgcn_exp2f(__builtin_fmaf(st[x], c, -shift)) * dp[x];
             if (partial) {
 #pragma unroll
                 for (int x = 0; x < 16; ++x) {
@@ -554,7 +572,10 @@ __global__ __launch_bounds__(256, (WAVES<T, DP>)) void dq_kernel(const Params p)
                 rho += a;
                 if (i < first) continue;
             }
-            if (is_f16<T>()) scale_col(st, sc, acc);
+            if (is_f16<T>()) {
+                const float by = shrink_col(st, acc);
+                if (by != 1.f) { sc *= by; rho *= by; shift = lse2 - __builtin_amdgcn_logf(sc); }
+            }
 #pragma unroll
             for (int f = 0; f < NP; ++f) {
                 const typename M::Frag df = M::from_acc(st, f);
@@ -563,7 +584,7 @@ __global__ __launch_bounds__(256, (WAVES<T, DP>)) void dq_kernel(const Params p)
             }
         }
     }
-    rho += other_half(rho);
+    rho = (rho + other_half(rho)) / sc;
     if (!rok) return;
     const float un = p.scale / sc;
     if (p.splits > 1) {                                              // part: sums, part_ml [split][row]: rho
@@ -572,24 +593,21 @@ __global__ __launch_bounds__(256, (WAVES<T, DP>)) void dq_kernel(const Params p)
         if (h == 0 && w.split == 0) { p.lse2[at] = lse2; p.ndelta[at] = nd; }
         return;
     }
-    store_row<T, DP>(acc, p.dq.p + w.b * p.dq.b + (s.q0 + token) * p.dq.t + head * p.dq.h, h, p.D, un);
+    store_row<T, DP>(acc, p.dq.p + w.b * p.dq.b + (w.q0 + token) * p.dq.t + head * p.dq.h, h, p.D, un);
     if (h == 0) { p.lse2[at] = lse2; p.ndelta[at] = nd - rho; }
 }
 
 template <class T>
 __global__ __launch_bounds__(256) void dq_join_kernel(const Params p) {
-    join_rows(p, [&](const Where& w, const Seq& s, int token, int head, long long at, int d) {
-        float v[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f}, rho = 0.f;
-        for (int i = 0; i < p.splits; ++i) {
-            rho += p.part_ml[i * p.part_rows + at];
-            if (d < p.D) {
-                const f32x4* x = reinterpret_cast<const f32x4*>(p.part + (i * p.part_rows + at) * p.D + d);
+    join_rows(p, [&](const Where& w, int token, int head, long long at) {
+        const int lane = threadIdx.x & 63, d = (lane & 15) * 8;
+        float v[8], rho = 0.f;
+        for (int i = lane; i < p.splits; i += 64) rho += p.part_ml[i * p.part_rows + at];
 #pragma unroll
-                for (int e = 0; e < 8; ++e) v[e] += x[e / 4][e % 4];
-            }
-        }
-        if (d < p.D) store8<T>(p.dq.p + w.b * p.dq.b + (s.q0 + token) * p.dq.t + head * p.dq.h, d, v);
-        if (d == 0) p.ndelta[at] -= rho;
+        for (int x = 32; x; x >>= 1) rho += __shfl_xor(rho, x, 64);
+        sum_splits(p.part + at * p.D, p.part_rows * p.D, p.splits, p.D, v);
+        if (lane < 16 && d < p.D) store8<T>(p.dq.p + w.b * p.dq.b + (w.q0 + token) * p.dq.t + head * p.dq.h, d, v);
+        if (lane == 0) p.ndelta[at] -= rho;
     });
 }
 
@@ -602,12 +620,11 @@ __global__ __launch_bounds__(256, (DKV_WAVES<T, DP>)) void dkv_kernel(const Para
     float* const s_row = reinterpret_cast<float*>(smem + 4 * IMG);
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, l31 = lane & 31, h = lane >> 5;
     const Where w = where(p, false);
-    const Seq s = sequence(p, w.b);
-    if (w.tile * QB >= s.kl) return;
-    const int off = s.kl - s.ql;
+    if (w.tile * QB >= w.kl) return;
+    const int off = w.kl - w.ql;
     const int kw = w.tile * QB + wave * 32, kj = kw + l31;           // this wave's first key, this lane's
-    const bool in = kj < s.kl;
-    const long long row = s.k0 + (in ? kj : 0);
+    const bool in = kj < w.kl;
+    const long long row = w.k0 + (in ? kj : 0);
     const bool live = in && (!p.key_mask || p.key_mask[w.b * p.mask_b + row]);
     typename M::Frag kf[NF], vf[NF];
     load_row<T, DP>(kf, p.k.p + w.b * p.k.b + row * p.k.t + w.kvh * p.k.h, h, p.D, live);
@@ -621,9 +638,9 @@ __global__ __launch_bounds__(256, (DKV_WAVES<T, DP>)) void dkv_kernel(const Para
     clear(dk);
     clear(dv);
     const float c = p.scale * LOG2E, lift = is_f16<T>() ? 15.f : 0.f;
-    float sc = is_f16<T>() ? 0x1p100f : 1.f;
+    float sc = is_f16<T>() ? 0x1p45f : 1.f;                          // (with the 2^15 of P: 2^60 in all)
     const int qbegin = p.causal ? max(0, w.tile * QB - off) : 0;                 // first query that sees the first key
-    const int per_head = qbegin < s.ql ? (s.ql - qbegin + R - 1) / R : 0;
+    const int per_head = qbegin < w.ql ? (w.ql - qbegin + R - 1) / R : 0;
     int step = 0, steps = per_head * p.group;
     if (p.splits > 1) {
         const int per = (steps + p.splits - 1) / p.splits;
@@ -633,21 +650,21 @@ __global__ __launch_bounds__(256, (DKV_WAVES<T, DP>)) void dkv_kernel(const Para
     // The walk: tiles of R queries, head after head.
     struct At { int head, qt; } next{w.kvh * p.group, qbegin};
     if (step < steps) { next.head += step / per_head; next.qt += step % per_head * R; }
-    auto advance = [&](At a) { return a.qt + R < s.ql ? At{a.head, a.qt + R} : At{a.head + 1, qbegin}; };
+    auto advance = [&](At a) { return a.qt + R < w.ql ? At{a.head, a.qt + R} : At{a.head + 1, qbegin}; };
     const Stage<T, DP, R> sq(p.q.t, p.D), sg(p.dout.t, p.D);
-    const char* const qbase = p.q.p + w.b * p.q.b + s.q0 * p.q.t;
-    const char* const gbase = p.dout.p + w.b * p.dout.b + s.q0 * p.dout.t;
-    const long long first_row = w.b * p.lse_b + s.q0;
+    const char* const qbase = p.q.p + w.b * p.q.b + w.q0 * p.q.t;
+    const char* const gbase = p.dout.p + w.b * p.dout.b + w.q0 * p.dout.t;
+    const long long first_row = w.b * p.lse_b + w.q0;
     if (p.D < DP) zero_images(smem, 4 * IMG);
     // Rows that see nothing are not read (their lse2 is +inf).  Under a causal mask alone they lie before qbegin; a key mask can leave any
     // row empty, so its lse2 is looked at first, a tile ahead.
     float ahead = 0.f;
     auto fetch = [&](At a) {
-        if (p.key_mask) ahead = a.qt + lane < s.ql ? p.lse2[first_row + a.head * p.lse_h + a.qt + lane] : INFINITY;
+        if (p.key_mask) ahead = a.qt + lane < w.ql ? p.lse2[first_row + a.head * p.lse_h + a.qt + lane] : INFINITY;
     };
     auto issue = [&](At a, int buf) {
         const long long at = first_row + a.head * p.lse_h + a.qt + lane;
-        const unsigned long long bits = p.key_mask ? __ballot(ahead != INFINITY) : first_bits(s.ql - a.qt);
+        const unsigned long long bits = p.key_mask ? __ballot(ahead != INFINITY) : first_bits(w.ql - a.qt);
         sq.issue(smem + buf * 2 * IMG, qbase + a.qt * p.q.t + a.head * p.q.h, bits);
         sg.issue(smem + buf * 2 * IMG + IMG, gbase + a.qt * p.dout.t + a.head * p.dout.h, bits);
         const bool there = (bits >> lane) & 1;                       // (R = 32: the upper half is never read)
@@ -671,11 +688,11 @@ __global__ __launch_bounds__(256, (DKV_WAVES<T, DP>)) void dkv_kernel(const Para
             next = advance(next);
             if (step + 2 < steps) fetch(next);
         }
-        if (kw >= s.kl || (p.causal && qt + R - 1 < kw - off)) continue;
+        if (kw >= w.kl || (p.causal && qt + R - 1 < kw - off)) continue;
         const char* const img_q = smem + buf * 2 * IMG;
         const char* const img_g = img_q + IMG;
         const bool partial = p.causal && kw + 31 - off > qt;
-#pragma unroll
+#pragma unroll (DP * (int)sizeof(T) <= 128 ? 2 : 1)
         for (int sub = 0; sub < R / 32; ++sub) {
             const float* const sl = s_row + buf * 128 + sub * 32 + 4 * h;
             f32x16 st, dp;
@@ -702,7 +719,11 @@ __global__ __launch_bounds__(256, (DKV_WAVES<T, DP>)) void dkv_kernel(const Para
                     dp[x] *= pr;
                 }
             }
-            if (is_f16<T>()) scale_col(dp, sc, dk);
+            if (is_f16<T>()) {
+#pragma unroll
+                for (int x = 0; x < 16; ++x) dp[x] *= sc;
+                sc *= shrink_col(dp, dk);
+            }
 #pragma unroll
             for (int f = 0; f < NP; ++f) {
                 const typename M::Frag pf = M::from_acc(st, f), df = M::from_acc(dp, f);
@@ -730,22 +751,17 @@ __global__ __launch_bounds__(256, (DKV_WAVES<T, DP>)) void dkv_kernel(const Para
 template <class T>
 __global__ __launch_bounds__(256) void dkv_join_kernel(const Params p) {
     Params one = p;
-    one.splits = QB / 16;
+    one.splits = QB / JOIN;
     const Where w = where(one, false);
-    const Seq s = sequence(p, w.b);
-    const int j = w.tile * QB + w.split * 16 + (threadIdx.x >> 4), d = (threadIdx.x & 15) * 8;
-    if (j >= s.kl || d >= p.D) return;
-    const long long row = s.k0 + j, at = w.b * p.krow_b + w.kvh * p.krow_h + row;
+    const int j = w.tile * QB + w.split * JOIN + (threadIdx.x >> 6), lane = threadIdx.x & 63, d = (lane & 15) * 8;
+    if (j >= w.kl) return;
+    const long long row = w.k0 + j, at = w.b * p.krow_b + w.kvh * p.krow_h + row;
 #pragma unroll
     for (int which = 0; which < 2; ++which) {
-        float v[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
-        for (int i = 0; i < p.splits; ++i) {
-            const f32x4* x = reinterpret_cast<const f32x4*>(p.part + ((2 * i + which) * p.part_rows + at) * p.D + d);
-#pragma unroll
-            for (int e = 0; e < 8; ++e) v[e] += x[e / 4][e % 4];
-        }
+        float v[8];
+        sum_splits(p.part + (which * p.part_rows + at) * p.D, 2 * p.part_rows * p.D, p.splits, p.D, v);
         const Ten& t = which ? p.dv : p.dk;
-        store8<T>(t.p + w.b * t.b + row * t.t + w.kvh * t.h, d, v);
+        if (lane < 16 && d < p.D) store8<T>(t.p + w.b * t.b + row * t.t + w.kvh * t.h, d, v);
     }
 }
 
@@ -759,7 +775,7 @@ int run_fwd(const Params& p, hipStream_t s) {
     hipLaunchKernelGGL((fwd_kernel<T, DP>), dim3(grid_of(p, p.splits)), dim3(256), lds, s, p);
     DPC_LAUNCH_CHECK();
     if (p.splits > 1) {
-        hipLaunchKernelGGL((fwd_join_kernel<T>), dim3(grid_of(p, QB / 16)), dim3(256), 0, s, p);
+        hipLaunchKernelGGL((fwd_join_kernel<T>), dim3(grid_of(p, QB / JOIN)), dim3(256), 0, s, p);
         DPC_LAUNCH_CHECK();
     }
     return DPC_OK;
@@ -778,7 +794,7 @@ int run_bwd(const Params& pq, const Params& pk, hipStream_t s) {
         hipLaunchKernelGGL((dq_kernel<T, DP>), dim3(grid_of(pq, pq.splits)), dim3(256), lds, s, pq);
         DPC_LAUNCH_CHECK();
         if (pq.splits > 1) {
-            hipLaunchKernelGGL((dq_join_kernel<T>), dim3(grid_of(pq, QB / 16)), dim3(256), 0, s, pq);
+            hipLaunchKernelGGL((dq_join_kernel<T>), dim3(grid_of(pq, QB / JOIN)), dim3(256), 0, s, pq);
             DPC_LAUNCH_CHECK();
         }
     }
@@ -786,7 +802,7 @@ int run_bwd(const Params& pq, const Params& pk, hipStream_t s) {
         hipLaunchKernelGGL((dkv_kernel<T, DP>), dim3(grid_of(pk, pk.splits)), dim3(256), lds_k, s, pk);
         DPC_LAUNCH_CHECK();
         if (pk.splits > 1) {
-            hipLaunchKernelGGL((dkv_join_kernel<T>), dim3(grid_of(pk, QB / 16)), dim3(256), 0, s, pk);
+            hipLaunchKernelGGL((dkv_join_kernel<T>), dim3(grid_of(pk, QB / JOIN)), dim3(256), 0, s, pk);
             DPC_LAUNCH_CHECK();
         }
     }

@@ -21,8 +21,8 @@ static int check(const dpc_seq_attn* a, bool backward) {
     DPC_REQUIRE(a->head_dim >= 8 && a->head_dim <= 128 && a->head_dim % 8 == 0, "seq_attn: head_dim must be a multiple of 8 up to 128");
     DPC_REQUIRE((a->q_len + 2ll * QB) * (a->heads / a->kv_heads) < (1ll << 31) && a->k_len < (1ll << 31) - 2 * QB, "seq_attn: sequence too long");
     DPC_REQUIRE(a->scale > 0.f && std::isfinite(a->scale), "seq_attn: scale must be positive and finite");
-    DPC_REQUIRE(!a->seqs || ((a->q_tiles || !a->n_q_tiles) && (a->k_tiles || !a->n_k_tiles) && a->n_q_tiles >= 0 && a->n_k_tiles >= 0),
-                "seq_attn: sequences need their block lists");
+    DPC_REQUIRE(!a->q_tiles == !a->k_tiles && a->n_q_tiles >= 0 && a->n_k_tiles >= 0 && (a->q_tiles || a->n_q_tiles + a->n_k_tiles == 0) &&
+                    ((size_t)a->q_tiles | (size_t)a->k_tiles) % 32 == 0, "seq_attn: both block lists, on 32 bytes, or neither");
     if (a->batch == 0) return DPC_OK;
     const int es = a->type == DPC_SEQ_F32 ? 4 : 2;
     const char* msg = "seq_attn: tensors must not be null; bases and strides must be multiples of 16 bytes, token strides below 2^25 bytes";
@@ -45,7 +45,6 @@ static Params params(const dpc_seq_attn* a) {
     p.lse = a->lse; p.lse_b = a->lse_stride_b; p.lse_h = a->lse_stride_h;
     p.krow_b = a->k_row_stride_b; p.krow_h = a->k_row_stride_h;
     p.key_mask = a->key_mask; p.mask_b = a->mask_stride_b;
-    p.seqs = a->seqs;
     p.heads = a->heads; p.kv_heads = a->kv_heads; p.group = a->heads / a->kv_heads; p.D = a->head_dim;
     p.q_len = a->q_len; p.k_len = a->k_len; p.causal = a->causal != 0; p.scale = a->scale;
     return p;
@@ -53,22 +52,23 @@ static Params params(const dpc_seq_attn* a) {
 
 // Blocks and splits.  A CU holds two workgroups, the card 512.  Where the blocks alone do not fill 3/4 of them, the axis that a block walks
 // along (keys; for dK/dV the query rows of the group) is split over as many workgroups as fit, each with at least four tiles to walk;
-// the partial sums are joined in order by a second launch.  dK/dV under a causal mask: the first keys' blocks walk far longer than the last
-// ones', so twice as many workgroups are made and the card evens them out (causal bf16 2 x 4096, 16/4 heads of 128: 561 -> 388 us, the join 14 -> 24).
+// the partial sums are joined in order by a second launch.  Under a causal mask over (nearly) square scores the blocks' walks differ by the
+// length of the sequence and the longest one decides while all are resident: twice as many workgroups are made, and the card evens them out (dK/dV of
+// causal bf16 2 x 4096, 16/4 heads of 128: 561 -> 388 us, the join 14 -> 24).
 // Returns false when the grid would pass 2^31.
 constexpr int SLOTS = 512;
 static bool plan_grid(Params& p, const dpc_seq_attn* a, bool keys) {
-    p.tiles = a->seqs ? (keys ? a->k_tiles : a->q_tiles) : nullptr;
+    p.tiles = keys ? a->k_tiles : a->q_tiles;
     p.tiles_per_seq = cdiv(keys ? a->k_len : a->q_len, QB);
-    const long long n = a->seqs ? (keys ? a->n_k_tiles : a->n_q_tiles) : (long long)a->batch * p.tiles_per_seq;
+    const long long n = p.tiles ? (keys ? a->n_k_tiles : a->n_q_tiles) : (long long)a->batch * p.tiles_per_seq;
     p.subs = keys ? 1 : cdiv((long long)std::min(a->q_len, QB) * p.group, QB);
     const long long blocks = n * p.kv_heads * p.subs;
     const long long walk = keys ? (long long)p.group * cdiv(a->q_len, KB) : cdiv(a->k_len, KB);
-    const int slots = keys && p.causal && 2ll * a->q_len > a->k_len ? 2 * SLOTS : SLOTS;
+    const int slots = p.causal && 2ll * a->q_len > a->k_len ? 2 * SLOTS : SLOTS;
     p.splits = blocks == 0 || blocks >= slots * 3 / 4 ? 1 : (int)std::max<long long>(1, std::min<long long>(slots / blocks, walk / 4));
     p.n_tiles = (int)n;
     p.part_rows = keys ? a->k_rows : a->lse_rows;
-    return n < (1ll << 31) && blocks * std::max(p.splits, QB / 16) < (1ll << 31);
+    return n < (1ll << 31) && blocks * std::max(p.splits, QB / JOIN) < (1ll << 31);
 }
 
 static size_t part_bytes(const Params& p, int per_row) {

@@ -382,16 +382,15 @@ class SequencePlan:
         self.k_whole = self.packed_layout or min(kl) == k_max
         rows, q0, k0 = [], 0, 0
         for a, b in zip(ql, kl):
-            rows.append((q0, a, k0, b))
+            rows.append((q0, a, k0, b, 0, 0))
             if self.packed_layout:
                 q0, k0 = q0 + a, k0 + b
-        tiles = [self._tiles(ql, kl), self._tiles(kl, ql)]
-        flat = torch.tensor([v for r in rows for v in r] + [v for t in tiles for e in t for v in e], dtype=torch.int32)
-        self.table = flat.to(device)                                    # (a blocking copy: whole for whatever stream uses it)
+        tiles = [[e + rows[e[0]] for e in self._tiles(*by)] for by in ((ql, kl), (kl, ql))]
+        # (a blocking copy: whole for whatever stream uses it)
+        self.table = torch.tensor(tiles[0] + tiles[1] or [(0,) * 8], dtype=torch.int32).to(device)
         self.stream = _stream(self.table.get_device())
         self.counts = tuple(len(t) for t in tiles)
-        at = self.table.data_ptr()
-        self.pointers = (at, at + 16 * len(rows), at + 16 * len(rows) + 8 * len(tiles[0]))
+        self.pointers = (self.table.data_ptr(), self.table.data_ptr() + 32 * len(tiles[0]))
         self.q_longest, self.k_longest, self.q_total, self.k_total = max(ql), max(kl), sum(ql), sum(kl)
 
     @staticmethod
@@ -432,19 +431,19 @@ def _attention_args(q, k, v, causal, scale, key_mask, plan):
         raise ValueError(f"key_mask: bool of shape {tuple(k.shape[:-2])}")
     d = _device(q, k, v, key_mask, plan and plan.table)
     if plan is None:
-        seqs, sizes, n_seq, q_len, k_len = (0, 0, 0), (0, 0), B, Tq, Tk
+        blocks, sizes, n_seq, q_len, k_len = (0, 0), (0, 0), B, Tq, Tk
     else:
         n_seq, q_len, k_len = len(plan.q_lengths), plan.q_longest, plan.k_longest
         want = ((1, plan.q_total), (1, plan.k_total)) if packed else ((n_seq, plan.q_max), (n_seq, plan.k_max))
         if ((B, Tq), (Bk, Tk)) != want:
             raise ValueError(f"the plan is for q {want[0]} and k {want[1]} (batch, tokens), got {(B, Tq)} and {(Bk, Tk)}")
         _in_use(plan, d)
-        seqs, sizes = plan.pointers, plan.counts
+        blocks, sizes = plan.pointers, plan.counts
     if key_mask is not None:
         key_mask = key_mask.contiguous()
     es = _BYTES[t]
     lse_b, mask_b, krow_b = (0, 0, 0) if packed else (H * Tq, Tk, Hk * Tk)
-    tail = (0 if key_mask is None else key_mask.data_ptr(), mask_b, *seqs, *sizes, _TYPE[t], n_seq, H, Hk, D, q_len, k_len, 1 if causal else 0,
+    tail = (0 if key_mask is None else key_mask.data_ptr(), mask_b, *blocks, *sizes, _TYPE[t], n_seq, H, Hk, D, q_len, k_len, 1 if causal else 0,
             B * H * Tq, B * Hk * Tk, krow_b, Tk, scale)
     return d, _lay(q, es), _lay(k, es), _lay(v, es), ((H, Tq) if packed else (B, H, Tq)), (lse_b, Tq), tail, key_mask
 

@@ -453,9 +453,9 @@ int dpc_seq_rotary_run(const dpc_seq_rotary* a, dpc_stream_t stream);
  * head h / (heads / kv_heads).  Visible: key_mask[j] != 0 (uint8, NULL: all) and, with causal, j <= i + k_len - q_len of the
  * sequence.  A query that sees nothing gives out = 0, lse = -inf and no gradient.  Keys that the mask takes out are never read into a product:
  * they may hold anything.  lse [batch][heads][tokens] = log sum exp S (natural), contiguous in tokens.
- * Dense: every sequence has q_len / k_len tokens, seqs == NULL.  Otherwise seqs [batch][4] = (first query row, queries, first key row,
- * keys), rows counted from the batch's own base (stride_b = 0: packed), q_len / k_len the longest; q_tiles / k_tiles [n][2] =
- * (sequence, block of 128 rows) list every block once, in launch order; rows that no sequence covers are not written.
+ * Dense: every sequence has q_len / k_len tokens, q_tiles == k_tiles == NULL.  Otherwise q_tiles / k_tiles [n][8] list every block of 128
+ * query / key rows once, in launch order, as (sequence, block, first query row, queries, first key row, keys, 0, 0) of the sequence, rows
+ * counted from the batch entry's own base (stride_b = 0: packed); q_len / k_len are the longest.  Rows that no sequence covers are not written.
  * head_dim: a multiple of 8, at most 128.  Tensor bases and strides: multiples of 16 bytes; token
  * strides below 2^25 bytes. */
 typedef struct dpc_seq_attn {
@@ -465,7 +465,7 @@ typedef struct dpc_seq_attn {
     dpc_seq_tensor dout, dq, dk, dv;         /* backward only */
     const uint8_t* key_mask;
     int64_t mask_stride_b;
-    const int32_t *seqs, *q_tiles, *k_tiles;
+    const int32_t *q_tiles, *k_tiles;        /* on 32 bytes */
     int32_t n_q_tiles, n_k_tiles;
     int32_t type, batch, heads, kv_heads, head_dim, q_len, k_len, causal;
     int64_t lse_rows;                        /* rows of lse: batch (packed: 1) * heads * tokens */

@@ -135,7 +135,7 @@ def _attn(**kw):
 @pytest.mark.parametrize("kw", [
     dict(type=3), dict(batch=-1), dict(q_len=-1), dict(heads=3, kv_heads=2), dict(kv_heads=0), dict(head_dim=36), dict(head_dim=0), dict(head_dim=256),
     dict(scale=0.0), dict(scale=float("inf")), dict(q=_lib.SeqTensor(None, 0, 0, 0)), dict(k=_lib.SeqTensor(4100, 256, 64, 32)),
-    dict(v=_lib.SeqTensor(4096, 256, 63, 32)), dict(lse=None), dict(seqs=4096, n_q_tiles=1),
+    dict(v=_lib.SeqTensor(4096, 256, 63, 32)), dict(lse=None), dict(q_tiles=4096, n_q_tiles=1), dict(n_q_tiles=1), dict(q_tiles=4112, k_tiles=4096, n_q_tiles=1),
 ])
 def test_attention_entries_refuse(kw):
     L = _lib.lib()
