@@ -15,6 +15,8 @@
 // is; sums and statistics stay fp32.  fp16 has only 2^-14 as its smallest full-precision number: P is carried as 2^15 P and dS under a running power of
 // two per column (shrink_col), both undone in fp32 at the end.
 #pragma once
+#include <algorithm>
+
 #include "common.h"
 
 namespace dpc {
@@ -113,7 +115,7 @@ struct Params {
     float *lse2, *ndelta;                          // backward: lse in powers of two (+inf: a row that sees nothing) and -D, numbered like lse
     float *part, *part_ml;                         // splits: partial sums [split][row][D] and per-row scalars (layout at each kernel)
     long long part_rows;
-    int heads, kv_heads, group, D, q_len, k_len, causal, n_tiles, tiles_per_seq, subs, splits;
+    int heads, kv_heads, group, D, q_len, k_len, causal, n_tiles, tiles_per_seq, subs, splits, few;
     float scale;
 };
 
@@ -165,36 +167,42 @@ __device__ __forceinline__ unsigned lds_offset(const void* p) {
     return __builtin_amdgcn_readfirstlane((unsigned)(size_t)(__attribute__((address_space(3))) const char*)p);
 }
 
-// ROWS x DP tiles of one tensor, global -> LDS by 256 threads.  The tile's base is the wave's, a lane adds one 32-bit offset (64 rows
-// stay within 2^31 bytes: checked at the entry), so a whole tile costs no address arithmetic.  Rows whose bit is 0 become zero; columns >= D
-// are never written: zero_images() clears them once.
-template <class T, int DP, int ROWS = KB>
+// ROWS x DP tiles of one tensor, global -> LDS by NT threads (a workgroup, or each wave its own).  The tile's base is the wave's, a lane adds one
+// 32-bit offset (64 rows stay within 2^31 bytes: checked at the entry), so a whole tile costs no address arithmetic.  Rows whose bit is 0
+// become zero; columns >= D are never written: zero_images() clears them once.
+template <class T, int DP, int ROWS = KB, int NT = 256>
 struct Stage {
-    static constexpr int CH = Image<T, DP>::CH, N = ROWS * CH / 256, STEP = 256 / CH;
-    static constexpr bool EVEN = 256 % CH == 0 && STEP % 16 == 0;     // round i is round 0, STEP rows further, with the same swizzle
-    static_assert(ROWS * CH % 256 == 0, "whole rounds");
+    static constexpr int CH = Image<T, DP>::CH, N = ROWS * CH / NT, STEP = NT / CH;
+    static constexpr bool EVEN = NT % CH == 0 && STEP % 16 == 0;      // round i is round 0, STEP rows further, with the same swizzle
+    static_assert(ROWS * CH % NT == 0, "whole rounds");
     unsigned off[EVEN ? 1 : N];
     long long st;
     int width;                                                       // bytes of a row
-    __device__ static __forceinline__ int row(int i) { return (threadIdx.x + 256 * i) / CH; }
-    __device__ static __forceinline__ int col(int i) { return (((threadIdx.x + 256 * i) % CH) ^ Image<T, DP>::swz(row(i))) * 16; }
+    __device__ static __forceinline__ int row(int i) { return (threadIdx.x % NT + NT * i) / CH; }
+    __device__ static __forceinline__ int col(int i) { return (((threadIdx.x % NT + NT * i) % CH) ^ Image<T, DP>::swz(row(i))) * 16; }
     __device__ __forceinline__ Stage(long long stride, int D) : st(stride), width(D * (int)sizeof(T)) {
 #pragma unroll
         for (int i = 0; i < (EVEN ? 1 : N); ++i) off[i] = (unsigned)(row(i) * st + col(i));
     }
     __device__ __forceinline__ void issue(char* img, const char* base, unsigned long long bits) const {
-        const unsigned at = lds_offset(img) + __builtin_amdgcn_readfirstlane((threadIdx.x >> 6) * 1024);
+        const unsigned at = lds_offset(img) + __builtin_amdgcn_readfirstlane((threadIdx.x % NT >> 6) * 1024);
         const bool all = ROWS == 64 ? bits == ~0ull : (unsigned)bits == ~0u;
         if (all && width == DP * (int)sizeof(T)) {
 #pragma unroll
-            for (int i = 0; i < N; ++i) copy16(EVEN ? base + i * STEP * st : base, off[EVEN ? 0 : i], at + i * 4096);
+            for (int i = 0; i < N; ++i) copy16(EVEN ? base + i * STEP * st : base, off[EVEN ? 0 : i], at + i * NT * 16);
+            return;
+        }
+        if (all) {
+#pragma unroll
+            for (int i = 0; i < N; ++i)
+                if (col(i) < width) copy16(EVEN ? base + i * STEP * st : base, off[EVEN ? 0 : i], at + i * NT * 16);
             return;
         }
 #pragma unroll
         for (int i = 0; i < N; ++i) {
             const char* src = base + (EVEN ? i * STEP * st : 0) + off[EVEN ? 0 : i];
             if (!((bits >> row(i)) & 1)) src = reinterpret_cast<const char*>(FILL);
-            if (col(i) < width) copy16(src, at + i * 4096);
+            if (col(i) < width) copy16(src, at + i * NT * 16);
         }
     }
 };
@@ -286,7 +294,7 @@ __global__ __launch_bounds__(256, (WAVES<T, DP>)) void fwd_kernel(const Params p
     typedef Mma<T> M;
     constexpr int NF = DP / M::KS, NP = 32 / M::KS, ND = DP / 32, IMG = KB * Image<T, DP>::PITCH;
     extern __shared__ __attribute__((aligned(16))) char smem[];       // [2][K, V]
-    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, l31 = lane & 31, h = lane >> 5;
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), l31 = lane & 31, h = lane >> 5;
     const Where w = where(p, true);
     const int rows = w.ql * p.group, r0 = w.tile * QB * p.group + w.sub * QB;       // (tokens < 2^31 / 128 a sequence is far beyond memory x heads)
     if (r0 >= min(rows, (w.tile + 1) * QB * p.group)) return;
@@ -391,16 +399,155 @@ __global__ __launch_bounds__(256, (WAVES<T, DP>)) void fwd_kernel(const Params p
     if (h == 0) p.lse[at] = l == 0.f ? -INFINITY : (m - lift + __builtin_amdgcn_logf(l)) * LN2;
 }
 
-// Joining the splits: a workgroup has 4 rows, a wave one: lane = 16 slices of 8 columns x 4 slices of the splits, whose loads are in flight together.
-constexpr int JOIN = 4;
-template <class F> __device__ __forceinline__ void join_rows(const Params& p, F f) {
+template <class T> __device__ __forceinline__ void store8(char* row, int d, const float (&v)[8]) {
+#pragma unroll
+    for (int e = 0; e < 8; e += 4)
+        *reinterpret_cast<typename Mma<T>::Quad*>(row + (d + e) * (int)sizeof(T)) = __builtin_convertvector((f32x4{v[e], v[e + 1], v[e + 2], v[e + 3]}), typename Mma<T>::Quad);
+}
+// Few rows (at most 32 of a sequence and key head: single tokens, short drafts): nothing to share, so each of the four waves walks over tiles
+// of 32 keys of its own, copied by itself into its own LDS, without barriers; the waves' sums are joined through LDS at the end.  Bound by the
+// keys' and values' bytes: 64 KB are in flight a CU.
+template <class T, int DP> constexpr bool FEW = Image<T, DP>::PITCH * 32 * 16 <= 128 * 1024;
+template <class T, int DP>
+__global__ __launch_bounds__(256) void few_kernel(const Params p) {
+    typedef Mma<T> M;
+    constexpr int NF = DP / M::KS, NP = 32 / M::KS, ND = DP / 32, IMG = 32 * Image<T, DP>::PITCH, OP = DP + 4;      // OP: floats of a row of sums
+    extern __shared__ __attribute__((aligned(16))) char smem[];       // [wave][2][K, V]; then [wave][32][OP] sums, [wave][32][2] maximum and sum
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), l31 = lane & 31, h = lane >> 5;
+    const Where w = where(p, true);
+    const int rows = w.ql * p.group;                                 // <= 32: block 0 has them all
+    if (w.tile * QB >= w.ql) return;
+    const int off = w.kl - w.ql;
+    const bool rok = l31 < rows;
+    const int token = (rok ? l31 : 0) / p.group, head = w.kvh * p.group + (rok ? l31 : 0) % p.group;
+    const int kend = p.causal ? min(w.kl, w.ql + off) : w.kl;
+    const int per = (max(kend, 0) + 32 * 4 * p.splits - 1) / (32 * 4 * p.splits) * 32 * 4;       // keys of a split: whole rounds of the four waves
+    const int from = w.split * per + wave * 32, to = min(kend, w.split * per + per);
+    char* const mine = smem + wave * 4 * IMG;
+    const char* const kbase = p.k.p + w.b * p.k.b + w.k0 * p.k.t + w.kvh * p.k.h;
+    const char* const vbase = p.v.p + w.b * p.v.b + w.k0 * p.v.t + w.kvh * p.v.h;
+    KeyBits kb{p.key_mask ? p.key_mask + w.b * p.mask_b + w.k0 : nullptr, w.kl, lane, 0};
+    typename M::Frag qf[NF];
+    load_row<T, DP>(qf, p.q.p + w.b * p.q.b + (w.q0 + token) * p.q.t + head * p.q.h, h, p.D, rok);
+    const Stage<T, DP, 32, 64> sk(p.k.t, p.D), sv(p.v.t, p.D);
+    if (p.D < DP) zero_images(smem, 16 * IMG);
+    f32x16 o[ND];
+    clear(o);
+    const float c = p.scale * LOG2E, lift = is_f16<T>() ? 7.f : 0.f;
+    float m = -INFINITY, l = 0.f;
+    unsigned cur = 0;
+    auto issue = [&](int kt, int buf) {
+        cur = (unsigned)kb.bits(kt);
+        sk.issue(mine + buf * 2 * IMG, kbase + kt * p.k.t, cur);
+        sv.issue(mine + buf * 2 * IMG + IMG, vbase + kt * p.v.t, cur);
+        kb.fetch(kt + 128);
+    };
+    if (from < to) { kb.fetch(from); issue(from, 0); }
+    int buf = 0;
+    for (int kt = from; kt < to; kt += 128, buf ^= 1) {
+        const unsigned bits = cur;
+        copies_done();                                               // (this wave's own copies; its reads of the other buffer are in registers)
+        if (kt + 128 < to) issue(kt + 128, buf ^ 1);
+        if (bits == 0) continue;
+        const char* const img_k = mine + buf * 2 * IMG;
+        const char* const img_v = img_k + IMG;
+        f32x16 st[1];
+        clear(st);
+#pragma unroll
+        for (int f = 0; f < NF; ++f) st[0] = M::mma(M::template row<DP>(img_k, l31, f, h), qf[f], st[0]);
+        if (bits != ~0u || (p.causal && kt + 31 > off)) {
+            const int last = p.causal ? token + off - kt : 32;
+#pragma unroll
+            for (int x = 0; x < 16; ++x) {
+                const int j = rowmap(x, h);
+                if (!((bits >> j) & 1) || j > last) st[0][x] = -INFINITY;
+            }
+        }
+        float tm = st[0][0];
+#pragma unroll
+        for (int x = 1; x < 16; ++x) tm = fmaxf(tm, st[0][x]);
+        tm = fmaxf(tm, other_half(tm)) * c;
+        if (__any(tm > m + 8.f)) {
+            const float mn = fmaxf(m, tm), alpha = mn == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m - mn);
+            m = mn;
+            l *= alpha;
+            times(o, alpha);
+        }
+        const float sub0 = (m == -INFINITY ? 0.f : m) - lift;
+#pragma unroll
+        for (int x = 0; x < 16; ++x) {
+            st[0][x] = __builtin_amdgcn_exp2f(__builtin_fmaf(st[0][x], c, -sub0));
+            l += st[0][x];
+        }
+#pragma unroll
+        for (int f = 0; f < NP; ++f) {
+            const typename M::Frag pf = M::from_acc(st[0], f);
+#pragma unroll
+            for (int dt = 0; dt < ND; ++dt) o[dt] = M::mma(M::template col<DP>(img_v, 0, f, dt, lane), pf, o[dt]);
+        }
+    }
+    l += other_half(l);
+    __syncthreads();                                                 // (the tiles' LDS becomes the sums')
+    float* const s_o = reinterpret_cast<float*>(smem);
+    float2* const s_ml = reinterpret_cast<float2*>(smem + 4 * 32 * OP * sizeof(float));
+    store_row<T, DP, f32x4>(o, reinterpret_cast<char*>(s_o + (wave * 32 + l31) * OP), h, p.D, 1.f);
+    if (h == 0) s_ml[wave * 32 + l31] = float2{m, l};
+    __syncthreads();
+    const int r = tid >> 3;                                          // 8 threads a row, 16 columns each
+    if (r >= rows) return;
+    const long long at = w.b * p.lse_b + (w.kvh * p.group + r % p.group) * p.lse_h + w.q0 + r / p.group;
+    float M0 = -INFINITY, L = 0.f, a[4];
+#pragma unroll
+    for (int x = 0; x < 4; ++x) M0 = fmaxf(M0, s_ml[x * 32 + r].x);
+#pragma unroll
+    for (int x = 0; x < 4; ++x) {                                    // (a NaN sum counts whatever its maximum)
+        const float2 ml = s_ml[x * 32 + r];
+        a[x] = ml.y == 0.f ? 0.f : ml.x == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(ml.x - M0);
+        L = __builtin_fmaf(ml.y, a[x], L);
+    }
+    const float inv = p.splits > 1 ? 1.f : L == 0.f ? 0.f : 1.f / L;
+    for (int d = (tid & 7) * 8; d < p.D; d += 64) {
+        float v[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int x = 0; x < 4; ++x) {
+            if (a[x] == 0.f) continue;
+#pragma unroll
+            for (int e = 0; e < 8; ++e) v[e] = __builtin_fmaf(s_o[(x * 32 + r) * OP + d + e], a[x], v[e]);
+        }
+#pragma unroll
+        for (int e = 0; e < 8; ++e) v[e] *= inv;
+        if (p.splits > 1) store8<float>(reinterpret_cast<char*>(p.part + (w.split * p.part_rows + at) * p.D), d, v);
+        else store8<T>(p.out.p + w.b * p.out.b + (w.q0 + r / p.group) * p.out.t + (w.kvh * p.group + r % p.group) * p.out.h, d, v);
+    }
+    if ((tid & 7) == 0) {
+        if (p.splits > 1) *reinterpret_cast<float2*>(p.part_ml + 2 * (w.split * p.part_rows + at)) = float2{M0 - lift, L};
+        else p.lse[at] = L == 0.f ? -INFINITY : (M0 - lift + __builtin_amdgcn_logf(L)) * LN2;
+    }
+}
+
+// Joining the splits: 16 lanes of 8 columns a row.  Many splits: a wave a row, its four groups of lanes take a quarter of the splits each (SL = 4);
+// up to 8: four rows a wave (SL = 1; the partial sums of 9990 rows in 5 splits: 8.9 -> 6.5 us).  A lane's loads are in flight together.
+constexpr int join_slices(int splits) { return splits > 8 ? 4 : 1; }
+template <int SL> struct Join {
+    static constexpr int ROWS = 16 / SL;                             // of a workgroup
+    int row, slice, d;
+    __device__ __forceinline__ Join() : row(threadIdx.x / (16 * SL)), slice(threadIdx.x / 16 % SL), d(threadIdx.x % 16 * 8) {}
+    __device__ __forceinline__ bool first() const { return slice == 0; }
+    template <class F> __device__ __forceinline__ float over_slices(float v, F f) const {
+        if (SL == 4) { v = f(v, __shfl_xor(v, 16, 64)); v = f(v, __shfl_xor(v, 32, 64)); }
+        return v;
+    }
+    __device__ __forceinline__ float sum(float v) const { return over_slices(v, [](float x, float y) { return x + y; }); }
+};
+template <int SL, class F> __device__ __forceinline__ void join_rows(const Params& p, F f) {
     Params one = p;
-    one.splits = QB / JOIN;                                          // (the same block numbering, JOIN rows each)
+    one.splits = QB / Join<SL>::ROWS;                                // (the same block numbering, ROWS rows each)
     const Where w = where(one, true);
-    const int rows = w.ql * p.group, r = w.tile * QB * p.group + w.sub * QB + w.split * JOIN + (threadIdx.x >> 6);
+    const Join<SL> j;
+    const int rows = w.ql * p.group, r = w.tile * QB * p.group + w.sub * QB + w.split * Join<SL>::ROWS + j.row;
     if (r >= min(rows, (w.tile + 1) * QB * p.group)) return;
     const int token = r / p.group, head = w.kvh * p.group + r % p.group;
-    f(w, token, head, w.b * p.lse_b + head * p.lse_h + w.q0 + token);
+    f(w, j, token, head, w.b * p.lse_b + head * p.lse_h + w.q0 + token);
 }
 __device__ __forceinline__ void load8(const float* row, int d, int D, float (&v)[8]) {
 #pragma unroll
@@ -410,61 +557,47 @@ __device__ __forceinline__ void load8(const float* row, int d, int D, float (&v)
         for (int i = 0; i < 4; ++i) v[e + i] = x[i];
     }
 }
-template <class T> __device__ __forceinline__ void store8(char* row, int d, const float (&v)[8]) {
-#pragma unroll
-    for (int e = 0; e < 8; e += 4)
-        *reinterpret_cast<typename Mma<T>::Quad*>(row + (d + e) * (int)sizeof(T)) = __builtin_convertvector((f32x4{v[e], v[e + 1], v[e + 2], v[e + 3]}), typename Mma<T>::Quad);
-}
-// Sum over i of row i of part (rows `stride` apart), in a fixed order: v in the first 16 lanes
-__device__ __forceinline__ void sum_splits(const float* part, long long stride, int n, int D, float (&v)[8]) {
-    const int lane = threadIdx.x & 63, d = (lane & 15) * 8;
+// Sum over the splits' rows (`stride` apart), in a fixed order
+template <int SL> __device__ __forceinline__ void sum_splits(const Join<SL>& j, const float* part, long long stride, int n, int D, float (&v)[8]) {
 #pragma unroll
     for (int e = 0; e < 8; ++e) v[e] = 0.f;
 #pragma unroll 4
-    for (int i = lane >> 4; i < n; i += 4) {
+    for (int i = j.slice; i < n; i += SL) {
         float x[8];
-        load8(part + i * stride, d, D, x);
+        load8(part + i * stride, j.d, D, x);
 #pragma unroll
         for (int e = 0; e < 8; ++e) v[e] += x[e];
     }
 #pragma unroll
-    for (int e = 0; e < 8; ++e) {
-        v[e] += __shfl_xor(v[e], 16, 64);
-        v[e] += __shfl_xor(v[e], 32, 64);
-    }
+    for (int e = 0; e < 8; ++e) v[e] = j.sum(v[e]);
 }
 
-template <class T>
+template <class T, int SL>
 __global__ __launch_bounds__(256) void fwd_join_kernel(const Params p) {
-    join_rows(p, [&](const Where& w, int token, int head, long long at) {
-        const int lane = threadIdx.x & 63, d = (lane & 15) * 8;
+    join_rows<SL>(p, [&](const Where& w, const Join<SL>& j, int token, int head, long long at) {
         // the largest maximum (splits that saw nothing have -inf and sum 0; a NaN sum counts whatever its maximum: it has to come out)
         float m = -INFINITY;
-        for (int i = lane; i < p.splits; i += 64) m = fmaxf(m, p.part_ml[2 * (i * p.part_rows + at)]);
-#pragma unroll
-        for (int x = 32; x; x >>= 1) m = fmaxf(m, __shfl_xor(m, x, 64));
+#pragma unroll 4
+        for (int i = j.slice; i < p.splits; i += SL) m = fmaxf(m, p.part_ml[2 * (i * p.part_rows + at)]);
+        m = j.over_slices(m, [](float x, float y) { return fmaxf(x, y); });
         float l = 0.f, v[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
 #pragma unroll 4
-        for (int i = lane >> 4; i < p.splits; i += 4) {
+        for (int i = j.slice; i < p.splits; i += SL) {
             const float2 ml = *reinterpret_cast<const float2*>(p.part_ml + 2 * (i * p.part_rows + at));
             float x[8];
-            load8(p.part + (i * p.part_rows + at) * p.D, d, p.D, x);
+            load8(p.part + (i * p.part_rows + at) * p.D, j.d, p.D, x);
             const float a = ml.y == 0.f ? 0.f : ml.x == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(ml.x - m);
             l = __builtin_fmaf(ml.y, a, l);
 #pragma unroll
             for (int e = 0; e < 8; ++e) v[e] = __builtin_fmaf(x[e], a, v[e]);
         }
-#pragma unroll
-        for (int x = 16; x <= 32; x += 16) {
-            l += __shfl_xor(l, x, 64);
-#pragma unroll
-            for (int e = 0; e < 8; ++e) v[e] += __shfl_xor(v[e], x, 64);
-        }
+        l = j.sum(l);
         const float inv = l == 0.f ? 0.f : 1.f / l;
 #pragma unroll
-        for (int e = 0; e < 8; ++e) v[e] *= inv;
-        if (lane < 16 && d < p.D) store8<T>(p.out.p + w.b * p.out.b + (w.q0 + token) * p.out.t + head * p.out.h, d, v);
-        if (lane == 0) p.lse[at] = l == 0.f ? -INFINITY : (m + __builtin_amdgcn_logf(l)) * LN2;
+        for (int e = 0; e < 8; ++e) v[e] = j.sum(v[e]) * inv;
+        if (!j.first()) return;
+        if (j.d < p.D) store8<T>(p.out.p + w.b * p.out.b + (w.q0 + token) * p.out.t + head * p.out.h, j.d, v);
+        if (j.d == 0) p.lse[at] = l == 0.f ? -INFINITY : (m + __builtin_amdgcn_logf(l)) * LN2;
     });
 }
 
@@ -477,7 +610,7 @@ __global__ __launch_bounds__(256, (WAVES<T, DP>)) void dq_kernel(const Params p)
     constexpr int NF = DP / M::KS, NP = 32 / M::KS, ND = DP / 32, IMG = KB * Image<T, DP>::PITCH;
     constexpr bool FIX = sizeof(T) == 2;
     extern __shared__ __attribute__((aligned(16))) char smem[];       // [2][K, V]
-    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, l31 = lane & 31, h = lane >> 5;
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), l31 = lane & 31, h = lane >> 5;
     const Where w = where(p, true);
     const int rows = w.ql * p.group, r0 = w.tile * QB * p.group + w.sub * QB;
     if (r0 >= min(rows, (w.tile + 1) * QB * p.group)) return;
@@ -597,17 +730,17 @@ __global__ __launch_bounds__(256, (WAVES<T, DP>)) void dq_kernel(const Params p)
     if (h == 0) { p.lse2[at] = lse2; p.ndelta[at] = nd - rho; }
 }
 
-template <class T>
+template <class T, int SL>
 __global__ __launch_bounds__(256) void dq_join_kernel(const Params p) {
-    join_rows(p, [&](const Where& w, int token, int head, long long at) {
-        const int lane = threadIdx.x & 63, d = (lane & 15) * 8;
+    join_rows<SL>(p, [&](const Where& w, const Join<SL>& j, int token, int head, long long at) {
         float v[8], rho = 0.f;
-        for (int i = lane; i < p.splits; i += 64) rho += p.part_ml[i * p.part_rows + at];
-#pragma unroll
-        for (int x = 32; x; x >>= 1) rho += __shfl_xor(rho, x, 64);
-        sum_splits(p.part + at * p.D, p.part_rows * p.D, p.splits, p.D, v);
-        if (lane < 16 && d < p.D) store8<T>(p.dq.p + w.b * p.dq.b + (w.q0 + token) * p.dq.t + head * p.dq.h, d, v);
-        if (lane == 0) p.ndelta[at] -= rho;
+#pragma unroll 4
+        for (int i = j.slice; i < p.splits; i += SL) rho += p.part_ml[i * p.part_rows + at];
+        rho = j.sum(rho);
+        sum_splits<SL>(j, p.part + at * p.D, p.part_rows * p.D, p.splits, p.D, v);
+        if (!j.first()) return;
+        if (j.d < p.D) store8<T>(p.dq.p + w.b * p.dq.b + (w.q0 + token) * p.dq.t + head * p.dq.h, j.d, v);
+        if (j.d == 0) p.ndelta[at] -= rho;
     });
 }
 
@@ -616,9 +749,10 @@ __global__ __launch_bounds__(256, (DKV_WAVES<T, DP>)) void dkv_kernel(const Para
     typedef Mma<T> M;
     constexpr int NF = DP / M::KS, NP = 32 / M::KS, ND = DP / 32, R = RB<T, DP>, IMG = R * Image<T, DP>::PITCH;
     constexpr bool VL = V_LDS<T, DP>;
+    constexpr int UN = DP * (int)sizeof(T) <= 128 ? 2 : 1;           // (more would spill)
     extern __shared__ __attribute__((aligned(16))) char smem[];       // [2][Q, dO], [2][lse2, -D][64], then the waves' V fragments
     float* const s_row = reinterpret_cast<float*>(smem + 4 * IMG);
-    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, l31 = lane & 31, h = lane >> 5;
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), l31 = lane & 31, h = lane >> 5;
     const Where w = where(p, false);
     if (w.tile * QB >= w.kl) return;
     const int off = w.kl - w.ql;
@@ -692,7 +826,7 @@ __global__ __launch_bounds__(256, (DKV_WAVES<T, DP>)) void dkv_kernel(const Para
         const char* const img_q = smem + buf * 2 * IMG;
         const char* const img_g = img_q + IMG;
         const bool partial = p.causal && kw + 31 - off > qt;
-#pragma unroll (DP * (int)sizeof(T) <= 128 ? 2 : 1)
+#pragma unroll UN
         for (int sub = 0; sub < R / 32; ++sub) {
             const float* const sl = s_row + buf * 128 + sub * 32 + 4 * h;
             f32x16 st, dp;
@@ -748,36 +882,51 @@ __global__ __launch_bounds__(256, (DKV_WAVES<T, DP>)) void dkv_kernel(const Para
     store_row<T, DP>(dv, p.dv.p + w.b * p.dv.b + row * p.dv.t + w.kvh * p.dv.h, h, p.D, un);
 }
 
-template <class T>
+template <class T, int SL>
 __global__ __launch_bounds__(256) void dkv_join_kernel(const Params p) {
     Params one = p;
-    one.splits = QB / JOIN;
+    one.splits = QB / Join<SL>::ROWS;
     const Where w = where(one, false);
-    const int j = w.tile * QB + w.split * JOIN + (threadIdx.x >> 6), lane = threadIdx.x & 63, d = (lane & 15) * 8;
-    if (j >= w.kl) return;
-    const long long row = w.k0 + j, at = w.b * p.krow_b + w.kvh * p.krow_h + row;
+    const Join<SL> j;
+    const int key = w.tile * QB + w.split * Join<SL>::ROWS + j.row;
+    if (key >= w.kl) return;
+    const long long row = w.k0 + key, at = w.b * p.krow_b + w.kvh * p.krow_h + row;
 #pragma unroll
     for (int which = 0; which < 2; ++which) {
         float v[8];
-        sum_splits(p.part + (which * p.part_rows + at) * p.D, 2 * p.part_rows * p.D, p.splits, p.D, v);
+        sum_splits<SL>(j, p.part + (which * p.part_rows + at) * p.D, 2 * p.part_rows * p.D, p.splits, p.D, v);
         const Ten& t = which ? p.dv : p.dk;
-        if (lane < 16 && d < p.D) store8<T>(t.p + w.b * t.b + row * t.t + w.kvh * t.h, d, v);
+        if (j.first() && j.d < p.D) store8<T>(t.p + w.b * t.b + row * t.t + w.kvh * t.h, j.d, v);
     }
 }
 
 inline int grid_of(const Params& p, int splits) { return p.n_tiles * p.kv_heads * p.subs * splits; }
+constexpr int JOIN = QB / Join<4>::ROWS;                             // most workgroups that join a block
+#define DPC_SEQ_JOIN(kernel, p)                                                                                                             \
+    if ((p).splits > 1) {                                                                                                                    \
+        if (join_slices((p).splits) == 4) hipLaunchKernelGGL((kernel<T, 4>), dim3(grid_of(p, QB / Join<4>::ROWS)), dim3(256), 0, s, p);      \
+        else hipLaunchKernelGGL((kernel<T, 1>), dim3(grid_of(p, QB / Join<1>::ROWS)), dim3(256), 0, s, p);                                   \
+        DPC_LAUNCH_CHECK();                                                                                                                  \
+    }
 
 template <class T, int DP>
 int run_fwd(const Params& p, hipStream_t s) {
     constexpr int lds = 4 * KB * Image<T, DP>::PITCH;
-    static DeviceOnce once;
-    if (!once) { DPC_HIP(hipFuncSetAttribute((const void*)fwd_kernel<T, DP>, hipFuncAttributeMaxDynamicSharedMemorySize, lds)); once = true; }
-    hipLaunchKernelGGL((fwd_kernel<T, DP>), dim3(grid_of(p, p.splits)), dim3(256), lds, s, p);
-    DPC_LAUNCH_CHECK();
-    if (p.splits > 1) {
-        hipLaunchKernelGGL((fwd_join_kernel<T>), dim3(grid_of(p, QB / JOIN)), dim3(256), 0, s, p);
-        DPC_LAUNCH_CHECK();
+    if constexpr (FEW<T, DP>) {
+        if (p.few) {
+            constexpr int lds_few = std::max(16 * 32 * Image<T, DP>::PITCH, 4 * 32 * ((DP + 4) * 4 + 8));
+            static DeviceOnce few;
+            if (!few) { DPC_HIP(hipFuncSetAttribute((const void*)few_kernel<T, DP>, hipFuncAttributeMaxDynamicSharedMemorySize, lds_few)); few = true; }
+            hipLaunchKernelGGL((few_kernel<T, DP>), dim3(grid_of(p, p.splits)), dim3(256), lds_few, s, p);
+        }
     }
+    if (!p.few) {
+        static DeviceOnce once;
+        if (!once) { DPC_HIP(hipFuncSetAttribute((const void*)fwd_kernel<T, DP>, hipFuncAttributeMaxDynamicSharedMemorySize, lds)); once = true; }
+        hipLaunchKernelGGL((fwd_kernel<T, DP>), dim3(grid_of(p, p.splits)), dim3(256), lds, s, p);
+    }
+    DPC_LAUNCH_CHECK();
+    DPC_SEQ_JOIN(fwd_join_kernel, p)
     return DPC_OK;
 }
 
@@ -793,18 +942,12 @@ int run_bwd(const Params& pq, const Params& pk, hipStream_t s) {
     if (pq.n_tiles) {
         hipLaunchKernelGGL((dq_kernel<T, DP>), dim3(grid_of(pq, pq.splits)), dim3(256), lds, s, pq);
         DPC_LAUNCH_CHECK();
-        if (pq.splits > 1) {
-            hipLaunchKernelGGL((dq_join_kernel<T>), dim3(grid_of(pq, QB / JOIN)), dim3(256), 0, s, pq);
-            DPC_LAUNCH_CHECK();
-        }
+        DPC_SEQ_JOIN(dq_join_kernel, pq)
     }
     if (pk.n_tiles) {
         hipLaunchKernelGGL((dkv_kernel<T, DP>), dim3(grid_of(pk, pk.splits)), dim3(256), lds_k, s, pk);
         DPC_LAUNCH_CHECK();
-        if (pk.splits > 1) {
-            hipLaunchKernelGGL((dkv_join_kernel<T>), dim3(grid_of(pk, QB / JOIN)), dim3(256), 0, s, pk);
-            DPC_LAUNCH_CHECK();
-        }
+        DPC_SEQ_JOIN(dkv_join_kernel, pk)
     }
     return DPC_OK;
 }

@@ -57,7 +57,7 @@ static Params params(const dpc_seq_attn* a) {
 // causal bf16 2 x 4096, 16/4 heads of 128: 561 -> 388 us, the join 14 -> 24).
 // Returns false when the grid would pass 2^31.
 constexpr int SLOTS = 512;
-static bool plan_grid(Params& p, const dpc_seq_attn* a, bool keys) {
+static bool plan_grid(Params& p, const dpc_seq_attn* a, bool keys, bool forward) {
     p.tiles = keys ? a->k_tiles : a->q_tiles;
     p.tiles_per_seq = cdiv(keys ? a->k_len : a->q_len, QB);
     const long long n = p.tiles ? (keys ? a->n_k_tiles : a->n_q_tiles) : (long long)a->batch * p.tiles_per_seq;
@@ -65,10 +65,14 @@ static bool plan_grid(Params& p, const dpc_seq_attn* a, bool keys) {
     const long long blocks = n * p.kv_heads * p.subs;
     const long long walk = keys ? (long long)p.group * cdiv(a->q_len, KB) : cdiv(a->k_len, KB);
     const int slots = p.causal && 2ll * a->q_len > a->k_len ? 2 * SLOTS : SLOTS;
-    p.splits = blocks == 0 || blocks >= slots * 3 / 4 ? 1 : (int)std::max<long long>(1, std::min<long long>(slots / blocks, walk / 4));
+    // At most 32 rows of a sequence and key head: few_kernel (its LDS allows rows of 256 bytes), one workgroup resident a CU, two made: sequences differ in length.
+    // A split has two tiles a wave at least.  One token, 8 x 16384 keys, 32/8 heads of 128, bf16: 113 us by fwd_kernel, 98 so (4.1 TB/s), 100 with 256 workgroups.
+    p.few = forward && (long long)a->q_len * p.group <= 32 && (a->head_dim + 31) / 32 * 32 * (a->type == DPC_SEQ_F32 ? 4 : 2) <= 256;
+    if (p.few) p.splits = blocks == 0 ? 1 : (int)std::max<long long>(1, std::min<long long>(SLOTS / blocks, a->k_len / 256));
+    else p.splits = blocks == 0 || blocks >= slots * 3 / 4 ? 1 : (int)std::max<long long>(1, std::min<long long>(slots / blocks, walk / 4));
     p.n_tiles = (int)n;
     p.part_rows = keys ? a->k_rows : a->lse_rows;
-    return n < (1ll << 31) && blocks * std::max(p.splits, QB / JOIN) < (1ll << 31);
+    return n < (1ll << 31) && blocks * std::max(p.splits, JOIN) < (1ll << 31);
 }
 
 static size_t part_bytes(const Params& p, int per_row) {
@@ -80,7 +84,7 @@ static Plan plan_of(const dpc_seq_attn* a, bool backward) {
     Plan w{};
     w.q = params(a);
     w.k = w.q;
-    w.ok = plan_grid(w.q, a, false) && (!backward || plan_grid(w.k, a, true));
+    w.ok = plan_grid(w.q, a, false, !backward) && (!backward || plan_grid(w.k, a, true, false));
     if (backward) {
         w.rows = align_up((size_t)a->lse_rows * sizeof(float), 256);
         w.bytes = 2 * w.rows + std::max(part_bytes(w.q, a->head_dim + 1), part_bytes(w.k, 2 * a->head_dim));
