@@ -23,7 +23,7 @@ import math
 
 import torch
 
-from ... import _lib
+from ... import _lib, sequence
 from .video_diffusion_pytorch_conv3d import _relative_position_bucket, _rotary_tables
 
 
@@ -386,7 +386,16 @@ class _SAttn(_AttnBase):
 
 
 class _MAttn(_AttnBase):
-    """mid_spatial_attn (:455-457): dense attention over the pixels of a frame, no rotary, no bias."""
+    """mid_spatial_attn (:455-457): dense attention over the pixels of a frame, no rotary, no bias.  Up to 256 pixels (S64: 16 x 16) the
+    whole-image operators dpc_attention_core / dpc_attention_bwd; beyond (S128: 32 x 32) diffphycon_amd.sequence on views of the packed qkv, whose
+    forward leaves the log-sum-exp that its backward recomputes the probabilities from."""
+
+    WHOLE = 256
+
+    def _heads(self, qkv, dims):
+        """q, k, v as [frames, pixels, heads, 32] views of a packed [rows, 3 heads 32] tensor."""
+        B, F, H, W = dims
+        return qkv.view(B * F, H * W, 3, self.ctx.heads, 32).unbind(2)
 
     def __init__(self, ctx, p, Cc):
         super().__init__(ctx, p, Cc, ".fn.fn.fn", False)
@@ -395,22 +404,28 @@ class _MAttn(_AttnBase):
         B, F, H, W = dims
         st, qkv = self._pre(x, dims)
         att = self.ctx.empty(x.shape[0], self.ctx.heads * 32)
-        _lib.check(_lib.lib().dpc_attention_core(_lib.ptr(qkv), _lib.ptr(att), self.ctx.heads, H * W, B * F, 1, H * W, 0, 1, None, None, None,
-                                                 _lib.stream()))
+        lse = None
+        if H * W <= self.WHOLE:
+            _lib.check(_lib.lib().dpc_attention_core(_lib.ptr(qkv), _lib.ptr(att), self.ctx.heads, H * W, B * F, 1, H * W, 0, 1, None, None, None,
+                                                     _lib.stream()))
+        else:
+            _, lse = sequence.attention_forward(*self._heads(qkv, dims), out=att.view(B * F, H * W, self.ctx.heads, 32))
         y = self.co.fwd(att, dims, resid=x)
-        self.tape = (x, st, qkv, att, dims)
+        self.tape = (x, st, qkv, att, lse, dims)
         return y
 
     def backward(self, dy):
-        x, st, qkv, att, dims = self.tape
+        x, st, qkv, att, lse, dims = self.tape
         self.tape = None
         B, F, H, W = dims
-        if H * W > 256:
-            raise NotImplementedError("mid_spatial_attn backward: at most 256 pixels per frame at the bottleneck (S64: 16 x 16)")
         self.co.wgrad([att], dy, dims)
         d_att = self.co.dgrad(dy, dims)
         dqkv = torch.empty_like(qkv)
-        _lib.check(_lib.lib().dpc_attention_bwd(_lib.ptr(qkv), _lib.ptr(d_att), _lib.ptr(dqkv), self.ctx.heads, B * F, H * W, _lib.stream()))
+        if lse is None:
+            _lib.check(_lib.lib().dpc_attention_bwd(_lib.ptr(qkv), _lib.ptr(d_att), _lib.ptr(dqkv), self.ctx.heads, B * F, H * W, _lib.stream()))
+        else:
+            heads = (B * F, H * W, self.ctx.heads, 32)
+            sequence.attention_backward(d_att.view(heads), *self._heads(qkv, dims), att.view(heads), lse, grads=self._heads(dqkv, dims))
         del d_att
         return self._post_backward(x, st, qkv, att, dqkv, dy, dims)
 
