@@ -263,7 +263,7 @@ class RotaryTable:
         z = torch.polar(torch.full((), self.attention_factor, dtype=torch.float64, device=device), angle)
         self.table = torch.view_as_real(z).float().contiguous()                        # [max_positions, rotary_dim / 2, 2]
         torch.cuda.current_stream(self.table.device).synchronize()                     # whole for whatever stream uses it
-        self.stream = _stream(self.table.get_device())
+        self.stream, self.address, self.interleaved = _stream(self.table.get_device()), self.table.data_ptr(), layout == "interleaved"
 
 
 def _rotary(q, k, table, positions, start, out, transpose):
@@ -278,9 +278,12 @@ def _rotary(q, k, table, positions, start, out, transpose):
     B, T, H, D = (1, *shape) if packed else shape
     Hk = 0
     if k is not None:
-        if k.shape[:-2] != shape[:-2] or k.shape[-1] != D:
-            raise ValueError(f"q {tuple(shape)} and k {tuple(k.shape)} must agree but for the heads")
-        Hk = k.shape[-2]
+        ks = k.shape
+        if len(ks) != len(shape) or (1, *ks)[-4] != B or ks[-3] != T or ks[-1] != D:
+            raise ValueError(f"q {tuple(shape)} and k {tuple(ks)} must agree but for the heads")
+        Hk = ks[-2]
+    if H < 1 or (k is not None and Hk < 1):
+        raise ValueError("at least one head")
     if table.rotary_dim > D:
         raise ValueError(f"the table's rotary_dim {table.rotary_dim} exceeds the head's {D}")
     pos_b = 0
@@ -299,21 +302,35 @@ def _rotary(q, k, table, positions, start, out, transpose):
     _in_use(table, d)
     if out is None:
         yq, yk = q.new_empty(shape), None if k is None else k.new_empty(k.shape)
+        lyq, lyk = (yq.data_ptr(), T * H * D, H * D, D), _NONE if k is None else (yk.data_ptr(), T * Hk * D, Hk * D, D)
     else:
         yq, yk = _rotary_out(q, k, out)
-    if B * T * H * D == 0 and (k is None or k.numel() == 0):
+        lyq, lyk = _place(yq), _NONE if k is None else _place(yk)
+    if B * T == 0:
         return yq, yk
     q = q if q.stride(-1) == 1 else q.contiguous()
-    k = k if k is None or k.stride(-1) == 1 else k.contiguous()
-    if positions is not None and not (positions.dtype == torch.int64 and positions.is_contiguous()):
-        positions = positions.to(torch.int64).contiguous()
-    none = (0, 0, 0, 0)
-    a = _lib.SEQ_ROTARY_BYTES.pack(q.data_ptr(), *_strides(q), *(none if k is None else (k.data_ptr(), *_strides(k))),
-                                   yq.data_ptr(), *_strides(yq), *(none if k is None else (yk.data_ptr(), *_strides(yk))), table.table.data_ptr(),
-                                   0 if positions is None else positions.data_ptr(), pos_b, start, table.max_positions, t, B, T, H, Hk, D,
-                                   table.rotary_dim, table.layout == "interleaved", transpose)
+    lk = _NONE
+    if k is not None:
+        k = k if k.stride(-1) == 1 else k.contiguous()
+        lk = _place(k)
+    at = 0
+    if positions is not None:
+        if positions.dtype != torch.int64 or not positions.is_contiguous():
+            positions = positions.to(torch.int64).contiguous()
+        at = positions.data_ptr()
+    a = _lib.SEQ_ROTARY_BYTES.pack(*_place(q), *lk, *lyq, *lyk, table.address, at, pos_b, start, table.max_positions, t, B, T, H, Hk, D,
+                                   table.rotary_dim, table.interleaved, transpose)
     _lib.check(_lib.lib().dpc_seq_rotary_run(a, _stream(d)))
     return yq, yk
+
+
+_NONE = (0, 0, 0, 0)
+
+
+def _place(x):
+    """Address and strides of batch, token, head."""
+    s = x.stride()
+    return (x.data_ptr(), *s[:3]) if len(s) == 4 else (x.data_ptr(), 0, s[0], s[1])
 
 
 def _rotary_out(q, k, out):
