@@ -17,7 +17,7 @@
 #pragma once
 #include <algorithm>
 
-#include "common.h"
+#include "seq_div.h"
 
 namespace dpc {
 namespace seqattn {
@@ -115,7 +115,8 @@ struct Params {
     float *lse2, *ndelta;                          // backward: lse in powers of two (+inf: a row that sees nothing) and -D, numbered like lse
     float *part, *part_ml;                         // splits: partial sums [split][row][D] and per-row scalars (layout at each kernel)
     long long part_rows;
-    int heads, kv_heads, group, D, q_len, k_len, causal, n_tiles, tiles_per_seq, subs, splits, few;
+    int heads, kv_heads, group, D, q_len, k_len, causal, n_tiles, tiles_per_seq, pairs, splits, few;
+    Div by_split, by_sub, by_kv, by_group, by_pair, by_tile;         // splits, sub-blocks of a block, kv_heads, group, blocks of a (sequence, key head), pairs
     float scale;
 };
 
@@ -128,23 +129,27 @@ __device__ __forceinline__ Where where(const Params& p, bool last_first) {
     int id = blockIdx.x;
     w.ql = p.q_len; w.kl = p.k_len; w.q0 = w.k0 = 0;
     if (p.tiles) {
-        w.split = id % p.splits; id /= p.splits;
-        w.sub = id % p.subs; id /= p.subs;
-        w.kvh = id % p.kv_heads;
-        id /= p.kv_heads;
-        const int* e = p.tiles + 8 * id;
+        w.split = p.by_split.take(id);
+        w.sub = p.by_sub.take(id);
+        w.kvh = p.by_kv.take(id);
+        const int* e = p.tiles + 8 * (long long)id;
         w.b = e[0]; w.tile = e[1]; w.q0 = e[2]; w.ql = e[3]; w.k0 = e[4]; w.kl = e[5];
         return w;
     }
-    const int per = p.tiles_per_seq * p.subs * p.splits, pairs = p.n_tiles / p.tiles_per_seq * p.kv_heads;
     int pair, i;
-    if (pairs % 8 == 0) { const int x = id & 7, j = id >> 3; pair = x * (pairs / 8) + j / per; i = j % per; }
-    else { pair = id % pairs; i = id / pairs; }
-    w.split = i % p.splits; i /= p.splits;
-    w.sub = i % p.subs; i /= p.subs;
+    if (p.pairs % 8 == 0) {
+        pair = id >> 3;
+        i = p.by_pair.take(pair);
+        pair += (id & 7) * (p.pairs >> 3);
+    } else {
+        i = id;
+        pair = p.by_tile.take(i);
+    }
+    w.split = p.by_split.take(i);
+    w.sub = p.by_sub.take(i);
     w.tile = last_first ? p.tiles_per_seq - 1 - i : i;
-    w.b = pair / p.kv_heads;
-    w.kvh = pair % p.kv_heads;
+    w.kvh = p.by_kv.take(pair);
+    w.b = pair;
     return w;
 }
 
@@ -300,9 +305,10 @@ __global__ __launch_bounds__(256, (WAVES<T, DP>)) void fwd_kernel(const Params p
     if (r0 >= min(rows, (w.tile + 1) * QB * p.group)) return;
     const int off = w.kl - w.ql, rw = r0 + wave * 32, r = rw + l31;   // this wave's first row, this lane's
     const bool rok = r < rows;
-    const int token = (rok ? r : r0) / p.group, head = w.kvh * p.group + (rok ? r : r0) % p.group;
-    const int t_first = rw / p.group, t_last = (rw + 31) / p.group;   // this wave's tokens
-    int kend = p.causal ? min(w.kl, min((r0 + QB - 1) / p.group, w.ql - 1) + 1 + off) : w.kl, kbegin = 0;
+    int token = rok ? r : r0;
+    const int head = w.kvh * p.group + p.by_group.take(token);
+    const int t_first = p.by_group(rw), t_last = p.by_group(rw + 31);   // this wave's tokens
+    int kend = p.causal ? min(w.kl, min((int)p.by_group(r0 + QB - 1), w.ql - 1) + 1 + off) : w.kl, kbegin = 0;
     if (p.splits > 1) {                                              // whole tiles, at least four
         const int per = max(4, (max(kend, 0) + KB * p.splits - 1) / (KB * p.splits)) * KB;
         kbegin = w.split * per;
@@ -419,7 +425,8 @@ __global__ __launch_bounds__(256) void few_kernel(const Params p) {
     if (w.tile * QB >= w.ql) return;
     const int off = w.kl - w.ql;
     const bool rok = l31 < rows;
-    const int token = (rok ? l31 : 0) / p.group, head = w.kvh * p.group + (rok ? l31 : 0) % p.group;
+    int token = rok ? l31 : 0;
+    const int head = w.kvh * p.group + p.by_group.take(token);
     const int kend = p.causal ? min(w.kl, w.ql + off) : w.kl;
     const int per = (max(kend, 0) + 32 * 4 * p.splits - 1) / (32 * 4 * p.splits) * 32 * 4;       // keys of a split: whole rounds of the four waves
     const int from = w.split * per + wave * 32, to = min(kend, w.split * per + per);
@@ -495,7 +502,9 @@ __global__ __launch_bounds__(256) void few_kernel(const Params p) {
     __syncthreads();
     const int r = tid >> 3;                                          // 8 threads a row, 16 columns each
     if (r >= rows) return;
-    const long long at = w.b * p.lse_b + (w.kvh * p.group + r % p.group) * p.lse_h + w.q0 + r / p.group;
+    int rt = r;
+    const int rh = w.kvh * p.group + p.by_group.take(rt);
+    const long long at = w.b * p.lse_b + rh * p.lse_h + w.q0 + rt;
     float M0 = -INFINITY, L = 0.f, a[4];
 #pragma unroll
     for (int x = 0; x < 4; ++x) M0 = fmaxf(M0, s_ml[x * 32 + r].x);
@@ -517,7 +526,7 @@ __global__ __launch_bounds__(256) void few_kernel(const Params p) {
 #pragma unroll
         for (int e = 0; e < 8; ++e) v[e] *= inv;
         if (p.splits > 1) store8<float>(reinterpret_cast<char*>(p.part + (w.split * p.part_rows + at) * p.D), d, v);
-        else store8<T>(p.out.p + w.b * p.out.b + (w.q0 + r / p.group) * p.out.t + (w.kvh * p.group + r % p.group) * p.out.h, d, v);
+        else store8<T>(p.out.p + w.b * p.out.b + (w.q0 + rt) * p.out.t + rh * p.out.h, d, v);
     }
     if ((tid & 7) == 0) {
         if (p.splits > 1) *reinterpret_cast<float2*>(p.part_ml + 2 * (w.split * p.part_rows + at)) = float2{M0 - lift, L};
@@ -540,13 +549,12 @@ template <int SL> struct Join {
     __device__ __forceinline__ float sum(float v) const { return over_slices(v, [](float x, float y) { return x + y; }); }
 };
 template <int SL, class F> __device__ __forceinline__ void join_rows(const Params& p, F f) {
-    Params one = p;
-    one.splits = QB / Join<SL>::ROWS;                                // (the same block numbering, ROWS rows each)
-    const Where w = where(one, true);
+    const Where w = where(p, true);                                  // (split: which ROWS rows of the block)
     const Join<SL> j;
     const int rows = w.ql * p.group, r = w.tile * QB * p.group + w.sub * QB + w.split * Join<SL>::ROWS + j.row;
     if (r >= min(rows, (w.tile + 1) * QB * p.group)) return;
-    const int token = r / p.group, head = w.kvh * p.group + r % p.group;
+    int token = r;
+    const int head = w.kvh * p.group + p.by_group.take(token);
     f(w, j, token, head, w.b * p.lse_b + head * p.lse_h + w.q0 + token);
 }
 __device__ __forceinline__ void load8(const float* row, int d, int D, float (&v)[8]) {
@@ -616,9 +624,10 @@ __global__ __launch_bounds__(256, (WAVES<T, DP>)) void dq_kernel(const Params p)
     if (r0 >= min(rows, (w.tile + 1) * QB * p.group)) return;
     const int off = w.kl - w.ql, rw = r0 + wave * 32, r = rw + l31;
     const bool rok = r < rows;
-    const int token = (rok ? r : r0) / p.group, head = w.kvh * p.group + (rok ? r : r0) % p.group;
-    const int t_first = rw / p.group, t_last = (rw + 31) / p.group;
-    int kend = p.causal ? min(w.kl, min((r0 + QB - 1) / p.group, w.ql - 1) + 1 + off) : w.kl, kbegin = 0;
+    int token = rok ? r : r0;
+    const int head = w.kvh * p.group + p.by_group.take(token);
+    const int t_first = p.by_group(rw), t_last = p.by_group(rw + 31);
+    int kend = p.causal ? min(w.kl, min((int)p.by_group(r0 + QB - 1), w.ql - 1) + 1 + off) : w.kl, kbegin = 0;
     if (p.splits > 1) {
         const int per = max(4, (max(kend, 0) + KB * p.splits - 1) / (KB * p.splits)) * KB;
         kbegin = w.split * per;
@@ -884,9 +893,7 @@ __global__ __launch_bounds__(256, (DKV_WAVES<T, DP>)) void dkv_kernel(const Para
 
 template <class T, int SL>
 __global__ __launch_bounds__(256) void dkv_join_kernel(const Params p) {
-    Params one = p;
-    one.splits = QB / Join<SL>::ROWS;
-    const Where w = where(one, false);
+    const Where w = where(p, false);
     const Join<SL> j;
     const int key = w.tile * QB + w.split * Join<SL>::ROWS + j.row;
     if (key >= w.kl) return;
@@ -900,13 +907,21 @@ __global__ __launch_bounds__(256) void dkv_join_kernel(const Params p) {
     }
 }
 
-inline int grid_of(const Params& p, int splits) { return p.n_tiles * p.kv_heads * p.subs * splits; }
+// p with every block in n parts (splits, or the rows that a join's workgroup has)
+inline Params in_parts(Params p, int n) {
+    p.by_split = Div(n);
+    p.by_pair = Div(std::max(1u, p.tiles_per_seq * p.by_sub.d * n));
+    return p;
+}
+inline int grid_of(const Params& p) { return p.n_tiles * p.kv_heads * (int)(p.by_sub.d * p.by_split.d); }
 constexpr int JOIN = QB / Join<4>::ROWS;                             // most workgroups that join a block
-#define DPC_SEQ_JOIN(kernel, p)                                                                                                             \
-    if ((p).splits > 1) {                                                                                                                    \
-        if (join_slices((p).splits) == 4) hipLaunchKernelGGL((kernel<T, 4>), dim3(grid_of(p, QB / Join<4>::ROWS)), dim3(256), 0, s, p);      \
-        else hipLaunchKernelGGL((kernel<T, 1>), dim3(grid_of(p, QB / Join<1>::ROWS)), dim3(256), 0, s, p);                                   \
-        DPC_LAUNCH_CHECK();                                                                                                                  \
+#define DPC_SEQ_JOIN(kernel, p)                                                                     \
+    if ((p).splits > 1) {                                                                            \
+        const bool many = join_slices((p).splits) == 4;                                              \
+        const Params j = in_parts(p, QB / (many ? Join<4>::ROWS : Join<1>::ROWS));                   \
+        if (many) hipLaunchKernelGGL((kernel<T, 4>), dim3(grid_of(j)), dim3(256), 0, s, j);          \
+        else hipLaunchKernelGGL((kernel<T, 1>), dim3(grid_of(j)), dim3(256), 0, s, j);               \
+        DPC_LAUNCH_CHECK();                                                                          \
     }
 
 template <class T, int DP>
@@ -917,13 +932,13 @@ int run_fwd(const Params& p, hipStream_t s) {
             constexpr int lds_few = std::max(16 * 32 * Image<T, DP>::PITCH, 4 * 32 * ((DP + 4) * 4 + 8));
             static DeviceOnce few;
             if (!few) { DPC_HIP(hipFuncSetAttribute((const void*)few_kernel<T, DP>, hipFuncAttributeMaxDynamicSharedMemorySize, lds_few)); few = true; }
-            hipLaunchKernelGGL((few_kernel<T, DP>), dim3(grid_of(p, p.splits)), dim3(256), lds_few, s, p);
+            hipLaunchKernelGGL((few_kernel<T, DP>), dim3(grid_of(p)), dim3(256), lds_few, s, p);
         }
     }
     if (!p.few) {
         static DeviceOnce once;
         if (!once) { DPC_HIP(hipFuncSetAttribute((const void*)fwd_kernel<T, DP>, hipFuncAttributeMaxDynamicSharedMemorySize, lds)); once = true; }
-        hipLaunchKernelGGL((fwd_kernel<T, DP>), dim3(grid_of(p, p.splits)), dim3(256), lds, s, p);
+        hipLaunchKernelGGL((fwd_kernel<T, DP>), dim3(grid_of(p)), dim3(256), lds, s, p);
     }
     DPC_LAUNCH_CHECK();
     DPC_SEQ_JOIN(fwd_join_kernel, p)
@@ -940,12 +955,12 @@ int run_bwd(const Params& pq, const Params& pk, hipStream_t s) {
         once = true;
     }
     if (pq.n_tiles) {
-        hipLaunchKernelGGL((dq_kernel<T, DP>), dim3(grid_of(pq, pq.splits)), dim3(256), lds, s, pq);
+        hipLaunchKernelGGL((dq_kernel<T, DP>), dim3(grid_of(pq)), dim3(256), lds, s, pq);
         DPC_LAUNCH_CHECK();
         DPC_SEQ_JOIN(dq_join_kernel, pq)
     }
     if (pk.n_tiles) {
-        hipLaunchKernelGGL((dkv_kernel<T, DP>), dim3(grid_of(pk, pk.splits)), dim3(256), lds_k, s, pk);
+        hipLaunchKernelGGL((dkv_kernel<T, DP>), dim3(grid_of(pk)), dim3(256), lds_k, s, pk);
         DPC_LAUNCH_CHECK();
         DPC_SEQ_JOIN(dkv_join_kernel, pk)
     }

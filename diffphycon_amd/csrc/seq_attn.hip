@@ -61,8 +61,8 @@ static bool plan_grid(Params& p, const dpc_seq_attn* a, bool keys, bool forward)
     p.tiles = keys ? a->k_tiles : a->q_tiles;
     p.tiles_per_seq = cdiv(keys ? a->k_len : a->q_len, QB);
     const long long n = p.tiles ? (keys ? a->n_k_tiles : a->n_q_tiles) : (long long)a->batch * p.tiles_per_seq;
-    p.subs = keys ? 1 : cdiv((long long)std::min(a->q_len, QB) * p.group, QB);
-    const long long blocks = n * p.kv_heads * p.subs;
+    const int subs = keys ? 1 : std::max(1, cdiv((long long)std::min(a->q_len, QB) * p.group, QB));
+    const long long blocks = n * p.kv_heads * subs;
     const long long walk = keys ? (long long)p.group * cdiv(a->q_len, KB) : cdiv(a->k_len, KB);
     const int slots = p.causal && 2ll * a->q_len > a->k_len ? 2 * SLOTS : SLOTS;
     // At most 32 rows of a sequence and key head: few_kernel (its LDS allows rows of 256 bytes), one workgroup resident a CU, two made: sequences differ in length.
@@ -71,6 +71,9 @@ static bool plan_grid(Params& p, const dpc_seq_attn* a, bool keys, bool forward)
     if (p.few) p.splits = blocks == 0 ? 1 : (int)std::max<long long>(1, std::min<long long>(SLOTS / blocks, a->k_len / 256));
     else p.splits = blocks == 0 || blocks >= slots * 3 / 4 ? 1 : (int)std::max<long long>(1, std::min<long long>(slots / blocks, walk / 4));
     p.n_tiles = (int)n;
+    p.pairs = a->batch * p.kv_heads;
+    p.by_sub = Div(subs); p.by_kv = Div(p.kv_heads); p.by_group = Div(p.group); p.by_tile = Div(std::max(1, p.pairs));
+    p = in_parts(p, p.splits);
     p.part_rows = keys ? a->k_rows : a->lse_rows;
     return n < (1ll << 31) && blocks * std::max(p.splits, JOIN) < (1ll << 31);
 }

@@ -5,23 +5,12 @@
 // Rows that do not start on 16 bytes, or halves that do not, go one pair at a time.
 #include <algorithm>
 
-#include "common.h"
+#include "seq_div.h"
 
 namespace dpc {
 namespace seqrot {
 
 struct Ten { char* p; long long b, t, h; };      // strides in elements
-
-// n / d for 0 <= n < 2^31 by a multiplication: with s = ceil(log2 d) and m = floor(2^32 (2^s - d) / d) + 1, n / d = (mulhi(n, m) + n) >> s
-struct Div {
-    unsigned d, m, s;
-    Div() : Div(1) {}
-    explicit Div(unsigned x) : d(x), m(0), s(0) {
-        while ((1ull << s) < d) ++s;
-        m = (unsigned)(((1ull << 32) * ((1ull << s) - d)) / d + 1);
-    }
-    __device__ __forceinline__ unsigned operator()(unsigned n) const { return (__umulhi(n, m) + n) >> s; }
-};
 
 struct Params {
     Ten xq, xk, yq, yk;
