@@ -115,14 +115,17 @@ struct Params {
     float *lse2, *ndelta;                          // backward: lse in powers of two (+inf: a row that sees nothing) and -D, numbered like lse
     float *part, *part_ml;                         // splits: partial sums [split][row][D] and per-row scalars (layout at each kernel)
     long long part_rows;
-    int heads, kv_heads, group, D, q_len, k_len, causal, n_tiles, tiles_per_seq, pairs, splits, few;
-    Div by_split, by_sub, by_kv, by_group, by_pair, by_tile;         // splits, sub-blocks of a block, kv_heads, group, blocks of a (sequence, key head), pairs
+    int heads, kv_heads, group, D, q_len, k_len, causal, n_tiles, tiles_per_seq, band_tiles, pairs, splits, few;
+    // splits, sub-blocks of a block, kv_heads, group, pairs; workgroups of a pair in a band of blocks and in the last band, of a band on an XCD
+    Div by_split, by_sub, by_kv, by_group, by_tile, by_pair, by_last, by_band;
     float scale;
 };
 
 // Which block of which (sequence, key head) a workgroup has.  Workgroups go round the 8 XCDs, each with its own L2: the blocks of one
-// (sequence, key head), which read the same keys and values, stay on one XCD where the pairs divide evenly; the blocks with most work
-// (under a causal mask the last queries', the first keys') come first.  A query block is `subs` sub-blocks of QB rows (rows = tokens x heads of the group).
+// (sequence, key head), which read the same keys and values, stay on one XCD where the pairs divide evenly, and follow each other.  Under a causal mask
+// they differ in work (the last queries', the first keys' have most): then the quarter with most work of every pair comes first, so that
+// none of it is left for the end (pair after pair: 20 to 40 % of the card idle at the end; all pairs' heaviest blocks first: keys and values leave L2
+// in between).  A query block is `subs` sub-blocks of QB rows (rows = tokens x heads of the group).
 struct Where { int b, tile, kvh, sub, split, ql, kl; long long q0, k0; };
 __device__ __forceinline__ Where where(const Params& p, bool last_first) {
     Where w;
@@ -138,8 +141,9 @@ __device__ __forceinline__ Where where(const Params& p, bool last_first) {
     }
     int pair, i;
     if (p.pairs % 8 == 0) {
-        pair = id >> 3;
-        i = p.by_pair.take(pair);
+        int band = id >> 3;
+        pair = p.by_band.take(band);                                 // place within the band
+        i = ((band + 1) * p.band_tiles < p.tiles_per_seq ? p.by_pair : p.by_last).take(pair) + band * (int)p.by_pair.d;
         pair += (id & 7) * (p.pairs >> 3);
     } else {
         i = id;
@@ -910,7 +914,11 @@ __global__ __launch_bounds__(256) void dkv_join_kernel(const Params p) {
 // p with every block in n parts (splits, or the rows that a join's workgroup has)
 inline Params in_parts(Params p, int n) {
     p.by_split = Div(n);
-    p.by_pair = Div(std::max(1u, p.tiles_per_seq * p.by_sub.d * n));
+    const int t = std::max(1, p.tiles_per_seq), per = (int)p.by_sub.d * n;
+    p.band_tiles = p.causal ? (t + 3) / 4 : t;
+    p.by_pair = Div(p.band_tiles * per);
+    p.by_last = Div((t - (t - 1) / p.band_tiles * p.band_tiles) * per);
+    p.by_band = Div(std::max(1u, p.by_pair.d * (p.pairs / 8)));
     return p;
 }
 inline int grid_of(const Params& p) { return p.n_tiles * p.kv_heads * (int)(p.by_sub.d * p.by_split.d); }

@@ -402,19 +402,31 @@ class SequencePlan:
             rows.append((q0, a, k0, b, 0, 0))
             if self.packed_layout:
                 q0, k0 = q0 + a, k0 + b
-        tiles = [[e + rows[e[0]] for e in self._tiles(*by)] for by in ((ql, kl), (kl, ql))]
+        # block lists: of queries and of keys, for full and for causal scores
+        lists = [[e + rows[e[0]] for e in self._tiles(ql, kl, keys, causal)] for causal in (False, True) for keys in (False, True)]
         # (a blocking copy: whole for whatever stream uses it)
-        self.table = torch.tensor(tiles[0] + tiles[1] or [(0,) * 8], dtype=torch.int32).to(device)
+        self.table = torch.tensor([e for t in lists for e in t] or [(0,) * 8], dtype=torch.int32).to(device)
         self.stream = _stream(self.table.get_device())
-        self.counts = tuple(len(t) for t in tiles)
-        self.pointers = (self.table.data_ptr(), self.table.data_ptr() + 32 * len(tiles[0]))
+        self.counts = (len(lists[0]), len(lists[1]))
+        q, k = (32 * n for n in self.counts)
+        at = self.table.data_ptr()
+        self.pointers = ((at, at + q), (at + q + k, at + q + k + q))            # by causal
         self.q_longest, self.k_longest, self.q_total, self.k_total = max(ql), max(kl), sum(ql), sum(kl)
 
     @staticmethod
-    def _tiles(lengths, other):
-        """(sequence, block of 128) of every block, those of the longest sequences first."""
-        order = sorted(range(len(lengths)), key=lambda b: -min(lengths[b], 1) * other[b])
-        return [(b, t) for b in order for t in reversed(range((lengths[b] + 127) // 128))]
+    def _tiles(ql, kl, keys, causal):
+        """(sequence, block of 128) of every block of queries (or keys): in four classes of work, most first, within a class sequence by sequence."""
+        blocks = []
+        for b, (nq, nk) in enumerate(zip(ql, kl)):
+            for t in range(((nk if keys else nq) + 127) // 128):
+                if keys:
+                    work = nq - max(0, 128 * t - (nk - nq)) if causal else nq
+                else:
+                    work = min(nk, 128 * (t + 1) + nk - nq) if causal else nk
+                blocks.append((max(0, work), b, t))
+        most = max((w for w, _, _ in blocks), default=0) or 1
+        order = sorted(blocks, key=lambda e: (-(4 * e[0] // (most + 1)), -(kl if not keys else ql)[e[1]], e[1], -e[0]))
+        return [(b, t) for _, b, t in order]
 
     @classmethod
     def packed(cls, q_lengths, k_lengths=None, device="cuda"):
@@ -455,7 +467,7 @@ def _attention_args(q, k, v, causal, scale, key_mask, plan):
         if ((B, Tq), (Bk, Tk)) != want:
             raise ValueError(f"the plan is for q {want[0]} and k {want[1]} (batch, tokens), got {(B, Tq)} and {(Bk, Tk)}")
         _in_use(plan, d)
-        blocks, sizes = plan.pointers, plan.counts
+        blocks, sizes = plan.pointers[1 if causal else 0], plan.counts
     if key_mask is not None:
         key_mask = key_mask.contiguous()
     es = _BYTES[t]

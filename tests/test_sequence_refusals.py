@@ -66,10 +66,16 @@ def test_plan_refuses_lengths_beyond_the_padding_and_the_cpu():
         S.SequencePlan.packed([3, 4], device="cpu")
 
 
-def test_plan_lists_every_block_once_longest_first():
-    t = S.SequencePlan._tiles([0, 300, 1, 128], [5, 300, 1, 400])
-    assert sorted(t) == [(1, 0), (1, 1), (1, 2), (2, 0), (3, 0)]
-    assert t[0] == (3, 0) and t.index((1, 2)) < t.index((1, 0)) < t.index((2, 0))
+def test_plan_lists_every_block_once_most_work_first():
+    ql, kl = [0, 300, 1, 128, 700], [5, 300, 1, 400, 600]
+    for causal in (False, True):
+        q = S.SequencePlan._tiles(ql, kl, False, causal)
+        k = S.SequencePlan._tiles(ql, kl, True, causal)
+        assert sorted(q) == [(b, t) for b in range(5) for t in range((ql[b] + 127) // 128)]
+        assert sorted(k) == [(b, t) for b in range(5) for t in range((kl[b] + 127) // 128)]
+        assert q[0][0] == k[0][0] == 4 and q[-1] == (2, 0)
+    assert S.SequencePlan._tiles(ql, kl, False, True)[0] == (4, 5) and S.SequencePlan._tiles(ql, kl, True, True)[0] == (4, 0)
+    assert S.SequencePlan._tiles([0], [0], False, True) == []
 
 
 @pytest.mark.parametrize("kw", [
