@@ -16,7 +16,9 @@
 // two per column (shrink_col), both undone in fp32 at the end.
 #pragma once
 #include <algorithm>
+#include <type_traits>
 
+#include "bf16x6.h"
 #include "seq_div.h"
 
 namespace dpc {
@@ -24,6 +26,9 @@ namespace seqattn {
 
 constexpr float LOG2E = 1.4426950408889634f, LN2 = 0.6931471805599453f;
 constexpr int QB = 128;        // rows (queries, or keys in the dK/dV kernel) of a workgroup: 4 waves x 32
+#ifndef SPLITMAX
+#define SPLITMAX 64
+#endif
 constexpr int KB = 64;         // rows of the tile that is staged in LDS
 
 __device__ __forceinline__ int rowmap(int r, int h) { return (r & 3) + 8 * (r >> 2) + 4 * h; }
@@ -53,11 +58,11 @@ template <class T> struct Mma;
 template <class T, class F> struct Mma16 {   // the two 16-bit types
     typedef F Frag;
     static constexpr int KS = 16;            // contraction steps of one operand fragment
-    template <int DP> __device__ static __forceinline__ Frag row(const char* img, int r, int s, int h) {
+    template <int DP, int PLANE = 0> __device__ static __forceinline__ Frag row(const char* img, int r, int s, int h) {
         return *reinterpret_cast<const Frag*>(img + Image<T, DP>::off(r, 2 * s + h));
     }
     // fragment of the transposed tile: columns 32 dt .. + 31 as operand rows, contraction over tile rows r0 + 16 s .. in rowmap order
-    template <int DP> __device__ static __forceinline__ Frag col(const char* img, int r0, int s, int dt, int lane) {
+    template <int DP, int PLANE = 0> __device__ static __forceinline__ Frag col(const char* img, int r0, int s, int dt, int lane) {
         const int i = lane & 15, g = (lane >> 4) & 1, h = lane >> 5;
         const int r = 4 * h + (i >> 2);
         const int c = 4 * dt + 2 * g + ((i & 3) >> 1), o = (r0 + 16 * s) * Image<T, DP>::PITCH + (i & 1) * 8;       // (swz repeats every 16 rows)
@@ -65,6 +70,7 @@ template <class T, class F> struct Mma16 {   // the two 16-bit types
         const s16x4 b = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4)(img + o + Image<T, DP>::off(r + 8, c)));
         return __builtin_bit_cast(Frag, __builtin_shufflevector(a, b, 0, 1, 2, 3, 4, 5, 6, 7));
     }
+    __device__ static __forceinline__ float value(const Frag& f, int e) { return (float)f[e]; }
     __device__ static __forceinline__ Frag from_acc(const f32x16& v, int s) {
         f32x8 t;
 #pragma unroll
@@ -89,10 +95,10 @@ template <> struct Mma<float> {
         for (int e = 0; e < 4; ++e) c = __builtin_amdgcn_mfma_f32_32x32x2f32(a[e], b[e], c, 0, 0, 0);
         return c;
     }
-    template <int DP> __device__ static __forceinline__ Frag row(const char* img, int r, int s, int h) {
+    template <int DP, int PLANE = 0> __device__ static __forceinline__ Frag row(const char* img, int r, int s, int h) {
         return *reinterpret_cast<const Frag*>(img + Image<float, DP>::off(r, 2 * s + h));
     }
-    template <int DP> __device__ static __forceinline__ Frag col(const char* img, int r0, int s, int dt, int lane) {
+    template <int DP, int PLANE = 0> __device__ static __forceinline__ Frag col(const char* img, int r0, int s, int dt, int lane) {
         const int h = lane >> 5;
         Frag f;
 #pragma unroll
@@ -100,8 +106,41 @@ template <> struct Mma<float> {
             f[e] = *reinterpret_cast<const float*>(img + Image<float, DP>::off(r0 + 8 * s + 4 * h + e, 8 * dt + ((lane & 31) >> 2)) + (lane & 3) * 4);
         return f;
     }
+    __device__ static __forceinline__ float value(const Frag& f, int e) { return f[e]; }
     __device__ static __forceinline__ Frag from_acc(const f32x16& v, int s) { return Frag{v[4 * s], v[4 * s + 1], v[4 * s + 2], v[4 * s + 3]}; }
 };
+
+// fp32 by the bf16 matrix instructions: x = x1 + x2 + x3 in three bf16 parts, exactly (bf16x6.h), and six of the nine products -- what is left out is
+// below 2^-24 of |a b|, an fp32 product's own rounding.  6 / 16 of the native instruction's time.  An operand is three fragments, an image three 16-bit
+// images PLANE bytes apart; registers and LDS for that are there up to head size 64.
+struct Split3 {
+    typedef struct { bf16x8 p[3]; } Frag;
+    typedef f32x4 Quad;
+    typedef Mma<__bf16> B;
+    static constexpr int KS = 16;
+    __device__ static __forceinline__ f32x16 mma(const Frag& a, const Frag& b, f32x16 c) {
+        b6::mfma6(c, a.p, b.p);
+        return c;
+    }
+    template <int DP, int PLANE> __device__ static __forceinline__ Frag row(const char* img, int r, int s, int h) {
+        return Frag{{B::row<DP>(img, r, s, h), B::row<DP>(img + PLANE, r, s, h), B::row<DP>(img + 2 * PLANE, r, s, h)}};
+    }
+    template <int DP, int PLANE> __device__ static __forceinline__ Frag col(const char* img, int r0, int s, int dt, int lane) {
+        return Frag{{B::col<DP>(img, r0, s, dt, lane), B::col<DP>(img + PLANE, r0, s, dt, lane), B::col<DP>(img + 2 * PLANE, r0, s, dt, lane)}};
+    }
+    __device__ static __forceinline__ float value(const Frag& f, int e) { return (float)f.p[0][e] + ((float)f.p[1][e] + (float)f.p[2][e]); }
+    __device__ static __forceinline__ Frag of(const float (&v)[8]) {
+        Frag f;
+        b6::split8(v[0], v[1], v[2], v[3], v[4], v[5], v[6], v[7], f.p);
+        return f;
+    }
+    __device__ static __forceinline__ Frag from_acc(const f32x16& v, int s) {
+        const float t[8] = {v[8 * s], v[8 * s + 1], v[8 * s + 2], v[8 * s + 3], v[8 * s + 4], v[8 * s + 5], v[8 * s + 6], v[8 * s + 7]};
+        return of(t);
+    }
+};
+template <class T, int DP> constexpr bool SPLIT = sizeof(T) == 4 && DP <= SPLITMAX;
+template <class T, int DP> using Op = std::conditional_t<SPLIT<T, DP>, Split3, Mma<T>>;
 
 struct Ten { char* p; long long b, t, h; };        // strides in bytes
 
@@ -171,7 +210,7 @@ __device__ __forceinline__ void copy16(const char* base, unsigned off, unsigned 
 __device__ __forceinline__ void copy4(const char* src, unsigned lds) {
     asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dword %0, off" :: "v"(src), "s"(lds) : "memory", "m0");
 }
-__device__ __forceinline__ void copies_done() { asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); }
+__device__ __forceinline__ void copies_done() { asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory"); }
 __device__ __forceinline__ unsigned lds_offset(const void* p) {
     return __builtin_amdgcn_readfirstlane((unsigned)(size_t)(__attribute__((address_space(3))) const char*)p);
 }
@@ -219,17 +258,88 @@ __device__ __forceinline__ void zero_images(char* smem, int bytes) {  // (follow
     for (int i = threadIdx.x * 16; i < bytes; i += 256 * 16) *reinterpret_cast<uint4*>(smem + i) = uint4{0, 0, 0, 0};
     __syncthreads();
 }
+// Tiles of two tensors, one ahead: issue() starts the next one, commit() waits for it and for everyone's reads of the one before.  Copied past the
+// registers into two buffers in turn (one barrier), or, split into bf16 parts, through the registers into one (two).
+template <class T, int DP, int ROWS, bool S = SPLIT<T, DP>> struct Tiles {
+    static constexpr int IMG = ROWS * Image<T, DP>::PITCH, PLANE = 0, BYTES = 4 * IMG;
+    char* smem;
+    Stage<T, DP, ROWS> a, b;
+    int next = 0, ready = 0;
+    __device__ __forceinline__ Tiles(char* s, long long sta, long long stb, int D) : smem(s), a(sta, D), b(stb, D) {
+        if (D < DP) zero_images(smem, BYTES);
+    }
+    __device__ __forceinline__ void issue(const char* pa, const char* pb, unsigned long long bits) {
+        a.issue(smem + next * 2 * IMG, pa, bits);
+        b.issue(smem + next * 2 * IMG + IMG, pb, bits);
+    }
+    __device__ __forceinline__ void commit() {
+        copies_done();
+        __syncthreads();
+        ready = next;
+        next ^= 1;
+    }
+    __device__ __forceinline__ const char* img_a() const { return smem + ready * 2 * IMG; }
+    __device__ __forceinline__ const char* img_b() const { return img_a() + IMG; }
+};
+template <class T, int DP, int ROWS> struct Tiles<T, DP, ROWS, true> {
+    static constexpr int UNITS = DP / 8, N = ROWS * UNITS / 256, PLANE = ROWS * DP * 2, IMG = 3 * PLANE, BYTES = 2 * IMG;      // unit: 8 columns
+    static_assert(ROWS * UNITS % 256 == 0, "whole rounds");
+    char* smem;
+    long long st[2];
+    int D, next = 0, ready = 0;
+    f32x4 v[2][N][2];
+    __device__ __forceinline__ Tiles(char* s, long long sta, long long stb, int d) : smem(s), st{sta, stb}, D(d) {}
+    __device__ __forceinline__ void issue(const char* pa, const char* pb, unsigned long long bits) {
+#pragma unroll
+        for (int t = 0; t < 2; ++t)
+#pragma unroll
+            for (int i = 0; i < N; ++i) {
+                const int e = threadIdx.x + 256 * i, row = e / UNITS, c = e % UNITS;
+                const f32x4* src = reinterpret_cast<const f32x4*>((t ? pb : pa) + row * st[t] + c * 32);
+                const bool ok = ((bits >> row) & 1) && c * 8 < D;
+                v[t][i][0] = ok ? src[0] : f32x4{0.f, 0.f, 0.f, 0.f};
+                v[t][i][1] = ok ? src[1] : f32x4{0.f, 0.f, 0.f, 0.f};
+            }
+    }
+    __device__ __forceinline__ void commit() {
+        __syncthreads();
+#pragma unroll
+        for (int t = 0; t < 2; ++t)
+#pragma unroll
+            for (int i = 0; i < N; ++i) {
+                const int e = threadIdx.x + 256 * i, row = e / UNITS, c = e % UNITS;
+                const f32x4 x = v[t][i][0], y = v[t][i][1];
+                const float w[8] = {x[0], x[1], x[2], x[3], y[0], y[1], y[2], y[3]};
+                const Split3::Frag f = Split3::of(w);
+#pragma unroll
+                for (int k = 0; k < 3; ++k) *reinterpret_cast<bf16x8*>(smem + t * IMG + k * PLANE + Image<__bf16, DP>::off(row, c)) = f.p[k];
+            }
+        copies_done();
+        __syncthreads();
+        ready = next;
+        next ^= 1;
+    }
+    __device__ __forceinline__ const char* img_a() const { return smem; }
+    __device__ __forceinline__ const char* img_b() const { return smem + IMG; }
+};
 __device__ __forceinline__ unsigned long long first_bits(int n) { return n >= 64 ? ~0ull : n <= 0 ? 0ull : (1ull << n) - 1; }
 
 // operand fragments of one row (this lane's column of the product), zero where !ok
-template <class T, int DP>
-__device__ __forceinline__ void load_row(typename Mma<T>::Frag (&f)[DP / Mma<T>::KS], const char* row, int h, int D, bool ok) {
+template <class M, class T, int DP>
+__device__ __forceinline__ void load_row(typename M::Frag (&f)[DP / M::KS], const char* row, int h, int D, bool ok) {
 #pragma unroll
-    for (int s = 0; s < DP / Mma<T>::KS; ++s) {
-        uint4 v = {0, 0, 0, 0};
-        const int c = 2 * s + h;
-        if (ok && c * 16 < D * (int)sizeof(T)) v = *reinterpret_cast<const uint4*>(row + c * 16);
-        f[s] = __builtin_bit_cast(typename Mma<T>::Frag, v);
+    for (int s = 0; s < DP / M::KS; ++s) {
+        const int c = 2 * s + h;                                     // KS / 2 elements
+        if constexpr (std::is_same_v<M, Split3>) {
+            f32x4 x = {0.f, 0.f, 0.f, 0.f}, y = x;
+            if (ok && c * 8 < D) { x = reinterpret_cast<const f32x4*>(row + c * 32)[0]; y = reinterpret_cast<const f32x4*>(row + c * 32)[1]; }
+            const float w[8] = {x[0], x[1], x[2], x[3], y[0], y[1], y[2], y[3]};
+            f[s] = Split3::of(w);
+        } else {
+            uint4 v = {0, 0, 0, 0};
+            if (ok && c * 16 < D * (int)sizeof(T)) v = *reinterpret_cast<const uint4*>(row + c * 16);
+            f[s] = __builtin_bit_cast(typename M::Frag, v);
+        }
     }
 }
 
@@ -300,9 +410,10 @@ struct KeyBits {
 // Rows of a query block: row r = token r / group, head kvh * group + r % group, so that heads which share keys share the tile's loads.
 template <class T, int DP>
 __global__ __launch_bounds__(256, (WAVES<T, DP>)) void fwd_kernel(const Params p) {
-    typedef Mma<T> M;
-    constexpr int NF = DP / M::KS, NP = 32 / M::KS, ND = DP / 32, IMG = KB * Image<T, DP>::PITCH;
-    extern __shared__ __attribute__((aligned(16))) char smem[];       // [2][K, V]
+    typedef Op<T, DP> M;
+    typedef Tiles<T, DP, KB> Tl;
+    constexpr int NF = DP / M::KS, NP = 32 / M::KS, ND = DP / 32;
+    extern __shared__ __attribute__((aligned(16))) char smem[];       // tiles of K and V
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), l31 = lane & 31, h = lane >> 5;
     const Where w = where(p, true);
     const int rows = w.ql * p.group, r0 = w.tile * QB * p.group + w.sub * QB;       // (tokens < 2^31 / 128 a sequence is far beyond memory x heads)
@@ -322,7 +433,7 @@ __global__ __launch_bounds__(256, (WAVES<T, DP>)) void fwd_kernel(const Params p
     const char* const vbase = p.v.p + w.b * p.v.b + w.k0 * p.v.t + w.kvh * p.v.h;
     KeyBits kb{p.key_mask ? p.key_mask + w.b * p.mask_b + w.k0 : nullptr, w.kl, lane, 0};
     typename M::Frag qf[NF];
-    load_row<T, DP>(qf, p.q.p + w.b * p.q.b + (w.q0 + token) * p.q.t + head * p.q.h, h, p.D, rok);
+    load_row<M, T, DP>(qf, p.q.p + w.b * p.q.b + (w.q0 + token) * p.q.t + head * p.q.h, h, p.D, rok);
     f32x16 o[ND];
     clear(o);
     // Exponents in powers of two.  The running maximum m is only raised when a score exceeds it by 2^8, so the sums are rarely rescaled;
@@ -330,30 +441,26 @@ __global__ __launch_bounds__(256, (WAVES<T, DP>)) void fwd_kernel(const Params p
     const float c = p.scale * LOG2E, lift = is_f16<T>() ? 7.f : 0.f;
     float m = -INFINITY, l = 0.f;                                    // maximum (scaled), this lane's part of the sum
     unsigned long long cur = 0;
-    const Stage<T, DP> sk(p.k.t, p.D), sv(p.v.t, p.D);
-    if (p.D < DP) zero_images(smem, 4 * IMG);
-    auto issue = [&](int kt, int buf) {
+    Tl tl(smem, p.k.t, p.v.t, p.D);
+    auto issue = [&](int kt) {
         cur = kb.bits(kt);
-        sk.issue(smem + buf * 2 * IMG, kbase + kt * p.k.t, cur);
-        sv.issue(smem + buf * 2 * IMG + IMG, vbase + kt * p.v.t, cur);
+        tl.issue(kbase + kt * p.k.t, vbase + kt * p.v.t, cur);
         kb.fetch(kt + KB);
     };
-    if (kbegin < kend) { kb.fetch(kbegin); issue(kbegin, 0); }
-    int buf = 0;
-    for (int kt = kbegin; kt < kend; kt += KB, buf ^= 1) {
+    if (kbegin < kend) { kb.fetch(kbegin); issue(kbegin); }
+    for (int kt = kbegin; kt < kend; kt += KB) {
         const unsigned long long bits = cur;
-        copies_done();
-        __syncthreads();                                             // this tile is there, and everyone is done with the other buffer
-        if (kt + KB < kend) issue(kt + KB, buf ^ 1);
+        tl.commit();
+        if (kt + KB < kend) issue(kt + KB);
         if (rw >= rows || bits == 0 || (p.causal && kt > t_last + off)) continue;
-        const char* const img_k = smem + buf * 2 * IMG;
-        const char* const img_v = img_k + IMG;
+        const char* const img_k = tl.img_a();
+        const char* const img_v = tl.img_b();
         f32x16 st[2];
         clear(st);
 #pragma unroll
         for (int f = 0; f < NF; ++f)
 #pragma unroll
-            for (int sub = 0; sub < 2; ++sub) st[sub] = M::mma(M::template row<DP>(img_k, sub * 32 + l31, f, h), qf[f], st[sub]);
+            for (int sub = 0; sub < 2; ++sub) st[sub] = M::mma(M::template row<DP, Tl::PLANE>(img_k, sub * 32 + l31, f, h), qf[f], st[sub]);
         if (bits != ~0ull || (p.causal && kt + KB - 1 > t_first + off)) {
             const int last = p.causal ? token + off - kt : KB;       // last visible key of the tile
 #pragma unroll
@@ -390,7 +497,7 @@ __global__ __launch_bounds__(256, (WAVES<T, DP>)) void fwd_kernel(const Params p
             for (int f = 0; f < NP; ++f) {
                 const typename M::Frag pf = M::from_acc(st[sub], f);
 #pragma unroll
-                for (int dt = 0; dt < ND; ++dt) o[dt] = M::mma(M::template col<DP>(img_v, sub * 32, f, dt, lane), pf, o[dt]);
+                for (int dt = 0; dt < ND; ++dt) o[dt] = M::mma(M::template col<DP, Tl::PLANE>(img_v, sub * 32, f, dt, lane), pf, o[dt]);
             }
     }
     l += other_half(l);
@@ -439,7 +546,7 @@ __global__ __launch_bounds__(256) void few_kernel(const Params p) {
     const char* const vbase = p.v.p + w.b * p.v.b + w.k0 * p.v.t + w.kvh * p.v.h;
     KeyBits kb{p.key_mask ? p.key_mask + w.b * p.mask_b + w.k0 : nullptr, w.kl, lane, 0};
     typename M::Frag qf[NF];
-    load_row<T, DP>(qf, p.q.p + w.b * p.q.b + (w.q0 + token) * p.q.t + head * p.q.h, h, p.D, rok);
+    load_row<M, T, DP>(qf, p.q.p + w.b * p.q.b + (w.q0 + token) * p.q.t + head * p.q.h, h, p.D, rok);
     const Stage<T, DP, 32, 64> sk(p.k.t, p.D), sv(p.v.t, p.D);
     if (p.D < DP) zero_images(smem, 16 * IMG);
     f32x16 o[ND];
@@ -618,10 +725,11 @@ __global__ __launch_bounds__(256) void fwd_join_kernel(const Params p) {
 // 256 keys -- where dP and D are of one size -- are swept once for D alone before they are swept for dQ.
 template <class T, int DP>
 __global__ __launch_bounds__(256, (WAVES<T, DP>)) void dq_kernel(const Params p) {
-    typedef Mma<T> M;
-    constexpr int NF = DP / M::KS, NP = 32 / M::KS, ND = DP / 32, IMG = KB * Image<T, DP>::PITCH;
+    typedef Op<T, DP> M;
+    typedef Tiles<T, DP, KB> Tl;
+    constexpr int NF = DP / M::KS, NP = 32 / M::KS, ND = DP / 32;
     constexpr bool FIX = sizeof(T) == 2;
-    extern __shared__ __attribute__((aligned(16))) char smem[];       // [2][K, V]
+    extern __shared__ __attribute__((aligned(16))) char smem[];       // tiles of K and V
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), l31 = lane & 31, h = lane >> 5;
     const Where w = where(p, true);
     const int rows = w.ql * p.group, r0 = w.tile * QB * p.group + w.sub * QB;
@@ -645,12 +753,12 @@ __global__ __launch_bounds__(256, (WAVES<T, DP>)) void dq_kernel(const Params p)
     const bool sees = lse != -INFINITY;                              // (a row that sees nothing takes no part, whatever it holds)
     const float lse2 = sees ? lse * LOG2E : INFINITY;
     typename M::Frag qf[NF], gf[NF];
-    load_row<T, DP>(qf, p.q.p + w.b * p.q.b + (w.q0 + token) * p.q.t + head * p.q.h, h, p.D, rok);
-    load_row<T, DP>(gf, p.dout.p + w.b * p.dout.b + (w.q0 + token) * p.dout.t + head * p.dout.h, h, p.D, rok);
+    load_row<M, T, DP>(qf, p.q.p + w.b * p.q.b + (w.q0 + token) * p.q.t + head * p.q.h, h, p.D, rok);
+    load_row<M, T, DP>(gf, p.dout.p + w.b * p.dout.b + (w.q0 + token) * p.dout.t + head * p.dout.h, h, p.D, rok);
     float nd = 0.f, rho = 0.f;                                       // -D, what D still misses (times sc)
     {
         typename M::Frag of[NF];
-        load_row<T, DP>(of, p.out.p + w.b * p.out.b + (w.q0 + token) * p.out.t + head * p.out.h, h, p.D, rok);
+        load_row<M, T, DP>(of, p.out.p + w.b * p.out.b + (w.q0 + token) * p.out.t + head * p.out.h, h, p.D, rok);
         if (!sees) {
 #pragma unroll
             for (int f = 0; f < NF; ++f) qf[f] = gf[f] = of[f] = typename M::Frag{};
@@ -658,7 +766,7 @@ __global__ __launch_bounds__(256, (WAVES<T, DP>)) void dq_kernel(const Params p)
 #pragma unroll
         for (int f = 0; f < NF; ++f)
 #pragma unroll
-            for (int e = 0; e < M::KS / 2; ++e) nd = __builtin_fmaf(-(float)of[f][e], (float)gf[f][e], nd);
+            for (int e = 0; e < M::KS / 2; ++e) nd = __builtin_fmaf(-M::value(of[f], e), M::value(gf[f], e), nd);
         nd += other_half(nd);
     }
     f32x16 acc[ND];
@@ -666,30 +774,27 @@ __global__ __launch_bounds__(256, (WAVES<T, DP>)) void dq_kernel(const Params p)
     const float c = p.scale * LOG2E;
     float sc = is_f16<T>() ? 0x1p60f : 1.f, shift = lse2 - (is_f16<T>() ? 60.f : 0.f);      // (fp16: the exponent brings the column's power of two along)
     unsigned long long cur = 0;
-    const Stage<T, DP> sk(p.k.t, p.D), sv(p.v.t, p.D);
-    if (p.D < DP) zero_images(smem, 4 * IMG);
-    auto issue = [&](int kt, int buf) {
+    Tl tl(smem, p.k.t, p.v.t, p.D);
+    auto issue = [&](int kt) {
         cur = kb.bits(kt);
-        sk.issue(smem + buf * 2 * IMG, kbase + kt * p.k.t, cur);
-        sv.issue(smem + buf * 2 * IMG + IMG, vbase + kt * p.v.t, cur);
+        tl.issue(kbase + kt * p.k.t, vbase + kt * p.v.t, cur);
     };
     const int tiles = kend > kbegin ? (kend - kbegin + KB - 1) / KB : 0;
     const int first = FIX && p.splits == 1 && tiles <= 4 ? tiles : 0;             // tiles of the sweep for D alone
     auto key = [&](int i) { return kbegin + (i < first ? i : i - first) * KB; };
-    if (tiles) { kb.fetch(key(0)); issue(key(0), 0); if (first + tiles > 1) kb.fetch(key(1)); }
+    if (tiles) { kb.fetch(key(0)); issue(key(0)); if (first + tiles > 1) kb.fetch(key(1)); }
     for (int i = 0; i < first + tiles; ++i) {
         const unsigned long long bits = cur;
-        const int kt = key(i), buf = i & 1;
-        copies_done();
-        __syncthreads();
+        const int kt = key(i);
+        tl.commit();
         if (i + 1 < first + tiles) {
-            issue(key(i + 1), buf ^ 1);
+            issue(key(i + 1));
             if (i + 2 < first + tiles) kb.fetch(key(i + 2));
         }
         if (FIX && i == first && first) { nd -= (rho + other_half(rho)) / sc; rho = 0.f; }
         if (rw >= rows || bits == 0 || (p.causal && kt > t_last + off)) continue;
-        const char* const img_k = smem + buf * 2 * IMG;
-        const char* const img_v = img_k + IMG;
+        const char* const img_k = tl.img_a();
+        const char* const img_v = tl.img_b();
         const bool partial = bits != ~0ull || (p.causal && kt + KB - 1 > t_first + off);
         const int last = p.causal ? token + off - kt : KB;
 #pragma unroll 1
@@ -699,8 +804,8 @@ __global__ __launch_bounds__(256, (WAVES<T, DP>)) void dq_kernel(const Params p)
             for (int x = 0; x < 16; ++x) { st[x] = 0.f; dp[x] = nd; }
 #pragma unroll
             for (int f = 0; f < NF; ++f) {
-                st = M::mma(M::template row<DP>(img_k, sub * 32 + l31, f, h), qf[f], st);
-                dp = M::mma(M::template row<DP>(img_v, sub * 32 + l31, f, h), gf[f], dp);
+                st = M::mma(M::template row<DP, Tl::PLANE>(img_k, sub * 32 + l31, f, h), qf[f], st);
+                dp = M::mma(M::template row<DP, Tl::PLANE>(img_v, sub * 32 + l31, f, h), gf[f], dp);
             }
 #pragma unroll
             for (int x = 0; x < 16; ++x) st[x] = __builtin_amdgcn_exp2f(__builtin_fmaf(st[x], c, -shift)) * dp[x];
@@ -726,7 +831,7 @@ __global__ __launch_bounds__(256, (WAVES<T, DP>)) void dq_kernel(const Params p)
             for (int f = 0; f < NP; ++f) {
                 const typename M::Frag df = M::from_acc(st, f);
 #pragma unroll
-                for (int dt = 0; dt < ND; ++dt) acc[dt] = M::mma(M::template col<DP>(img_k, sub * 32, f, dt, lane), df, acc[dt]);
+                for (int dt = 0; dt < ND; ++dt) acc[dt] = M::mma(M::template col<DP, Tl::PLANE>(img_k, sub * 32, f, dt, lane), df, acc[dt]);
             }
         }
     }
@@ -759,12 +864,14 @@ __global__ __launch_bounds__(256) void dq_join_kernel(const Params p) {
 
 template <class T, int DP>
 __global__ __launch_bounds__(256, (DKV_WAVES<T, DP>)) void dkv_kernel(const Params p) {
-    typedef Mma<T> M;
-    constexpr int NF = DP / M::KS, NP = 32 / M::KS, ND = DP / 32, R = RB<T, DP>, IMG = R * Image<T, DP>::PITCH;
+    constexpr int R = RB<T, DP>;
+    typedef Op<T, DP> M;
+    typedef Tiles<T, DP, R> Tl;
+    constexpr int NF = DP / M::KS, NP = 32 / M::KS, ND = DP / 32;
     constexpr bool VL = V_LDS<T, DP>;
     constexpr int UN = DP * (int)sizeof(T) <= 128 ? 2 : 1;           // (more would spill)
-    extern __shared__ __attribute__((aligned(16))) char smem[];       // [2][Q, dO], [2][lse2, -D][64], then the waves' V fragments
-    float* const s_row = reinterpret_cast<float*>(smem + 4 * IMG);
+    extern __shared__ __attribute__((aligned(16))) char smem[];       // tiles of Q and dO, [2][lse2, -D][64], then the waves' V fragments
+    float* const s_row = reinterpret_cast<float*>(smem + Tl::BYTES);
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), l31 = lane & 31, h = lane >> 5;
     const Where w = where(p, false);
     if (w.tile * QB >= w.kl) return;
@@ -774,9 +881,9 @@ __global__ __launch_bounds__(256, (DKV_WAVES<T, DP>)) void dkv_kernel(const Para
     const long long row = w.k0 + (in ? kj : 0);
     const bool live = in && (!p.key_mask || p.key_mask[w.b * p.mask_b + row]);
     typename M::Frag kf[NF], vf[NF];
-    load_row<T, DP>(kf, p.k.p + w.b * p.k.b + row * p.k.t + w.kvh * p.k.h, h, p.D, live);
-    load_row<T, DP>(vf, p.v.p + w.b * p.v.b + row * p.v.t + w.kvh * p.v.h, h, p.D, live);
-    typename M::Frag* const s_v = reinterpret_cast<typename M::Frag*>(smem + 4 * IMG + 1024) + wave * NF * 64 + lane;     // (each lane its own)
+    load_row<M, T, DP>(kf, p.k.p + w.b * p.k.b + row * p.k.t + w.kvh * p.k.h, h, p.D, live);
+    load_row<M, T, DP>(vf, p.v.p + w.b * p.v.b + row * p.v.t + w.kvh * p.v.h, h, p.D, live);
+    typename M::Frag* const s_v = reinterpret_cast<typename M::Frag*>(smem + Tl::BYTES + 1024) + wave * NF * 64 + lane;     // (each lane its own)
     if (VL) {
 #pragma unroll
         for (int f = 0; f < NF; ++f) s_v[f * 64] = vf[f];
@@ -798,50 +905,47 @@ __global__ __launch_bounds__(256, (DKV_WAVES<T, DP>)) void dkv_kernel(const Para
     struct At { int head, qt; } next{w.kvh * p.group, qbegin};
     if (step < steps) { next.head += step / per_head; next.qt += step % per_head * R; }
     auto advance = [&](At a) { return a.qt + R < w.ql ? At{a.head, a.qt + R} : At{a.head + 1, qbegin}; };
-    const Stage<T, DP, R> sq(p.q.t, p.D), sg(p.dout.t, p.D);
+    Tl tl(smem, p.q.t, p.dout.t, p.D);
     const char* const qbase = p.q.p + w.b * p.q.b + w.q0 * p.q.t;
     const char* const gbase = p.dout.p + w.b * p.dout.b + w.q0 * p.dout.t;
     const long long first_row = w.b * p.lse_b + w.q0;
-    if (p.D < DP) zero_images(smem, 4 * IMG);
     // Rows that see nothing are not read (their lse2 is +inf).  Under a causal mask alone they lie before qbegin; a key mask can leave any
     // row empty, so its lse2 is looked at first, a tile ahead.
     float ahead = 0.f;
     auto fetch = [&](At a) {
         if (p.key_mask) ahead = a.qt + lane < w.ql ? p.lse2[first_row + a.head * p.lse_h + a.qt + lane] : INFINITY;
     };
-    auto issue = [&](At a, int buf) {
+    auto issue = [&](At a) {
         const long long at = first_row + a.head * p.lse_h + a.qt + lane;
         const unsigned long long bits = p.key_mask ? __ballot(ahead != INFINITY) : first_bits(w.ql - a.qt);
-        sq.issue(smem + buf * 2 * IMG, qbase + a.qt * p.q.t + a.head * p.q.h, bits);
-        sg.issue(smem + buf * 2 * IMG + IMG, gbase + a.qt * p.dout.t + a.head * p.dout.h, bits);
+        tl.issue(qbase + a.qt * p.q.t + a.head * p.q.h, gbase + a.qt * p.dout.t + a.head * p.dout.h, bits);
         const bool there = (bits >> lane) & 1;                       // (R = 32: the upper half is never read)
-        if (wave == 0) copy4(reinterpret_cast<const char*>(there ? p.lse2 + at : FILL + 4), lds_offset(s_row + buf * 128));
-        if (wave == 1) copy4(reinterpret_cast<const char*>(there ? p.ndelta + at : FILL), lds_offset(s_row + buf * 128 + 64));
+        if (wave == 0) copy4(reinterpret_cast<const char*>(there ? p.lse2 + at : FILL + 4), lds_offset(s_row + tl.next * 128));
+        if (wave == 1) copy4(reinterpret_cast<const char*>(there ? p.ndelta + at : FILL), lds_offset(s_row + tl.next * 128 + 64));
     };
     At now = next;
     if (step < steps) {
         fetch(now);
-        issue(now, 0);
+        issue(now);
         next = advance(now);
         if (step + 1 < steps) fetch(next);
     }
-    for (int buf = 0; step < steps; ++step, buf ^= 1) {
+    for (; step < steps; ++step) {
         const int qt = now.qt;
-        copies_done();
-        __syncthreads();
+        tl.commit();
         if (step + 1 < steps) {
-            issue(next, buf ^ 1);
+            issue(next);
             now = next;
             next = advance(next);
             if (step + 2 < steps) fetch(next);
         }
         if (kw >= w.kl || (p.causal && qt + R - 1 < kw - off)) continue;
-        const char* const img_q = smem + buf * 2 * IMG;
-        const char* const img_g = img_q + IMG;
+        const char* const img_q = tl.img_a();
+        const char* const img_g = tl.img_b();
         const bool partial = p.causal && kw + 31 - off > qt;
 #pragma unroll UN
         for (int sub = 0; sub < R / 32; ++sub) {
-            const float* const sl = s_row + buf * 128 + sub * 32 + 4 * h;
+            const float* const sl = s_row + tl.ready * 128 + sub * 32 + 4 * h;
             f32x16 st, dp;
 #pragma unroll
             for (int g = 0; g < 4; ++g) {
@@ -851,8 +955,8 @@ __global__ __launch_bounds__(256, (DKV_WAVES<T, DP>)) void dkv_kernel(const Para
             }
 #pragma unroll
             for (int f = 0; f < NF; ++f) {
-                st = M::mma(M::template row<DP>(img_q, sub * 32 + l31, f, h), kf[f], st);
-                dp = M::mma(M::template row<DP>(img_g, sub * 32 + l31, f, h), VL ? s_v[f * 64] : vf[f], dp);
+                st = M::mma(M::template row<DP, Tl::PLANE>(img_q, sub * 32 + l31, f, h), kf[f], st);
+                dp = M::mma(M::template row<DP, Tl::PLANE>(img_g, sub * 32 + l31, f, h), VL ? s_v[f * 64] : vf[f], dp);
             }
 #pragma unroll
             for (int g = 0; g < 4; ++g) {
@@ -876,8 +980,8 @@ __global__ __launch_bounds__(256, (DKV_WAVES<T, DP>)) void dkv_kernel(const Para
                 const typename M::Frag pf = M::from_acc(st, f), df = M::from_acc(dp, f);
 #pragma unroll
                 for (int dt = 0; dt < ND; ++dt) {
-                    dv[dt] = M::mma(M::template col<DP>(img_g, sub * 32, f, dt, lane), pf, dv[dt]);
-                    dk[dt] = M::mma(M::template col<DP>(img_q, sub * 32, f, dt, lane), df, dk[dt]);
+                    dv[dt] = M::mma(M::template col<DP, Tl::PLANE>(img_g, sub * 32, f, dt, lane), pf, dv[dt]);
+                    dk[dt] = M::mma(M::template col<DP, Tl::PLANE>(img_q, sub * 32, f, dt, lane), df, dk[dt]);
                 }
             }
         }
@@ -934,7 +1038,7 @@ constexpr int JOIN = QB / Join<4>::ROWS;                             // most wor
 
 template <class T, int DP>
 int run_fwd(const Params& p, hipStream_t s) {
-    constexpr int lds = 4 * KB * Image<T, DP>::PITCH;
+    constexpr int lds = Tiles<T, DP, KB>::BYTES;
     if constexpr (FEW<T, DP>) {
         if (p.few) {
             constexpr int lds_few = std::max(16 * 32 * Image<T, DP>::PITCH, 4 * 32 * ((DP + 4) * 4 + 8));
@@ -955,7 +1059,7 @@ int run_fwd(const Params& p, hipStream_t s) {
 
 template <class T, int DP>
 int run_bwd(const Params& pq, const Params& pk, hipStream_t s) {
-    constexpr int lds = 4 * KB * Image<T, DP>::PITCH, lds_k = 4 * RB<T, DP> * Image<T, DP>::PITCH + 1024 + (V_LDS<T, DP> ? QB * Image<T, DP>::PITCH : 0);
+    constexpr int lds = Tiles<T, DP, KB>::BYTES, lds_k = Tiles<T, DP, RB<T, DP>>::BYTES + 1024 + (V_LDS<T, DP> ? QB * Image<T, DP>::PITCH : 0);
     static DeviceOnce once;
     if (!once) {
         DPC_HIP(hipFuncSetAttribute((const void*)dq_kernel<T, DP>, hipFuncAttributeMaxDynamicSharedMemorySize, lds));
