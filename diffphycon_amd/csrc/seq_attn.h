@@ -26,9 +26,6 @@ namespace seqattn {
 
 constexpr float LOG2E = 1.4426950408889634f, LN2 = 0.6931471805599453f;
 constexpr int QB = 128;        // rows (queries, or keys in the dK/dV kernel) of a workgroup: 4 waves x 32
-#ifndef SPLITMAX
-#define SPLITMAX 64
-#endif
 constexpr int KB = 64;         // rows of the tile that is staged in LDS
 
 __device__ __forceinline__ int rowmap(int r, int h) { return (r & 3) + 8 * (r >> 2) + 4 * h; }
@@ -112,7 +109,7 @@ template <> struct Mma<float> {
 
 // fp32 by the bf16 matrix instructions: x = x1 + x2 + x3 in three bf16 parts, exactly (bf16x6.h), and six of the nine products -- what is left out is
 // below 2^-24 of |a b|, an fp32 product's own rounding.  6 / 16 of the native instruction's time.  An operand is three fragments, an image three 16-bit
-// images PLANE bytes apart; registers and LDS for that are there up to head size 64.
+// images PLANE bytes apart.
 struct Split3 {
     typedef struct { bf16x8 p[3]; } Frag;
     typedef f32x4 Quad;
@@ -139,7 +136,7 @@ struct Split3 {
         return of(t);
     }
 };
-template <class T, int DP> constexpr bool SPLIT = sizeof(T) == 4 && DP <= SPLITMAX;
+template <class T, int DP> constexpr bool SPLIT = sizeof(T) == 4;
 template <class T, int DP> using Op = std::conditional_t<SPLIT<T, DP>, Split3, Mma<T>>;
 
 struct Ten { char* p; long long b, t, h; };        // strides in bytes
@@ -396,7 +393,7 @@ template <class T, int DP> constexpr int WAVES = DP * sizeof(T) <= 128 ? 3 : siz
 template <class T, int DP> constexpr int DKV_WAVES = WAVES<T, DP> < 2 ? 1 : 2;
 // dK/dV at head size 128: the two sums alone take 128 registers; the values' fragments wait in LDS (V_LDS) and the staged tile has 32 rows
 template <class T, int DP> constexpr bool V_LDS = DP == 128;
-template <class T, int DP> constexpr int RB = V_LDS<T, DP> ? 32 : 64;
+template <class T, int DP> constexpr int RB = DP == 128 ? 32 : 64;
 
 // The keys of a tile that take part, one tile ahead: without a key mask by the sequence's end, with one by a byte a lane
 struct KeyBits {
@@ -1059,7 +1056,8 @@ int run_fwd(const Params& p, hipStream_t s) {
 
 template <class T, int DP>
 int run_bwd(const Params& pq, const Params& pk, hipStream_t s) {
-    constexpr int lds = Tiles<T, DP, KB>::BYTES, lds_k = Tiles<T, DP, RB<T, DP>>::BYTES + 1024 + (V_LDS<T, DP> ? QB * Image<T, DP>::PITCH : 0);
+    constexpr int lds = Tiles<T, DP, KB>::BYTES, lds_k = Tiles<T, DP, RB<T, DP>>::BYTES + 1024 + (V_LDS<T, DP> ? 256 * (DP / Op<T, DP>::KS) * (int)sizeof(typename Op<T, DP>::Frag) : 0);
+    static_assert(lds_k <= 160 * 1024, "LDS of a CU");
     static DeviceOnce once;
     if (!once) {
         DPC_HIP(hipFuncSetAttribute((const void*)dq_kernel<T, DP>, hipFuncAttributeMaxDynamicSharedMemorySize, lds));
