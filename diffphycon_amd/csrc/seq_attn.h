@@ -212,6 +212,22 @@ __device__ __forceinline__ unsigned lds_offset(const void* p) {
     return __builtin_amdgcn_readfirstlane((unsigned)(size_t)(__attribute__((address_space(3))) const char*)p);
 }
 
+// Bits of 64 rows, tested by 32-bit shifts alone: a 64-bit shift whose amount is the last vector register that a wave has reads register 0 instead
+// when the wave's registers end the register file (seen in the fp32 kernel of 256 registers: masked keys counted; the build refuses such a shift).
+__device__ __forceinline__ bool bit(unsigned long long bits, int r) { return ((r & 32 ? (unsigned)(bits >> 32) : (unsigned)bits) >> (r & 31)) & 1; }
+// Which of the rows 32 sub + rowmap(x, h) of a tile take part: bit (x & 3) + 8 (x >> 2); `last` is the last one that this lane may see
+__device__ __forceinline__ unsigned part_of(unsigned long long bits, int sub, int last, int h) {
+    const unsigned word = sub ? (unsigned)(bits >> 32) : (unsigned)bits;
+    const int n = last + 1 - 32 * sub;
+    return (n <= 0 ? 0u : word & (~0u >> (32 - min(n, 32)))) >> (4 * h);
+}
+__device__ __forceinline__ unsigned all_or_none(unsigned part, int x) { return (unsigned)__builtin_amdgcn_sbfe((int)part, (x & 3) + 8 * (x >> 2), 1); }
+// v where the row takes part, else `other`
+__device__ __forceinline__ float where_part(unsigned part, int x, float v, float other) {
+    const unsigned m = all_or_none(part, x);
+    return __uint_as_float((__float_as_uint(v) & m) | (__float_as_uint(other) & ~m));
+}
+
 // ROWS x DP tiles of one tensor, global -> LDS by NT threads (a workgroup, or each wave its own).  The tile's base is the wave's, a lane adds one
 // 32-bit offset (64 rows stay within 2^31 bytes: checked at the entry), so a whole tile costs no address arithmetic.  Rows whose bit is 0
 // become zero; columns >= D are never written: zero_images() clears them once.
@@ -246,7 +262,7 @@ struct Stage {
 #pragma unroll
         for (int i = 0; i < N; ++i) {
             const char* src = base + (EVEN ? i * STEP * st : 0) + off[EVEN ? 0 : i];
-            if (!((bits >> row(i)) & 1)) src = reinterpret_cast<const char*>(FILL);
+            if (!bit(bits, row(i))) src = reinterpret_cast<const char*>(FILL);
             if (col(i) < width) copy16(src, at + i * NT * 16);
         }
     }
@@ -293,7 +309,7 @@ template <class T, int DP, int ROWS> struct Tiles<T, DP, ROWS, true> {
             for (int i = 0; i < N; ++i) {
                 const int e = threadIdx.x + 256 * i, row = e / UNITS, c = e % UNITS;
                 const f32x4* src = reinterpret_cast<const f32x4*>((t ? pb : pa) + row * st[t] + c * 32);
-                const bool ok = ((bits >> row) & 1) && c * 8 < D;
+                const bool ok = bit(bits, row) && c * 8 < D;
                 v[t][i][0] = ok ? src[0] : f32x4{0.f, 0.f, 0.f, 0.f};
                 v[t][i][1] = ok ? src[1] : f32x4{0.f, 0.f, 0.f, 0.f};
             }
@@ -461,12 +477,11 @@ __global__ __launch_bounds__(256, (WAVES<T, DP>)) void fwd_kernel(const Params p
         if (bits != ~0ull || (p.causal && kt + KB - 1 > t_first + off)) {
             const int last = p.causal ? token + off - kt : KB;       // last visible key of the tile
 #pragma unroll
-            for (int sub = 0; sub < 2; ++sub)
+            for (int sub = 0; sub < 2; ++sub) {
+                const unsigned part = part_of(bits, sub, last, h);
 #pragma unroll
-                for (int x = 0; x < 16; ++x) {
-                    const int j = sub * 32 + rowmap(x, h);
-                    if (!((bits >> j) & 1) || j > last) st[sub][x] = -INFINITY;
-                }
+                for (int x = 0; x < 16; ++x) st[sub][x] = where_part(part, x, st[sub][x], -INFINITY);
+            }
         }
         float tm = fmaxf(st[0][0], st[1][0]);
 #pragma unroll
@@ -571,12 +586,9 @@ __global__ __launch_bounds__(256) void few_kernel(const Params p) {
 #pragma unroll
         for (int f = 0; f < NF; ++f) st[0] = M::mma(M::template row<DP>(img_k, l31, f, h), qf[f], st[0]);
         if (bits != ~0u || (p.causal && kt + 31 > off)) {
-            const int last = p.causal ? token + off - kt : 32;
+            const unsigned part = part_of(bits, 0, p.causal ? token + off - kt : 32, h);
 #pragma unroll
-            for (int x = 0; x < 16; ++x) {
-                const int j = rowmap(x, h);
-                if (!((bits >> j) & 1) || j > last) st[0][x] = -INFINITY;
-            }
+            for (int x = 0; x < 16; ++x) st[0][x] = where_part(part, x, st[0][x], -INFINITY);
         }
         float tm = st[0][0];
 #pragma unroll
@@ -718,8 +730,9 @@ __global__ __launch_bounds__(256) void fwd_join_kernel(const Params p) {
 }
 
 // dQ, and for the dK/dV kernel lse2 and -D.  D = sum_d dO O with the 16-bit O misses what O's rounding lost; since the probabilities of a
-// row add up to 1, sum_j P (dP - D) is exactly that error, so the sweep adds it up and hands the corrected D on.  Rows that see at most
-// 256 keys -- where dP and D are of one size -- are swept once for D alone before they are swept for dQ.
+// row add up to 1, sum_j P (dP - D) is exactly that error, so the sweep adds it up and hands the corrected D on.  Where a block sees at most
+// 256 keys -- dP and D are of one size then, and a row of one or two keys has nothing but their difference -- it is swept once for D alone
+// before it is swept for dQ.  fp32 does so up to one tile, for the rows of few keys alone.
 template <class T, int DP>
 __global__ __launch_bounds__(256, (WAVES<T, DP>)) void dq_kernel(const Params p) {
     typedef Op<T, DP> M;
@@ -737,7 +750,8 @@ __global__ __launch_bounds__(256, (WAVES<T, DP>)) void dq_kernel(const Params p)
     const int head = w.kvh * p.group + p.by_group.take(token);
     const int t_first = p.by_group(rw), t_last = p.by_group(rw + 31);
     int kend = p.causal ? min(w.kl, min((int)p.by_group(r0 + QB - 1), w.ql - 1) + 1 + off) : w.kl, kbegin = 0;
-    if (p.splits > 1) {
+    const int kall = kend;
+    if (p.splits > 1) {                                              // as in the forward: at most 256 keys are one split's
         const int per = max(4, (max(kend, 0) + KB * p.splits - 1) / (KB * p.splits)) * KB;
         kbegin = w.split * per;
         kend = min(kend, kbegin + per);
@@ -775,51 +789,61 @@ __global__ __launch_bounds__(256, (WAVES<T, DP>)) void dq_kernel(const Params p)
     auto issue = [&](int kt) {
         cur = kb.bits(kt);
         tl.issue(kbase + kt * p.k.t, vbase + kt * p.v.t, cur);
+        kb.fetch(kt + KB);
     };
-    const int tiles = kend > kbegin ? (kend - kbegin + KB - 1) / KB : 0;
-    const int first = FIX && p.splits == 1 && tiles <= 4 ? tiles : 0;             // tiles of the sweep for D alone
-    auto key = [&](int i) { return kbegin + (i < first ? i : i - first) * KB; };
-    if (tiles) { kb.fetch(key(0)); issue(key(0)); if (first + tiles > 1) kb.fetch(key(1)); }
-    for (int i = 0; i < first + tiles; ++i) {
-        const unsigned long long bits = cur;
-        const int kt = key(i);
-        tl.commit();
-        if (i + 1 < first + tiles) {
-            issue(key(i + 1));
-            if (i + 2 < first + tiles) kb.fetch(key(i + 2));
+    // P (dP - D) of the tile's keys 32 sub .. (times sc)
+    auto terms = [&](f32x16& st, unsigned long long bits, int kt, int sub) {
+        f32x16 dp;
+#pragma unroll
+        for (int x = 0; x < 16; ++x) { st[x] = 0.f; dp[x] = nd; }
+#pragma unroll
+        for (int f = 0; f < NF; ++f) {
+            st = M::mma(M::template row<DP, Tl::PLANE>(tl.img_a(), sub * 32 + l31, f, h), qf[f], st);
+            dp = M::mma(M::template row<DP, Tl::PLANE>(tl.img_b(), sub * 32 + l31, f, h), gf[f], dp);
         }
-        if (FIX && i == first && first) { nd -= (rho + other_half(rho)) / sc; rho = 0.f; }
-        if (rw >= rows || bits == 0 || (p.causal && kt > t_last + off)) continue;
-        const char* const img_k = tl.img_a();
-        const char* const img_v = tl.img_b();
-        const bool partial = bits != ~0ull || (p.causal && kt + KB - 1 > t_first + off);
-        const int last = p.causal ? token + off - kt : KB;
+#pragma unroll
+        for (int x = 0; x < 16; ++x) st[x] = __builtin_amdgcn_exp2f(__builtin_fmaf(st[x], c, -shift)) * dp[x];
+        if (bits != ~0ull || (p.causal && kt + KB - 1 > t_first + off)) {
+            const unsigned part = part_of(bits, sub, p.causal ? token + off - kt : KB, h);
+#pragma unroll
+            for (int x = 0; x < 16; ++x) st[x] = where_part(part, x, st[x], 0.f);
+        }
+    };
+    auto add = [&](const f32x16& st) {
+        float a = 0.f;
+#pragma unroll
+        for (int x = 0; x < 16; ++x) a += st[x];
+        rho += a;
+    };
+    auto none = [&](unsigned long long bits, int kt) { return rw >= rows || bits == 0 || (p.causal && kt > t_last + off); };
+    if (kbegin < kend) { kb.fetch(kbegin); issue(kbegin); }
+    if (kbegin == 0 && kend == kall && kall > 0 && kall <= (FIX ? 4 : 1) * KB) {                  // the sweep for D alone
+        for (int kt = 0; kt < kall; kt += KB) {
+            const unsigned long long bits = cur;
+            tl.commit();
+            if (kt + KB >= kall) kb.fetch(0);
+            issue(kt + KB < kall ? kt + KB : 0);
+            if (none(bits, kt)) continue;
+#pragma unroll 1
+            for (int sub = 0; sub < 2; ++sub) {
+                f32x16 st;
+                terms(st, bits, kt, sub);
+                add(st);
+            }
+        }
+        nd -= (rho + other_half(rho)) / sc;
+        rho = 0.f;
+    }
+    for (int kt = kbegin; kt < kend; kt += KB) {
+        const unsigned long long bits = cur;
+        tl.commit();
+        if (kt + KB < kend) issue(kt + KB);
+        if (none(bits, kt)) continue;
 #pragma unroll 1
         for (int sub = 0; sub < 2; ++sub) {
-            f32x16 st, dp;
-#pragma unroll
-            for (int x = 0; x < 16; ++x) { st[x] = 0.f; dp[x] = nd; }
-#pragma unroll
-            for (int f = 0; f < NF; ++f) {
-                st = M::mma(M::template row<DP, Tl::PLANE>(img_k, sub * 32 + l31, f, h), qf[f], st);
-                dp = M::mma(M::template row<DP, Tl::PLANE>(img_v, sub * 32 + l31, f, h), gf[f], dp);
-            }
-#pragma unroll
-            for (int x = 0; x < 16; ++x) st[x] = __builtin_amdgcn_exp2f(__builtin_fmaf(st[x], c, -shift)) * dp[x];
-            if (partial) {
-#pragma unroll
-                for (int x = 0; x < 16; ++x) {
-                    const int j = sub * 32 + rowmap(x, h);
-                    if (!((bits >> j) & 1) || j > last) st[x] = 0.f;
-                }
-            }
-            if (FIX) {
-                float a = 0.f;
-#pragma unroll
-                for (int x = 0; x < 16; ++x) a += st[x];
-                rho += a;
-                if (i < first) continue;
-            }
+            f32x16 st;
+            terms(st, bits, kt, sub);
+            if (FIX) add(st);
             if (is_f16<T>()) {
                 const float by = shrink_col(st, acc);
                 if (by != 1.f) { sc *= by; rho *= by; shift = lse2 - __builtin_amdgcn_logf(sc); }
@@ -828,7 +852,7 @@ __global__ __launch_bounds__(256, (WAVES<T, DP>)) void dq_kernel(const Params p)
             for (int f = 0; f < NP; ++f) {
                 const typename M::Frag df = M::from_acc(st, f);
 #pragma unroll
-                for (int dt = 0; dt < ND; ++dt) acc[dt] = M::mma(M::template col<DP, Tl::PLANE>(img_k, sub * 32, f, dt, lane), df, acc[dt]);
+                for (int dt = 0; dt < ND; ++dt) acc[dt] = M::mma(M::template col<DP, Tl::PLANE>(tl.img_a(), sub * 32, f, dt, lane), df, acc[dt]);
             }
         }
     }
@@ -916,7 +940,7 @@ __global__ __launch_bounds__(256, (DKV_WAVES<T, DP>)) void dkv_kernel(const Para
         const long long at = first_row + a.head * p.lse_h + a.qt + lane;
         const unsigned long long bits = p.key_mask ? __ballot(ahead != INFINITY) : first_bits(w.ql - a.qt);
         tl.issue(qbase + a.qt * p.q.t + a.head * p.q.h, gbase + a.qt * p.dout.t + a.head * p.dout.h, bits);
-        const bool there = (bits >> lane) & 1;                       // (R = 32: the upper half is never read)
+        const bool there = bit(bits, lane);                          // (R = 32: the upper half is never read)
         if (wave == 0) copy4(reinterpret_cast<const char*>(there ? p.lse2 + at : FILL + 4), lds_offset(s_row + tl.next * 128));
         if (wave == 1) copy4(reinterpret_cast<const char*>(there ? p.ndelta + at : FILL), lds_offset(s_row + tl.next * 128 + 64));
     };

@@ -16,8 +16,9 @@ def rounded(x, t):
     return UNIT[t] * x.abs() + TINY[t]
 
 
-def attention(q, k, v, dout=None, causal=False, scale=None, mask=None):
-    """One head: q [n, D], k, v [m, D] -> {name: (value, bound)} of out, lse (and dq, dk, dv).  mask [m]: which keys take part."""
+def attention(q, k, v, dout=None, causal=False, scale=None, mask=None, swept=False):
+    """One head: q [n, D], k, v [m, D] -> {name: (value, bound)} of out, lse (and dq, dk, dv).  mask [m]: which keys take part.
+    swept: D = sum_d dout out is corrected by sum_j P_j (dP_j - D), so the rounding of `out` is not in it (blocks of at most 256 keys)."""
     t = q.dtype
     u = 0.0 if t == torch.float32 else UNIT[t]                        # P and dS are rounded only where the matrix operand is 16 bits
     q, k, v = q.double(), k.double(), v.double()
@@ -53,6 +54,9 @@ def attention(q, k, v, dout=None, causal=False, scale=None, mask=None):
     b_delta = (g.abs() * (b_out + (D + 2) * E * out.abs())).sum(1, keepdim=True)
     b_dP = (D + 2) * E * (g.abs() @ v.abs().T)
     relP = torch.expm1(torch.log1p(relP) + b_lse[:, None])            # P from the rounded lse
+    if swept:                                                         # what is left of D's error: times 1 - sum P, and the errors of the sweep's own sum
+        off = dP.abs() * 4 * E + b_dP + (dP - delta).abs() + b_delta
+        b_delta = (P * ((1 + relP) * (b_dP + 4 * E * (dP.abs() + delta.abs())) + (relP + (m + 4) * E) * off)).sum(1, keepdim=True)
     T = P * (dP - delta)
     b_T = P * (1 + relP) * (b_dP + b_delta + 4 * E * (dP.abs() + delta.abs())) + T.abs() * relP
     b_T = b_T + u * (T.abs() + b_T)

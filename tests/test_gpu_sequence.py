@@ -89,6 +89,45 @@ def test_attention_and_its_gradients(shape, t, dev):
 
 
 @pytest.mark.parametrize("t", TYPES, ids=str)
+@pytest.mark.parametrize("D", [32, 64, 96, 128])
+@pytest.mark.parametrize("causal,Lq,Lk", [(False, 236, 1), (False, 236, 11), (False, 150, 47), (True, 90, 90)])
+def test_attention_when_the_card_is_full(causal, Lq, Lk, D, t, dev):
+    """Every place on the card is taken, by one sequence over and over: each copy gives the first one's results, to the bit."""
+    from diffphycon_amd import sequence as S
+    B, H, Hk = 160, 10, 5
+    g = _gen(Lk + D)
+    one = lambda L, h: _randn(g, 1, L, h, D, dtype=t).expand(B, L, h, D)  # noqa: E731
+    q, k, v, dout = one(Lq, H), one(Lk, Hk), one(Lk, Hk), one(Lq, H)
+    for _ in range(2):
+        out, lse = S.attention_forward(q, k, v, causal=causal)
+        grads = S.attention_backward(dout, q, k, v, out, lse, causal=causal)
+        for x in (out, lse, *grads):
+            assert torch.equal(x, x[:1].expand_as(x))
+    _check_attention(q[:1], k[:1], v[:1], dout[:1], out[:1], lse[:1], [x[:1] for x in grads], [(Lq, Lk)], causal=causal)
+
+
+@pytest.mark.parametrize("t", TYPES[1:], ids=str)
+def test_attention_gradients_of_rows_with_few_keys(t, dev):
+    """Short sequences beside long ones that are split: what the rounding of `out` loses in D must not reach dq, nor dk.  A row of one key has no
+    gradient but dv's: what is left is fp32's rounding."""
+    from diffphycon_amd import sequence as S
+    ql, kl, H, D = [11, 4, 9, 1, 7], [961, 2, 61, 1, 250], 4, 64
+    g = _gen(23)
+    q, k, v, dout = _randn(g, sum(ql), H, D, dtype=t), _randn(g, sum(kl), H, D, dtype=t), _randn(g, sum(kl), H, D, dtype=t), _randn(g, sum(ql), H, D, dtype=t)
+    plan = S.SequencePlan.packed(ql, kl, device=dev)
+    out, lse = S.attention_forward(q, k, v, plan=plan)
+    dq, dk, _ = S.attention_backward(dout, q, k, v, out, lse, plan=plan)
+    q0 = k0 = 0
+    for nq, nk in zip(ql, kl):
+        for h in range(H):
+            a, b = (slice(q0, q0 + nq), h), (slice(k0, k0 + nk), h)
+            r = O.attention(q[a], k[b], v[b], dout[a], swept=nk <= 256)
+            _within("dq", dq[a], r["dq"][0], O.add_rounding(*r["dq"], t))
+            _within("dk", dk[b], r["dk"][0], O.add_rounding(*r["dk"], t))
+        q0, k0 = q0 + nq, k0 + nk
+
+
+@pytest.mark.parametrize("t", TYPES, ids=str)
 @pytest.mark.parametrize("causal", [False, True])
 def test_attention_masks(t, causal, dev):
     """Padded keys hold infinities and NaN; one batch entry has no key at all; one has holes."""
