@@ -457,8 +457,8 @@ __global__ __launch_bounds__(256, (WAVES<T, DP>)) void fwd_kernel(const Params p
     Tl tl(smem, p.k.t, p.v.t, p.D);
     auto issue = [&](int kt) {
         cur = kb.bits(kt);
-        tl.issue(kbase + kt * p.k.t, vbase + kt * p.v.t, cur);
-        kb.fetch(kt + KB);
+        kb.fetch(kt + KB);                                           // (before the copies: commit() waits for all of them)
+        if (cur) tl.issue(kbase + kt * p.k.t, vbase + kt * p.v.t, cur);
     };
     if (kbegin < kend) { kb.fetch(kbegin); issue(kbegin); }
     for (int kt = kbegin; kt < kend; kt += KB) {
@@ -568,9 +568,11 @@ __global__ __launch_bounds__(256) void few_kernel(const Params p) {
     unsigned cur = 0;
     auto issue = [&](int kt, int buf) {
         cur = (unsigned)kb.bits(kt);
-        sk.issue(mine + buf * 2 * IMG, kbase + kt * p.k.t, cur);
-        sv.issue(mine + buf * 2 * IMG + IMG, vbase + kt * p.v.t, cur);
-        kb.fetch(kt + 128);
+        kb.fetch(kt + 128);                                          // (before the copies: they are all waited for together)
+        if (cur) {
+            sk.issue(mine + buf * 2 * IMG, kbase + kt * p.k.t, cur);
+            sv.issue(mine + buf * 2 * IMG + IMG, vbase + kt * p.v.t, cur);
+        }
     };
     if (from < to) { kb.fetch(from); issue(from, 0); }
     int buf = 0;
@@ -788,8 +790,8 @@ __global__ __launch_bounds__(256, (WAVES<T, DP>)) void dq_kernel(const Params p)
     Tl tl(smem, p.k.t, p.v.t, p.D);
     auto issue = [&](int kt) {
         cur = kb.bits(kt);
-        tl.issue(kbase + kt * p.k.t, vbase + kt * p.v.t, cur);
-        kb.fetch(kt + KB);
+        kb.fetch(kt + KB);                                           // (before the copies: commit() waits for all of them)
+        if (cur) tl.issue(kbase + kt * p.k.t, vbase + kt * p.v.t, cur);
     };
     // P (dP - D) of the tile's keys 32 sub .. (times sc)
     auto terms = [&](f32x16& st, unsigned long long bits, int kt, int sub) {

@@ -65,10 +65,12 @@ static bool plan_grid(Params& p, const dpc_seq_attn* a, bool keys, bool forward)
     const long long blocks = n * p.kv_heads * subs;
     const long long walk = keys ? (long long)p.group * cdiv(a->q_len, KB) : cdiv(a->k_len, KB);
     const int slots = p.causal && 2ll * a->q_len > a->k_len ? 2 * SLOTS : SLOTS;
-    // At most 32 rows of a sequence and key head: few_kernel (its LDS allows rows of 256 bytes), one workgroup resident a CU, two made: sequences differ in length.
-    // A split has two tiles a wave at least.  One token, 8 x 16384 keys, 32/8 heads of 128, bf16: 113 us by fwd_kernel, 98 so (4.1 TB/s), 100 with 256 workgroups.
-    p.few = forward && (long long)a->q_len * p.group <= 32 && (a->head_dim + 31) / 32 * 32 * (a->type == DPC_SEQ_F32 ? 4 : 2) <= 256;
-    if (p.few) p.splits = blocks == 0 ? 1 : (int)std::max<long long>(1, std::min<long long>(SLOTS / blocks, a->k_len / 256));
+    // At most 32 rows of a sequence and key head: few_kernel (its LDS allows rows of 256 bytes), as many workgroups as are resident at once -- one a CU, two with
+    // rows of 128 bytes -- for each starts with empty loads in flight; a split has two tiles a wave at least.  One token, 32/8 heads of 128, bf16: 8 x 16384 keys
+    // 101 us (104 with 512 workgroups; a quarter masked 80, 95), 1 x 16384 keys 20 (25); by fwd_kernel the first takes 113.
+    const int row = (a->head_dim + 31) / 32 * 32 * (a->type == DPC_SEQ_F32 ? 4 : 2);
+    p.few = forward && (long long)a->q_len * p.group <= 32 && row <= 256;
+    if (p.few) p.splits = blocks == 0 ? 1 : (int)std::max<long long>(1, std::min<long long>((row <= 128 ? SLOTS : SLOTS / 2) / blocks, a->k_len / 256));
     else p.splits = blocks == 0 || blocks >= slots * 3 / 4 ? 1 : (int)std::max<long long>(1, std::min<long long>(slots / blocks, walk / 4));
     p.n_tiles = (int)n;
     p.pairs = a->batch * p.kv_heads;
