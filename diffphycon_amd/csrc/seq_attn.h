@@ -924,6 +924,8 @@ __global__ __launch_bounds__(256, (DKV_WAVES<T, DP>)) void dkv_kernel(const Para
         step = min(steps, w.split * per);
         steps = min(steps, step + per);
     }
+    const bool idle = !__any(live);                                  // (this wave's keys are all masked or behind the end)
+    if (p.key_mask && !__syncthreads_or(live)) steps = step;
     // The walk: tiles of R queries, head after head.
     struct At { int head, qt; } next{w.kvh * p.group, qbegin};
     if (step < steps) { next.head += step / per_head; next.qt += step % per_head * R; }
@@ -938,9 +940,10 @@ __global__ __launch_bounds__(256, (DKV_WAVES<T, DP>)) void dkv_kernel(const Para
     auto fetch = [&](At a) {
         if (p.key_mask) ahead = a.qt + lane < w.ql ? p.lse2[first_row + a.head * p.lse_h + a.qt + lane] : INFINITY;
     };
-    auto issue = [&](At a) {
+    auto issue = [&](At a, bool more) {
         const long long at = first_row + a.head * p.lse_h + a.qt + lane;
         const unsigned long long bits = p.key_mask ? __ballot(ahead != INFINITY) : first_bits(w.ql - a.qt);
+        if (more) fetch(advance(a));                                 // (before the copies: commit() waits for all of them)
         tl.issue(qbase + a.qt * p.q.t + a.head * p.q.h, gbase + a.qt * p.dout.t + a.head * p.dout.h, bits);
         const bool there = bit(bits, lane);                          // (R = 32: the upper half is never read)
         if (wave == 0) copy4(reinterpret_cast<const char*>(there ? p.lse2 + at : FILL + 4), lds_offset(s_row + tl.next * 128));
@@ -949,20 +952,18 @@ __global__ __launch_bounds__(256, (DKV_WAVES<T, DP>)) void dkv_kernel(const Para
     At now = next;
     if (step < steps) {
         fetch(now);
-        issue(now);
+        issue(now, step + 1 < steps);
         next = advance(now);
-        if (step + 1 < steps) fetch(next);
     }
     for (; step < steps; ++step) {
         const int qt = now.qt;
         tl.commit();
         if (step + 1 < steps) {
-            issue(next);
+            issue(next, step + 2 < steps);
             now = next;
             next = advance(next);
-            if (step + 2 < steps) fetch(next);
         }
-        if (kw >= w.kl || (p.causal && qt + R - 1 < kw - off)) continue;
+        if (idle || (p.causal && qt + R - 1 < kw - off)) continue;
         const char* const img_q = tl.img_a();
         const char* const img_g = tl.img_b();
         const bool partial = p.causal && kw + 31 - off > qt;
