@@ -860,6 +860,7 @@ __global__ __launch_bounds__(256, (WAVES<T, DP>)) void dq_kernel(const Params p)
     }
     rho = (rho + other_half(rho)) / sc;
     if (!rok) return;
+    if (w.kl == 1) clear(acc);                                       // (the softmax of one key is constant: P (dP - D) has only rounding to give)
     const float un = p.scale / sc;
     if (p.splits > 1) {                                              // part: sums, part_ml [split][row]: rho
         store_row<T, DP, f32x4>(acc, reinterpret_cast<char*>(p.part + (w.split * p.part_rows + at) * p.D), h, p.D, un);
@@ -1011,7 +1012,8 @@ __global__ __launch_bounds__(256, (DKV_WAVES<T, DP>)) void dkv_kernel(const Para
         }
     }
     if (!in) return;
-    if (!live) { clear(dk); clear(dv); }
+    if (!live || w.kl == 1) clear(dk);                               // (one key: as in the dQ kernel)
+    if (!live) clear(dv);
     const float un = is_f16<T>() ? 0x1p-15f : 1.f;                   // (P and with it dS carry 2^15)
     if (p.splits > 1) {                                              // part: [split][dK, dV][row][D]
         const long long at = w.b * p.krow_b + w.kvh * p.krow_h + row;

@@ -12,8 +12,9 @@ step calls `*_forward`, keeps what it returns, and calls `*_backward`.  A pre-no
 
 Element types: float32, float16, bfloat16 (one type per call); sums, statistics and norms are float32 whatever the type.  Kernels run on the
 current stream of the tensors' device and never synchronise; outputs and scratch come from torch's allocator on that stream, so calls may be
-captured into graphs.  Nothing is accumulated with atomics: results repeat bit for bit.  Arguments are checked on the host (ValueError /
-TypeError / RuntimeError); tensors must live on the GPU (no CPU path)."""
+captured into graphs (a graph that reads a RotaryTable or a SequencePlan needs it alive for as long as it is replayed).  Nothing is accumulated
+with atomics: results repeat bit for bit.  Arguments are checked on the host (ValueError / TypeError / RuntimeError); tensors must live on the
+GPU (no CPU path)."""
 import math
 
 import torch
@@ -248,6 +249,8 @@ class RotaryTable:
         device = torch.device(device)
         if device.type != "cuda":
             raise RuntimeError("libdpc needs device tensors (there is no CPU implementation)")
+        if torch.cuda.is_current_stream_capturing():
+            raise RuntimeError("a RotaryTable is computed and waited for: build it before the capture")
         exponent = -torch.arange(0, rotary_dim, 2, dtype=torch.float64) / rotary_dim
         f = (base * factor ** (rotary_dim / (rotary_dim - 2)) if scaling == "ntk" else base) ** exponent
         self.attention_factor = 1.0
@@ -486,7 +489,7 @@ def attention_forward(q, k, v, *, causal=False, scale=None, key_mask=None, plan=
     q [B, Lq, H, D], k and v [B, Lk, Hk, D] (or packed, see `SequencePlan`), H a multiple of Hk: query head h reads key / value head
     h // (H / Hk); D a multiple of 8 up to 128; scale defaults to D^-0.5.  causal: query i sees keys j <= i + Lk - Lq of its sequence.
     key_mask: bool [B, Lk] (packed: [tokens]), True = takes part; what masked keys and values hold never matters.  (A NaN or infinity in a
-    key or value that some query of the call sees may reach queries that the causal mask keeps from it, as 0 * NaN does in the formula.)  A
+    key or value that some query of the call sees may reach queries that the causal mask keeps from it, as 0 * NaN does in the formula.  float32 operands are split into bfloat16 parts: an infinity or a value above 3.38e38 gives NaN.)  A
     query that sees nothing gives zeros and lse -inf.  lse [B, H, Lq] (packed: [H, tokens]) float32 is the log of the softmax's
     denominator, which `attention_backward` needs.  Any strides; layouts whose head rows do not start on 16 bytes are copied first.  Rows of a padded
     plan that belong to no sequence are zero (lse -inf), or left as they were in a given `out` buffer."""

@@ -128,6 +128,25 @@ def test_attention_gradients_of_rows_with_few_keys(t, dev):
 
 
 @pytest.mark.parametrize("t", TYPES, ids=str)
+def test_attention_of_one_key_has_no_gradient_but_the_values(t, dev):
+    """The softmax of one key is 1 whatever the query and the key: their gradients are zero, not the rounding of P (dP - D)."""
+    from diffphycon_amd import sequence as S
+    g = _gen(31)
+    q, dout = _randn(g, 3, 40, 6, 80, dtype=t), _randn(g, 3, 40, 6, 80, dtype=t)
+    k, v = _randn(g, 3, 1, 2, 80, dtype=t), _randn(g, 3, 1, 2, 80, dtype=t)
+    out, lse = S.attention_forward(q, k, v)
+    dq, dk, dv = S.attention_backward(dout, q, k, v, out, lse)
+    assert not dq.any() and not dk.any()
+    _check_attention(q, k, v, dout, out, lse, (dq, dk, dv), [(40, 1)] * 3)
+    plan = S.SequencePlan.packed([40, 40, 40], [1, 0, 2], device=dev)
+    q, k, v, dout = q.reshape(120, 6, 80), k.reshape(3, 2, 80), v.reshape(3, 2, 80), dout.reshape(120, 6, 80)
+    out, lse = S.attention_forward(q, k, v, plan=plan)
+    grads = S.attention_backward(dout, q, k, v, out, lse, plan=plan)
+    assert not grads[0][:80].any() and grads[0][80:].any() and not grads[1][0].any() and grads[1][1:].any()
+    _check_attention(q, k, v, dout, out, lse, grads, [(40, 1), (40, 0), (40, 2)], packed=True)
+
+
+@pytest.mark.parametrize("t", TYPES, ids=str)
 @pytest.mark.parametrize("causal", [False, True])
 def test_attention_masks(t, causal, dev):
     """Padded keys hold infinities and NaN; one batch entry has no key at all; one has holes."""
@@ -536,3 +555,19 @@ def test_drawn_sizes(dev):
         out, lse = S.attention_forward(q, k, v, causal=causal, key_mask=mask)
         grads = S.attention_backward(dout, q, k, v, out, lse, causal=causal, key_mask=mask)
         _check_attention(q, k, v, dout, out, lse, grads, [(Lq, Lk)] * B, causal=causal, mask=mask)
+
+
+def test_tables_are_refused_in_a_capture(dev):
+    from diffphycon_amd import sequence as S
+    x = torch.ones(4, device=dev)
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        with pytest.raises(RuntimeError, match="before the capture"):
+            S.RotaryTable(8, 16)
+        with pytest.raises(RuntimeError, match="before the capture"):
+            S.SequencePlan.packed([3, 4])
+        y = x + 1
+    for _ in range(3):
+        g.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(y, x + 1)
