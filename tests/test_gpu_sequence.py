@@ -398,6 +398,25 @@ def test_rotary(B, T, H, Hk, D, R, layout, t, dev):
                 assert torch.equal(a, yq) and torch.equal(b, yk)
 
 
+@pytest.mark.parametrize("t", TYPES, ids=str)
+@pytest.mark.parametrize("layout", ["interleaved", "half"])
+@pytest.mark.parametrize("B,T,H,Hk,D,R", [(2, 4500, 13, 4, 80, 48), (1, 7, 3, 1, 512, 512), (1, 5, 2, 1, 1040, 1024), (3, 41, 5, 2, 264, 256), (1, 70, 9, 3, 24, 16), (1, 40, 4, 2, 27, 16)])
+def test_rotary_of_many_tokens_and_of_long_and_odd_heads(B, T, H, Hk, D, R, layout, t, dev):
+    from diffphycon_amd import sequence as S
+    g = _gen(T + R)
+    q, k = _randn(g, B, T, H, D, dtype=t), _randn(g, B, T, Hk, D, dtype=t)
+    table = S.RotaryTable(R, T + 9, layout=layout, device=dev)
+    full = (torch.arange(T, device=dev) + 9).expand(B, T)
+    yq, yk = S.rotary_forward(q, k, table, start=9)
+    for y, x in ((yq, q), (yk, k)):
+        _within("rotary", y, *O.rotary(x, full, table.frequencies, layout))
+    for in_q, in_k in ((True, True), (True, False), (False, True)):  # both in place, or one
+        a, b = q.clone(), k.clone()
+        oq, ok = a if in_q else torch.empty_like(a), b if in_k else torch.empty_like(b)
+        S.rotary_forward(a, b, table, start=9, out=(oq, ok))
+        assert torch.equal(oq, yq) and torch.equal(ok, yk)
+
+
 def test_rotary_frequencies(dev):
     """The scalings against their definitions, by hand, at pairs where they differ."""
     from diffphycon_amd import sequence as S
