@@ -43,6 +43,36 @@ template <class T, class P, int G, int N, bool VECT> struct Held {
             }
         }
     }
+    // A row that is on its way while another is worked on: ask() reads something in every lane and settled() puts zeros past the row's end.  (With the
+    // choice at the load, the compiler copies what was loaded, and waits for it, right behind the load: bf16 8191 x 4096 backward 49 us, so 43.  Rows of a
+    // wave or less, of which thousands are at work, lose by it: fp32 786432 x 64 120 us, 129.)
+    __device__ __forceinline__ void ask(const P* __restrict__ row, int lane, int C) {
+#pragma unroll
+        for (int n = 0; n < N; ++n) {
+            if (VECT) {
+                const int c = at<T, G, VECT>(lane, n, 0);
+                v[n] = *reinterpret_cast<const Q*>(row + (c < C ? c : 0));
+                continue;
+            }
+#pragma unroll
+            for (int e = 0; e < VEC<T>; ++e) { const int c = at<T, G, VECT>(lane, n, e); v[n][e] = row[c < C ? c : 0]; }
+        }
+    }
+    __device__ __forceinline__ Held settled(int lane, int C) const {
+        Held r;
+#pragma unroll
+        for (int n = 0; n < N; ++n) {
+            if (VECT) {
+                const uint4 w = __builtin_bit_cast(uint4, v[n]);
+                const unsigned m = at<T, G, VECT>(lane, n, 0) < C ? ~0u : 0u;
+                r.v[n] = __builtin_bit_cast(Q, uint4{w.x & m, w.y & m, w.z & m, w.w & m});
+                continue;
+            }
+#pragma unroll
+            for (int e = 0; e < VEC<T>; ++e) r.v[n][e] = at<T, G, VECT>(lane, n, e) < C ? v[n][e] : (P)0.f;
+        }
+        return r;
+    }
     __device__ __forceinline__ void fill(float x) {
 #pragma unroll
         for (int n = 0; n < N; ++n)
@@ -67,7 +97,7 @@ template <class T, int G, bool VECT> __device__ __forceinline__ void store(T* __
     }
 }
 
-// Sums of a and b over the G lanes of a group.  A group that is a whole workgroup (256, 1024) meets in LDS; `turn` alternates between two slots, so one
+// Sums of a and b over the G lanes of a group.  A group that is a whole workgroup (256 to 1024) meets in LDS; `turn` alternates between two slots, so one
 // barrier a call is enough.  (Every thread of the workgroup makes every call.)
 template <int G> __device__ __forceinline__ void group_sum(float& a, float& b, float2 (*s_red)[16], int& turn) {
 #pragma unroll
@@ -75,9 +105,17 @@ template <int G> __device__ __forceinline__ void group_sum(float& a, float& b, f
     if (G > 64) {
         if ((threadIdx.x & 63) == 0) s_red[turn][threadIdx.x >> 6] = float2{a, b};
         __syncthreads();
-        a = b = 0.f;
+        if (G <= 256) {
+            a = b = 0.f;
 #pragma unroll
-        for (int w = 0; w < G / 64; ++w) { a += s_red[turn][w].x; b += s_red[turn][w].y; }
+            for (int w = 0; w < G / 64; ++w) { a += s_red[turn][w].x; b += s_red[turn][w].y; }
+        } else {                                                     // (a lane a wave: reading all of 16 would take 32 registers)
+            const float2 z = s_red[turn][threadIdx.x & (G / 64 - 1)];
+            a = z.x;
+            b = z.y;
+#pragma unroll
+            for (int x = G / 128; x; x >>= 1) { a += __shfl_xor(a, x, 64); b += __shfl_xor(b, x, 64); }
+        }
         turn ^= 1;
     }
 }
@@ -198,6 +236,7 @@ template <class P> __device__ __forceinline__ void put_param(void* dst, int c, f
 template <class T, class P, int G, int N, bool VECT, int THREADS>
 __global__ __launch_bounds__(THREADS) void bwd_kernel(const BwdParams p) {
     constexpr int V = VEC<T>, R = THREADS / G;
+    constexpr bool WG_ROW = G > 64;                                   // few rows at once: the next one has to be on its way
     __shared__ float2 s_red[2][16];
     __shared__ float s_sum[R > 1 ? THREADS * N * V : 1];
     const int lane = threadIdx.x & (G - 1), grp = threadIdx.x / G;
@@ -218,28 +257,34 @@ __global__ __launch_bounds__(THREADS) void bwd_kernel(const BwdParams p) {
     float2 ns;
     auto fetch = [&](long long row) {
         row = min(row, p.rows - 1);
-        nx.load(x + row * p.xs, lane, p.C, 0.f);
-        ny.load(dy + row * p.dys, lane, p.C, 0.f);
+        if (WG_ROW) {
+            nx.ask(x + row * p.xs, lane, p.C);
+            ny.ask(dy + row * p.dys, lane, p.C);
+        } else {
+            nx.load(x + row * p.xs, lane, p.C, 0.f);
+            ny.load(dy + row * p.dys, lane, p.C, 0.f);
+        }
         ns = *reinterpret_cast<const float2*>(p.stats + 2 * row);
     };
     fetch(r);
     for (long long r0 = (long long)blockIdx.x * R; r0 < p.rows; r0 += step, r += step) {
-        const Held<T, T, G, N, VECT> hx = nx, hy = ny;
+        Held<T, T, G, N, VECT> hx = WG_ROW ? nx.settled(lane, p.C) : nx, hy = WG_ROW ? ny.settled(lane, p.C) : ny;
         const float mu = ns.x, rstd = ns.y;
         if (r0 + step < p.rows) fetch(r + step);
-        float xh[N][V], g[N][V], a = 0.f, b = 0.f;
+        float a = 0.f, b = 0.f;
+        auto xhat = [&](int n, int e) { return ((float)hx.v[n][e] - mu) * rstd; };
 #pragma unroll
         for (int n = 0; n < N; ++n)
 #pragma unroll
             for (int e = 0; e < V; ++e) {
-                xh[n][e] = ((float)hx.v[n][e] - mu) * rstd;
-                g[n][e] = (float)hy.v[n][e];                          // (0 past the row's end)
-                if (r >= p.rows) g[n][e] = 0.f;                      // (a group without a row reads the last one again)
-                dw[n][e] = __builtin_fmaf(g[n][e], xh[n][e], dw[n][e]);
-                db[n][e] += g[n][e];
-                g[n][e] *= (float)w.v[n][e];
-                a += g[n][e];
-                b = __builtin_fmaf(g[n][e], xh[n][e], b);
+                const float xh = xhat(n, e);
+                float g = (float)hy.v[n][e];                         // (0 past the row's end)
+                if (r >= p.rows) g = 0.f;                            // (a group without a row reads the last one again)
+                dw[n][e] = __builtin_fmaf(g, xh, dw[n][e]);
+                db[n][e] += g;
+                g *= (float)w.v[n][e];
+                a += g;
+                b = __builtin_fmaf(g, xh, b);
             }
         group_sum<G>(a, b, s_red, turn);
         a *= inv_c;
@@ -248,9 +293,10 @@ __global__ __launch_bounds__(THREADS) void bwd_kernel(const BwdParams p) {
             T* dx = reinterpret_cast<T*>(p.dx) + r * (long long)p.C;
 #pragma unroll
             for (int n = 0; n < N; ++n) {
+                float v[V];
 #pragma unroll
-                for (int e = 0; e < V; ++e) xh[n][e] = rstd * (g[n][e] - __builtin_fmaf(xh[n][e], b, a));
-                store<T, G, VECT>(dx, lane, n, p.C, xh[n]);
+                for (int e = 0; e < V; ++e) v[e] = rstd * ((float)hy.v[n][e] * (float)w.v[n][e] - __builtin_fmaf(xhat(n, e), b, a));
+                store<T, G, VECT>(dx, lane, n, p.C, v);
             }
         }
     }
@@ -275,7 +321,7 @@ __global__ __launch_bounds__(THREADS) void bwd_kernel(const BwdParams p) {
                 for (int q = 0; q < R; ++q) sum += s_sum[q * W + i];
             }
             const int c = at<T, G, VECT>(i % G, i / G / V, i / G % V);
-            if (R == 1) {                                            // (i = (n V + e) 256 + thread: this thread's own)
+            if (R == 1) {                                            // (i = (n V + e) G + thread: this thread's own)
 #pragma unroll
                 for (int n = 0; n < N; ++n)
 #pragma unroll
@@ -362,16 +408,17 @@ __global__ __launch_bounds__(1024) void param_kernel(const float* __restrict__ p
 
 // Lanes a row (G) and accesses a lane (N) by the row's 16-byte accesses: the fewest lanes that hold it in at most four accesses up to a wave
 // -- no barrier -- else a workgroup.  More accesses a lane cost registers, that is waves, that is loads in flight: bf16 rows of 4096 forward in
-// one wave of 8 accesses 41 us for 8191 rows, in four waves of 2 accesses 23 us (5.7 TB/s).
+// one wave of 8 accesses 41 us for 8191 rows, in four waves of 2 accesses 23 us (5.7 TB/s).  The backward pass holds four times as much a lane and
+// goes to workgroups of one access a lane earlier: bf16 8191 x 8192 in four accesses 119 us, in one 97; 30000 x 2048 84 and 80.
 template <int A, int B> using Shape = std::pair<std::integral_constant<int, A>, std::integral_constant<int, B>>;
-template <class F> int by_width(int acc, F f) {
+template <bool BWD, class F> int by_width(int acc, F f) {
     if (acc <= 4) return f(Shape<4, 1>{});
     if (acc <= 16) return f(Shape<16, 1>{});
     if (acc <= 64) return f(Shape<64, 1>{});
     if (acc <= 128) return f(Shape<64, 2>{});
-    if (acc <= 256) return f(Shape<64, 4>{});
-    if (acc <= 512) return f(Shape<256, 2>{});
-    if (acc <= 1024) return f(Shape<256, 4>{});
+    if (acc <= 256) return f(Shape<BWD ? 256 : 64, BWD ? 1 : 4>{});
+    if (acc <= 512) return f(Shape<BWD ? 512 : 256, BWD ? 1 : 2>{});
+    if (acc <= 1024) return f(Shape<BWD ? 1024 : 256, BWD ? 1 : 4>{});
     if (acc <= 2048) return f(Shape<1024, 2>{});
     return f(Shape<256, 0>{});
 }
@@ -386,7 +433,7 @@ static bool one_block(long long rows, int C, int es) { return rows * C <= ONE_BL
 
 template <class T, class P, bool VECT> int fwd(const FwdParams& p, hipStream_t s) {
     const int acc = (p.C + VEC<T> - 1) / VEC<T>;
-    return by_width(acc, [&](auto shape) {
+    return by_width<false>(acc, [&](auto shape) {
         constexpr int G = decltype(shape.first)::value, N = decltype(shape.second)::value;
         constexpr int THREADS = G > 256 ? G : 256, R = THREADS / G;
         const int grid = (int)std::min<long long>(FWD_BLOCKS, (p.rows + R - 1) / R);
@@ -399,7 +446,7 @@ template <class T, class P, bool VECT> int fwd(const FwdParams& p, hipStream_t s
 
 template <class T, class P, bool VECT> int bwd(const BwdParams& p, hipStream_t s) {
     const int acc = (p.C + VEC<T> - 1) / VEC<T>;
-    return by_width(acc, [&](auto shape) {
+    return by_width<true>(acc, [&](auto shape) {
         constexpr int G = decltype(shape.first)::value, N = decltype(shape.second)::value;
         if constexpr (G <= 64 && N == 1) {
             if (p.sums && !p.part) {
