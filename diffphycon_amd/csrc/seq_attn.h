@@ -10,10 +10,15 @@
 // and its P and dS are the B operands of dV^T += dO^T P and dK^T += Q^T dS.  No probability moves between lanes: the contraction runs
 // over the accumulator's own row order, and the other operand is read from LDS in that order (16-bit types: the LDS transpose read).
 //
-// One source for the three element types: Mma<T> hides the instruction (32x32x16 for 16 bits; for fp32 four 32x32x2, which multiply
-// exact fp32) and the operand layouts.  P and dS are rounded to the element type for the second product, as any 16-bit matrix operand
-// is; sums and statistics stay fp32.  fp16 has only 2^-14 as its smallest full-precision number: P is carried as 2^15 P and dS under a running power of
-// two per column (shrink_col), both undone in fp32 at the end.
+// One source for the three element types.  Mma<T> hides the 16-bit instruction (32x32x16) and the operand layouts; fp32 goes through the same
+// instruction as three bf16 parts (Split3), but for few rows, where the native fp32 one is used.  P and dS are rounded to the element type for the
+// second product, as any 16-bit matrix operand is; sums and statistics stay fp32.  fp16 has only 2^-14 as its smallest full-precision number: P is
+// carried as 2^7 P (forward) or 2^15 P and dS under a running power of two per column (shrink_col), both undone in fp32 at the end.
+//
+// What bounds it (counters at the sizes named at the kernels): head size 128 in 16 bits keeps the matrix units busy for half of the time (forward and dQ 890 to 920
+// TFLOP/s executed, a large library product 1050 to 1094), head size 64 the vector unit for two thirds (exponentials, maxima and masks: 560, 520 and
+// 490 TFLOP/s forward, dQ, dK/dV), fp32 the matrix units (six bf16 products for one: 165 to 190 TFLOP/s of fp32, the fp32 product itself reaches 150).
+// The backward pass executes seven products where five would do, for dQ and dK/dV are summed by different workgroups and nothing is added with atomics.
 #pragma once
 #include <algorithm>
 #include <type_traits>
@@ -108,7 +113,7 @@ template <> struct Mma<float> {
 };
 
 // fp32 by the bf16 matrix instructions: x = x1 + x2 + x3 in three bf16 parts, exactly (bf16x6.h), and six of the nine products -- what is left out is
-// below 2^-24 of |a b|, an fp32 product's own rounding.  6 / 16 of the native instruction's time.  An operand is three fragments, an image three 16-bit
+// below 2^-24 of |a b|, an fp32 product's own rounding.  6 / 16 of the native instruction's time (1 x 4096, 16 heads of 128: forward 1274 -> 771 us).  An operand is three fragments, an image three 16-bit
 // images PLANE bytes apart.
 struct Split3 {
     typedef struct { bf16x8 p[3]; } Frag;
@@ -403,11 +408,14 @@ template <int N> __device__ __forceinline__ float shrink_col(f32x16& t, f32x16 (
 }
 
 template <class T> __device__ __forceinline__ constexpr bool is_f16() { return __is_same(T, _Float16); }
-// Workgroups of a CU that the registers have to allow.  Rows of at most 128 bytes: three (packed fp16, D 64: forward 119 -> 99 us, dQ 181 -> 157
-// against two; four spill), but for dK/dV, whose two sums would spill (211 us at two, 222 at three).
+// Workgroups of a CU that the registers have to allow.  Rows of at most 128 bytes: three (packed fp16 24 x 1900, 12 heads of 64: forward 119 -> 99 us, dQ
+// 181 -> 157 against two; four would spill in dQ), but for dK/dV, whose two sums would spill (211 us at two, 222 at three).  fp32: two up to head size 64,
+// one beyond, whose operands of three parts fill the registers.  (fp32 dQ and dK/dV of head size 64 spill some ten and some forty registers, outside of
+// the innermost loops: 1 x 4096, 16 heads of 64, backward 1278 us, at one workgroup, without, 1480.)
 template <class T, int DP> constexpr int WAVES = DP * sizeof(T) <= 128 ? 3 : sizeof(T) == 2 || DP <= 64 ? 2 : 1;
 template <class T, int DP> constexpr int DKV_WAVES = WAVES<T, DP> < 2 ? 1 : 2;
-// dK/dV at head size 128: the two sums alone take 128 registers; the values' fragments wait in LDS (V_LDS) and the staged tile has 32 rows
+// dK/dV at head size 128: the two sums alone take 128 registers; the values' fragments wait in LDS (V_LDS) and the staged tile has 32 rows (fp32: 146 KB
+// of LDS in all)
 template <class T, int DP> constexpr bool V_LDS = DP == 128;
 template <class T, int DP> constexpr int RB = DP == 128 ? 32 : 64;
 
@@ -420,7 +428,10 @@ struct KeyBits {
     __device__ __forceinline__ unsigned long long bits(int kt) const { return mask ? __ballot(next != 0) : first_bits(kl - kt); }
 };
 
-// Rows of a query block: row r = token r / group, head kvh * group + r % group, so that heads which share keys share the tile's loads.
+// Forward.  Rows of a query block: row r = token r / group, head kvh * group + r % group, so that heads which share keys share the tile's loads.  One
+// pass over the keys with a running maximum and sum; 128 rows a workgroup, 32 a wave, tiles of 64 keys and values in two LDS buffers, one barrier a tile.
+// Causal bf16 2 x 4096, 16/4 heads of 128: 155 us (890 TFLOP/s); packed causal fp16 24 x 1900, 12 heads of 64: 93 us (560); fp32 32 x 1024, 8 heads of
+// 32: 209 us (165).
 template <class T, int DP>
 __global__ __launch_bounds__(256, (WAVES<T, DP>)) void fwd_kernel(const Params p) {
     typedef Op<T, DP> M;
@@ -535,7 +546,7 @@ template <class T> __device__ __forceinline__ void store8(char* row, int d, cons
 }
 // Few rows (at most 32 of a sequence and key head: single tokens, short drafts): nothing to share, so each of the four waves walks over tiles
 // of 32 keys of its own, copied by itself into its own LDS, without barriers; the waves' sums are joined through LDS at the end.  Bound by the
-// keys' and values' bytes: 64 KB are in flight a CU.
+// keys' and values' bytes: 64 KB are in flight a CU (one token, 8 x 16384 keys, 32/8 heads of 128, bf16: 97 us, 5.5 TB/s; 75 with a quarter masked).
 template <class T, int DP> constexpr bool FEW = Image<T, DP>::PITCH * 32 * 16 <= 128 * 1024;
 template <class T, int DP>
 __global__ __launch_bounds__(256) void few_kernel(const Params p) {
@@ -734,7 +745,8 @@ __global__ __launch_bounds__(256) void fwd_join_kernel(const Params p) {
 // dQ, and for the dK/dV kernel lse2 and -D.  D = sum_d dO O with the 16-bit O misses what O's rounding lost; since the probabilities of a
 // row add up to 1, sum_j P (dP - D) is exactly that error, so the sweep adds it up and hands the corrected D on.  Where a block sees at most
 // 256 keys -- dP and D are of one size then, and a row of one or two keys has nothing but their difference -- it is swept once for D alone
-// before it is swept for dQ.  fp32 does so up to one tile, for the rows of few keys alone.
+// before it is swept for dQ.  fp32 does so up to one tile, for the rows of few keys alone.  Tiles, split and bound as in the forward; three products:
+// 229, 149 and 268 us at its sizes (900, 520 and 190 TFLOP/s).
 template <class T, int DP>
 __global__ __launch_bounds__(256, (WAVES<T, DP>)) void dq_kernel(const Params p) {
     typedef Op<T, DP> M;
@@ -886,6 +898,9 @@ __global__ __launch_bounds__(256) void dq_join_kernel(const Params p) {
     });
 }
 
+// dK and dV.  128 keys a workgroup, 32 a wave, which stay in registers (V_LDS: or LDS) with their two sums, and a walk over tiles of query rows, head
+// after head of the group, so that shared heads are summed in fixed order.  Four products; lse2 and -D of a tile's rows come along into LDS and are the
+// start of the accumulator.  Bound as the forward: 348, 214 and 388 us at its sizes (790, 490 and 177 TFLOP/s), the join of the first's splits 23.
 template <class T, int DP>
 __global__ __launch_bounds__(256, (DKV_WAVES<T, DP>)) void dkv_kernel(const Params p) {
     constexpr int R = RB<T, DP>;
