@@ -79,6 +79,12 @@ template <class T, class F> struct Mma16 {   // the two 16-bit types
         for (int e = 0; e < 8; ++e) t[e] = v[8 * s + e];
         return __builtin_convertvector(t, Frag);
     }
+    __device__ static __forceinline__ Frag rest(const f32x16& v, int s, const Frag& f) {          // what from_acc's rounding left
+        f32x8 t;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) t[e] = v[8 * s + e] - (float)f[e];
+        return __builtin_convertvector(t, Frag);
+    }
 };
 template <> struct Mma<_Float16> : Mma16<_Float16, f16x8> {
     typedef f16x4 Quad;
@@ -407,6 +413,9 @@ template <int N> __device__ __forceinline__ float shrink_col(f32x16& t, f32x16 (
     return by;
 }
 
+// 16-bit types: sums of at most this many terms (dQ: a tile of keys) take P and dS in two parts, what the first one's rounding left being the second.  A
+// long sum averages those roundings; one of two or four terms would be off by up to 1.6 times what a computation in 32 bits, rounded once, is.
+constexpr int EXACT = 32;
 template <class T> __device__ __forceinline__ constexpr bool is_f16() { return __is_same(T, _Float16); }
 // Workgroups of a CU that the registers have to allow.  Rows of at most 128 bytes: three (packed fp16 24 x 1900, 12 heads of 64: forward 119 -> 99 us, dQ
 // 181 -> 157 against two; four would spill in dQ), but for dK/dV, whose two sums would spill (211 us at two, 222 at three).  fp32: two up to head size 64,
@@ -830,13 +839,21 @@ __global__ __launch_bounds__(256, (WAVES<T, DP>)) void dq_kernel(const Params p)
         rho += a;
     };
     auto none = [&](unsigned long long bits, int kt) { return rw >= rows || bits == 0 || (p.causal && kt > t_last + off); };
+    auto shrink = [&](f32x16& st) {
+        if (!is_f16<T>()) return;
+        const float by = shrink_col(st, acc);
+        if (by != 1.f) { sc *= by; rho *= by; shift = lse2 - __builtin_amdgcn_logf(sc); }
+    };
     if (kbegin < kend) { kb.fetch(kbegin); issue(kbegin); }
     if (kbegin == 0 && kend == kall && kall > 0 && kall <= (FIX ? 4 : 1) * KB) {                  // the sweep for D alone
+        const unsigned long long only = cur;
         for (int kt = 0; kt < kall; kt += KB) {
             const unsigned long long bits = cur;
             tl.commit();
-            if (kt + KB >= kall) kb.fetch(0);
-            issue(kt + KB < kall ? kt + KB : 0);
+            if (kall > KB) {
+                if (kt + KB >= kall) kb.fetch(0);
+                issue(kt + KB < kall ? kt + KB : 0);
+            }
             if (none(bits, kt)) continue;
 #pragma unroll 1
             for (int sub = 0; sub < 2; ++sub) {
@@ -847,6 +864,27 @@ __global__ __launch_bounds__(256, (WAVES<T, DP>)) void dq_kernel(const Params p)
         }
         nd -= (rho + other_half(rho)) / sc;
         rho = 0.f;
+        if (kall <= KB) {                                            // one tile: it is still there, and dS goes on in two parts (see EXACT)
+            kend = kbegin;
+            if (!none(only, 0))
+#pragma unroll 1
+                for (int sub = 0; sub < 2; ++sub) {
+                    f32x16 st;
+                    terms(st, only, 0, sub);
+                    if (FIX) add(st);
+                    shrink(st);
+#pragma unroll
+                    for (int f = 0; f < NP; ++f) {
+                        const typename M::Frag df = M::from_acc(st, f);
+#pragma unroll
+                        for (int dt = 0; dt < ND; ++dt) {
+                            const typename M::Frag kf = M::template col<DP, Tl::PLANE>(tl.img_a(), sub * 32, f, dt, lane);
+                            acc[dt] = M::mma(kf, df, acc[dt]);
+                            if constexpr (FIX) acc[dt] = M::mma(kf, M::rest(st, f, df), acc[dt]);
+                        }
+                    }
+                }
+        }
     }
     for (int kt = kbegin; kt < kend; kt += KB) {
         const unsigned long long bits = cur;
@@ -858,10 +896,7 @@ __global__ __launch_bounds__(256, (WAVES<T, DP>)) void dq_kernel(const Params p)
             f32x16 st;
             terms(st, bits, kt, sub);
             if (FIX) add(st);
-            if (is_f16<T>()) {
-                const float by = shrink_col(st, acc);
-                if (by != 1.f) { sc *= by; rho *= by; shift = lse2 - __builtin_amdgcn_logf(sc); }
-            }
+            shrink(st);
 #pragma unroll
             for (int f = 0; f < NP; ++f) {
                 const typename M::Frag df = M::from_acc(st, f);
@@ -900,7 +935,7 @@ __global__ __launch_bounds__(256) void dq_join_kernel(const Params p) {
 
 // dK and dV.  128 keys a workgroup, 32 a wave, which stay in registers (V_LDS: or LDS) with their two sums, and a walk over tiles of query rows, head
 // after head of the group, so that shared heads are summed in fixed order.  Four products; lse2 and -D of a tile's rows come along into LDS and are the
-// start of the accumulator.  Bound as the forward: 348, 214 and 388 us at its sizes (790, 490 and 177 TFLOP/s), the join of the first's splits 23.
+// start of the accumulator.  Bound as the forward: 335, 219 and 388 us at its sizes (820, 470 and 177 TFLOP/s), the join of the first's splits 23.
 template <class T, int DP>
 __global__ __launch_bounds__(256, (DKV_WAVES<T, DP>)) void dkv_kernel(const Params p) {
     constexpr int R = RB<T, DP>;
@@ -1023,6 +1058,15 @@ __global__ __launch_bounds__(256, (DKV_WAVES<T, DP>)) void dkv_kernel(const Para
                     dv[dt] = M::mma(M::template col<DP, Tl::PLANE>(img_g, sub * 32, f, dt, lane), pf, dv[dt]);
                     dk[dt] = M::mma(M::template col<DP, Tl::PLANE>(img_q, sub * 32, f, dt, lane), df, dk[dt]);
                 }
+                if constexpr (sizeof(T) == 2)
+                    if (w.ql - qbegin <= EXACT) {
+                        const typename M::Frag pr = M::rest(st, f, pf), dr = M::rest(dp, f, df);
+#pragma unroll
+                        for (int dt = 0; dt < ND; ++dt) {
+                            dv[dt] = M::mma(M::template col<DP, Tl::PLANE>(img_g, sub * 32, f, dt, lane), pr, dv[dt]);
+                            dk[dt] = M::mma(M::template col<DP, Tl::PLANE>(img_q, sub * 32, f, dt, lane), dr, dk[dt]);
+                        }
+                    }
             }
         }
     }

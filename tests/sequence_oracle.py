@@ -16,9 +16,10 @@ def rounded(x, t):
     return UNIT[t] * x.abs() + TINY[t]
 
 
-def attention(q, k, v, dout=None, causal=False, scale=None, mask=None, swept=False):
+def attention(q, k, v, dout=None, causal=False, scale=None, mask=None, swept=False, parts=False):
     """One head: q [n, D], k, v [m, D] -> {name: (value, bound)} of out, lse (and dq, dk, dv).  mask [m]: which keys take part.
-    swept: D = sum_d dout out is corrected by sum_j P_j (dP_j - D), so the rounding of `out` is not in it (blocks of at most 256 keys)."""
+    swept: D = sum_d dout out is corrected by sum_j P_j (dP_j - D), so the rounding of `out` is not in it (blocks of at most 256 keys).
+    parts: P and dS go into the gradients' products as two numbers of the element type (at most 64 keys and 32 queries): u^2 in place of u."""
     t = q.dtype
     u = 0.0 if t == torch.float32 else UNIT[t]                        # P and dS are rounded only where the matrix operand is 16 bits
     q, k, v = q.double(), k.double(), v.double()
@@ -59,6 +60,8 @@ def attention(q, k, v, dout=None, causal=False, scale=None, mask=None, swept=Fal
         b_delta = (P * ((1 + relP) * (b_dP + 4 * E * (dP.abs() + delta.abs())) + (relP + (m + 4) * E) * off)).sum(1, keepdim=True)
     T = P * (dP - delta)
     b_T = P * (1 + relP) * (b_dP + b_delta + 4 * E * (dP.abs() + delta.abs())) + T.abs() * relP
+    if parts:
+        u = u * u
     b_T = b_T + u * (T.abs() + b_T)
     if t == torch.float16:                                            # the column's power of two keeps its largest entry above 2^14: steps below 2^-14 are 2^-24
         b_T = b_T + 2.0 ** -39 * torch.maximum(T.abs().amax(0, keepdim=True) if n else T.new_zeros(1, m), T.abs().amax(1, keepdim=True) if m else T.new_zeros(n, 1))

@@ -127,6 +127,33 @@ def test_attention_gradients_of_rows_with_few_keys(t, dev):
         q0, k0 = q0 + nq, k0 + nk
 
 
+@pytest.mark.parametrize("t", TYPES[1:], ids=str)
+@pytest.mark.parametrize("D,causal", [(32, False), (64, True), (96, False), (128, True)])
+def test_attention_gradients_of_short_sequences_round_once(D, causal, t, dev):
+    """Sums of few terms do not average their operands' roundings: they take P and dS in two parts."""
+    from diffphycon_amd import sequence as S
+    ql, kl, H, Hk = [2, 7, 32, 1, 20, 3] + ([400] if causal else []), [2, 5, 64, 40, 33, 4] + ([3] if causal else []), 4, 2
+    g = _gen(41 + D)
+    q, k, v, dout = _randn(g, sum(ql), H, D, dtype=t), _randn(g, sum(kl), Hk, D, dtype=t), _randn(g, sum(kl), Hk, D, dtype=t), _randn(g, sum(ql), H, D, dtype=t)
+    plan = S.SequencePlan.packed(ql, kl, device=dev)
+    out, lse = S.attention_forward(q, k, v, causal=causal, plan=plan)
+    dq, dk, dv = S.attention_backward(dout, q, k, v, out, lse, causal=causal, plan=plan)
+    q0 = k0 = 0
+    for nq, nk in zip(ql, kl):
+        for hk in range(Hk):
+            b, sums = (slice(k0, k0 + nk), hk), None
+            for h in range(hk * 2, hk * 2 + 2):
+                a = (slice(q0, q0 + nq), h)
+                r = O.attention(q[a], k[b], v[b], dout[a], causal, swept=True, parts=True)
+                _within("dq", dq[a], r["dq"][0], O.add_rounding(*r["dq"], t))
+                part = [*r["dk"], *r["dv"]]
+                sums = part if sums is None else [x + y for x, y in zip(sums, part)]
+            chain = 2 * O.E * nq
+            _within("dk", dk[b], sums[0], O.add_rounding(sums[0], sums[1] * (1 + chain), t))
+            _within("dv", dv[b], sums[2], O.add_rounding(sums[2], sums[3] * (1 + chain), t))
+        q0, k0 = q0 + nq, k0 + nk
+
+
 @pytest.mark.parametrize("t", TYPES, ids=str)
 def test_attention_of_one_key_has_no_gradient_but_the_values(t, dev):
     """The softmax of one key is 1 whatever the query and the key: their gradients are zero, not the rounding of P (dP - D)."""
