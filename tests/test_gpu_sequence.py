@@ -203,6 +203,28 @@ def test_attention_masks(t, causal, dev):
 
 
 @pytest.mark.parametrize("t", TYPES, ids=str)
+@pytest.mark.parametrize("Lq,D,causal", [(150, 64, True), (70, 128, False), (5, 64, True), (300, 32, False)])
+def test_attention_masks_with_holes_of_whole_tiles(Lq, D, causal, t, dev):
+    """Tiles and blocks that no key takes part in are left out: between others, first, last, and all of them."""
+    from diffphycon_amd import sequence as S
+    B, Lk, H, Hk = 5, 900, 4, 2
+    g = _gen(61 + Lq)
+    q, k, v, dout = _randn(g, B, Lq, H, D, dtype=t), _randn(g, B, Lk, Hk, D, dtype=t), _randn(g, B, Lk, Hk, D, dtype=t), _randn(g, B, Lq, H, D, dtype=t)
+    mask = torch.ones(B, Lk, dtype=torch.bool)
+    mask[0, :400] = False
+    mask[1, 64:700] = False
+    mask[2, 130:] = False
+    mask[3] = torch.rand(Lk // 50, generator=g).repeat_interleave(50) < 0.3
+    mask[4] = False
+    mask[4, 640] = True
+    mask = mask.to(dev)
+    k[~mask], v[~mask] = math.nan, -math.inf
+    out, lse = S.attention_forward(q, k, v, causal=causal, key_mask=mask)
+    grads = S.attention_backward(dout, q, k, v, out, lse, causal=causal, key_mask=mask)
+    _check_attention(q, k, v, dout, out, lse, grads, [(Lq, Lk)] * B, causal=causal, mask=mask)
+
+
+@pytest.mark.parametrize("t", TYPES, ids=str)
 @pytest.mark.parametrize("causal", [False, True])
 def test_attention_packed(t, causal, dev):
     from diffphycon_amd import sequence as S
@@ -356,6 +378,21 @@ def test_layer_norm(rows, C, t, dev):
         assert dw.dtype == (wt or torch.float32) == db.dtype
         for name, got in (("y", y), ("dx", dx), ("dw", dw), ("db", db), ("mean", stats[:, :1]), ("rstd", stats[:, 1:])):
             _within(name, got, *r[name])
+
+
+@pytest.mark.parametrize("t", TYPES, ids=str)
+@pytest.mark.parametrize("rows,C", [(2500, 1540), (1100, 2056), (1301, 4104), (1100, 4099), (1037, 8200), (700, 12008)])
+def test_layer_norm_of_many_wide_rows(rows, C, t, dev):
+    """More rows than workgroups, in every width of a group: the next row is on its way while one is worked on."""
+    from diffphycon_amd import sequence as S
+    g = _gen(rows)
+    x, dy = _randn(g, rows, C, dtype=t, scale=1.5, shift=0.25), _randn(g, rows, C, dtype=t, scale=0.1)
+    w, b = _randn(g, C, scale=0.1, shift=1.0).to(t), _randn(g, C).to(t)
+    y, st = S.layer_norm_forward(x, w, b)
+    dx, dw, db = S.layer_norm_backward(dy, x, st, w)
+    r = O.layer_norm(x, w, b, 1e-5, dy, t)
+    for name, got in (("y", y), ("mean", st[:, :1]), ("rstd", st[:, 1:]), ("dx", dx), ("dw", dw), ("db", db)):
+        _within(name, got, *r[name])
 
 
 @pytest.mark.parametrize("t", TYPES, ids=str)
@@ -601,6 +638,33 @@ def test_drawn_sizes(dev):
         out, lse = S.attention_forward(q, k, v, causal=causal, key_mask=mask)
         grads = S.attention_backward(dout, q, k, v, out, lse, causal=causal, key_mask=mask)
         _check_attention(q, k, v, dout, out, lse, grads, [(Lq, Lk)] * B, causal=causal, mask=mask)
+
+
+def test_single_tokens_in_a_graph(dev):
+    """A step's attention over masked keys, captured with its splits and joins: every replay equals the eager call on what the cache then holds."""
+    from diffphycon_amd import sequence as S
+    g = _gen(51)
+    B, Lk, H, Hk, D = 3, 2500, 8, 2, 128
+    q, k, v = (_randn(g, B, n, h, D, dtype=torch.bfloat16) for n, h in ((1, H), (Lk, Hk), (Lk, Hk)))
+    mask = torch.zeros(B, Lk, dtype=torch.bool, device=dev)
+    S.attention_forward(q, k, v, key_mask=mask)
+    gr = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(gr):
+        out, lse = S.attention_forward(q, k, v, key_mask=mask)
+    for n in (0, 1, 33, 1024, 2500):
+        mask[:, :n] = True
+        if n == 1024:
+            mask[1, 5:900] = False
+        q.copy_(_randn(g, *q.shape, dtype=q.dtype))
+        want = S.attention_forward(q, k, v, key_mask=mask)
+        gr.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(out, want[0]) and torch.equal(lse, want[1]) and lse.isinf().all() == (n == 0)
+        for b in range(B):
+            for h in range(H):
+                r = O.attention(q[b, :, h], k[b, :, h // 4], v[b, :, h // 4], mask=mask[b])
+                _within("out", out[b, :, h], *r["out"])
+                _within("lse", lse[b, h], *r["lse"])
 
 
 def test_tables_are_refused_in_a_capture(dev):
