@@ -273,7 +273,8 @@ __global__ __launch_bounds__(THREADS) void bwd_kernel(const BwdParams p) {
         const float mu = ns.x, rstd = ns.y;
         if (r0 + step < p.rows) fetch(r + step);
         float a = 0.f, b = 0.f;
-        auto xhat = [&](int n, int e) { return ((float)hx.v[n][e] - mu) * rstd; };
+        // (past the row's end xh is 0 as dy is: (0 - mu) rstd may leave fp32's range where the row's own xh do not, and 0 * inf would reach every dx)
+        auto xhat = [&](int n, int e) { return ((float)hx.v[n][e] - mu) * (at<T, G, VECT>(lane, n, e) < p.C ? rstd : 0.f); };
 #pragma unroll
         for (int n = 0; n < N; ++n)
 #pragma unroll
