@@ -413,7 +413,7 @@ template <int N> __device__ __forceinline__ float shrink_col(f32x16& t, f32x16 (
     return by;
 }
 
-// 16-bit types: sums of at most this many terms (dQ: a tile of keys) take P and dS in two parts, what the first one's rounding left being the second.  A
+// 16-bit types: sums of at most this many terms (dQ: of as many keys as a tile has) take P and dS in two parts, what the first one's rounding left being the second.  A
 // long sum averages those roundings; one of two or four terms would be off by up to 1.6 times what a computation in 32 bits, rounded once, is.
 constexpr int EXACT = 32;
 template <class T> __device__ __forceinline__ constexpr bool is_f16() { return __is_same(T, _Float16); }
@@ -436,6 +436,19 @@ struct KeyBits {
     __device__ __forceinline__ void fetch(int kt) { if (mask) next = kt + lane < kl ? mask[kt + lane] : 0; }
     __device__ __forceinline__ unsigned long long bits(int kt) const { return mask ? __ballot(next != 0) : first_bits(kl - kt); }
 };
+
+// Keys among the first n that the mask lets through, counted until there are more than `most` (all of a wave's lanes; 512 bytes are asked for at a time)
+__device__ __forceinline__ int count_live(const unsigned char* mask, int n, int lane, int most) {
+    int live = 0;
+    for (int k0 = 0; k0 < n && live <= most; k0 += 512) {
+        unsigned char m[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) m[i] = k0 + 64 * i + lane < n ? mask[k0 + 64 * i + lane] : 0;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) live += __popcll(__ballot(m[i] != 0));
+    }
+    return live;
+}
 
 // Forward.  Rows of a query block: row r = token r / group, head kvh * group + r % group, so that heads which share keys share the tile's loads.  One
 // pass over the keys with a running maximum and sum; 128 rows a workgroup, 32 a wave, tiles of 64 keys and values in two LDS buffers, one barrier a tile.
@@ -754,7 +767,8 @@ __global__ __launch_bounds__(256) void fwd_join_kernel(const Params p) {
 // dQ, and for the dK/dV kernel lse2 and -D.  D = sum_d dO O with the 16-bit O misses what O's rounding lost; since the probabilities of a
 // row add up to 1, sum_j P (dP - D) is exactly that error, so the sweep adds it up and hands the corrected D on.  Where a block sees at most
 // 256 keys -- dP and D are of one size then, and a row of one or two keys has nothing but their difference -- it is swept once for D alone
-// before it is swept for dQ.  fp32 does so up to one tile, for the rows of few keys alone.  Tiles, split and bound as in the forward; three products:
+// before it is swept for dQ.  fp32 does so up to 64 keys, for the rows of few keys alone.  Seen keys are what counts, not the axis they lie on: a
+// key mask's are counted first, and the few that it leaves are one workgroup's, however the axis is split.  Tiles, split and bound as in the forward; three products:
 // 229, 149 and 268 us at its sizes (900, 520 and 190 TFLOP/s).
 template <class T, int DP>
 __global__ __launch_bounds__(256, (WAVES<T, DP>)) void dq_kernel(const Params p) {
@@ -762,6 +776,7 @@ __global__ __launch_bounds__(256, (WAVES<T, DP>)) void dq_kernel(const Params p)
     typedef Tiles<T, DP, KB> Tl;
     constexpr int NF = DP / M::KS, NP = 32 / M::KS, ND = DP / 32;
     constexpr bool FIX = sizeof(T) == 2;
+    constexpr int FEW_KEYS = (FIX ? 4 : 1) * KB;
     extern __shared__ __attribute__((aligned(16))) char smem[];       // tiles of K and V
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), l31 = lane & 31, h = lane >> 5;
     const Where w = where(p, true);
@@ -774,14 +789,10 @@ __global__ __launch_bounds__(256, (WAVES<T, DP>)) void dq_kernel(const Params p)
     const int t_first = p.by_group(rw), t_last = p.by_group(rw + 31);
     int kend = p.causal ? min(w.kl, min((int)p.by_group(r0 + QB - 1), w.ql - 1) + 1 + off) : w.kl, kbegin = 0;
     const int kall = kend;
-    if (p.splits > 1) {                                              // as in the forward: at most 256 keys are one split's
-        const int per = max(4, (max(kend, 0) + KB * p.splits - 1) / (KB * p.splits)) * KB;
-        kbegin = w.split * per;
-        kend = min(kend, kbegin + per);
-    }
+    const unsigned char* const mask = p.key_mask ? p.key_mask + w.b * p.mask_b + w.k0 : nullptr;
     const char* const kbase = p.k.p + w.b * p.k.b + w.k0 * p.k.t + w.kvh * p.k.h;
     const char* const vbase = p.v.p + w.b * p.v.b + w.k0 * p.v.t + w.kvh * p.v.h;
-    KeyBits kb{p.key_mask ? p.key_mask + w.b * p.mask_b + w.k0 : nullptr, w.kl, lane, 0};
+    KeyBits kb{mask, w.kl, lane, 0};
     const long long at = w.b * p.lse_b + head * p.lse_h + w.q0 + token;
     const float lse = rok ? p.lse[at] : -INFINITY;
     const bool sees = lse != -INFINITY;                              // (a row that sees nothing takes no part, whatever it holds)
@@ -789,6 +800,15 @@ __global__ __launch_bounds__(256, (WAVES<T, DP>)) void dq_kernel(const Params p)
     typename M::Frag qf[NF], gf[NF];
     load_row<M, T, DP>(qf, p.q.p + w.b * p.q.b + (w.q0 + token) * p.q.t + head * p.q.h, h, p.D, rok);
     load_row<M, T, DP>(gf, p.dout.p + w.b * p.dout.b + (w.q0 + token) * p.dout.t + head * p.dout.h, h, p.D, rok);
+    // keys that the block sees (more than FEW_KEYS: at least that many); the rows are on their way meanwhile
+    const int live = mask ? count_live(mask, kall, lane, FEW_KEYS) : kall;
+    const bool few = live > 0 && live <= FEW_KEYS;
+    if (p.splits > 1 && few) kend = w.split == 0 ? kall : 0;
+    else if (p.splits > 1) {                                         // as in the forward
+        const int per = max(4, (max(kend, 0) + KB * p.splits - 1) / (KB * p.splits)) * KB;
+        kbegin = w.split * per;
+        kend = min(kend, kbegin + per);
+    }
     float nd = 0.f, rho = 0.f;                                       // -D, what D still misses (times sc)
     {
         typename M::Frag of[NF];
@@ -845,12 +865,11 @@ __global__ __launch_bounds__(256, (WAVES<T, DP>)) void dq_kernel(const Params p)
         if (by != 1.f) { sc *= by; rho *= by; shift = lse2 - __builtin_amdgcn_logf(sc); }
     };
     if (kbegin < kend) { kb.fetch(kbegin); issue(kbegin); }
-    if (kbegin == 0 && kend == kall && kall > 0 && kall <= (FIX ? 4 : 1) * KB) {                  // the sweep for D alone
-        const unsigned long long only = cur;
+    if (few && kbegin < kend) {                                      // the sweep for D alone
         for (int kt = 0; kt < kall; kt += KB) {
             const unsigned long long bits = cur;
             tl.commit();
-            if (kall > KB) {
+            if (kall > KB) {                                         // (one tile stays where it is)
                 if (kt + KB >= kall) kb.fetch(0);
                 issue(kt + KB < kall ? kt + KB : 0);
             }
@@ -864,32 +883,14 @@ __global__ __launch_bounds__(256, (WAVES<T, DP>)) void dq_kernel(const Params p)
         }
         nd -= (rho + other_half(rho)) / sc;
         rho = 0.f;
-        if (kall <= KB) {                                            // one tile: it is still there, and dS goes on in two parts (see EXACT)
-            kend = kbegin;
-            if (!none(only, 0))
-#pragma unroll 1
-                for (int sub = 0; sub < 2; ++sub) {
-                    f32x16 st;
-                    terms(st, only, 0, sub);
-                    if (FIX) add(st);
-                    shrink(st);
-#pragma unroll
-                    for (int f = 0; f < NP; ++f) {
-                        const typename M::Frag df = M::from_acc(st, f);
-#pragma unroll
-                        for (int dt = 0; dt < ND; ++dt) {
-                            const typename M::Frag kf = M::template col<DP, Tl::PLANE>(tl.img_a(), sub * 32, f, dt, lane);
-                            acc[dt] = M::mma(kf, df, acc[dt]);
-                            if constexpr (FIX) acc[dt] = M::mma(kf, M::rest(st, f, df), acc[dt]);
-                        }
-                    }
-                }
-        }
     }
+    const bool kept = few && kall <= KB, parts = FIX && few && live <= KB;       // (dS in two parts: see EXACT)
     for (int kt = kbegin; kt < kend; kt += KB) {
         const unsigned long long bits = cur;
-        tl.commit();
-        if (kt + KB < kend) issue(kt + KB);
+        if (!kept) {
+            tl.commit();
+            if (kt + KB < kend) issue(kt + KB);
+        }
         if (none(bits, kt)) continue;
 #pragma unroll 1
         for (int sub = 0; sub < 2; ++sub) {
@@ -902,6 +903,12 @@ __global__ __launch_bounds__(256, (WAVES<T, DP>)) void dq_kernel(const Params p)
                 const typename M::Frag df = M::from_acc(st, f);
 #pragma unroll
                 for (int dt = 0; dt < ND; ++dt) acc[dt] = M::mma(M::template col<DP, Tl::PLANE>(tl.img_a(), sub * 32, f, dt, lane), df, acc[dt]);
+                if constexpr (FIX)
+                    if (parts) {
+                        const typename M::Frag dr = M::rest(st, f, df);
+#pragma unroll
+                        for (int dt = 0; dt < ND; ++dt) acc[dt] = M::mma(M::template col<DP, Tl::PLANE>(tl.img_a(), sub * 32, f, dt, lane), dr, acc[dt]);
+                    }
             }
         }
     }

@@ -30,3 +30,82 @@ def test_layer_norm_gradient_of_a_far_constant_row(C, pad, t, dev):
     _within("dx", dx, value, O.add_rounding(value, rstd * O.E * (6 * z.abs() + (C + 10) * size), t))
     assert not dw.any()
     _within("db", db, dy.double().sum(0), O.add_rounding(dy.double().sum(0), 9 * O.E * dy.double().abs().sum(0), t))
+
+
+# ---------------------------------------------------------------------------------------------------------------- attention: few keys under a mask
+def _few(B, Lk, seen, seed):
+    """A mask that leaves `seen` keys of Lk in each batch entry, spread over all of them."""
+    g = torch.Generator().manual_seed(seed)
+    mask = torch.zeros(B, Lk, dtype=torch.bool)
+    for b in range(B):
+        mask[b, torch.randperm(Lk, generator=g)[:seen]] = True
+    return mask
+
+
+@pytest.mark.parametrize("t", TYPES, ids=str)
+@pytest.mark.parametrize("D", [32, 64, 96, 128])
+@pytest.mark.parametrize("seen", [1, 2, 5, 20, 60])
+def test_attention_gradients_of_few_keys_under_a_mask(seen, D, t, dev):
+    """Few keys among many: the gradients are as exact as those of a short sequence.  Once with the keys split over workgroups, once with the card full."""
+    from diffphycon_amd import sequence as S
+    for B, H, Hk in ((3, 4, 2), (40, 10, 10)):
+        Lq, Lk = 30, 900
+        g = _gen(seen + D)
+        mask = _few(B, Lk, seen, seen).to(dev)
+        q, k, v, dout = _randn(g, B, Lq, H, D, dtype=t), _randn(g, B, Lk, Hk, D, dtype=t), _randn(g, B, Lk, Hk, D, dtype=t), _randn(g, B, Lq, H, D, dtype=t)
+        k[~mask], v[~mask] = math.nan, math.inf
+        out, lse = S.attention_forward(q, k, v, key_mask=mask)
+        dq, dk, dv = S.attention_backward(dout, q, k, v, out, lse, key_mask=mask)
+        for b in sorted({0, 1, B - 1}):
+            for hk in range(Hk):
+                sums = None
+                for h in range(hk * (H // Hk), (hk + 1) * (H // Hk)):
+                    r = O.attention(q[b, :, h], k[b, :, hk], v[b, :, hk], dout[b, :, h], mask=mask[b], swept=True, parts=True)
+                    _within("dq", dq[b, :, h], r["dq"][0], O.add_rounding(*r["dq"], t))
+                    part = [*r["dk"], *r["dv"]]
+                    sums = part if sums is None else [x + y for x, y in zip(sums, part)]
+                chain = (H // Hk) * O.E * Lq
+                _within("dk", dk[b, :, hk], sums[0], O.add_rounding(sums[0], sums[1] * (1 + chain), t))
+                _within("dv", dv[b, :, hk], sums[2], O.add_rounding(sums[2], sums[3] * (1 + chain), t))
+
+
+@pytest.mark.parametrize("t", TYPES[1:], ids=str)
+@pytest.mark.parametrize("D,H,Hk", [(32, 2, 2), (64, 6, 2), (128, 2, 1)])
+def test_attention_gradients_behind_left_padding(D, H, Hk, t, dev):
+    """Causal sequences that start behind padding: their first rows see one key, two keys, ...  A block sees at most the real tokens."""
+    from diffphycon_amd import sequence as S
+    L, first = 700, [690, 640, 500, 447, 130]
+    B = len(first)
+    g = _gen(D)
+    q, k, v, dout = _randn(g, B, L, H, D, dtype=t), _randn(g, B, L, Hk, D, dtype=t), _randn(g, B, L, Hk, D, dtype=t), _randn(g, B, L, H, D, dtype=t)
+    mask = (torch.arange(L)[None] >= torch.tensor(first)[:, None]).to(dev)
+    k[~mask], v[~mask] = math.nan, math.inf
+    out, lse = S.attention_forward(q, k, v, causal=True, key_mask=mask)
+    dq, dk, dv = S.attention_backward(dout, q, k, v, out, lse, causal=True, key_mask=mask)
+    for b, f in enumerate(first):
+        last = L if L - f <= 256 else 256                            # rows of blocks that see at most 256 keys
+        for h in range(H):
+            r = O.attention(q[b, :, h], k[b, :, h // (H // Hk)], v[b, :, h // (H // Hk)], dout[b, :, h], True, mask=mask[b], swept=True, parts=L - f <= 64)
+            _within("dq", dq[b, :last, h], *(x[:last] for x in (r["dq"][0], O.add_rounding(*r["dq"], t))))
+        assert not dq[b, :f].any() and not dk[b, :f].any() and not dv[b, :f].any()
+    _check_attention(q.masked_fill(~mask[:, :, None, None], 0.0), k, v, dout.masked_fill(~mask[:, :, None, None], 0.0), out, lse, (dq, dk, dv), [(L, L)] * B, causal=True, mask=mask)
+
+
+@pytest.mark.parametrize("t", TYPES[1:], ids=str)
+def test_attention_gradients_of_few_keys_are_the_same_masked_and_packed(t, dev):
+    """The keys that a mask leaves, gathered into a plan's sequences: either way the gradients are rounded once, from values some 2 u^2 of their terms
+    apart (u: half a step).  Such a pair rounds apart in a share u k of the elements (k: terms over result, below 16), by 2 u: 2 u (u k)^(1/2) < u / 2 in norm."""
+    from diffphycon_amd import sequence as S
+    B, Lq, Lk, H, D, seen = 4, 25, 1300, 3, 64, 7
+    g = _gen(77)
+    mask = _few(B, Lk, seen, 3).to(dev)
+    q, k, v, dout = _randn(g, B, Lq, H, D, dtype=t), _randn(g, B, Lk, H, D, dtype=t), _randn(g, B, Lk, H, D, dtype=t), _randn(g, B, Lq, H, D, dtype=t)
+    out, lse = S.attention_forward(q, k, v, key_mask=mask)
+    a = S.attention_backward(dout, q, k, v, out, lse, key_mask=mask)
+    plan = S.SequencePlan.packed([Lq] * B, [seen] * B, device=dev)
+    p = [q.flatten(0, 1), k[mask], v[mask]]
+    out, lse = S.attention_forward(*p, plan=plan)
+    b = S.attention_backward(dout.flatten(0, 1), *p, out, lse, plan=plan)
+    for x, y in ((a[0].flatten(0, 1), b[0]), (a[1][mask], b[1]), (a[2][mask], b[2])):
+        x, y = x.double(), y.double()
+        assert ((x - y).norm() / y.norm()).item() <= O.UNIT[t] / 2
