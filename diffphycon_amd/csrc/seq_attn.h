@@ -437,17 +437,17 @@ struct KeyBits {
     __device__ __forceinline__ unsigned long long bits(int kt) const { return mask ? __ballot(next != 0) : first_bits(kl - kt); }
 };
 
-// Keys among the first n that the mask lets through, counted until there are more than `most` (all of a wave's lanes; 512 bytes are asked for at a time)
-__device__ __forceinline__ int count_live(const unsigned char* mask, int n, int lane, int most) {
-    int live = 0;
-    for (int k0 = 0; k0 < n && live <= most; k0 += 512) {
-        unsigned char m[8];
+// How many of the rows from .. to - 1 takes_part(row) holds for, counted until there are more than `most` (by all lanes of a wave; 512 rows are asked for at a time)
+template <class F> __device__ __forceinline__ int count_rows(int from, int to, int lane, int most, F takes_part) {
+    int n = 0;
+    for (int r0 = from; r0 < to && n <= most; r0 += 512) {
+        bool in[8];
 #pragma unroll
-        for (int i = 0; i < 8; ++i) m[i] = k0 + 64 * i + lane < n ? mask[k0 + 64 * i + lane] : 0;
+        for (int i = 0; i < 8; ++i) in[i] = r0 + 64 * i + lane < to && takes_part(r0 + 64 * i + lane);
 #pragma unroll
-        for (int i = 0; i < 8; ++i) live += __popcll(__ballot(m[i] != 0));
+        for (int i = 0; i < 8; ++i) n += __popcll(__ballot(in[i]));
     }
-    return live;
+    return n;
 }
 
 // Forward.  Rows of a query block: row r = token r / group, head kvh * group + r % group, so that heads which share keys share the tile's loads.  One
@@ -801,7 +801,7 @@ __global__ __launch_bounds__(256, (WAVES<T, DP>)) void dq_kernel(const Params p)
     load_row<M, T, DP>(qf, p.q.p + w.b * p.q.b + (w.q0 + token) * p.q.t + head * p.q.h, h, p.D, rok);
     load_row<M, T, DP>(gf, p.dout.p + w.b * p.dout.b + (w.q0 + token) * p.dout.t + head * p.dout.h, h, p.D, rok);
     // keys that the block sees (more than FEW_KEYS: at least that many); the rows are on their way meanwhile
-    const int live = mask ? count_live(mask, kall, lane, FEW_KEYS) : kall;
+    const int live = mask ? count_rows(0, kall, lane, FEW_KEYS, [&](int j) { return mask[j] != 0; }) : kall;
     const bool few = live > 0 && live <= FEW_KEYS;
     if (p.splits > 1 && few) kend = w.split == 0 ? kall : 0;
     else if (p.splits > 1) {                                         // as in the forward
@@ -982,6 +982,10 @@ __global__ __launch_bounds__(256, (DKV_WAVES<T, DP>)) void dkv_kernel(const Para
         step = min(steps, w.split * per);
         steps = min(steps, step + per);
     }
+    // Queries of a head that take part (more than EXACT: at least that many)
+    const int seeing = p.key_mask && sizeof(T) == 2
+                           ? count_rows(qbegin, w.ql, lane, EXACT, [&](int i) { return p.lse2[w.b * p.lse_b + w.kvh * p.group * p.lse_h + w.q0 + i] != INFINITY; })
+                           : w.ql - qbegin;
     const bool idle = !__any(live);                                  // (this wave's keys are all masked or behind the end)
     if (p.key_mask && !__syncthreads_or(live)) steps = step;
     // The walk: tiles of R queries, head after head.
@@ -1066,7 +1070,7 @@ __global__ __launch_bounds__(256, (DKV_WAVES<T, DP>)) void dkv_kernel(const Para
                     dk[dt] = M::mma(M::template col<DP, Tl::PLANE>(img_q, sub * 32, f, dt, lane), df, dk[dt]);
                 }
                 if constexpr (sizeof(T) == 2)
-                    if (w.ql - qbegin <= EXACT) {
+                    if (seeing <= EXACT) {
                         const typename M::Frag pr = M::rest(st, f, pf), dr = M::rest(dp, f, df);
 #pragma unroll
                         for (int dt = 0; dt < ND; ++dt) {

@@ -109,3 +109,27 @@ def test_attention_gradients_of_few_keys_are_the_same_masked_and_packed(t, dev):
     for x, y in ((a[0].flatten(0, 1), b[0]), (a[1][mask], b[1]), (a[2][mask], b[2])):
         x, y = x.double(), y.double()
         assert ((x - y).norm() / y.norm()).item() <= O.UNIT[t] / 2
+
+
+@pytest.mark.parametrize("t", TYPES[1:], ids=str)
+@pytest.mark.parametrize("D", [32, 64, 96, 128])
+def test_attention_key_gradients_of_few_queries_behind_left_padding(D, t, dev):
+    """A key behind left padding is seen by as many queries as there are real tokens from it on: sums of few terms, however long the axis is."""
+    from diffphycon_amd import sequence as S
+    L, first, H, Hk = 500, [498, 490, 470], 4, 2
+    B = len(first)
+    g = _gen(D)
+    q, k, v, dout = _randn(g, B, L, H, D, dtype=t), _randn(g, B, L, Hk, D, dtype=t), _randn(g, B, L, Hk, D, dtype=t), _randn(g, B, L, H, D, dtype=t)
+    mask = (torch.arange(L)[None] >= torch.tensor(first)[:, None]).to(dev)
+    out, lse = S.attention_forward(q, k, v, causal=True, key_mask=mask)
+    dq, dk, dv = S.attention_backward(dout, q, k, v, out, lse, causal=True, key_mask=mask)
+    for b in range(B):
+        for hk in range(Hk):
+            sums = None
+            for h in (2 * hk, 2 * hk + 1):
+                r = O.attention(q[b, :, h], k[b, :, hk], v[b, :, hk], dout[b, :, h], True, mask=mask[b], swept=True, parts=True)
+                part = [*r["dk"], *r["dv"]]
+                sums = part if sums is None else [x + y for x, y in zip(sums, part)]
+            chain = 2 * O.E * L
+            _within("dk", dk[b, :, hk], sums[0], O.add_rounding(sums[0], sums[1] * (1 + chain), t))
+            _within("dv", dv[b, :, hk], sums[2], O.add_rounding(sums[2], sums[3] * (1 + chain), t))
