@@ -984,7 +984,7 @@ __global__ __launch_bounds__(256, (DKV_WAVES<T, DP>)) void dkv_kernel(const Para
     }
     // Queries of a head that take part (more than EXACT: at least that many)
     const int seeing = p.key_mask && sizeof(T) == 2
-                           ? count_rows(qbegin, w.ql, lane, EXACT, [&](int i) { return p.lse2[w.b * p.lse_b + w.kvh * p.group * p.lse_h + w.q0 + i] != INFINITY; })
+                           ? count_rows(qbegin, w.ql, lane, EXACT, [&](int i) { return p.lse[w.b * p.lse_b + w.kvh * p.group * p.lse_h + w.q0 + i] != -INFINITY; })
                            : w.ql - qbegin;
     const bool idle = !__any(live);                                  // (this wave's keys are all masked or behind the end)
     if (p.key_mask && !__syncthreads_or(live)) steps = step;
@@ -996,15 +996,15 @@ __global__ __launch_bounds__(256, (DKV_WAVES<T, DP>)) void dkv_kernel(const Para
     const char* const qbase = p.q.p + w.b * p.q.b + w.q0 * p.q.t;
     const char* const gbase = p.dout.p + w.b * p.dout.b + w.q0 * p.dout.t;
     const long long first_row = w.b * p.lse_b + w.q0;
-    // Rows that see nothing are not read (their lse2 is +inf).  Under a causal mask alone they lie before qbegin; a key mask can leave any
-    // row empty, so its lse2 is looked at first, a tile ahead.
+    // Rows that see nothing are not read (lse = -inf; lse2 cannot tell them from rows whose lse is +inf).  Under a causal mask alone they lie before
+    // qbegin; a key mask can leave any row empty, so its lse is looked at first, a tile ahead.
     float ahead = 0.f;
     auto fetch = [&](At a) {
-        if (p.key_mask) ahead = a.qt + lane < w.ql ? p.lse2[first_row + a.head * p.lse_h + a.qt + lane] : INFINITY;
+        if (p.key_mask) ahead = a.qt + lane < w.ql ? p.lse[first_row + a.head * p.lse_h + a.qt + lane] : -INFINITY;
     };
     auto issue = [&](At a, bool more) {
         const long long at = first_row + a.head * p.lse_h + a.qt + lane;
-        const unsigned long long bits = p.key_mask ? __ballot(ahead != INFINITY) : first_bits(w.ql - a.qt);
+        const unsigned long long bits = p.key_mask ? __ballot(ahead != -INFINITY) : first_bits(w.ql - a.qt);
         if (more) fetch(advance(a));                                 // (before the copies: commit() waits for all of them)
         tl.issue(qbase + a.qt * p.q.t + a.head * p.q.h, gbase + a.qt * p.dout.t + a.head * p.dout.h, bits);
         const bool there = bit(bits, lane);                          // (R = 32: the upper half is never read)

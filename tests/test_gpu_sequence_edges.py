@@ -133,3 +133,24 @@ def test_attention_key_gradients_of_few_queries_behind_left_padding(D, t, dev):
             chain = 2 * O.E * L
             _within("dk", dk[b, :, hk], sums[0], O.add_rounding(sums[0], sums[1] * (1 + chain), t))
             _within("dv", dv[b, :, hk], sums[2], O.add_rounding(sums[2], sums[3] * (1 + chain), t))
+
+
+@pytest.mark.parametrize("t", TYPES, ids=str)
+@pytest.mark.parametrize("bad", [math.inf, math.nan])
+def test_attention_gradients_of_an_infinite_row_do_not_depend_on_a_mask(bad, t, dev):
+    """A row whose log-sum-exp is +inf (scores that overflowed, as torch.logsumexp gives it) or NaN takes part: with a mask that lets every key through dk and
+    dv are what they are without one.  Only -inf is a row that sees nothing."""
+    from diffphycon_amd import sequence as S
+    g = _gen(81)
+    B, Lq, Lk, H, D = 2, 40, 300, 2, 64
+    q, k, v, dout = _randn(g, B, Lq, H, D, dtype=t), _randn(g, B, Lk, H, D, dtype=t), _randn(g, B, Lk, H, D, dtype=t), _randn(g, B, Lq, H, D, dtype=t)
+    out, lse = S.attention_forward(q, k, v)
+    q[0, 7, 1], lse[0, 1, 7] = math.inf, bad
+    plain = S.attention_backward(dout, q, k, v, out, lse)
+    masked = S.attention_backward(dout, q, k, v, out, lse, key_mask=torch.ones(B, Lk, dtype=torch.bool, device=dev))
+    for x, y in zip(plain, masked):
+        assert torch.equal(x.isnan(), y.isnan()) and torch.equal(x.nan_to_num(), y.nan_to_num())
+    assert plain[1][0, :, 1].isnan().all() and not plain[1][1].isnan().any()
+    lse[0, 1, 7] = -math.inf
+    masked = S.attention_backward(dout, q, k, v, out, lse, key_mask=torch.ones(B, Lk, dtype=torch.bool, device=dev))
+    assert not any(x.isnan().any() for x in masked) and not masked[0][0, 7, 1].any()
