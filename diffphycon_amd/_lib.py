@@ -80,12 +80,12 @@ class SeqAttn(C.Structure):
                 ("key_mask", C.c_void_p), ("mask_stride_b", C.c_int64), ("q_tiles", C.c_void_p), ("k_tiles", C.c_void_p),
                 ("n_q_tiles", C.c_int32), ("n_k_tiles", C.c_int32), ("type", C.c_int32), ("batch", C.c_int32), ("heads", C.c_int32),
                 ("kv_heads", C.c_int32), ("head_dim", C.c_int32), ("q_len", C.c_int32), ("k_len", C.c_int32), ("causal", C.c_int32),
-                ("lse_rows", C.c_int64), ("k_rows", C.c_int64), ("k_row_stride_b", C.c_int64), ("k_row_stride_h", C.c_int64), ("scale", C.c_float)]
+                ("lse_rows", C.c_int64), ("scale", C.c_float)]
 
 
 # The two structures above as one struct.pack each: a call per microsecond matters for single tokens, and ctypes takes one per field.
 SEQ_ROTARY_BYTES = struct.Struct("<21q9i4x")
-SEQ_ATTN_BYTES = struct.Struct("<39q10i4qf4x")
+SEQ_ATTN_BYTES = struct.Struct("<39q10iqf4x")
 assert SEQ_ROTARY_BYTES.size == C.sizeof(SeqRotary) and SEQ_ATTN_BYTES.size == C.sizeof(SeqAttn)
 
 

@@ -121,7 +121,7 @@ using namespace dpc;
 
 extern "C" {
 
-int dpc_version(void) { return 102; }
+int dpc_version(void) { return 103; }
 int dpc_set_cu_budget(int cus) {
     DPC_REQUIRE(cus >= 0, "set_cu_budget: negative");
     g_cu_budget.store(cus, std::memory_order_relaxed);

@@ -155,13 +155,16 @@ struct Ten { char* p; long long b, t, h; };        // strides in bytes
 struct Params {
     Ten q, k, v, out, dout, dq, dk, dv;
     float* lse;
-    long long lse_b, lse_h, krow_b, krow_h;        // row numbers of q (as in lse) and of k
+    long long lse_b, lse_h;                        // row numbers of q, as in lse
     const unsigned char* key_mask;
     long long mask_b;
     const int* tiles;                              // [..][8] = (sequence, block, first query, queries, first key, keys, ..) or null (dense)
     float *lse2, *ndelta;                          // backward: lse in powers of two (+inf: a row that sees nothing) and -D, numbered like lse
-    float *part, *part_ml;                         // splits: partial sums [split][row][D] and per-row scalars (layout at each kernel)
+    // splits: partial sums [split][row][D] and per-row scalars (layout at each kernel).  Rows are numbered block by block, not as they lie in the
+    // tensors: scratch goes by the blocks that there are, and a plan of short sequences in a long buffer has few.
+    float *part, *part_ml;
     long long part_rows;
+    int block_rows;                                // most rows that a block has
     int heads, kv_heads, group, D, q_len, k_len, causal, n_tiles, tiles_per_seq, band_tiles, pairs, splits, few;
     // splits, sub-blocks of a block, kv_heads, group, pairs; workgroups of a pair in a band of blocks and in the last band, of a band on an XCD
     Div by_split, by_sub, by_kv, by_group, by_tile, by_pair, by_last, by_band;
@@ -173,13 +176,18 @@ struct Params {
 // they differ in work (the last queries', the first keys' have most): then the quarter with most work of every pair comes first, so that
 // none of it is left for the end (pair after pair: 20 to 40 % of the card idle at the end; all pairs' heaviest blocks first: keys and values leave L2
 // in between).  A query block is `subs` sub-blocks of QB rows (rows = tokens x heads of the group).
-struct Where { int b, tile, kvh, sub, split, ql, kl; long long q0, k0; };
+struct Where {
+    int b, tile, kvh, sub, split, ql, kl, block;                     // block: which of all blocks, of (sequence, key head) too
+    long long q0, k0;
+    __device__ __forceinline__ long long part(const Params& p, int row) const { return (long long)block * p.block_rows + row; }
+};
 __device__ __forceinline__ Where where(const Params& p, bool last_first) {
     Where w;
     int id = blockIdx.x;
     w.ql = p.q_len; w.kl = p.k_len; w.q0 = w.k0 = 0;
     if (p.tiles) {
         w.split = p.by_split.take(id);
+        w.block = id;
         w.sub = p.by_sub.take(id);
         w.kvh = p.by_kv.take(id);
         const int* e = p.tiles + 8 * (long long)id;
@@ -197,6 +205,7 @@ __device__ __forceinline__ Where where(const Params& p, bool last_first) {
         pair = p.by_tile.take(i);
     }
     w.split = p.by_split.take(i);
+    w.block = pair * p.tiles_per_seq * (int)p.by_sub.d + i;
     w.sub = p.by_sub.take(i);
     w.tile = last_first ? p.tiles_per_seq - 1 - i : i;
     w.kvh = p.by_kv.take(pair);
@@ -549,9 +558,10 @@ __global__ __launch_bounds__(256, (WAVES<T, DP>)) void fwd_kernel(const Params p
     if (!rok) return;
     const long long at = w.b * p.lse_b + head * p.lse_h + w.q0 + token;
     if (p.splits > 1) {                                              // part: sums, part_ml [split][row][2]: maximum and sum
-        store_row<T, DP, f32x4>(o, reinterpret_cast<char*>(p.part + (w.split * p.part_rows + at) * p.D), h, p.D, 1.f);
+        const long long pr = w.split * p.part_rows + w.part(p, wave * 32 + l31);
+        store_row<T, DP, f32x4>(o, reinterpret_cast<char*>(p.part + pr * p.D), h, p.D, 1.f);
         if (h == 0) {
-            float* ml = p.part_ml + 2 * (w.split * p.part_rows + at);
+            float* ml = p.part_ml + 2 * pr;
             ml[0] = m - lift;
             ml[1] = l;
         }
@@ -659,7 +669,7 @@ __global__ __launch_bounds__(256) void few_kernel(const Params p) {
     if (r >= rows) return;
     int rt = r;
     const int rh = w.kvh * p.group + p.by_group.take(rt);
-    const long long at = w.b * p.lse_b + rh * p.lse_h + w.q0 + rt;
+    const long long at = w.b * p.lse_b + rh * p.lse_h + w.q0 + rt, pr = w.split * p.part_rows + w.part(p, r);
     float M0 = -INFINITY, L = 0.f, a[4];
 #pragma unroll
     for (int x = 0; x < 4; ++x) M0 = fmaxf(M0, s_ml[x * 32 + r].x);
@@ -680,11 +690,11 @@ __global__ __launch_bounds__(256) void few_kernel(const Params p) {
         }
 #pragma unroll
         for (int e = 0; e < 8; ++e) v[e] *= inv;
-        if (p.splits > 1) store8<float>(reinterpret_cast<char*>(p.part + (w.split * p.part_rows + at) * p.D), d, v);
+        if (p.splits > 1) store8<float>(reinterpret_cast<char*>(p.part + pr * p.D), d, v);
         else store8<T>(p.out.p + w.b * p.out.b + (w.q0 + rt) * p.out.t + rh * p.out.h, d, v);
     }
     if ((tid & 7) == 0) {
-        if (p.splits > 1) *reinterpret_cast<float2*>(p.part_ml + 2 * (w.split * p.part_rows + at)) = float2{M0 - lift, L};
+        if (p.splits > 1) *reinterpret_cast<float2*>(p.part_ml + 2 * pr) = float2{M0 - lift, L};
         else p.lse[at] = L == 0.f ? -INFINITY : (M0 - lift + __builtin_amdgcn_logf(L)) * LN2;
     }
 }
@@ -706,11 +716,11 @@ template <int SL> struct Join {
 template <int SL, class F> __device__ __forceinline__ void join_rows(const Params& p, F f) {
     const Where w = where(p, true);                                  // (split: which ROWS rows of the block)
     const Join<SL> j;
-    const int rows = w.ql * p.group, r = w.tile * QB * p.group + w.sub * QB + w.split * Join<SL>::ROWS + j.row;
+    const int rows = w.ql * p.group, in = w.split * Join<SL>::ROWS + j.row, r = w.tile * QB * p.group + w.sub * QB + in;
     if (r >= min(rows, (w.tile + 1) * QB * p.group)) return;
     int token = r;
     const int head = w.kvh * p.group + p.by_group.take(token);
-    f(w, j, token, head, w.b * p.lse_b + head * p.lse_h + w.q0 + token);
+    f(w, j, token, head, w.b * p.lse_b + head * p.lse_h + w.q0 + token, w.part(p, in));
 }
 __device__ __forceinline__ void load8(const float* row, int d, int D, float (&v)[8]) {
 #pragma unroll
@@ -737,18 +747,18 @@ template <int SL> __device__ __forceinline__ void sum_splits(const Join<SL>& j, 
 
 template <class T, int SL>
 __global__ __launch_bounds__(256) void fwd_join_kernel(const Params p) {
-    join_rows<SL>(p, [&](const Where& w, const Join<SL>& j, int token, int head, long long at) {
+    join_rows<SL>(p, [&](const Where& w, const Join<SL>& j, int token, int head, long long at, long long pr) {
         // the largest maximum (splits that saw nothing have -inf and sum 0; a NaN sum counts whatever its maximum: it has to come out)
         float m = -INFINITY;
 #pragma unroll 4
-        for (int i = j.slice; i < p.splits; i += SL) m = fmaxf(m, p.part_ml[2 * (i * p.part_rows + at)]);
+        for (int i = j.slice; i < p.splits; i += SL) m = fmaxf(m, p.part_ml[2 * (i * p.part_rows + pr)]);
         m = j.over_slices(m, [](float x, float y) { return fmaxf(x, y); });
         float l = 0.f, v[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
 #pragma unroll 4
         for (int i = j.slice; i < p.splits; i += SL) {
-            const float2 ml = *reinterpret_cast<const float2*>(p.part_ml + 2 * (i * p.part_rows + at));
+            const float2 ml = *reinterpret_cast<const float2*>(p.part_ml + 2 * (i * p.part_rows + pr));
             float x[8];
-            load8(p.part + (i * p.part_rows + at) * p.D, j.d, p.D, x);
+            load8(p.part + (i * p.part_rows + pr) * p.D, j.d, p.D, x);
             const float a = ml.y == 0.f ? 0.f : ml.x == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(ml.x - m);
             l = __builtin_fmaf(ml.y, a, l);
 #pragma unroll
@@ -917,8 +927,9 @@ __global__ __launch_bounds__(256, (WAVES<T, DP>)) void dq_kernel(const Params p)
     if (w.kl == 1) clear(acc);                                       // (the softmax of one key is constant: P (dP - D) has only rounding to give)
     const float un = p.scale / sc;
     if (p.splits > 1) {                                              // part: sums, part_ml [split][row]: rho
-        store_row<T, DP, f32x4>(acc, reinterpret_cast<char*>(p.part + (w.split * p.part_rows + at) * p.D), h, p.D, un);
-        if (h == 0) p.part_ml[w.split * p.part_rows + at] = rho;
+        const long long pr = w.split * p.part_rows + w.part(p, wave * 32 + l31);
+        store_row<T, DP, f32x4>(acc, reinterpret_cast<char*>(p.part + pr * p.D), h, p.D, un);
+        if (h == 0) p.part_ml[pr] = rho;
         if (h == 0 && w.split == 0) { p.lse2[at] = lse2; p.ndelta[at] = nd; }
         return;
     }
@@ -928,12 +939,12 @@ __global__ __launch_bounds__(256, (WAVES<T, DP>)) void dq_kernel(const Params p)
 
 template <class T, int SL>
 __global__ __launch_bounds__(256) void dq_join_kernel(const Params p) {
-    join_rows<SL>(p, [&](const Where& w, const Join<SL>& j, int token, int head, long long at) {
+    join_rows<SL>(p, [&](const Where& w, const Join<SL>& j, int token, int head, long long at, long long pr) {
         float v[8], rho = 0.f;
 #pragma unroll 4
-        for (int i = j.slice; i < p.splits; i += SL) rho += p.part_ml[i * p.part_rows + at];
+        for (int i = j.slice; i < p.splits; i += SL) rho += p.part_ml[i * p.part_rows + pr];
         rho = j.sum(rho);
-        sum_splits<SL>(j, p.part + at * p.D, p.part_rows * p.D, p.splits, p.D, v);
+        sum_splits<SL>(j, p.part + pr * p.D, p.part_rows * p.D, p.splits, p.D, v);
         if (!j.first()) return;
         if (j.d < p.D) store8<T>(p.dq.p + w.b * p.dq.b + (w.q0 + token) * p.dq.t + head * p.dq.h, j.d, v);
         if (j.d == 0) p.ndelta[at] -= rho;
@@ -1086,9 +1097,9 @@ __global__ __launch_bounds__(256, (DKV_WAVES<T, DP>)) void dkv_kernel(const Para
     if (!live) clear(dv);
     const float un = is_f16<T>() ? 0x1p-15f : 1.f;                   // (P and with it dS carry 2^15)
     if (p.splits > 1) {                                              // part: [split][dK, dV][row][D]
-        const long long at = w.b * p.krow_b + w.kvh * p.krow_h + row;
-        store_row<T, DP, f32x4>(dk, reinterpret_cast<char*>(p.part + ((2 * w.split) * p.part_rows + at) * p.D), h, p.D, p.scale * un / sc);
-        store_row<T, DP, f32x4>(dv, reinterpret_cast<char*>(p.part + ((2 * w.split + 1) * p.part_rows + at) * p.D), h, p.D, un);
+        const long long pr = w.part(p, wave * 32 + l31);
+        store_row<T, DP, f32x4>(dk, reinterpret_cast<char*>(p.part + ((2 * w.split) * p.part_rows + pr) * p.D), h, p.D, p.scale * un / sc);
+        store_row<T, DP, f32x4>(dv, reinterpret_cast<char*>(p.part + ((2 * w.split + 1) * p.part_rows + pr) * p.D), h, p.D, un);
         return;
     }
     store_row<T, DP>(dk, p.dk.p + w.b * p.dk.b + row * p.dk.t + w.kvh * p.dk.h, h, p.D, p.scale * un / sc);
@@ -1099,13 +1110,13 @@ template <class T, int SL>
 __global__ __launch_bounds__(256) void dkv_join_kernel(const Params p) {
     const Where w = where(p, false);
     const Join<SL> j;
-    const int key = w.tile * QB + w.split * Join<SL>::ROWS + j.row;
+    const int in = w.split * Join<SL>::ROWS + j.row, key = w.tile * QB + in;
     if (key >= w.kl) return;
-    const long long row = w.k0 + key, at = w.b * p.krow_b + w.kvh * p.krow_h + row;
+    const long long row = w.k0 + key, pr = w.part(p, in);
 #pragma unroll
     for (int which = 0; which < 2; ++which) {
         float v[8];
-        sum_splits<SL>(j, p.part + (which * p.part_rows + at) * p.D, 2 * p.part_rows * p.D, p.splits, p.D, v);
+        sum_splits<SL>(j, p.part + (which * p.part_rows + pr) * p.D, 2 * p.part_rows * p.D, p.splits, p.D, v);
         const Ten& t = which ? p.dv : p.dk;
         if (j.first() && j.d < p.D) store8<T>(t.p + w.b * t.b + row * t.t + w.kvh * t.h, j.d, v);
     }

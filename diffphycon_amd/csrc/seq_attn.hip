@@ -43,7 +43,6 @@ static Params params(const dpc_seq_attn* a) {
     p.q = ten(a->q); p.k = ten(a->k); p.v = ten(a->v); p.out = ten(a->out);
     p.dout = ten(a->dout); p.dq = ten(a->dq); p.dk = ten(a->dk); p.dv = ten(a->dv);
     p.lse = a->lse; p.lse_b = a->lse_stride_b; p.lse_h = a->lse_stride_h;
-    p.krow_b = a->k_row_stride_b; p.krow_h = a->k_row_stride_h;
     p.key_mask = a->key_mask; p.mask_b = a->mask_stride_b;
     p.heads = a->heads; p.kv_heads = a->kv_heads; p.group = a->heads / a->kv_heads; p.D = a->head_dim;
     p.q_len = a->q_len; p.k_len = a->k_len; p.causal = a->causal != 0; p.scale = a->scale;
@@ -76,7 +75,8 @@ static bool plan_grid(Params& p, const dpc_seq_attn* a, bool keys, bool forward)
     p.pairs = a->batch * p.kv_heads;
     p.by_sub = Div(subs); p.by_kv = Div(p.kv_heads); p.by_group = Div(p.group); p.by_tile = Div(std::max(1, p.pairs));
     p = in_parts(p, p.splits);
-    p.part_rows = keys ? a->k_rows : a->lse_rows;
+    p.block_rows = keys ? std::min(a->k_len, QB) : (int)std::min<long long>((long long)a->q_len * p.group, QB);
+    p.part_rows = blocks * p.block_rows;
     return n < (1ll << 31) && blocks * std::max(p.splits, JOIN) < (1ll << 31);
 }
 
@@ -122,7 +122,7 @@ int dpc_seq_attn_fwd(const dpc_seq_attn* a, void* ws, size_t ws_bytes, dpc_strea
     DPC_REQUIRE(w.bytes == 0 || (ws && ws_bytes >= w.bytes), "seq_attn: workspace too small");
     if (w.q.n_tiles == 0) return DPC_OK;
     w.q.part = reinterpret_cast<float*>(align_up((size_t)ws, 256));
-    w.q.part_ml = w.q.part + (size_t)w.q.splits * a->lse_rows * a->head_dim;
+    w.q.part_ml = w.q.part + (size_t)w.q.splits * w.q.part_rows * a->head_dim;
     hipStream_t s = (hipStream_t)stream;
     ProfScope prof(PROF_ATTN, 4.0 * a->batch * a->heads * (double)a->q_len * a->k_len * a->head_dim, 0, s);
     return a->type == DPC_SEQ_F32 ? fwd_f32(w.q, s) : a->type == DPC_SEQ_F16 ? fwd_f16(w.q, s) : fwd_bf16(w.q, s);

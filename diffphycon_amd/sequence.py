@@ -474,9 +474,9 @@ def _attention_args(q, k, v, causal, scale, key_mask, plan):
     if key_mask is not None:
         key_mask = key_mask.contiguous()
     es = _BYTES[t]
-    lse_b, mask_b, krow_b = (0, 0, 0) if packed else (H * Tq, Tk, Hk * Tk)
+    lse_b, mask_b = (0, 0) if packed else (H * Tq, Tk)
     tail = (0 if key_mask is None else key_mask.data_ptr(), mask_b, *blocks, *sizes, _TYPE[t], n_seq, H, Hk, D, q_len, k_len, 1 if causal else 0,
-            B * H * Tq, B * Hk * Tk, krow_b, Tk, scale)
+            B * H * Tq, scale)
     return d, _lay(q, es), _lay(k, es), _lay(v, es), ((H, Tq) if packed else (B, H, Tq)), (lse_b, Tq), tail, key_mask
 
 

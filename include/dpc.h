@@ -469,10 +469,10 @@ typedef struct dpc_seq_attn {
     int32_t n_q_tiles, n_k_tiles;
     int32_t type, batch, heads, kv_heads, head_dim, q_len, k_len, causal;
     int64_t lse_rows;                        /* rows of lse: batch (packed: 1) * heads * tokens */
-    int64_t k_rows, k_row_stride_b, k_row_stride_h;   /* the same numbering for k: batch (packed: 1) * kv_heads * tokens; 0 and tokens when packed */
     float scale;                             /* > 0 */
 } dpc_seq_attn;
-/* Scratch of one call (0: none): partial sums where long rows are split over workgroups; backward: two floats a query row. */
+/* Scratch of one call (0: none): partial sums where long rows are split over workgroups, by the blocks of 128 rows that there are, at most 1024 of them
+ * over all splits; backward: two floats a row of lse. */
 size_t dpc_seq_attn_workspace_bytes(const dpc_seq_attn* a, int backward);
 int dpc_seq_attn_fwd(const dpc_seq_attn* a, void* ws, size_t ws_bytes, dpc_stream_t stream);
 /* dq, dk, dv from dout and the forward's out and lse: the probabilities are computed again from q, k and lse. */

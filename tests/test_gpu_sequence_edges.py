@@ -154,3 +154,22 @@ def test_attention_gradients_of_an_infinite_row_do_not_depend_on_a_mask(bad, t, 
     lse[0, 1, 7] = -math.inf
     masked = S.attention_backward(dout, q, k, v, out, lse, key_mask=torch.ones(B, Lk, dtype=torch.bool, device=dev))
     assert not any(x.isnan().any() for x in masked) and not masked[0][0, 7, 1].any()
+
+
+@pytest.mark.parametrize("t", TYPES, ids=str)
+@pytest.mark.parametrize("H,Hk,D", [(6, 2, 64), (2, 2, 128)])
+@pytest.mark.parametrize("causal", [False, True])
+def test_attention_of_few_sequences_in_a_long_buffer(H, Hk, D, causal, t, dev):
+    """Long and short sequences of a padded plan whose walks are split: partial sums are numbered by the blocks that the plan has."""
+    from diffphycon_amd import sequence as S
+    ql, kl, Lq, Lk = [1100, 3, 0, 140, 1], [1500, 700, 9, 140, 0], 1300, 1600
+    B = len(ql)
+    g = _gen(H + D)
+    q, k, v, dout = _randn(g, B, Lq, H, D, dtype=t), _randn(g, B, Lk, Hk, D, dtype=t), _randn(g, B, Lk, Hk, D, dtype=t), _randn(g, B, Lq, H, D, dtype=t)
+    plan = S.SequencePlan.padded(ql, Lq, kl, Lk, device=dev)
+    out, lse = S.attention_forward(q, k, v, causal=causal, plan=plan)
+    grads = S.attention_backward(dout, q, k, v, out, lse, causal=causal, plan=plan)
+    _check_attention(q, k, v, dout, out, lse, grads, list(zip(ql, kl)), causal=causal)
+    plan = S.SequencePlan.padded([1] * B, Lq, kl, Lk, device=dev)    # one token a sequence: few rows, many splits
+    out, lse = S.attention_forward(q, k, v, causal=causal, plan=plan)
+    _check_attention(q, k, v, None, out, lse, None, list(zip([1] * B, kl)), causal=causal)
