@@ -7,10 +7,11 @@
 namespace dpc {
 namespace seqattn {
 
+constexpr long long MAX_TOKEN_STRIDE = ((1ll << 31) - 4096) / 64;    // bytes: 64 rows within 2^31, for a lane's offset in a tile is 32 bits
+
 static bool bad_tensor(const dpc_seq_tensor& t, int es) {
-    // (64 rows within 2^31 bytes: a lane's offset in a tile is 32 bits)
     return !t.p || ((size_t)t.p | (size_t)(t.stride_b * es) | (size_t)(t.stride_t * es) | (size_t)(t.stride_h * es)) % 16 != 0 ||
-           t.stride_t < 0 || t.stride_t * es > ((1ll << 31) - 4096) / 64;
+           t.stride_t < 0 || t.stride_t * es > MAX_TOKEN_STRIDE;
 }
 
 static int check(const dpc_seq_attn* a, bool backward) {
@@ -25,7 +26,7 @@ static int check(const dpc_seq_attn* a, bool backward) {
                     ((size_t)a->q_tiles | (size_t)a->k_tiles) % 32 == 0, "seq_attn: both block lists, on 32 bytes, or neither");
     if (a->batch == 0) return DPC_OK;
     const int es = a->type == DPC_SEQ_F32 ? 4 : 2;
-    const char* msg = "seq_attn: tensors must not be null; bases and strides must be multiples of 16 bytes, token strides below 2^25 bytes";
+    const char* msg = "seq_attn: tensors must not be null; bases and strides must be multiples of 16 bytes, token strides at most 2^25 - 64 bytes";
     if (a->q_len) DPC_REQUIRE(!bad_tensor(a->q, es) && !bad_tensor(a->out, es) && a->lse, msg);
     if (a->q_len && a->k_len) DPC_REQUIRE(!bad_tensor(a->k, es) && !bad_tensor(a->v, es), msg);
     if (backward) {

@@ -23,6 +23,7 @@ from . import _lib
 
 _TYPE = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}
 _BYTES = {torch.float32: 4, torch.float16: 2, torch.bfloat16: 2}
+_FAR = ((1 << 31) - 4096) // 64                                      # bytes between tokens at most: 64 rows of a tile within 2^31 bytes (seq_attn.hip: MAX_TOKEN_STRIDE)
 
 
 # ------------------------------------------------------------------------------------------------------------------ checks
@@ -64,9 +65,9 @@ def _in_use(owner, d):
 
 
 def _ok16(x, es):
-    """Whether a kernel can read x as it lies: last axis contiguous, base and strides on 16 bytes, tokens less than 2^25 bytes apart."""
+    """Whether a kernel can read x as it lies: last axis contiguous, base and strides on 16 bytes, tokens at most _FAR bytes apart."""
     s = [n if m > 1 else 0 for n, m in zip(x.stride()[:-1], x.shape[:-1])]
-    return x.stride(-1) == 1 and not any(n * es & 15 for n in s) and x.data_ptr() & 15 == 0 and s[-2] * es < 1 << 25
+    return x.stride(-1) == 1 and not any(n * es & 15 for n in s) and x.data_ptr() & 15 == 0 and s[-2] * es <= _FAR
 
 
 def _lay(x, es):
@@ -77,7 +78,7 @@ def _lay(x, es):
         b = 0
         t, h, d = x.stride()
     p = x.data_ptr()
-    if d == 1 and not (p | b * es | t * es | h * es) & 15 and t * es < 1 << 25:
+    if d == 1 and not (p | b * es | t * es | h * es) & 15 and t * es <= _FAR:
         return x, p, b, t, h
     if x.numel() and not _ok16(x, es):
         x = x.clone(memory_format=torch.contiguous_format)

@@ -173,3 +173,19 @@ def test_attention_of_few_sequences_in_a_long_buffer(H, Hk, D, causal, t, dev):
     plan = S.SequencePlan.padded([1] * B, Lq, kl, Lk, device=dev)    # one token a sequence: few rows, many splits
     out, lse = S.attention_forward(q, k, v, causal=causal, plan=plan)
     _check_attention(q, k, v, None, out, lse, None, list(zip([1] * B, kl)), causal=causal)
+
+
+@pytest.mark.parametrize("far", [2 ** 25 - 128, 2 ** 25 - 64, 2 ** 25 - 48, 2 ** 25 - 16, 2 ** 25])
+def test_attention_of_tokens_far_apart(far, dev):
+    """Token strides at the border of what a kernel reads in place (bytes): the same results, to the bit, as from contiguous tensors."""
+    from diffphycon_amd import sequence as S
+    g = _gen(91)
+    t, L, D = torch.bfloat16, 70, 64
+    k, q, dout = (_randn(g, 1, L, 1, D, dtype=t) for _ in range(3))
+    wide = torch.empty(L * far // 2, dtype=t, device=dev).as_strided((1, L, 1, D), (0, far // 2, D, 1))
+    wide.copy_(k)
+    out, lse = S.attention_forward(q, k, k, causal=True)
+    o2, l2 = S.attention_forward(q, wide, wide, causal=True)
+    assert torch.equal(out, o2) and torch.equal(lse, l2)
+    for a, b in zip(S.attention_backward(dout, q, k, k, out, lse, causal=True), S.attention_backward(dout, q, wide, wide, out, lse, causal=True)):
+        assert torch.equal(a, b)

@@ -39,3 +39,22 @@ def test_scratch_of_a_padded_plan_goes_by_its_sequences_not_by_the_buffer():
             for causal in (0, 1):
                 a = _attn(batch=B, heads=H, kv_heads=Hk, head_dim=D, q_len=Lq, k_len=Lk, causal=causal, lse_rows=B * H * Lq)
                 assert need(a, 1) <= 8 * a.lse_rows + 1024 * 128 * 2 * D * 4 + 4096 and need(a, 0) <= 1024 * 128 * (D + 2) * 4 + 4096
+
+
+# ---------------------------------------------------------------------------------------------------------------- strides
+@pytest.mark.parametrize("es,dtype", [(2, torch.bfloat16), (4, torch.float32)])
+def test_token_strides_are_copied_exactly_where_the_entry_refuses_them(es, dtype):
+    """Around the largest token stride that a kernel reads (64 rows within 2^31 bytes): a layout that is not copied is one that the entry takes."""
+    need = _lib.lib().dpc_seq_attn_workspace_bytes
+    taken = set()
+    for stride in range((1 << 25) - 160, (1 << 25) + 33, 16):
+        x = torch.empty(stride // es + 8, dtype=dtype).as_strided((1, 2, 1, 8), (0, stride // es, 8, 1))
+        as_is = S._lay(x, es)[0] is x
+        assert as_is == S._ok16(x, es)
+        a = _attn(type=0 if es == 4 else 2, head_dim=8, q=_lib.SeqTensor(4096, 0, stride // es, 8))
+        entry = need(C.byref(a), 1) > 0
+        assert as_is == entry, (stride, as_is, entry)
+        if not entry:
+            assert b"token strides" in _lib.lib().dpc_last_error()
+        taken.add(entry)
+    assert taken == {True, False}
