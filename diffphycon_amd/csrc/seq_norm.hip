@@ -387,24 +387,30 @@ __global__ __launch_bounds__(256) void bwd_wide_kernel(const BwdParams p) {
     }
 }
 
-// dweight / dbias: 32 columns x 32 slices of the partial rows a workgroup; slices are joined in order
+// dweight / dbias: 32 columns x 32 slices of the partial rows a workgroup, which goes on by whole grids (a launch holds fewer than 2^32 threads); slices
+// are joined in order
+constexpr int PARAM_BLOCKS = 1 << 16;
 template <class P>
 __global__ __launch_bounds__(1024) void param_kernel(const float* __restrict__ part, void* dw, void* db, int nblk, int C) {
     __shared__ float s[32][33];
-    const int half = blockIdx.y, col = threadIdx.x & 31, slice = threadIdx.x >> 5, c = blockIdx.x * 32 + col;
+    const int half = blockIdx.y, col = threadIdx.x & 31, slice = threadIdx.x >> 5;
     void* out = half ? db : dw;
     if (!out) return;
-    float sum = 0.f;
-    if (c < C) {
+    for (int c0 = blockIdx.x * 32; c0 < C; c0 += gridDim.x * 32) {
+        const int c = c0 + col;
+        float sum = 0.f;
+        if (c < C) {
 #pragma unroll 8
-        for (int k = slice; k < nblk; k += 32) sum += part[((long long)k * 2 + half) * C + c];
-    }
-    s[slice][col] = sum;
-    __syncthreads();
-    if (slice == 0 && c < C) {
-        double t = 0.0;
-        for (int k = 0; k < 32; ++k) t += (double)s[k][col];
-        put_param<P>(out, c, (float)t);
+            for (int k = slice; k < nblk; k += 32) sum += part[((long long)k * 2 + half) * C + c];
+        }
+        s[slice][col] = sum;
+        __syncthreads();
+        if (slice == 0 && c < C) {
+            double t = 0.0;
+            for (int k = 0; k < 32; ++k) t += (double)s[k][col];
+            put_param<P>(out, c, (float)t);
+        }
+        __syncthreads();
     }
 }
 
@@ -426,6 +432,7 @@ template <bool BWD, class F> int by_width(int acc, F f) {
 }
 
 constexpr int FWD_BLOCKS = 2048;
+constexpr int MAX_C = 1 << 30;                // columns are counted in 32 bits, a step of 2048 accesses past the last one included
 // Workgroups of the backward pass: each writes one row of partial sums (8 C bytes, read once more), which may cost some 10 % of the rows' own traffic,
 // but two workgroups a CU are there in any case.
 static int bwd_blocks(long long rows, int es) { return (int)std::min(rows, std::min(2048ll, std::max(512ll, rows * es / 64))); }
@@ -463,7 +470,7 @@ template <class T, class P, bool VECT> int bwd(const BwdParams& p, hipStream_t s
         else hipLaunchKernelGGL((bwd_kernel<T, P, G, N, VECT, THREADS>), dim3(grid), dim3(THREADS), 0, s, p);
         DPC_LAUNCH_CHECK();
         if (!p.sums) return (int)DPC_OK;
-        hipLaunchKernelGGL((param_kernel<P>), dim3((p.C + 31) / 32, 2), dim3(1024), 0, s, p.part, p.dw, p.db, grid, p.C);
+        hipLaunchKernelGGL((param_kernel<P>), dim3(std::min((p.C + 31) / 32, PARAM_BLOCKS), 2), dim3(1024), 0, s, p.part, p.dw, p.db, grid, p.C);
         DPC_LAUNCH_CHECK();
         return (int)DPC_OK;
     });
@@ -495,7 +502,7 @@ int dpc_seq_norm_fwd(const void* x, const void* weight, const void* bias, void* 
                      int64_t x_stride, float eps, int type, int wtype, dpc_stream_t stream) {
     DPC_REQUIRE(type >= DPC_SEQ_F32 && type <= DPC_SEQ_BF16, "seq_norm: unknown element type");
     DPC_REQUIRE(wtype == DPC_SEQ_F32 || wtype == type, "seq_norm: weight and bias are fp32 or of the element type");
-    DPC_REQUIRE(rows >= 0 && C >= 1 && eps > 0.f, "seq_norm: rows >= 0, C >= 1, eps > 0");
+    DPC_REQUIRE(rows >= 0 && C >= 1 && C <= MAX_C && eps > 0.f, "seq_norm: rows >= 0, 1 <= C <= 2^30, eps > 0");
     if (rows == 0) return DPC_OK;
     DPC_REQUIRE(x && y && stats && (rows == 1 || x_stride >= C), "seq_norm: null argument or overlapping rows");
     hipStream_t s = (hipStream_t)stream;
@@ -506,7 +513,7 @@ int dpc_seq_norm_fwd(const void* x, const void* weight, const void* bias, void* 
 }
 
 size_t dpc_seq_norm_bwd_workspace_bytes(int64_t rows, int C, int type) {
-    if (rows < 1 || C < 1 || one_block(rows, C, type == DPC_SEQ_F32 ? 4 : 2)) return 0;
+    if (rows < 1 || C < 1 || C > MAX_C || one_block(rows, C, type == DPC_SEQ_F32 ? 4 : 2)) return 0;
     return (size_t)bwd_blocks(rows, type == DPC_SEQ_F32 ? 4 : 2) * 2 * (size_t)C * sizeof(float) + 256;
 }
 
@@ -515,7 +522,7 @@ int dpc_seq_norm_bwd(const void* dy, const void* x, const float* stats, const vo
                      dpc_stream_t stream) {
     DPC_REQUIRE(type >= DPC_SEQ_F32 && type <= DPC_SEQ_BF16, "seq_norm_bwd: unknown element type");
     DPC_REQUIRE(wtype == DPC_SEQ_F32 || wtype == type, "seq_norm_bwd: weight and bias are fp32 or of the element type");
-    DPC_REQUIRE(rows >= 1 && C >= 1, "seq_norm_bwd: rows >= 1, C >= 1");
+    DPC_REQUIRE(rows >= 1 && C >= 1 && C <= MAX_C, "seq_norm_bwd: rows >= 1, 1 <= C <= 2^30");
     DPC_REQUIRE(dy && x && stats && dx && (rows == 1 || (x_stride >= C && (dy_stride >= C || dy_stride == 0))), "seq_norm_bwd: null argument or overlapping rows");
     const int sums = dweight || dbias, es = type == DPC_SEQ_F32 ? 4 : 2;
     const size_t need = sums ? dpc_seq_norm_bwd_workspace_bytes(rows, C, type) : 0;

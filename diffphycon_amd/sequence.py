@@ -155,13 +155,13 @@ def _matrix(x, n):
 def layer_norm_forward(x, weight=None, bias=None, eps=1e-5):
     """y = (x - mean) / sqrt(variance + eps) * weight + bias over the last axis (biased variance) -> (y, stats).
 
-    x: any shape [..., C], C >= 1, any strides; weight, bias: [C] of float32 or of x's type, or None.  stats [rows, 2] float32 = (mean,
+    x: any shape [..., C], C from 1 to 2^30, any strides; weight, bias: [C] of float32 or of x's type, or None.  stats [rows, 2] float32 = (mean,
     1 / sqrt(variance + eps)) is what `layer_norm_backward` needs."""
     if _elsewhere(x):
         with torch.cuda.device(x.device):
             return layer_norm_forward(x, weight, bias, eps)
-    if x.dim() < 1 or x.shape[-1] < 1:
-        raise ValueError("x: at least one axis of at least one element")
+    if x.dim() < 1 or not 1 <= x.shape[-1] <= 1 << 30:
+        raise ValueError("x: at least one axis, the last one of 1 to 2^30 elements")
     if not 0 < eps < math.inf:
         raise ValueError("eps must be positive and finite")
     t = _TYPE[_type(x)]
@@ -189,8 +189,8 @@ def layer_norm_backward(dy, x, stats, weight=None, param_grads=True, param_dtype
             return layer_norm_backward(dy, x, stats, weight, param_grads, param_dtype)
     if dy.shape != x.shape:
         raise ValueError(f"dy {tuple(dy.shape)} must have x's shape {tuple(x.shape)}")
-    if x.dim() < 1 or x.shape[-1] < 1:
-        raise ValueError("x: at least one axis of at least one element")
+    if x.dim() < 1 or not 1 <= x.shape[-1] <= 1 << 30:
+        raise ValueError("x: at least one axis, the last one of 1 to 2^30 elements")
     t = _TYPE[_type(x, dy)]
     _norm_params(x, weight, None)
     n = x.shape[-1]

@@ -419,7 +419,7 @@ int dpc_adam_ema_step(float* w, const float* g, float* m, float* v, float* ema, 
  * whatever the element type; nothing is accumulated with atomics, so results repeat bit for bit. */
 enum dpc_seq_type { DPC_SEQ_F32 = 0, DPC_SEQ_F16 = 1, DPC_SEQ_BF16 = 2 };
 
-/* y = (x - mean) * rstd * weight + bias over the last axis of x [rows][C] (x rows x_stride elements apart, y contiguous);
+/* y = (x - mean) * rstd * weight + bias over the last axis of x [rows][C], C <= 2^30 (x rows x_stride elements apart, y contiguous);
  * weight / bias [C] of type wtype (fp32 or type) or NULL; stats [rows][2] = (mean, rstd), rstd = (variance + eps)^-1/2. */
 int dpc_seq_norm_fwd(const void* x, const void* weight, const void* bias, void* y, float* stats, int64_t rows, int C,
                      int64_t x_stride, float eps, int type, int wtype, dpc_stream_t stream);

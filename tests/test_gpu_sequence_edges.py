@@ -189,3 +189,26 @@ def test_attention_of_tokens_far_apart(far, dev):
     assert torch.equal(out, o2) and torch.equal(lse, l2)
     for a, b in zip(S.attention_backward(dout, q, k, k, out, lse, causal=True), S.attention_backward(dout, q, wide, wide, out, lse, causal=True)):
         assert torch.equal(a, b)
+
+
+def test_layer_norm_of_a_very_wide_row(dev):
+    """2^27 + 264 columns: the parameters' gradients have more columns than one launch has threads for a column each."""
+    from diffphycon_amd import sequence as S
+    n = 2 ** 27 + 264
+    g = torch.Generator(device=dev).manual_seed(5)
+    x = torch.randn(1, n, generator=g, device=dev).to(torch.bfloat16)
+    dy = torch.randn(1, n, generator=g, device=dev).to(torch.bfloat16)
+    y, st = S.layer_norm_forward(x)
+    dx, dw, db = S.layer_norm_backward(dy, x, st)
+    assert torch.equal(db, dy[0].float())                            # (one row: its own elements)
+    xh = (x[0].float() - st[0, 0]) * st[0, 1]
+    assert ((dw - dy[0].float() * xh).abs() <= 4 * O.E * dw.abs() + 1e-37).all()
+    assert ((y[0].float() - xh).abs() <= O.UNIT[torch.bfloat16] * xh.abs() * 1.001 + 1e-37).all()
+    assert abs(st[0, 0].item() - x.double().mean().item()) < 1e-6
+    # dx: a lane adds at most n / 256 + 8 terms one by one, so a mean over the row is off by less than that many 2^-24 of its terms' mean size.  (That the
+    # elements of dx add up to 0 is lost in their rounding: g lies on bf16's grid, and mean(g), 2^-13 here, is less than its step.)
+    gx = dy[0].double() * xh.double()
+    a, b, rstd = dy.double().mean(), gx.mean(), st[0, 1].double()
+    off = (n / 256 + 24) * O.E * rstd * (dy.double().abs().mean() + xh.double().abs() * gx.abs().mean())
+    value = rstd * (dy[0].double() - a - xh.double() * b)
+    assert ((dx[0].double() - value).abs() <= O.UNIT[torch.bfloat16] * (value.abs() + off) + off + 8 * O.E * (dy[0].double().abs() + 1)).all()

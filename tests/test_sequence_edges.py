@@ -58,3 +58,22 @@ def test_token_strides_are_copied_exactly_where_the_entry_refuses_them(es, dtype
             assert b"token strides" in _lib.lib().dpc_last_error()
         taken.add(entry)
     assert taken == {True, False}
+
+
+# ---------------------------------------------------------------------------------------------------------------- sizes
+@pytest.mark.parametrize("n", [(1 << 30) + 1, 1 << 31, (1 << 32) + 8])
+def test_layer_norm_refuses_rows_beyond_its_range(n):
+    """A width that the entry's 32 bits cannot hold is refused, not cut off; rows are at most 2^30 elements wide."""
+    x = torch.zeros(1).expand(1, n)
+    st = torch.zeros(1, 2)
+    for f in (lambda: S.layer_norm_forward(x), lambda: S.layer_norm_backward(x, x, st), lambda: S.layer_norm_forward(x[:0]), lambda: S.layer_norm_backward(x[:0], x[:0], st[:0])):
+        with pytest.raises(ValueError, match="2\\^30"):
+            f()
+
+
+def test_layer_norm_entries_refuse_rows_beyond_their_range():
+    L, p = _lib.lib(), C.c_void_p(4096)
+    assert L.dpc_seq_norm_fwd(p, None, None, p, p, 1, (1 << 30) + 1, 1 << 31, 1e-5, 0, 0, None) < 0 and b"C" in L.dpc_last_error()
+    need = L.dpc_seq_norm_bwd_workspace_bytes(1, 1 << 30, 0)
+    assert need >= 2 * (1 << 30) * 4 and L.dpc_seq_norm_bwd_workspace_bytes(1, (1 << 30) + 1, 0) == 0
+    assert L.dpc_seq_norm_bwd(p, p, p, None, p, p, p, 1, (1 << 30) + 1, 1 << 31, 1 << 31, 0, 0, p, 1 << 40, None) < 0
