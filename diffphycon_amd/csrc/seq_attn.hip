@@ -55,7 +55,7 @@ static Params params(const dpc_seq_attn* a) {
 // the partial sums are joined in order by a second launch.  Under a causal mask over (nearly) square scores the blocks' walks differ by the
 // length of the sequence and the longest one decides while all are resident: twice as many workgroups are made, and the card evens them out (dK/dV of
 // causal bf16 2 x 4096, 16/4 heads of 128: 561 -> 388 us, the join 14 -> 24).
-// Returns false when the grid would pass 2^31.
+// Returns false when a launch would have 2^32 threads or more.
 constexpr int SLOTS = 512;
 static bool plan_grid(Params& p, const dpc_seq_attn* a, bool keys, bool forward) {
     p.tiles = keys ? a->k_tiles : a->q_tiles;
@@ -78,7 +78,7 @@ static bool plan_grid(Params& p, const dpc_seq_attn* a, bool keys, bool forward)
     p = in_parts(p, p.splits);
     p.block_rows = keys ? std::min(a->k_len, QB) : (int)std::min<long long>((long long)a->q_len * p.group, QB);
     p.part_rows = blocks * p.block_rows;
-    return n < (1ll << 31) && blocks * std::max(p.splits, JOIN) < (1ll << 31);
+    return n < (1ll << 31) && blocks * (p.splits > 1 ? std::max(p.splits, JOIN) : 1) < (1ll << 24);
 }
 
 static size_t part_bytes(const Params& p, int per_row) {

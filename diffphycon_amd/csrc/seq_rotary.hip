@@ -153,6 +153,8 @@ __global__ __launch_bounds__(256) void rotary_kernel(const Params p) {
     }
 }
 
+constexpr unsigned MAX_GRID = 1u << 24;          // workgroups of 256 threads along an axis: a launch holds fewer than 2^32
+
 static bool aligned(const dpc_seq_tensor& t, int es) {
     return !t.p || ((size_t)t.p | (size_t)(t.stride_b * es) | (size_t)(t.stride_t * es) | (size_t)(t.stride_h * es)) % 16 == 0;
 }
@@ -189,6 +191,7 @@ template <class T> int run(const dpc_seq_rotary* a, hipStream_t s) {
         p.per_wg = 64 / items;
         p.work = p.total * groups;
         const dim3 grid((p.work + 4ll * p.per_wg - 1) / (4 * p.per_wg));
+        DPC_REQUIRE(grid.x < MAX_GRID, "seq_rotary: grid too large");
         if (four) hipLaunchKernelGGL((rotary_half_kernel<T, 4>), grid, dim3(256), 0, s, p);
         else hipLaunchKernelGGL((rotary_half_kernel<T, 1>), grid, dim3(256), 0, s, p);
         DPC_LAUNCH_CHECK();
@@ -196,7 +199,8 @@ template <class T> int run(const dpc_seq_rotary* a, hipStream_t s) {
     }
     p.per_wg = std::max(1, 256 / per_token);
     p.work = p.per_wg * per_token;
-    const dim3 grid((p.total + p.per_wg - 1) / p.per_wg, (p.work + 255) / 256);
+    const dim3 grid((p.total + (long long)p.per_wg - 1) / p.per_wg, (p.work + 255) / 256);
+    DPC_REQUIRE(grid.x < MAX_GRID, "seq_rotary: grid too large");
     if (vec && four) hipLaunchKernelGGL((rotary_kernel<T, VV, 4>), grid, dim3(256), 0, s, p);
     else if (vec) hipLaunchKernelGGL((rotary_kernel<T, VV, 1>), grid, dim3(256), 0, s, p);
     else if (four) hipLaunchKernelGGL((rotary_kernel<T, 1, 4>), grid, dim3(256), 0, s, p);

@@ -288,6 +288,8 @@ def _rotary(q, k, table, positions, start, out, transpose):
         Hk = ks[-2]
     if H < 1 or (k is not None and Hk < 1):
         raise ValueError("at least one head")
+    if (B | T | H | Hk | D) >> 31:
+        raise ValueError(f"q {tuple(shape)}: axes of 2^31 or more are not supported")
     if table.rotary_dim > D:
         raise ValueError(f"the table's rotary_dim {table.rotary_dim} exceeds the head's {D}")
     pos_b = 0
@@ -457,6 +459,8 @@ def _attention_args(q, k, v, causal, scale, key_mask, plan):
         raise ValueError(f"head size {D}: multiples of 8 up to 128 are supported")
     if B != Bk:
         raise ValueError("q and k must have one batch size")
+    if (B | Tq | Tk | H) >> 31:
+        raise ValueError(f"q {tuple(q.shape)} and k {tuple(k.shape)}: axes of 2^31 or more are not supported")
     scale = D ** -0.5 if scale is None else float(scale)
     if not 0 < scale < math.inf:
         raise ValueError("scale must be positive and finite")

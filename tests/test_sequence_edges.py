@@ -77,3 +77,33 @@ def test_layer_norm_entries_refuse_rows_beyond_their_range():
     need = L.dpc_seq_norm_bwd_workspace_bytes(1, 1 << 30, 0)
     assert need >= 2 * (1 << 30) * 4 and L.dpc_seq_norm_bwd_workspace_bytes(1, (1 << 30) + 1, 0) == 0
     assert L.dpc_seq_norm_bwd(p, p, p, None, p, p, p, 1, (1 << 30) + 1, 1 << 31, 1 << 31, 0, 0, p, 1 << 40, None) < 0
+
+
+def test_attention_and_rotary_refuse_sizes_beyond_32_bits_in_their_own_manner():
+    """Broadcast tensors of 2^31 rows cost nothing to make: ValueError, not the packing's own error (nor RuntimeError: shapes come before devices)."""
+    z, far = torch.zeros(1, 1, 1, 8), 1 << 31
+    many, long, wide = z.expand(far, 1, 1, 8), z.expand(1, far, 1, 8), z.expand(1, 1, far, 8)
+    for q, k in ((many, many), (long, z), (z, long), (wide, z), (long, long)):
+        with pytest.raises(ValueError, match="2\\^31"):
+            S.attention_forward(q, k, k)
+        with pytest.raises(ValueError, match="2\\^31"):
+            S.attention_backward(q, q, k, k, q, torch.zeros(1, 1, 1))
+    table = type("T", (), dict(table=torch.zeros(16, 4, 2), rotary_dim=8, max_positions=1 << 40, layout="half", stream=None))
+    for q in (many, long, wide, torch.zeros(1, 1, 1, 1).expand(1, 1, 1, far)):
+        for k in (q, None):
+            with pytest.raises(ValueError, match="2\\^31"):
+                S.rotary_forward(q, k, table)
+
+
+def test_entries_refuse_launches_of_more_threads_than_32_bits_count():
+    """Before anything is launched: 2^24 workgroups of 256 threads are one launch too many."""
+    L = _lib.lib()
+    a = _attn(batch=1 << 24, heads=1, lse_rows=1 << 26)
+    ws = C.c_void_p(1 << 20)
+    for rc in (L.dpc_seq_attn_fwd(C.byref(a), ws, 1 << 40, None), L.dpc_seq_attn_bwd(C.byref(a), ws, 1 << 40, None)):
+        assert rc < 0 and b"grid too large" in L.dpc_last_error()
+    T = _lib.SeqTensor(4096, 0, 64 * 128, 128)
+    for interleaved in (0, 1):
+        a = _lib.SeqRotary(xq=T, yq=_lib.SeqTensor(8192, 0, 64 * 128, 128), table=4096, max_positions=1 << 30, type=0, batch=1, tokens=1 << 25, heads=64, head_dim=128, rotary_dim=128,
+                           interleaved=interleaved)
+        assert L.dpc_seq_rotary_run(C.byref(a), None) < 0 and b"grid too large" in L.dpc_last_error()
