@@ -459,6 +459,14 @@ template <class F> __device__ __forceinline__ int count_rows(int from, int to, i
     return n;
 }
 
+// What a row's sum l of exponentials, relative to 2^m, makes of it: 1 / l and the log-sum-exp; 0 and -inf for a row that saw no key.  A sum of 0 over some keys
+// is none of that: scores from 2^30 on are further from their maximum by its rounding than an exponent holds, and the row becomes NaN.
+__device__ __forceinline__ bool sees_none(float m, float l) { return l == 0.f && m == -INFINITY; }
+__device__ __forceinline__ float inverse(float m, float l) { return sees_none(m, l) ? 0.f : 1.f / l; }
+__device__ __forceinline__ float lse_of(float m, float l) {
+    return l != 0.f ? (m + __builtin_amdgcn_logf(l)) * LN2 : sees_none(m, l) ? -INFINITY : __builtin_nanf("");
+}
+
 // Forward.  Rows of a query block: row r = token r / group, head kvh * group + r % group, so that heads which share keys share the tile's loads.  One
 // pass over the keys with a running maximum and sum; 128 rows a workgroup, 32 a wave, tiles of 64 keys and values in two LDS buffers, one barrier a tile.
 // Causal bf16 2 x 4096, 16/4 heads of 128: 155 us (890 TFLOP/s); packed causal fp16 24 x 1900, 12 heads of 64: 93 us (560); fp32 32 x 1024, 8 heads of
@@ -567,8 +575,8 @@ __global__ __launch_bounds__(256, (WAVES<T, DP>)) void fwd_kernel(const Params p
         }
         return;
     }
-    store_row<T, DP>(o, p.out.p + w.b * p.out.b + (w.q0 + token) * p.out.t + head * p.out.h, h, p.D, l == 0.f ? 0.f : 1.f / l);
-    if (h == 0) p.lse[at] = l == 0.f ? -INFINITY : (m - lift + __builtin_amdgcn_logf(l)) * LN2;
+    store_row<T, DP>(o, p.out.p + w.b * p.out.b + (w.q0 + token) * p.out.t + head * p.out.h, h, p.D, inverse(m, l));
+    if (h == 0) p.lse[at] = lse_of(m - lift, l);
 }
 
 template <class T> __device__ __forceinline__ void store8(char* row, int d, const float (&v)[8]) {
@@ -679,7 +687,7 @@ __global__ __launch_bounds__(256) void few_kernel(const Params p) {
         a[x] = ml.y == 0.f ? 0.f : ml.x == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(ml.x - M0);
         L = __builtin_fmaf(ml.y, a[x], L);
     }
-    const float inv = p.splits > 1 ? 1.f : L == 0.f ? 0.f : 1.f / L;
+    const float inv = p.splits > 1 ? 1.f : inverse(M0, L);
     for (int d = (tid & 7) * 8; d < p.D; d += 64) {
         float v[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
 #pragma unroll
@@ -695,7 +703,7 @@ __global__ __launch_bounds__(256) void few_kernel(const Params p) {
     }
     if ((tid & 7) == 0) {
         if (p.splits > 1) *reinterpret_cast<float2*>(p.part_ml + 2 * pr) = float2{M0 - lift, L};
-        else p.lse[at] = L == 0.f ? -INFINITY : (M0 - lift + __builtin_amdgcn_logf(L)) * LN2;
+        else p.lse[at] = lse_of(M0 - lift, L);
     }
 }
 
@@ -765,12 +773,12 @@ __global__ __launch_bounds__(256) void fwd_join_kernel(const Params p) {
             for (int e = 0; e < 8; ++e) v[e] = __builtin_fmaf(x[e], a, v[e]);
         }
         l = j.sum(l);
-        const float inv = l == 0.f ? 0.f : 1.f / l;
+        const float inv = inverse(m, l);
 #pragma unroll
         for (int e = 0; e < 8; ++e) v[e] = j.sum(v[e]) * inv;
         if (!j.first()) return;
         if (j.d < p.D) store8<T>(p.out.p + w.b * p.out.b + (w.q0 + token) * p.out.t + head * p.out.h, j.d, v);
-        if (j.d == 0) p.lse[at] = l == 0.f ? -INFINITY : (m + __builtin_amdgcn_logf(l)) * LN2;
+        if (j.d == 0) p.lse[at] = lse_of(m, l);
     });
 }
 

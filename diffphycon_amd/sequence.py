@@ -493,11 +493,14 @@ def attention_forward(q, k, v, *, causal=False, scale=None, key_mask=None, plan=
 
     q [B, Lq, H, D], k and v [B, Lk, Hk, D] (or packed, see `SequencePlan`), H a multiple of Hk: query head h reads key / value head
     h // (H / Hk); D a multiple of 8 up to 128; scale defaults to D^-0.5.  causal: query i sees keys j <= i + Lk - Lq of its sequence.
-    key_mask: bool [B, Lk] (packed: [tokens]), True = takes part; what masked keys and values hold never matters.  (A NaN or infinity in a
-    key or value that some query of the call sees may reach queries that the causal mask keeps from it, as 0 * NaN does in the formula.  float32 operands are split into bfloat16 parts: an infinity or a value above 3.38e38 gives NaN.)  A
-    query that sees nothing gives zeros and lse -inf.  lse [B, H, Lq] (packed: [H, tokens]) float32 is the log of the softmax's
-    denominator, which `attention_backward` needs.  Any strides; layouts whose head rows do not start on 16 bytes are copied first.  Rows of a padded
-    plan that belong to no sequence are zero (lse -inf), or left as they were in a given `out` buffer."""
+    key_mask: bool [B, Lk] (packed: [tokens]), True = takes part; what masked keys and values hold never matters.  A query that sees nothing
+    gives zeros and lse -inf.  lse [B, H, Lq] (packed: [H, tokens]) float32 is the log of the softmax's denominator, which
+    `attention_backward` needs.  Any strides; layouts whose head rows do not start on 16 bytes are copied first.  Rows of a padded plan that
+    belong to no sequence are zero (lse -inf), or left as they were in a given `out` buffer.
+
+    Large values: a NaN or infinity in a key or value that some query of the call sees may reach queries that the causal mask keeps from it, as
+    0 * NaN does in the formula.  float32 operands are split into bfloat16 parts: an infinity or a value above 3.38e38 gives NaN.  Scores are
+    held in 32 bits: probabilities are off by up to 2^-22 times the score, relative, and scores beyond 2^30 may make their query NaN."""
     if _elsewhere(q):
         with torch.cuda.device(q.device):
             return attention_forward(q, k, v, causal=causal, scale=scale, key_mask=key_mask, plan=plan, out=out)

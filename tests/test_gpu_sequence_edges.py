@@ -212,3 +212,27 @@ def test_layer_norm_of_a_very_wide_row(dev):
     off = (n / 256 + 24) * O.E * rstd * (dy.double().abs().mean() + xh.double().abs() * gx.abs().mean())
     value = rstd * (dy[0].double() - a - xh.double() * b)
     assert ((dx[0].double() - value).abs() <= O.UNIT[torch.bfloat16] * (value.abs() + off) + off + 8 * O.E * (dy[0].double().abs() + 1)).all()
+
+
+@pytest.mark.parametrize("t", [torch.float32, torch.bfloat16], ids=str)
+@pytest.mark.parametrize("Lq,Lk", [(1, 8), (1, 2000), (60, 64), (200, 1500)])
+@pytest.mark.parametrize("score", [127, 101, 60, 41, 33, 8])
+def test_attention_scores_beyond_fp32_are_not_rows_that_see_nothing(score, Lq, Lk, t, dev):
+    """A row of equal scores 1.75 * 2^score.  The first overflows when it is counted in powers of two, the others are further from a whole step of fp32 than
+    an exponent reaches: NaN, in the row alone, never the zeros and -inf of a row without keys.  The last is ordinary: the keys share the row."""
+    from diffphycon_amd import sequence as S
+    g = _gen(95)
+    q, k, v = (_randn(g, 1, n, 2, 16, dtype=t) for n in (Lq, Lk, Lk))
+    row = Lq // 2
+    k[0, :, 1, 0] = 1.75 * 2.0 ** (score // 2)
+    q[0, :, 1, 0], q[0, row, 1] = 0.0, 0.0
+    q[0, row, 1, 0] = 2.0 ** (score - score // 2)
+    out, lse = S.attention_forward(q, k, v, scale=1.0)
+    mean = v[0, :, 1].double().mean(0)
+    if score == 8:
+        assert ((out[0, row, 1].double() - mean).abs() <= 0.02).all() and abs(lse[0, 1, row].item() - 448 - math.log(Lk)) <= 1e-3
+    else:
+        assert not torch.isneginf(lse[0, 1, row]) and (lse[0, 1, row].isnan() or score < 127)
+        assert out[0, row, 1].isnan().all() or ((out[0, row, 1].double() - mean).abs() <= 0.02).all()
+    out[0, row, 1], lse[0, 1, row] = 0.0, 0.0
+    assert out.isfinite().all() and lse.isfinite().all()
