@@ -96,29 +96,39 @@ def _shares(a, b):
 
 
 def _overlap(a, b):
-    """Whether a and b may share an element: equal strides and a shift inside one row of the larger axes keep views of one projection apart."""
+    """Whether a and b may share an element: equal strides and a shift that fits into a row of the two inner axes, and into every step of the
+    outer ones, keep views of one projection apart."""
     if not (a.numel() and b.numel()) or not _shares(a, b):
         return False
     if a.dim() == b.dim() and a.dim() >= 2 and a.stride()[:-2] == b.stride()[:-2]:
         wide = lambda t: (t.shape[-2] - 1) * t.stride(-2) + (t.shape[-1] - 1) * t.stride(-1) + 1
         (lo, wl), (hi, wh) = sorted(((a.storage_offset(), wide(a)), (b.storage_offset(), wide(b))))
-        outer = min((s for s, n in zip(a.stride()[:-2], a.shape[:-2]) if n > 1), default=None)
-        if hi - lo >= wl and (outer is None or (hi - lo) + wh <= outer):
+        reach, apart = hi - lo + wh, hi - lo >= wl
+        for s, n in sorted(zip(a.stride()[:-2], map(max, a.shape, b.shape))):
+            if n > 1:
+                apart, reach = apart and s >= reach, reach + s * (n - 1)
+        if apart:
             return False
     last = lambda t: t.storage_offset() + sum((n - 1) * s for n, s in zip(t.shape, t.stride()))
     return a.storage_offset() <= last(b) and b.storage_offset() <= last(a)
+
+
+def _distinct(x):
+    """Whether every element of x has a place of its own: each axis steps over all that the smaller strides reach."""
+    reach = 0
+    for s, n in sorted((s, n) for s, n in zip(x.stride(), x.shape) if n > 1):
+        if s <= reach:
+            return False
+        reach += s * (n - 1)
+    return True
 
 
 def _written(x, like, name, inputs):
     """Checks a caller's output buffer: shape, type, layout of distinct elements, and no element shared with an input."""
     if x.shape != like.shape or x.dtype != like.dtype:
         raise ValueError(f"{name}: expected shape {tuple(like.shape)} of {like.dtype}, got {tuple(x.shape)} of {x.dtype}")
-    order = sorted((s, n) for s, n in zip(x.stride(), x.shape) if n > 1)
-    reach = 0
-    for s, n in order:
-        if s <= reach:
-            raise ValueError(f"{name}: elements of the buffer overlap")
-        reach += s * (n - 1)
+    if x.numel() and not _distinct(x):
+        raise ValueError(f"{name}: elements of the buffer overlap")
     if x.numel() and not _ok16(x, x.element_size()):
         raise ValueError(f"{name}: the last axis must be contiguous, base and strides multiples of 16 bytes")
     if any(_overlap(x, i) for i in inputs):

@@ -107,3 +107,33 @@ def test_entries_refuse_launches_of_more_threads_than_32_bits_count():
         a = _lib.SeqRotary(xq=T, yq=_lib.SeqTensor(8192, 0, 64 * 128, 128), table=4096, max_positions=1 << 30, type=0, batch=1, tokens=1 << 25, heads=64, head_dim=128, rotary_dim=128,
                            interleaved=interleaved)
         assert L.dpc_seq_rotary_run(C.byref(a), None) < 0 and b"grid too large" in L.dpc_last_error()
+
+
+# ---------------------------------------------------------------------------------------------------------------- buffers that overlap
+def _elements(x):
+    at = torch.tensor([x.storage_offset()])
+    for n, s in zip(x.shape, x.stride()):
+        at = (at[:, None] + torch.arange(n) * s).flatten()
+    return set(at.tolist())
+
+
+def test_overlap_finds_every_shared_element():
+    """Pairs of views of one storage with equal outer strides, batches that are no whole number of tokens apart among them: never "apart" where an element is
+    shared; and views of one projection, padded or not, are apart."""
+    base, g = torch.zeros(4000), torch.Generator().manual_seed(2)
+    r = lambda lo, hi: int(torch.randint(lo, hi, (1,), generator=g))  # noqa: E731
+    apart = 0
+    for _ in range(4000):
+        outer = (r(1, 60), r(1, 60))
+        sizes = (r(1, 4), r(1, 4), r(1, 4), r(1, 5))
+        a, b = (base.as_strided(sizes, (*outer, r(1, 9), 1), r(0, 40)) for _ in range(2))
+        shared = bool(_elements(a) & _elements(b))
+        found = S._overlap(a, b)
+        assert found or not shared, (a.shape, a.stride(), a.storage_offset(), b.stride(), b.storage_offset())
+        apart += not found
+    assert apart > 500
+    a = base.as_strided((2, 2, 1, 3), (10, 7, 3, 1))                 # rows at 0, 7, 10, 17; the other's at 3, 10, 13, 20
+    assert S._overlap(a, base.as_strided((2, 2, 1, 3), (10, 7, 3, 1), 3))
+    for stride_b in (5 * 96, 5 * 96 + 17):
+        q, k, v = (base.as_strided((2, 5, 4, 8), (stride_b, 96, 8, 1), 32 * i) for i in range(3))
+        assert not S._overlap(q, k) and not S._overlap(k, v) and not S._overlap(q, v)
