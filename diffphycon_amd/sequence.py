@@ -358,7 +358,7 @@ def _rotary_out(q, k, out):
     for y, x in zip(ys, xs):
         if y.shape != x.shape or y.dtype != x.dtype or y.device != x.device:
             raise ValueError("out: shape, type and device of the input")
-        if y.numel() and y.stride(-1) != 1 or any(s == 0 and n > 1 for s, n in zip(y.stride(), y.shape)):
+        if y.numel() and (y.stride(-1) != 1 or not _distinct(y)):
             raise ValueError("out: the last axis must be contiguous and elements distinct")
         for z in xs:
             itself = z is x and y.data_ptr() == z.data_ptr() and y.stride() == z.stride()

@@ -137,3 +137,18 @@ def test_overlap_finds_every_shared_element():
     for stride_b in (5 * 96, 5 * 96 + 17):
         q, k, v = (base.as_strided((2, 5, 4, 8), (stride_b, 96, 8, 1), 32 * i) for i in range(3))
         assert not S._overlap(q, k) and not S._overlap(k, v) and not S._overlap(q, v)
+
+
+def test_rotary_refuses_buffers_whose_own_elements_overlap():
+    """In place or not: two threads would write one element.  Views of a projection and of a buffer with gaps are fine."""
+    base = torch.zeros(4096)
+    q = torch.zeros(2, 4, 3, 8)
+    fine = [torch.zeros_like(q), torch.zeros(2, 4, 5, 8)[:, :, 1:4], base.as_strided((2, 4, 3, 8), (8, 16, 64, 1)), torch.zeros(3, 4, 2, 8).transpose(0, 2)]
+    for y in fine:
+        assert S._rotary_out(q, None, (y,))[0] is y
+    for y in (base.as_strided((2, 4, 3, 8), (96, 16, 8, 1)), base.as_strided((2, 4, 3, 8), (96, 24, 4, 1)), base.as_strided((2, 4, 3, 8), (40, 24, 8, 1)), q[:, :1].expand_as(q)):
+        with pytest.raises(ValueError):
+            S._rotary_out(q, None, (y,))
+    x = base.as_strided((1, 4, 3, 8), (96, 16, 8, 1))                # in place on an input that overlaps itself
+    with pytest.raises(ValueError):
+        S._rotary_out(x, None, (x,))
