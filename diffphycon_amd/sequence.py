@@ -257,6 +257,8 @@ class RotaryTable:
             raise ValueError("scaling 'ntk' needs rotary_dim >= 4")
         if scaling == "ramp" and not (len(turns) == 2 and 0 <= turns[0] < turns[1]):
             raise ValueError("turns: two rising numbers")
+        if scaling == "ramp" and trained_positions is not None and not float(trained_positions) > 0:
+            raise ValueError("trained_positions must be positive")
         device = torch.device(device)
         if device.type != "cuda":
             raise RuntimeError("libdpc needs device tensors (there is no CPU implementation)")

@@ -152,3 +152,10 @@ def test_rotary_refuses_buffers_whose_own_elements_overlap():
     x = base.as_strided((1, 4, 3, 8), (96, 16, 8, 1))                # in place on an input that overlaps itself
     with pytest.raises(ValueError):
         S._rotary_out(x, None, (x,))
+
+
+@pytest.mark.parametrize("kw", [dict(trained_positions=float("nan")), dict(trained_positions=0), dict(trained_positions=-5.0),
+                                dict(turns=(1.0, float("nan")))])
+def test_rotary_table_refuses_a_ramp_without_meaning(kw):
+    with pytest.raises(ValueError):
+        S.RotaryTable(8, 16, scaling="ramp", factor=2.0, **kw)
