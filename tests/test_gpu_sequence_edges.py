@@ -236,3 +236,22 @@ def test_attention_scores_beyond_fp32_are_not_rows_that_see_nothing(score, Lq, L
         assert out[0, row, 1].isnan().all() or ((out[0, row, 1].double() - mean).abs() <= 0.02).all()
     out[0, row, 1], lse[0, 1, row] = 0.0, 0.0
     assert out.isfinite().all() and lse.isfinite().all()
+
+
+@pytest.mark.parametrize("t", TYPES, ids=str)
+@pytest.mark.parametrize("B,H,Hk,Lq,Lk,D,causal", [
+    (4, 2, 2, 641, 641, 64, True), (8, 4, 2, 769, 769, 32, True), (2, 4, 4, 1100, 1100, 128, True), (1, 16, 8, 641, 1100, 96, True),          # split walks
+    (16, 8, 8, 641, 641, 32, True), (32, 8, 8, 513, 200, 32, True), (8, 8, 8, 1100, 1100, 64, True), (2, 16, 8, 1300, 257, 64, True),         # whole ones
+    (8, 2, 2, 700, 1030, 64, False), (16, 16, 8, 300, 513, 32, False),
+])
+def test_attention_blocks_of_many_pairs(B, H, Hk, Lq, Lk, D, causal, t, dev):
+    """(sequence, key head) pairs by the eight, whose blocks follow each other on one XCD, under a causal mask in bands (5 to 11 blocks: bands of 2 and 3, the
+    last one shorter): every block is computed, with and without splits of the walks.  Buffers hold NaN before."""
+    from diffphycon_amd import sequence as S
+    g = _gen(Lq + D + B)
+    q, k, v, dout = (torch.randn(B, n, h, D, generator=g).to(t).to(dev) for n, h in ((Lq, H), (Lk, Hk), (Lk, Hk), (Lq, H)))
+    out = torch.full_like(q, math.nan)
+    _, lse = S.attention_forward(q, k, v, causal=causal, out=out)
+    grads = tuple(torch.full_like(x, math.nan) for x in (q, k, v))
+    S.attention_backward(dout, q, k, v, out, lse, causal=causal, grads=grads)
+    _check_attention(q, k, v, dout, out, lse, grads, [(Lq, Lk)] * B, causal=causal)
