@@ -147,8 +147,8 @@ struct Split3 {
         return of(t);
     }
 };
-template <class T, int DP> constexpr bool SPLIT = sizeof(T) == 4;
-template <class T, int DP> using Op = std::conditional_t<SPLIT<T, DP>, Split3, Mma<T>>;
+template <class T> constexpr bool SPLIT = sizeof(T) == 4;
+template <class T> using Op = std::conditional_t<SPLIT<T>, Split3, Mma<T>>;
 
 struct Ten { char* p; long long b, t, h; };        // strides in bytes
 
@@ -293,7 +293,7 @@ __device__ __forceinline__ void zero_images(char* smem, int bytes) {  // (follow
 }
 // Tiles of two tensors, one ahead: issue() starts the next one, commit() waits for it and for everyone's reads of the one before.  Copied past the
 // registers into two buffers in turn (one barrier), or, split into bf16 parts, through the registers into one (two).
-template <class T, int DP, int ROWS, bool S = SPLIT<T, DP>> struct Tiles {
+template <class T, int DP, int ROWS, bool S = SPLIT<T>> struct Tiles {
     static constexpr int IMG = ROWS * Image<T, DP>::PITCH, PLANE = 0, BYTES = 4 * IMG;
     char* smem;
     Stage<T, DP, ROWS> a, b;
@@ -473,7 +473,7 @@ __device__ __forceinline__ float lse_of(float m, float l) {
 // 32: 209 us (165).
 template <class T, int DP>
 __global__ __launch_bounds__(256, (WAVES<T, DP>)) void fwd_kernel(const Params p) {
-    typedef Op<T, DP> M;
+    typedef Op<T> M;
     typedef Tiles<T, DP, KB> Tl;
     constexpr int NF = DP / M::KS, NP = 32 / M::KS, ND = DP / 32;
     extern __shared__ __attribute__((aligned(16))) char smem[];       // tiles of K and V
@@ -790,7 +790,7 @@ __global__ __launch_bounds__(256) void fwd_join_kernel(const Params p) {
 // 229, 149 and 268 us at its sizes (900, 520 and 190 TFLOP/s).
 template <class T, int DP>
 __global__ __launch_bounds__(256, (WAVES<T, DP>)) void dq_kernel(const Params p) {
-    typedef Op<T, DP> M;
+    typedef Op<T> M;
     typedef Tiles<T, DP, KB> Tl;
     constexpr int NF = DP / M::KS, NP = 32 / M::KS, ND = DP / 32;
     constexpr bool FIX = sizeof(T) == 2;
@@ -965,7 +965,7 @@ __global__ __launch_bounds__(256) void dq_join_kernel(const Params p) {
 template <class T, int DP>
 __global__ __launch_bounds__(256, (DKV_WAVES<T, DP>)) void dkv_kernel(const Params p) {
     constexpr int R = RB<T, DP>;
-    typedef Op<T, DP> M;
+    typedef Op<T> M;
     typedef Tiles<T, DP, R> Tl;
     constexpr int NF = DP / M::KS, NP = 32 / M::KS, ND = DP / 32;
     constexpr bool VL = V_LDS<T, DP>;
@@ -1174,7 +1174,7 @@ int run_fwd(const Params& p, hipStream_t s) {
 
 template <class T, int DP>
 int run_bwd(const Params& pq, const Params& pk, hipStream_t s) {
-    constexpr int lds = Tiles<T, DP, KB>::BYTES, lds_k = Tiles<T, DP, RB<T, DP>>::BYTES + 1024 + (V_LDS<T, DP> ? 256 * (DP / Op<T, DP>::KS) * (int)sizeof(typename Op<T, DP>::Frag) : 0);
+    constexpr int lds = Tiles<T, DP, KB>::BYTES, lds_k = Tiles<T, DP, RB<T, DP>>::BYTES + 1024 + (V_LDS<T, DP> ? 256 * (DP / Op<T>::KS) * (int)sizeof(typename Op<T>::Frag) : 0);
     static_assert(lds_k <= 160 * 1024, "LDS of a CU");
     static DeviceOnce once;
     if (!once) {

@@ -126,7 +126,7 @@ struct FwdParams {
     void* y;
     float* stats;
     long long rows, xs;
-    int C, w32, vec;
+    int C, vec;
     float eps;
 };
 
@@ -229,7 +229,7 @@ struct BwdParams {
     void *dx, *dw, *db;        // dw, db: written by the kernel itself when it is one workgroup (part null)
     float* part;               // [gridDim.x][2][C] sums of dy xh and dy
     long long rows, dys, xs;
-    int C, w32, vec, sums;
+    int C, vec, sums;
 };
 
 template <class P> __device__ __forceinline__ void put_param(void* dst, int c, float v) { if (dst) reinterpret_cast<P*>(dst)[c] = (P)v; }
@@ -507,7 +507,7 @@ int dpc_seq_norm_fwd(const void* x, const void* weight, const void* bias, void* 
     DPC_REQUIRE(x && y && stats && (rows == 1 || x_stride >= C), "seq_norm: null argument or overlapping rows");
     hipStream_t s = (hipStream_t)stream;
     const int es = type == DPC_SEQ_F32 ? 4 : 2;
-    const FwdParams p{x, weight, bias, y, stats, rows, x_stride, C, wtype == DPC_SEQ_F32, vector_rows({x, y}, x_stride, 0, C, es, weight, bias, wtype == DPC_SEQ_F32 ? 4 : 2), eps};
+    const FwdParams p{x, weight, bias, y, stats, rows, x_stride, C, vector_rows({x, y}, x_stride, 0, C, es, weight, bias, wtype == DPC_SEQ_F32 ? 4 : 2), eps};
     ProfScope prof(PROF_LN, 0, 2.0 * (double)rows * C * es, s);
     return by_type(p, type, wtype, [&](auto t, auto w, auto v) { return fwd<decltype(t), decltype(w), decltype(v)::value>(p, s); });
 }
@@ -529,7 +529,7 @@ int dpc_seq_norm_bwd(const void* dy, const void* x, const float* stats, const vo
     DPC_REQUIRE(need == 0 || (ws && ws_bytes >= need), "seq_norm_bwd: workspace too small");
     hipStream_t s = (hipStream_t)stream;
     const BwdParams p{dy, x, weight, stats, dx, dweight, dbias, need ? reinterpret_cast<float*>(align_up((size_t)ws, 256)) : nullptr, rows, dy_stride, x_stride, C,
-                      wtype == DPC_SEQ_F32, vector_rows({dy, x, dx}, dy_stride, x_stride, C, es, weight, nullptr, wtype == DPC_SEQ_F32 ? 4 : 2), sums};
+                      vector_rows({dy, x, dx}, dy_stride, x_stride, C, es, weight, nullptr, wtype == DPC_SEQ_F32 ? 4 : 2), sums};
     ProfScope prof(PROF_LN, 0, 3.0 * (double)rows * C * es, s);
     return by_type(p, type, wtype, [&](auto t, auto w, auto v) { return bwd<decltype(t), decltype(w), decltype(v)::value>(p, s); });
 }

@@ -454,7 +454,7 @@ int dpc_seq_rotary_run(const dpc_seq_rotary* a, dpc_stream_t stream);
  * sequence.  A query that sees nothing gives out = 0, lse = -inf and no gradient.  Keys that the mask takes out are never read into a product:
  * they may hold anything.  lse [batch][heads][tokens] = log sum exp S (natural), contiguous in tokens.
  * Dense: every sequence has q_len / k_len tokens, q_tiles == k_tiles == NULL.  Otherwise q_tiles / k_tiles [n][8] list every block of 128
- * query / key rows once, in launch order, as (sequence, block, first query row, queries, first key row, keys, 0, 0) of the sequence, rows
+ * query / key rows once, in launch order, as (sequence, block, first query row, queries, first key row, keys, then two words that are not read) of the sequence, rows
  * counted from the batch entry's own base (stride_b = 0: packed); q_len / k_len are the longest.  Rows that no sequence covers are not written.
  * head_dim: a multiple of 8, at most 128.  Tensor bases and strides: multiples of 16 bytes; token
  * strides at most 2^25 - 64 bytes. */
