@@ -64,6 +64,19 @@ def _in_use(owner, d):
         owner.table.record_stream(torch.cuda.current_stream(d))
 
 
+class _Tables:
+    """An owner of a device tensor `table` that is whole for whatever stream uses it; copies (copy.deepcopy, pickle) own and address their own."""
+
+    def _settle(self):
+        if self.table.is_cuda:
+            torch.cuda.current_stream(self.table.device).synchronize()
+            self.stream = _stream(self.table.get_device())
+
+    def __setstate__(self, state):
+        self.__dict__.update(state)
+        self._settle()
+
+
 def _ok16(x, es):
     """Whether a kernel can read x as it lies: last axis contiguous, base and strides on 16 bytes, tokens at most _FAR bytes apart."""
     s = [n if m > 1 else 0 for n, m in zip(x.stride()[:-1], x.shape[:-1])]
@@ -227,7 +240,7 @@ def layer_norm_backward(dy, x, stats, weight=None, param_grads=True, param_dtype
 
 
 # ------------------------------------------------------------------------------------------------------------------ rotary positions
-class RotaryTable:
+class RotaryTable(_Tables):
     """Cosines and sines of the rotary angles for positions 0 .. max_positions - 1 (computed in 64 bits, kept in float32 on the device).
 
     Pair i < rotary_dim / 2 turns by position * f_i with f_i = base^(-2 i / rotary_dim); `layout` says which elements are a pair:
@@ -278,8 +291,8 @@ class RotaryTable:
         angle = torch.arange(max_positions, dtype=torch.float64, device=device)[:, None] * f.to(device)
         z = torch.polar(torch.full((), self.attention_factor, dtype=torch.float64, device=device), angle)
         self.table = torch.view_as_real(z).float().contiguous()                        # [max_positions, rotary_dim / 2, 2]
-        torch.cuda.current_stream(self.table.device).synchronize()                     # whole for whatever stream uses it
-        self.stream, self.address, self.interleaved = _stream(self.table.get_device()), self.table.data_ptr(), layout == "interleaved"
+        self.interleaved = layout == "interleaved"
+        self._settle()
 
 
 def _rotary(q, k, table, positions, start, out, transpose):
@@ -336,7 +349,7 @@ def _rotary(q, k, table, positions, start, out, transpose):
         if positions.dtype != torch.int64 or not positions.is_contiguous():
             positions = positions.to(torch.int64).contiguous()
         at = positions.data_ptr()
-    a = _lib.SEQ_ROTARY_BYTES.pack(*_place(q), *lk, *lyq, *lyk, table.address, at, pos_b, start, table.max_positions, t, B, T, H, Hk, D,
+    a = _lib.SEQ_ROTARY_BYTES.pack(*_place(q), *lk, *lyq, *lyk, table.table.data_ptr(), at, pos_b, start, table.max_positions, t, B, T, H, Hk, D,
                                    table.rotary_dim, table.interleaved, transpose)
     _lib.check(_lib.lib().dpc_seq_rotary_run(a, _stream(d)))
     return yq, yk
@@ -387,7 +400,7 @@ def rotary_backward(dq, dk, table, positions=None, start=0, out=None):
 
 
 # ------------------------------------------------------------------------------------------------------------------ attention
-class SequencePlan:
+class SequencePlan(_Tables):
     """Sequences of different lengths for `attention_forward` / `attention_backward`: checked here, laid out once, used for many calls.
 
     `packed`: q is [sum(q_lengths), H, D], the sequences one behind the other; k and v alike.  `padded`: q is [B, q_max, H, D], sequence b
@@ -422,13 +435,11 @@ class SequencePlan:
                 q0, k0 = q0 + a, k0 + b
         # block lists: of queries and of keys, for full and for causal scores
         lists = [[e + rows[e[0]] for e in self._tiles(ql, kl, keys, causal)] for causal in (False, True) for keys in (False, True)]
-        # (a blocking copy: whole for whatever stream uses it)
         self.table = torch.tensor([e for t in lists for e in t] or [(0,) * 8], dtype=torch.int32).to(device)
-        self.stream = _stream(self.table.get_device())
+        self._settle()
         self.counts = (len(lists[0]), len(lists[1]))
         q, k = (32 * n for n in self.counts)
-        at = self.table.data_ptr()
-        self.pointers = ((at, at + q), (at + q + k, at + q + k + q))            # by causal
+        self.offsets = ((0, q), (q + k, q + k + q))                             # of the lists in the table (bytes), by causal
         self.q_longest, self.k_longest, self.q_total, self.k_total = max(ql), max(kl), sum(ql), sum(kl)
 
     @staticmethod
@@ -487,7 +498,8 @@ def _attention_args(q, k, v, causal, scale, key_mask, plan):
         if ((B, Tq), (Bk, Tk)) != want:
             raise ValueError(f"the plan is for q {want[0]} and k {want[1]} (batch, tokens), got {(B, Tq)} and {(Bk, Tk)}")
         _in_use(plan, d)
-        blocks, sizes = plan.pointers[1 if causal else 0], plan.counts
+        at, (of_q, of_k) = plan.table.data_ptr(), plan.offsets[1 if causal else 0]
+        blocks, sizes = (at + of_q, at + of_k), plan.counts
     if key_mask is not None:
         key_mask = key_mask.contiguous()
     es = _BYTES[t]

@@ -255,3 +255,41 @@ def test_attention_blocks_of_many_pairs(B, H, Hk, Lq, Lk, D, causal, t, dev):
     grads = tuple(torch.full_like(x, math.nan) for x in (q, k, v))
     S.attention_backward(dout, q, k, v, out, lse, causal=causal, grads=grads)
     _check_attention(q, k, v, dout, out, lse, grads, [(Lq, Lk)] * B, causal=causal)
+
+
+@pytest.mark.parametrize("how", ["deepcopy", "pickle", "save"])
+def test_copies_of_tables_and_plans_stand_alone(how, dev, tmp_path):
+    """A copied model copies its RotaryTable and SequencePlan: the copies read their own memory, when the originals are gone too, on any stream."""
+    import copy
+    import pickle
+
+    from diffphycon_amd import sequence as S
+
+    def copied(x):
+        if how == "deepcopy":
+            return copy.deepcopy(x)
+        if how == "pickle":
+            return pickle.loads(pickle.dumps(x))
+        torch.save(x, tmp_path / "x.pt")
+        return torch.load(tmp_path / "x.pt", weights_only=False)     # (a file this test wrote)
+
+    g = _gen(99)
+    q, k, v, dout = (_randn(g, 200, 2, 64, dtype=torch.bfloat16) for _ in range(4))
+    table, plan = S.RotaryTable(64, 300, layout="half", device=dev), S.SequencePlan.packed([150, 0, 50], device=dev)
+    turned = S.rotary_forward(q, k, table, start=7)
+    out, lse = S.attention_forward(*turned, v, causal=True, plan=plan)
+    grads = S.attention_backward(dout, *turned, v, out, lse, causal=True, plan=plan)
+    t2, p2 = copied(table), copied(plan)
+    assert t2.table.data_ptr() != table.table.data_ptr() and p2.table.data_ptr() != plan.table.data_ptr()
+    table.table.fill_(math.nan)                                      # (the originals' memory means something else by now)
+    plan.table.zero_()
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    for stream in (torch.cuda.current_stream(), side):
+        with torch.cuda.stream(stream):
+            again = S.rotary_forward(q, k, t2, start=7)
+            o2, l2 = S.attention_forward(*again, v, causal=True, plan=p2)
+            g2 = S.attention_backward(dout, *again, v, o2, l2, causal=True, plan=p2)
+        torch.cuda.synchronize()
+        for a, b in zip((*turned, out, lse, *grads), (*again, o2, l2, *g2)):
+            assert torch.equal(a, b)
