@@ -485,8 +485,8 @@ def _attention_args(q, k, v, causal, scale, key_mask, plan):
     if (B | Tq | Tk | H) >> 31:
         raise ValueError(f"q {tuple(q.shape)} and k {tuple(k.shape)}: axes of 2^31 or more are not supported")
     scale = D ** -0.5 if scale is None else float(scale)
-    if not 0 < scale < math.inf:
-        raise ValueError("scale must be positive and finite")
+    if not 2.0 ** -126 <= scale < 2.0 ** 127:
+        raise ValueError("scale must be positive and finite (2^-126 to 2^127)")
     if key_mask is not None and (key_mask.dtype != torch.bool or key_mask.shape != k.shape[:-2]):
         raise ValueError(f"key_mask: bool of shape {tuple(k.shape[:-2])}")
     d = _device(q, k, v, key_mask, plan and plan.table)
@@ -550,7 +550,8 @@ def attention_forward(q, k, v, *, causal=False, scale=None, key_mask=None, plan=
 
 
 def attention_backward(dout, q, k, v, out, lse, *, causal=False, scale=None, key_mask=None, plan=None, grads=None):
-    """Gradients of `attention_forward` -> (dq, dk, dv); the other arguments as in the forward call, out and lse what it returned.
+    """Gradients of `attention_forward` -> (dq, dk, dv); the other arguments as in the forward call, out and lse what it returned.  Rows of a
+    padded plan that belong to no sequence get zeros, or stay as they were in given buffers.
 
     The probabilities are computed again from q, k and lse.  Gradients of a key / value head are summed over the query heads that read it.  Masked
     keys get zero gradients.  grads: buffers for (dq, dk, dv), e.g. views of one packed projection gradient; they must not overlap."""

@@ -159,3 +159,13 @@ def test_rotary_refuses_buffers_whose_own_elements_overlap():
 def test_rotary_table_refuses_a_ramp_without_meaning(kw):
     with pytest.raises(ValueError):
         S.RotaryTable(8, 16, scaling="ramp", factor=2.0, **kw)
+
+
+@pytest.mark.parametrize("scale", [1e39, 3.5e38, 1e-60, 1e-39])
+def test_attention_refuses_scales_beyond_fp32(scale):
+    """A scale that 32 bits make 0 or infinity is refused as one that is 0 or infinity is."""
+    q = torch.zeros(1, 2, 1, 8)
+    with pytest.raises(ValueError, match="scale"):
+        S.attention_forward(q, q, q, scale=scale)
+    with pytest.raises(ValueError, match="scale"):
+        S.attention_backward(q, q, q, q, q, torch.zeros(1, 1, 2), scale=scale)
