@@ -286,6 +286,14 @@ struct Stage {
             if (col(i) < width) copy16(src, at + i * NT * 16);
         }
     }
+    __device__ __forceinline__ void issue_rows(char* img, const char* base, const int* rows, unsigned long long bits) const {      // (rows: in LDS)
+        const unsigned at = lds_offset(img) + __builtin_amdgcn_readfirstlane((threadIdx.x % NT >> 6) * 1024);
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+            const char* src = bit(bits, row(i)) ? base + rows[row(i)] * st + col(i) : reinterpret_cast<const char*>(FILL);
+            if (col(i) < width) copy16(src, at + i * NT * 16);
+        }
+    }
 };
 __device__ __forceinline__ void zero_images(char* smem, int bytes) {  // (followed by the barrier before the first read)
     for (int i = threadIdx.x * 16; i < bytes; i += 256 * 16) *reinterpret_cast<uint4*>(smem + i) = uint4{0, 0, 0, 0};
@@ -305,6 +313,10 @@ template <class T, int DP, int ROWS, bool S = SPLIT<T>> struct Tiles {
         a.issue(smem + next * 2 * IMG, pa, bits);
         b.issue(smem + next * 2 * IMG + IMG, pb, bits);
     }
+    __device__ __forceinline__ void issue_rows(const char* pa, const char* pb, const int* rows, unsigned long long bits) {
+        a.issue_rows(smem + next * 2 * IMG, pa, rows, bits);
+        b.issue_rows(smem + next * 2 * IMG + IMG, pb, rows, bits);
+    }
     __device__ __forceinline__ void commit() {
         copies_done();
         __syncthreads();
@@ -323,13 +335,19 @@ template <class T, int DP, int ROWS> struct Tiles<T, DP, ROWS, true> {
     f32x4 v[2][N][2];
     __device__ __forceinline__ Tiles(char* s, long long sta, long long stb, int d) : smem(s), st{sta, stb}, D(d) {}
     __device__ __forceinline__ void issue(const char* pa, const char* pb, unsigned long long bits) {
+        fetch(pa, pb, bits, [](int row, bool) { return row; });
+    }
+    __device__ __forceinline__ void issue_rows(const char* pa, const char* pb, const int* rows, unsigned long long bits) {
+        fetch(pa, pb, bits, [&](int row, bool ok) { return ok ? rows[row] : 0; });
+    }
+    template <class F> __device__ __forceinline__ void fetch(const char* pa, const char* pb, unsigned long long bits, F place) {
 #pragma unroll
         for (int t = 0; t < 2; ++t)
 #pragma unroll
             for (int i = 0; i < N; ++i) {
                 const int e = threadIdx.x + 256 * i, row = e / UNITS, c = e % UNITS;
-                const f32x4* src = reinterpret_cast<const f32x4*>((t ? pb : pa) + row * st[t] + c * 32);
                 const bool ok = bit(bits, row) && c * 8 < D;
+                const f32x4* src = reinterpret_cast<const f32x4*>((t ? pb : pa) + place(row, ok) * st[t] + c * 32);
                 v[t][i][0] = ok ? src[0] : f32x4{0.f, 0.f, 0.f, 0.f};
                 v[t][i][1] = ok ? src[1] : f32x4{0.f, 0.f, 0.f, 0.f};
             }
@@ -425,6 +443,8 @@ template <int N> __device__ __forceinline__ float shrink_col(f32x16& t, f32x16 (
 // 16-bit types: sums of at most this many terms (dQ: of as many keys as a tile has) take P and dS in two parts, what the first one's rounding left being the second.  A
 // long sum averages those roundings; one of two or four terms would be off by up to 1.6 times what a computation in 32 bits, rounded once, is.
 constexpr int EXACT = 32;
+// Blocks that see at most this many keys are swept for D before dQ (see there)
+template <class T> constexpr int FEW_KEYS = (sizeof(T) == 2 ? 4 : 1) * KB;
 template <class T> __device__ __forceinline__ constexpr bool is_f16() { return __is_same(T, _Float16); }
 // Workgroups of a CU that the registers have to allow.  Rows of at most 128 bytes: three (packed fp16 24 x 1900, 12 heads of 64: forward 119 -> 99 us, dQ
 // 181 -> 157 against two; four would spill in dQ), but for dK/dV, whose two sums would spill (211 us at two, 222 at three).  fp32: two up to head size 64,
@@ -446,17 +466,55 @@ struct KeyBits {
     __device__ __forceinline__ unsigned long long bits(int kt) const { return mask ? __ballot(next != 0) : first_bits(kl - kt); }
 };
 
-// How many of the rows from .. to - 1 takes_part(row) holds for, counted until there are more than `most` (by all lanes of a wave; 512 rows are asked for at a time)
+// How many of the rows from .. to - 1 takes_part(row) holds for, counted until there are more than `most` (by all lanes of a wave)
 template <class F> __device__ __forceinline__ int count_rows(int from, int to, int lane, int most, F takes_part) {
     int n = 0;
-    for (int r0 = from; r0 < to && n <= most; r0 += 512) {
-        bool in[8];
+    for (int r0 = from; r0 < to && n <= most; r0 += 128) {
+        bool in[2];
 #pragma unroll
-        for (int i = 0; i < 8; ++i) in[i] = r0 + 64 * i + lane < to && takes_part(r0 + 64 * i + lane);
-#pragma unroll
-        for (int i = 0; i < 8; ++i) n += __popcll(__ballot(in[i]));
+        for (int i = 0; i < 2; ++i) in[i] = r0 + 64 * i + lane < to && takes_part(r0 + 64 * i + lane);
+        n += __popcll(__ballot(in[0])) + __popcll(__ballot(in[1]));
     }
     return n;
+}
+// How many of the first n keys a mask lets through, counted until there are more than `most`, and the first `most` of them, in order, into `list` (LDS; four
+// more words follow it).  By all 256 threads of a workgroup, 16 keys each at a time.
+__device__ __forceinline__ int list_keys(const unsigned char* mask, int n, int most, int* list) {
+    int* const totals = list + most;
+    int live = 0;
+    for (int k0 = 0; k0 < n && live <= most; k0 += 256 * 16) {
+        const int k = k0 + (int)threadIdx.x * 16;
+        unsigned char m[16] = {};
+        if (k + 16 <= n) __builtin_memcpy(m, mask + k, 16);
+        else
+            for (int i = 0; i < 16; ++i) m[i] = k + i < n ? mask[k + i] : 0;
+        int mine = 0;
+#pragma unroll
+        for (int i = 0; i < 16; ++i) mine += m[i] != 0;
+        int upto = mine;                                             // of this wave, up to this thread
+#pragma unroll
+        for (int x = 1; x < 64; x <<= 1) {
+            const int other = __shfl_up(upto, x, 64);
+            if ((int)(threadIdx.x & 63) >= x) upto += other;
+        }
+        __syncthreads();                                             // (the totals of the round before have been read)
+        if ((threadIdx.x & 63) == 63) totals[threadIdx.x >> 6] = upto;
+        __syncthreads();
+        int at = live + upto - mine;
+#pragma unroll
+        for (int w = 0; w < 4; ++w) {
+            if (w < (int)(threadIdx.x >> 6)) at += totals[w];
+            live += totals[w];
+        }
+#pragma unroll
+        for (int i = 0; i < 16; ++i)
+            if (m[i] != 0) {
+                if (at < most) list[at] = k + i;
+                ++at;
+            }
+    }
+    __syncthreads();
+    return __builtin_amdgcn_readfirstlane(live);
 }
 
 // What a row's sum l of exponentials, relative to 2^m, makes of it: 1 / l and the log-sum-exp; 0 and -inf for a row that saw no key.  A sum of 0 over some keys
@@ -786,7 +844,7 @@ __global__ __launch_bounds__(256) void fwd_join_kernel(const Params p) {
 // row add up to 1, sum_j P (dP - D) is exactly that error, so the sweep adds it up and hands the corrected D on.  Where a block sees at most
 // 256 keys -- dP and D are of one size then, and a row of one or two keys has nothing but their difference -- it is swept once for D alone
 // before it is swept for dQ.  fp32 does so up to 64 keys, for the rows of few keys alone.  Seen keys are what counts, not the axis they lie on: a
-// key mask's are counted first, and the few that it leaves are one workgroup's, however the axis is split.  Tiles, split and bound as in the forward; three products:
+// key mask's are counted first, and the few that it leaves are gathered.  Tiles, split and bound as in the forward; three products:
 // 229, 149 and 268 us at its sizes (900, 520 and 190 TFLOP/s).
 template <class T, int DP>
 __global__ __launch_bounds__(256, (WAVES<T, DP>)) void dq_kernel(const Params p) {
@@ -794,8 +852,8 @@ __global__ __launch_bounds__(256, (WAVES<T, DP>)) void dq_kernel(const Params p)
     typedef Tiles<T, DP, KB> Tl;
     constexpr int NF = DP / M::KS, NP = 32 / M::KS, ND = DP / 32;
     constexpr bool FIX = sizeof(T) == 2;
-    constexpr int FEW_KEYS = (FIX ? 4 : 1) * KB;
-    extern __shared__ __attribute__((aligned(16))) char smem[];       // tiles of K and V
+    extern __shared__ __attribute__((aligned(16))) char smem[];       // tiles of K and V, then FEW_KEYS places of keys and 4 words
+    int* const s_live = reinterpret_cast<int*>(smem + Tl::BYTES);
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), l31 = lane & 31, h = lane >> 5;
     const Where w = where(p, true);
     const int rows = w.ql * p.group, r0 = w.tile * QB * p.group + w.sub * QB;
@@ -803,30 +861,45 @@ __global__ __launch_bounds__(256, (WAVES<T, DP>)) void dq_kernel(const Params p)
     const int off = w.kl - w.ql, rw = r0 + wave * 32, r = rw + l31;
     const bool rok = r < rows;
     int token = rok ? r : r0;
-    const int head = w.kvh * p.group + p.by_group.take(token);
+    int head = w.kvh * p.group + p.by_group.take(token);
     const int t_first = p.by_group(rw), t_last = p.by_group(rw + 31);
     int kend = p.causal ? min(w.kl, min((int)p.by_group(r0 + QB - 1), w.ql - 1) + 1 + off) : w.kl, kbegin = 0;
-    const int kall = kend;
+    int kall = kend;
     const unsigned char* const mask = p.key_mask ? p.key_mask + w.b * p.mask_b + w.k0 : nullptr;
     const char* const kbase = p.k.p + w.b * p.k.b + w.k0 * p.k.t + w.kvh * p.k.h;
     const char* const vbase = p.v.p + w.b * p.v.b + w.k0 * p.v.t + w.kvh * p.v.h;
-    KeyBits kb{mask, w.kl, lane, 0};
-    const long long at = w.b * p.lse_b + head * p.lse_h + w.q0 + token;
+    long long at = w.b * p.lse_b + head * p.lse_h + w.q0 + token;
     const float lse = rok ? p.lse[at] : -INFINITY;
     const bool sees = lse != -INFINITY;                              // (a row that sees nothing takes no part, whatever it holds)
     const float lse2 = sees ? lse * LOG2E : INFINITY;
     typename M::Frag qf[NF], gf[NF];
     load_row<M, T, DP>(qf, p.q.p + w.b * p.q.b + (w.q0 + token) * p.q.t + head * p.q.h, h, p.D, rok);
     load_row<M, T, DP>(gf, p.dout.p + w.b * p.dout.b + (w.q0 + token) * p.dout.t + head * p.dout.h, h, p.D, rok);
-    // keys that the block sees (more than FEW_KEYS: at least that many); the rows are on their way meanwhile
-    const int live = mask ? count_rows(0, kall, lane, FEW_KEYS, [&](int j) { return mask[j] != 0; }) : kall;
-    const bool few = live > 0 && live <= FEW_KEYS;
-    if (p.splits > 1 && few) kend = w.split == 0 ? kall : 0;
-    else if (p.splits > 1) {                                         // as in the forward
+    // Keys that the block sees (more than FEW_KEYS: at least that many); the rows are on their way meanwhile.  The few that a mask leaves are gathered: from
+    // here on they are a sequence of their own, one split's.
+    const int live = mask ? list_keys(mask, kall, FEW_KEYS<T>, s_live) : kall;
+    const bool few = live <= FEW_KEYS<T>, gather = mask && few;
+    int last = token + off, wave_first = t_first + off, wave_last = t_last + off;          // last key that this row, the wave's first and last row may see
+    if (gather) {
+        kall = live;
+        last = kall - 1;
+        if (p.causal) {                                              // (how many of the list lie at most at token + off)
+            int n = 0;
+            for (int step = FEW_KEYS<T>; step; step >>= 1) n += n + step <= kall && s_live[n + step - 1] <= token + off ? step : 0;
+            last = n - 1;
+        }
+        wave_first = -1;
+        wave_last = kall;
+    }
+    if (few) {
+        kend = w.split == 0 ? kall : 0;
+    } else if (p.splits > 1) {                                       // as in the forward
         const int per = max(4, (max(kend, 0) + KB * p.splits - 1) / (KB * p.splits)) * KB;
         kbegin = w.split * per;
         kend = min(kend, kbegin + per);
     }
+    const bool kept = kall <= KB;                                    // one tile stays where it is
+    KeyBits kb{gather ? nullptr : mask, gather ? live : w.kl, lane, 0};
     float nd = 0.f, rho = 0.f;                                       // -D, what D still misses (times sc)
     {
         typename M::Frag of[NF];
@@ -850,7 +923,8 @@ __global__ __launch_bounds__(256, (WAVES<T, DP>)) void dq_kernel(const Params p)
     auto issue = [&](int kt) {
         cur = kb.bits(kt);
         kb.fetch(kt + KB);                                           // (before the copies: commit() waits for all of them)
-        if (cur) tl.issue(kbase + kt * p.k.t, vbase + kt * p.v.t, cur);
+        if (FIX && gather) tl.issue_rows(kbase, vbase, s_live + kt, cur);
+        else if (cur) tl.issue(kbase + kt * p.k.t, vbase + kt * p.v.t, cur);
     };
     // P (dP - D) of the tile's keys 32 sub .. (times sc)
     auto terms = [&](f32x16& st, unsigned long long bits, int kt, int sub) {
@@ -864,8 +938,8 @@ __global__ __launch_bounds__(256, (WAVES<T, DP>)) void dq_kernel(const Params p)
         }
 #pragma unroll
         for (int x = 0; x < 16; ++x) st[x] = __builtin_amdgcn_exp2f(__builtin_fmaf(st[x], c, -shift)) * dp[x];
-        if (bits != ~0ull || (p.causal && kt + KB - 1 > t_first + off)) {
-            const unsigned part = part_of(bits, sub, p.causal ? token + off - kt : KB, h);
+        if (bits != ~0ull || (p.causal && kt + KB - 1 > wave_first)) {
+            const unsigned part = part_of(bits, sub, p.causal ? last - kt : KB, h);
 #pragma unroll
             for (int x = 0; x < 16; ++x) st[x] = where_part(part, x, st[x], 0.f);
         }
@@ -876,20 +950,25 @@ __global__ __launch_bounds__(256, (WAVES<T, DP>)) void dq_kernel(const Params p)
         for (int x = 0; x < 16; ++x) a += st[x];
         rho += a;
     };
-    auto none = [&](unsigned long long bits, int kt) { return rw >= rows || bits == 0 || (p.causal && kt > t_last + off); };
+    auto none = [&](unsigned long long bits, int kt) { return rw >= rows || bits == 0 || (p.causal && kt > wave_last); };
     auto shrink = [&](f32x16& st) {
         if (!is_f16<T>()) return;
         const float by = shrink_col(st, acc);
         if (by != 1.f) { sc *= by; rho *= by; shift = lse2 - __builtin_amdgcn_logf(sc); }
     };
-    if (kbegin < kend) { kb.fetch(kbegin); issue(kbegin); }
+    if (!FIX && gather) {                                            // (one tile at most)
+        if (kbegin < kend) tl.issue_rows(kbase, vbase, s_live, cur = kb.bits(0));
+    } else if (kbegin < kend) {
+        kb.fetch(kbegin);
+        issue(kbegin);
+    }
     if (few && kbegin < kend) {                                      // the sweep for D alone
-        for (int kt = 0; kt < kall; kt += KB) {
+        for (int kt = kbegin; kt < kend; kt += KB) {
             const unsigned long long bits = cur;
             tl.commit();
-            if (kall > KB) {                                         // (one tile stays where it is)
-                if (kt + KB >= kall) kb.fetch(0);
-                issue(kt + KB < kall ? kt + KB : 0);
+            if (!kept) {
+                if (kt + KB >= kend) kb.fetch(kbegin);
+                issue(kt + KB < kend ? kt + KB : kbegin);
             }
             if (none(bits, kt)) continue;
 #pragma unroll 1
@@ -902,7 +981,7 @@ __global__ __launch_bounds__(256, (WAVES<T, DP>)) void dq_kernel(const Params p)
         nd -= (rho + other_half(rho)) / sc;
         rho = 0.f;
     }
-    const bool kept = few && kall <= KB, parts = FIX && few && live <= KB;       // (dS in two parts: see EXACT)
+    const bool parts = FIX && live <= KB;                            // (dS in two parts: see EXACT)
     for (int kt = kbegin; kt < kend; kt += KB) {
         const unsigned long long bits = cur;
         if (!kept) {
@@ -932,6 +1011,15 @@ __global__ __launch_bounds__(256, (WAVES<T, DP>)) void dq_kernel(const Params p)
     }
     rho = (rho + other_half(rho)) / sc;
     if (!rok) return;
+    // fp32, short of registers, works the row's place out anew, from the thread's number: kept over the loops it makes them spill (32 x 1024, 8 heads of 32:
+    // 293 -> 309 us).  16 bits keep it: 2 x 4096, 16/4 heads of 128 is 7 % slower without.
+    if constexpr (sizeof(T) == 4) {
+        int again = tid;
+        asm volatile("" : "+v"(again));
+        token = rw + (again & 31);
+        head = w.kvh * p.group + p.by_group.take(token);
+        at = w.b * p.lse_b + head * p.lse_h + w.q0 + token;
+    }
     if (w.kl == 1) clear(acc);                                       // (the softmax of one key is constant: P (dP - D) has only rounding to give)
     const float un = p.scale / sc;
     if (p.splits > 1) {                                              // part: sums, part_ml [split][row]: rho
@@ -1001,10 +1089,6 @@ __global__ __launch_bounds__(256, (DKV_WAVES<T, DP>)) void dkv_kernel(const Para
         step = min(steps, w.split * per);
         steps = min(steps, step + per);
     }
-    // Queries of a head that take part (more than EXACT: at least that many)
-    const int seeing = p.key_mask && sizeof(T) == 2
-                           ? count_rows(qbegin, w.ql, lane, EXACT, [&](int i) { return p.lse[w.b * p.lse_b + w.kvh * p.group * p.lse_h + w.q0 + i] != -INFINITY; })
-                           : w.ql - qbegin;
     const bool idle = !__any(live);                                  // (this wave's keys are all masked or behind the end)
     if (p.key_mask && !__syncthreads_or(live)) steps = step;
     // The walk: tiles of R queries, head after head.
@@ -1036,6 +1120,10 @@ __global__ __launch_bounds__(256, (DKV_WAVES<T, DP>)) void dkv_kernel(const Para
         issue(now, step + 1 < steps);
         next = advance(now);
     }
+    // Queries of a head that take part (more than EXACT: at least that many; asked for while the first tile is on its way)
+    const int seeing = p.key_mask && sizeof(T) == 2 && step < steps
+                           ? count_rows(qbegin, w.ql, lane, EXACT, [&](int i) { return p.lse[first_row + w.kvh * p.group * p.lse_h + i] != -INFINITY; })
+                           : w.ql - qbegin;
     for (; step < steps; ++step) {
         const int qt = now.qt;
         tl.commit();
@@ -1174,7 +1262,7 @@ int run_fwd(const Params& p, hipStream_t s) {
 
 template <class T, int DP>
 int run_bwd(const Params& pq, const Params& pk, hipStream_t s) {
-    constexpr int lds = Tiles<T, DP, KB>::BYTES, lds_k = Tiles<T, DP, RB<T, DP>>::BYTES + 1024 + (V_LDS<T, DP> ? 256 * (DP / Op<T>::KS) * (int)sizeof(typename Op<T>::Frag) : 0);
+    constexpr int lds = Tiles<T, DP, KB>::BYTES + (FEW_KEYS<T> + 4) * (int)sizeof(int), lds_k = Tiles<T, DP, RB<T, DP>>::BYTES + 1024 + (V_LDS<T, DP> ? 256 * (DP / Op<T>::KS) * (int)sizeof(typename Op<T>::Frag) : 0);
     static_assert(lds_k <= 160 * 1024, "LDS of a CU");
     static DeviceOnce once;
     if (!once) {

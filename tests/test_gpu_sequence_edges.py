@@ -293,3 +293,30 @@ def test_copies_of_tables_and_plans_stand_alone(how, dev, tmp_path):
         torch.cuda.synchronize()
         for a, b in zip((*turned, out, lse, *grads), (*again, o2, l2, *g2)):
             assert torch.equal(a, b)
+
+
+@pytest.mark.parametrize("t", TYPES, ids=str)
+@pytest.mark.parametrize("H,Hk,D", [(4, 2, 64), (3, 3, 128), (2, 1, 32)])
+@pytest.mark.parametrize("causal", [False, True])
+def test_attention_gradients_of_keys_far_apart(H, Hk, D, causal, t, dev):
+    """1 to 256 keys among 4500, which are gathered (257 are not), in packed sequences that start anywhere: the masks' bytes lie on no boundary.  Under the causal
+    mask rows of one block see different numbers of them."""
+    from diffphycon_amd import sequence as S
+    ql, kl, seen = [300, 37, 200, 130, 64, 1], [4500, 4097, 1301, 700, 263, 300], [256, 3, 130, 65, 64, 257]
+    g = _gen(D + H)
+    q, k, v, dout = _randn(g, sum(ql), H, D, dtype=t), _randn(g, sum(kl), Hk, D, dtype=t), _randn(g, sum(kl), Hk, D, dtype=t), _randn(g, sum(ql), H, D, dtype=t)
+    mask = torch.cat([_few(1, nk, n, nk)[0] for nk, n in zip(kl, seen)]).to(dev)
+    k[~mask], v[~mask] = math.nan, math.inf
+    plan = S.SequencePlan.packed(ql, kl, device=dev)
+    out, lse = S.attention_forward(q, k, v, causal=causal, key_mask=mask, plan=plan)
+    grads = S.attention_backward(dout, q, k, v, out, lse, causal=causal, key_mask=mask, plan=plan)
+    _check_attention(q, k, v, dout, out, lse, grads, list(zip(ql, kl)), packed=True, causal=causal, mask=mask)
+    few = 64 if t == torch.float32 else 256
+    q0 = k0 = 0
+    for nq, nk, n in zip(ql, kl, seen):
+        for h in range(H):
+            a, b = (slice(q0, q0 + nq), h), (slice(k0, k0 + nk), h // (H // Hk))
+            if n <= few:
+                r = O.attention(q[a], k[b], v[b], dout[a], causal, mask=mask[k0:k0 + nk], swept=True, parts=n <= 64)
+                _within("dq", grads[0][a], r["dq"][0], O.add_rounding(*r["dq"], t))
+        q0, k0 = q0 + nq, k0 + nk
