@@ -15,9 +15,11 @@
 // second product, as any 16-bit matrix operand is; sums and statistics stay fp32.  fp16 has only 2^-14 as its smallest full-precision number: P is
 // carried as 2^7 P (forward) or 2^15 P and dS under a running power of two per column (shrink_col), both undone in fp32 at the end.
 //
-// What bounds it (counters at the sizes named at the kernels): head size 128 in 16 bits keeps the matrix units busy for half of the time (forward and dQ 890 to 920
-// TFLOP/s executed, a large library product 1050 to 1094), head size 64 the vector unit for two thirds (exponentials, maxima and masks: 560, 520 and
-// 490 TFLOP/s forward, dQ, dK/dV), fp32 the matrix units (six bf16 products for one: 165 to 190 TFLOP/s of fp32, the fp32 product itself reaches 150).
+// What bounds it (counters at the sizes named at the kernels; figures of one card, on which a large library product reaches 1248 TFLOP/s in bf16, 1184 in fp16 and
+// 154 in fp32): in 16 bits the matrix and the vector units take turns, and neither is a bound yet.  Head size 128: busy 0.47 and 0.46 of the time in the
+// forward (900 TFLOP/s executed), 0.50 and 0.43 in dQ (915), 0.44 and 0.38 in dK/dV (875); head size 64, with more exponentials, maxima and masks for a
+// product: 0.33 and 0.64 (575), 0.30 and 0.67 (535), 0.27 and 0.53 (500).  fp32, six bf16 products for one, overlaps them
+// better: 0.53 to 0.63 and, for the vector units split operands, 0.62 to 0.71 (165 to 185 of fp32's products).
 // The backward pass executes seven products where five would do, for dQ and dK/dV are summed by different workgroups and nothing is added with atomics.
 #pragma once
 #include <algorithm>
@@ -119,8 +121,8 @@ template <> struct Mma<float> {
 };
 
 // fp32 by the bf16 matrix instructions: x = x1 + x2 + x3 in three bf16 parts, exactly (bf16x6.h), and six of the nine products -- what is left out is
-// below 2^-24 of |a b|, an fp32 product's own rounding.  6 / 16 of the native instruction's time (1 x 4096, 16 heads of 128: forward 1274 -> 771 us).  An operand is three fragments, an image three 16-bit
-// images PLANE bytes apart.
+// below 2^-24 of |a b|, an fp32 product's own rounding.  6 / 16 of the native instruction's time (1 x 4096, 16 heads of 128: the forward takes
+// 0.6 of the time that it took with those).  An operand is three fragments, an image three 16-bit images PLANE bytes apart.
 struct Split3 {
     typedef struct { bf16x8 p[3]; } Frag;
     typedef f32x4 Quad;
@@ -440,16 +442,16 @@ template <int N> __device__ __forceinline__ float shrink_col(f32x16& t, f32x16 (
     return by;
 }
 
-// 16-bit types: sums of at most this many terms (dQ: of as many keys as a tile has) take P and dS in two parts, what the first one's rounding left being the second.  A
-// long sum averages those roundings; one of two or four terms would be off by up to 1.6 times what a computation in 32 bits, rounded once, is.
+// 16-bit types: sums of at most this many terms (dQ: of as many keys as a tile has) take P and dS in two parts, what the first one's rounding left being the
+// second.  The terms are those of a block that take part: what a key mask leaves out does not count.  A long sum averages those roundings; one of two or four terms would be off by up to 1.6 times what a computation in 32 bits, rounded once, is.
 constexpr int EXACT = 32;
 // Blocks that see at most this many keys are swept for D before dQ (see there)
 template <class T> constexpr int FEW_KEYS = (sizeof(T) == 2 ? 4 : 1) * KB;
 template <class T> __device__ __forceinline__ constexpr bool is_f16() { return __is_same(T, _Float16); }
-// Workgroups of a CU that the registers have to allow.  Rows of at most 128 bytes: three (packed fp16 24 x 1900, 12 heads of 64: forward 119 -> 99 us, dQ
-// 181 -> 157 against two; four would spill in dQ), but for dK/dV, whose two sums would spill (211 us at two, 222 at three).  fp32: two up to head size 64,
-// one beyond, whose operands of three parts fill the registers.  (fp32 dQ and dK/dV of head size 64 spill some ten and some forty registers, outside of
-// the innermost loops: 1 x 4096, 16 heads of 64, backward 1278 us, at one workgroup, without, 1480.)
+// Workgroups of a CU that the registers have to allow.  Rows of at most 128 bytes: three (packed fp16 24 x 1900, 12 heads of 64: forward 17 % and dQ 13 %
+// faster than at two; four would spill in dQ), but for dK/dV, whose two sums would spill (5 % slower at three).  fp32: two up to head size 64, one beyond,
+// whose operands of three parts fill the registers.  (fp32 dQ and dK/dV of head size 64 spill some five and some forty registers, outside of the
+// innermost loops: 1 x 4096, 16 heads of 64, backward 1265 us; at one workgroup, where nothing spills, 16 % slower.)
 template <class T, int DP> constexpr int WAVES = DP * sizeof(T) <= 128 ? 3 : sizeof(T) == 2 || DP <= 64 ? 2 : 1;
 template <class T, int DP> constexpr int DKV_WAVES = WAVES<T, DP> < 2 ? 1 : 2;
 // dK/dV at head size 128: the two sums alone take 128 registers; the values' fragments wait in LDS (V_LDS) and the staged tile has 32 rows (fp32: 146 KB
@@ -527,7 +529,7 @@ __device__ __forceinline__ float lse_of(float m, float l) {
 
 // Forward.  Rows of a query block: row r = token r / group, head kvh * group + r % group, so that heads which share keys share the tile's loads.  One
 // pass over the keys with a running maximum and sum; 128 rows a workgroup, 32 a wave, tiles of 64 keys and values in two LDS buffers, one barrier a tile.
-// Causal bf16 2 x 4096, 16/4 heads of 128: 155 us (890 TFLOP/s); packed causal fp16 24 x 1900, 12 heads of 64: 93 us (560); fp32 32 x 1024, 8 heads of
+// Causal bf16 2 x 4096, 16/4 heads of 128: 152 us (900 TFLOP/s); packed causal fp16 24 x 1900, 12 heads of 64: 90 us (575); fp32 32 x 1024, 8 heads of
 // 32: 209 us (165).
 template <class T, int DP>
 __global__ __launch_bounds__(256, (WAVES<T, DP>)) void fwd_kernel(const Params p) {
@@ -644,7 +646,7 @@ template <class T> __device__ __forceinline__ void store8(char* row, int d, cons
 }
 // Few rows (at most 32 of a sequence and key head: single tokens, short drafts): nothing to share, so each of the four waves walks over tiles
 // of 32 keys of its own, copied by itself into its own LDS, without barriers; the waves' sums are joined through LDS at the end.  Bound by the
-// keys' and values' bytes: 64 KB are in flight a CU (one token, 8 x 16384 keys, 32/8 heads of 128, bf16: 97 us, 5.5 TB/s; 75 with a quarter masked).
+// keys' and values' bytes: 64 KB are in flight a CU (one token, 8 x 16384 keys, 32/8 heads of 128, bf16: 100 us, 5.4 TB/s; 76 with a quarter masked).
 template <class T, int DP> constexpr bool FEW = Image<T, DP>::PITCH * 32 * 16 <= 128 * 1024;
 template <class T, int DP>
 __global__ __launch_bounds__(256) void few_kernel(const Params p) {
@@ -766,7 +768,7 @@ __global__ __launch_bounds__(256) void few_kernel(const Params p) {
 }
 
 // Joining the splits: 16 lanes of 8 columns a row.  Many splits: a wave a row, its four groups of lanes take a quarter of the splits each (SL = 4);
-// up to 8: four rows a wave (SL = 1; the partial sums of 9990 rows in 5 splits: 8.9 -> 6.5 us).  A lane's loads are in flight together.
+// up to 8: four rows a wave (SL = 1; the partial sums of 9990 rows in 5 splits take 5.8 us, a quarter less than with a wave a row).  A lane's loads are in flight together.
 constexpr int join_slices(int splits) { return splits > 8 ? 4 : 1; }
 template <int SL> struct Join {
     static constexpr int ROWS = 16 / SL;                             // of a workgroup
@@ -845,7 +847,7 @@ __global__ __launch_bounds__(256) void fwd_join_kernel(const Params p) {
 // 256 keys -- dP and D are of one size then, and a row of one or two keys has nothing but their difference -- it is swept once for D alone
 // before it is swept for dQ.  fp32 does so up to 64 keys, for the rows of few keys alone.  Seen keys are what counts, not the axis they lie on: a
 // key mask's are counted first, and the few that it leaves are gathered.  Tiles, split and bound as in the forward; three products:
-// 229, 149 and 268 us at its sizes (900, 520 and 190 TFLOP/s).
+// 225, 146 and 278 us at its sizes (915, 535 and 185 TFLOP/s).
 template <class T, int DP>
 __global__ __launch_bounds__(256, (WAVES<T, DP>)) void dq_kernel(const Params p) {
     typedef Op<T> M;
@@ -1012,7 +1014,7 @@ __global__ __launch_bounds__(256, (WAVES<T, DP>)) void dq_kernel(const Params p)
     rho = (rho + other_half(rho)) / sc;
     if (!rok) return;
     // fp32, short of registers, works the row's place out anew, from the thread's number: kept over the loops it makes them spill (32 x 1024, 8 heads of 32:
-    // 293 -> 309 us).  16 bits keep it: 2 x 4096, 16/4 heads of 128 is 7 % slower without.
+    // 5 % slower).  16 bits keep it: 2 x 4096, 16/4 heads of 128 is 7 % slower without.
     if constexpr (sizeof(T) == 4) {
         int again = tid;
         asm volatile("" : "+v"(again));
@@ -1049,7 +1051,7 @@ __global__ __launch_bounds__(256) void dq_join_kernel(const Params p) {
 
 // dK and dV.  128 keys a workgroup, 32 a wave, which stay in registers (V_LDS: or LDS) with their two sums, and a walk over tiles of query rows, head
 // after head of the group, so that shared heads are summed in fixed order.  Four products; lse2 and -D of a tile's rows come along into LDS and are the
-// start of the accumulator.  Bound as the forward: 335, 219 and 388 us at its sizes (820, 470 and 177 TFLOP/s), the join of the first's splits 23.
+// start of the accumulator.  Bound as the forward: 315, 208 and 382 us at its sizes (875, 500 and 180 TFLOP/s), the join of the first's splits 23.
 template <class T, int DP>
 __global__ __launch_bounds__(256, (DKV_WAVES<T, DP>)) void dkv_kernel(const Params p) {
     constexpr int R = RB<T, DP>;

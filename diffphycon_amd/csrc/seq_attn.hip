@@ -54,7 +54,7 @@ static Params params(const dpc_seq_attn* a) {
 // along (keys; for dK/dV the query rows of the group) is split over as many workgroups as fit, each with at least four tiles to walk;
 // the partial sums are joined in order by a second launch.  Under a causal mask over (nearly) square scores the blocks' walks differ by the
 // length of the sequence and the longest one decides while all are resident: twice as many workgroups are made, and the card evens them out (dK/dV of
-// causal bf16 2 x 4096, 16/4 heads of 128: 561 -> 388 us, the join 14 -> 24).
+// causal bf16 2 x 4096, 16/4 heads of 128: 28 % less with its join of 23 us, which was 14).
 // Returns false when a launch would have 2^32 threads or more.
 constexpr int SLOTS = 512;
 static bool plan_grid(Params& p, const dpc_seq_attn* a, bool keys, bool forward) {
@@ -66,8 +66,8 @@ static bool plan_grid(Params& p, const dpc_seq_attn* a, bool keys, bool forward)
     const long long walk = keys ? (long long)p.group * cdiv(a->q_len, KB) : cdiv(a->k_len, KB);
     const int slots = p.causal && 2ll * a->q_len > a->k_len ? 2 * SLOTS : SLOTS;
     // At most 32 rows of a sequence and key head: few_kernel (its LDS allows rows of 256 bytes), as many workgroups as are resident at once -- one a CU, two with
-    // rows of 128 bytes -- for each starts with empty loads in flight; a split has two tiles a wave at least.  One token, 32/8 heads of 128, bf16: 8 x 16384 keys
-    // 101 us (104 with 512 workgroups; a quarter masked 80, 95), 1 x 16384 keys 20 (25); by fwd_kernel the first takes 113.
+    // rows of 128 bytes -- for each starts with empty loads in flight; a split has two tiles a wave at least.  One token, 32/8 heads of 128, bf16, against
+    // 512 workgroups: 8 x 16384 keys 3 % faster, a quarter of them masked 16 %, 1 x 16384 keys 20 %; fwd_kernel takes 12 % longer for the first.
     const int row = (a->head_dim + 31) / 32 * 32 * (a->type == DPC_SEQ_F32 ? 4 : 2);
     p.few = forward && (long long)a->q_len * p.group <= 32 && row <= 256;
     if (p.few) p.splits = blocks == 0 ? 1 : (int)std::max<long long>(1, std::min<long long>((row <= 128 ? SLOTS : SLOTS / 2) / blocks, a->k_len / 256));

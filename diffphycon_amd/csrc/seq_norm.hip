@@ -5,8 +5,9 @@
 // of G lanes (4, 16, 64 or a whole workgroup; N accesses of 16 bytes a lane), so that the centred second sum of the variance -- no
 // E[x^2] - mu^2 cancellation -- costs no second read.  Rows too wide for that (over 2048 accesses) are read again from L2.
 // The backward pass keeps dw and db in registers over all rows of a group, adds the groups of a workgroup in LDS and writes one row of
-// partial sums per workgroup; a second kernel adds those in fixed order.
-// fp32 786432 x 64: forward 72 us (5.6 TB/s), backward 121 (5.0) and 7 for the sums; bf16 8191 x 4096: 23 (5.8), 43 (4.7) and 5.
+// partial sums per workgroup; a second kernel adds those in fixed order (in fp32, the last 32 of a column in double).
+// fp32 786432 x 64: forward 71 us (5.7 TB/s), backward 120 (5.0) and 7 for the sums; bf16 8191 x 4096: 23 (5.7), 47 (4.3; 42 on another card) and 5.
+// Rows over 2048 accesses add dw and db in global memory, row by row, 16 bytes an element beside the row's own 12: fp32 4000 x 12000 forward 107 us, backward 481.
 #include <algorithm>
 #include <initializer_list>
 #include <type_traits>
@@ -45,8 +46,8 @@ template <class T, class P, int G, int N, bool VECT> struct Held {
         }
     }
     // A row that is on its way while another is worked on: ask() reads something in every lane and settled() puts zeros past the row's end.  (With the
-    // choice at the load, the compiler copies what was loaded, and waits for it, right behind the load: bf16 8191 x 4096 backward 49 us, so 43.  Rows of a
-    // wave or less, of which thousands are at work, lose by it: fp32 786432 x 64 120 us, 129.)
+    // choice at the load, the compiler copies what was loaded, and waits for it, right behind the load: bf16 8191 x 4096 backward 14 % slower.  Rows of
+    // a wave or less, of which thousands are at work, lose by ask(): fp32 786432 x 64 7 %.)
     __device__ __forceinline__ void ask(const P* __restrict__ row, int lane, int C) {
 #pragma unroll
         for (int n = 0; n < N; ++n) {
@@ -416,8 +417,8 @@ __global__ __launch_bounds__(1024) void param_kernel(const float* __restrict__ p
 
 // Lanes a row (G) and accesses a lane (N) by the row's 16-byte accesses: the fewest lanes that hold it in at most four accesses up to a wave
 // -- no barrier -- else a workgroup.  More accesses a lane cost registers, that is waves, that is loads in flight: bf16 rows of 4096 forward in
-// one wave of 8 accesses 41 us for 8191 rows, in four waves of 2 accesses 23 us (5.7 TB/s).  The backward pass holds four times as much a lane and
-// goes to workgroups of one access a lane earlier: bf16 8191 x 8192 in four accesses 119 us, in one 97; 30000 x 2048 84 and 80.
+// one wave of 8 accesses take 1.8 times as long as in four waves of 2.  The backward pass holds four times as much a lane and goes to workgroups of one
+// access a lane earlier: bf16 8191 x 8192 in four accesses 119 us, in one 97; 30000 x 2048 84 and 80.
 template <int A, int B> using Shape = std::pair<std::integral_constant<int, A>, std::integral_constant<int, B>>;
 template <bool BWD, class F> int by_width(int acc, F f) {
     if (acc <= 4) return f(Shape<4, 1>{});

@@ -3,8 +3,8 @@
 // Bound by bytes: every element is read and written once.  A thread owns one chunk of a token's head and walks over heads with the chunk's cosines in
 // registers.  Interleaved: a chunk is 16 bytes of pairs, or of the pass-through part.  Half layout: a chunk is any 16 bytes of the head, the lanes of a
 // head read it in one piece, and the pair's other halves come from the lane that has them -- were they loaded, every line of memory would be touched by
-// two loads and two stores (2 x 8192 tokens, 40 heads of 128, 96 of them turned, bf16: 80 -> 68 us).  Rows that do not start on 16 bytes, or halves that
-// do not, go one pair at a time.  A copy's rate: 5.4 TB/s there, 5.3 for fp32 1536 x 32 tokens, 16 heads of 32 (38 us).
+// two loads and two stores (2 x 8192 tokens, 40 heads of 128, 96 of them turned, bf16: 81 -> 64 us).  Rows that do not start on 16 bytes, or halves that
+// do not, go one pair at a time.  A copy's rate: 5.3 TB/s there, 5.2 for fp32 1536 x 32 tokens, 16 heads of 32 (39 us).
 #include <algorithm>
 
 #include "seq_div.h"
