@@ -9,6 +9,8 @@ namespace seqattn {
 
 constexpr long long MAX_TOKEN_STRIDE = ((1ll << 31) - 4096) / 64;    // bytes: 64 rows within 2^31, for a lane's offset in a tile is 32 bits
 
+constexpr long long MAX_KEYS = (1ll << 31) - (1 << 17);             // keys are counted in 32 bits, up to 128 times 512 splits behind the last one
+
 static bool bad_tensor(const dpc_seq_tensor& t, int es) {
     return !t.p || ((size_t)t.p | (size_t)(t.stride_b * es) | (size_t)(t.stride_t * es) | (size_t)(t.stride_h * es)) % 16 != 0 ||
            t.stride_t < 0 || t.stride_t * es > MAX_TOKEN_STRIDE;
@@ -20,7 +22,7 @@ static int check(const dpc_seq_attn* a, bool backward) {
     DPC_REQUIRE(a->batch >= 0 && a->q_len >= 0 && a->k_len >= 0, "seq_attn: negative size");
     DPC_REQUIRE(a->heads >= 1 && a->kv_heads >= 1 && a->heads % a->kv_heads == 0, "seq_attn: heads must be a multiple of kv_heads");
     DPC_REQUIRE(a->head_dim >= 8 && a->head_dim <= 128 && a->head_dim % 8 == 0, "seq_attn: head_dim must be a multiple of 8 up to 128");
-    DPC_REQUIRE((a->q_len + 2ll * QB) * (a->heads / a->kv_heads) < (1ll << 31) && a->k_len < (1ll << 31) - 2 * QB, "seq_attn: sequence too long");
+    DPC_REQUIRE((a->q_len + 2ll * QB) * (a->heads / a->kv_heads) < (1ll << 31) && a->k_len <= MAX_KEYS, "seq_attn: sequence too long");
     DPC_REQUIRE(a->scale > 0.f && std::isfinite(a->scale), "seq_attn: scale must be positive and finite");
     DPC_REQUIRE(!a->q_tiles == !a->k_tiles && a->n_q_tiles >= 0 && a->n_k_tiles >= 0 && (a->q_tiles || a->n_q_tiles + a->n_k_tiles == 0) &&
                     ((size_t)a->q_tiles | (size_t)a->k_tiles) % 32 == 0, "seq_attn: both block lists, on 32 bytes, or neither");

@@ -169,3 +169,14 @@ def test_attention_refuses_scales_beyond_fp32(scale):
         S.attention_forward(q, q, q, scale=scale)
     with pytest.raises(ValueError, match="scale"):
         S.attention_backward(q, q, q, q, q, torch.zeros(1, 1, 2), scale=scale)
+
+
+def test_attention_entries_refuse_key_axes_whose_splits_would_pass_32_bits():
+    """Splits are whole tiles, up to 512 of them: the last one ends up to 2^16 behind the last key, and that has to be a 32-bit number too."""
+    L = _lib.lib()
+    for k_len, fine in (((1 << 31) - (1 << 17), True), ((1 << 31) - (1 << 17) + 1, False), ((1 << 31) - 300, False), ((1 << 31) - 257, False)):
+        for q_len in (1, 40):
+            a = _attn(q_len=q_len, k_len=k_len)
+            assert (L.dpc_seq_attn_workspace_bytes(C.byref(a), 0) > 0) == fine, (q_len, k_len)
+            if not fine:
+                assert L.dpc_seq_attn_fwd(C.byref(a), C.c_void_p(4096), 1 << 40, None) < 0 and b"too long" in L.dpc_last_error()
