@@ -457,7 +457,7 @@ int dpc_seq_rotary_run(const dpc_seq_rotary* a, dpc_stream_t stream);
  * query / key rows once, in launch order, as (sequence, block, first query row, queries, first key row, keys, then two words that are not read) of the sequence, rows
  * counted from the batch entry's own base (stride_b = 0: packed); q_len / k_len are the longest.  Rows that no sequence covers are not written.
  * head_dim: a multiple of 8, at most 128.  Tensor bases and strides: multiples of 16 bytes; token
- * strides at most 2^25 - 64 bytes. */
+ * strides at most 2^25 - 64 bytes; k_len at most 2^31 - 2^17. */
 typedef struct dpc_seq_attn {
     dpc_seq_tensor q, k, v, out;             /* forward: out is written; backward: read */
     float* lse;
